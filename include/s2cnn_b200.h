@@ -2,7 +2,7 @@
  * s2cnn_b200 - C ABI of the B200-native spectral hot path of s2cnn.
  *
  * Every entry point takes plain pointers and sizes.  Device pointers must be float32, contiguous,
- * 16-byte aligned and live on the current CUDA device; `stream` is a cudaStream_t passed as void*
+ * 16-byte aligned (but see "sequences of signals") and live on the current CUDA device; `stream` is a cudaStream_t passed as void*
  * (NULL = the legacy default stream).  All functions return 0 on success and a non-zero status
  * otherwise, with a message available from s2c_last_error() (thread-local).  Nothing is thrown
  * across the boundary.  Except for the constant tables (built and uploaded on the first call that
@@ -317,6 +317,62 @@ int s2c_so3_rotate_spectrum(const float* U, const float* x, float* z, int b, lon
  * render_model, examples/shrec17/dataset.py:53-95 (trimesh / pyembree ray casting on the host). */
 int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, const float* grid,
                           int nr, float* out, void* stream);
+
+/* ---- sequences of signals ------------------------------------------------------------------- */
+/* Operators of a model over signals in order (frames, shells, rings): attention with a learned bias by
+ * buckets of the relative position, layer norm, dropout, each with its gradient (no counterpart in the
+ * reference).  `dtype` is the type of every value array of a call: 0 float32, 1 bfloat16; arithmetic
+ * and sums are float32 for both.  These arrays need no more alignment than their type.  Results and
+ * gradients are the same to the last bit in every call on the same inputs.
+ *
+ * A call of s2c_attention, q [batch][lq][heads][dim], k and v [batch][lk][kv_heads][dim], any strides
+ * (in elements, of the first three axes; the last is contiguous), dim <= 128, heads a multiple of
+ * kv_heads (query head h reads key head h / (heads / kv_heads)):
+ *   seen(i, j) = i < q_length and j < kv_length and (not causal or j <= i + start)
+ *   out(i)     = sum_j softmax_j(scale q(i).k(j) + bias[bucket_of[clamp(j - i - start, +-reach) + reach]][head]) v(j)
+ * over the seen j; 0 where a query sees nothing.  start, q_length and kv_length are those of the batch entry
+ * (device int32 [batch]; NULL: q_start, lq, lk; lengths outside 0 .. lq / lk are clamped).  bias
+ * [n_buckets][heads] and bucket_of (device int32 [2 reach + 1]; an entry outside 0 .. n_buckets - 1 means no
+ * bias) come together or are both NULL.  reach <= 2048, n_buckets <= 1024.  Rows of k and v that no query sees
+ * are not read.  (Under `causal`, what a tile of 128 queries sees is read by the whole tile: an infinity or NaN
+ * among those values may reach its other queries.) */
+typedef struct s2c_attention_desc {
+  int dtype, batch, lq, lk, heads, kv_heads, dim;
+  long q_stride[3], k_stride[3], v_stride[3];      /* batch entry, position, head */
+  int causal;
+  float scale;
+  int q_start;
+  const int *q_starts, *q_lengths, *kv_lengths;
+  const int* bucket_of;
+  int n_buckets, reach;
+} s2c_attention_desc;
+/* out [batch][lq][heads][dim].  saved (NULL: no backward pass follows): s2c_attention_saved_bytes() bytes that
+ * s2c_attention_backward reads, 16-byte aligned. */
+size_t s2c_attention_workspace(const s2c_attention_desc* desc);
+size_t s2c_attention_saved_bytes(const s2c_attention_desc* desc);
+int s2c_attention(const s2c_attention_desc* desc, const void* q, const void* k, const void* v, const void* bias, void* out,
+                  void* saved, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients dq, dk, dv (laid out as out and as k without gaps) and dbias (NULL: not wanted) from that of out
+ * (dout, laid out as out).  Computes the probabilities again; nothing of size lq * lk is stored. */
+size_t s2c_attention_backward_workspace(const s2c_attention_desc* desc);
+int s2c_attention_backward(const s2c_attention_desc* desc, const void* q, const void* k, const void* v, const void* bias,
+                           const void* out, const void* saved, const void* dout, void* dq, void* dk, void* dv, void* dbias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last of [rows][cols], cols <= 16384; weight or
+ * bias NULL: 1, 0.  stats: [rows][2] floats (mean, 1 / sqrt(var + eps)) for the backward pass, or NULL. */
+int s2c_layer_norm(int dtype, const void* x, const void* weight, const void* bias, void* y, float* stats, long rows, int cols,
+                   float eps, void* stream);
+size_t s2c_layer_norm_backward_workspace(long rows, int cols);
+/* dx, dweight, dbias: NULL where not wanted; the workspace is needed for the latter two. */
+int s2c_layer_norm_backward(int dtype, const void* x, const void* weight, const float* stats, const void* dy, void* dx,
+                            void* dweight, void* dbias, long rows, int cols, void* workspace, size_t workspace_bytes,
+                            void* stream);
+/* out[i] = residual[i] + (word(i) >= floor(probability 2^32) ? x[i] / (1 - probability) : 0), 0 <= probability
+ * < 1, residual NULL: 0.  word(i) is word i % 4 of Philox-4x32 with seven rounds at counter (i / 4, step), key
+ * seed (64 bits each, low words first); it is computed, never stored, and the gradient is the same call on the
+ * gradient of out without a residual. */
+int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long n, double probability,
+                unsigned long long seed, unsigned long long step, void* stream);
 
 /* ---- test hooks (not part of the drop-in surface; no counterpart in the reference) ------------ */
 /* Path selection for the test-suite, so that every kernel variant can be compared with the oracle

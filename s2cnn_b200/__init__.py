@@ -13,6 +13,8 @@ from .s2_mm import s2_mm
 from .so3_mm import so3_mm
 from .soft import (S2Convolution, SO3Convolution, SO3Shortcut, so3_integrate, so3_relu_integrate,
                    so3_rotation)
+from .sequence import (attention, layer_norm, dropout, relative_buckets, RelativeBias, LayerNorm, Dropout,
+                       SequenceBlock)
 from .fuse import fuse
 from . import models, projection
 from .tables import set_table_cache_dir
@@ -22,5 +24,7 @@ __all__ = [
     "so3_near_identity_grid", "so3_equatorial_grid", "so3_soft_grid", "s2_mm", "so3_mm",
     "so3_rotation",
     "S2Convolution", "SO3Convolution", "SO3Shortcut", "so3_integrate", "so3_relu_integrate",
+    "attention", "layer_norm", "dropout", "relative_buckets", "RelativeBias", "LayerNorm", "Dropout",
+    "SequenceBlock",
     "fuse", "models", "projection", "set_table_cache_dir",
 ]

@@ -6,7 +6,7 @@ wrap the host-emulation build that the CPU test-suite compiles from the same sou
 """
 import ctypes
 import os
-from ctypes import c_char_p, c_double, c_float, c_int, c_long, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_float, c_int, c_long, c_size_t, c_ulonglong, c_void_p, POINTER
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CUDA_LIB_PATH = os.path.join(_HERE, "lib", "libs2cnn_b200.so")
@@ -96,6 +96,15 @@ _SIGNATURES = {
     "s2c_so3_rotation_matrices": (c_int, [c_int, c_double, c_double, c_double, _P]),
     "s2c_so3_rotate_spectrum": (c_int, [_P, _P, _P, c_int, c_long, c_int, _P]),
     "s2c_project_on_sphere": (c_int, [_P, c_int, _P, c_int, _P, c_int, _P, _P]),
+    "s2c_attention_workspace": (c_size_t, [_P]),
+    "s2c_attention_saved_bytes": (c_size_t, [_P]),
+    "s2c_attention": (c_int, [_P] * 8 + [c_size_t, _P]),
+    "s2c_attention_backward_workspace": (c_size_t, [_P]),
+    "s2c_attention_backward": (c_int, [_P] * 13 + [c_size_t, _P]),
+    "s2c_layer_norm": (c_int, [c_int, _P, _P, _P, _P, _P, c_long, c_int, c_float, _P]),
+    "s2c_layer_norm_backward_workspace": (c_size_t, [c_long, c_int]),
+    "s2c_layer_norm_backward": (c_int, [c_int] + [_P] * 7 + [c_long, c_int, _P, c_size_t, _P]),
+    "s2c_dropout": (c_int, [c_int, _P, _P, _P, c_long, c_double, c_ulonglong, c_ulonglong, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -16,6 +16,7 @@ from concurrent.futures import ThreadPoolExecutor
 PKG = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(PKG, "csrc", "lib.cu")
 PARTS_SRC = os.path.join(PKG, "csrc", "parts.cu")
+SEQ_SRC = os.path.join(PKG, "csrc", "sequence.cu")
 N_PARTS = 18
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libs2cnn_b200.so")
@@ -92,6 +93,7 @@ def build(force=False, verbose=False):
     with tempfile.TemporaryDirectory(dir=LIB_DIR) as tmp:
         jobs = [(PARTS_SRC, ["-DS2C_PART=%d" % k], os.path.join(tmp, "part%d.o" % k)) for k in range(N_PARTS)]
         jobs.append((SRC, [], os.path.join(tmp, "lib.o")))
+        jobs.append((SEQ_SRC, [], os.path.join(tmp, "sequence.o")))
         with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
             list(pool.map(lambda j: run([nvcc] + flags + j[1] + ["-c", j[0], "-o", j[2]]), jobs))
         out = os.path.join(tmp, "lib.so")

@@ -66,6 +66,8 @@ struct Ctx {
   // barrier among the 32 threads of a warp (every warp of the block must call it equally often:
   // the emulation build implements it as a block barrier)
   __device__ __forceinline__ void sync_warp() const { __syncwarp(); }
+  // exchange within a warp, by every thread of the block (as sync_warp)
+  __device__ __forceinline__ float shfl_xor(float v, int mask) const { return __shfl_xor_sync(0xffffffffu, v, mask); }
 };
 
 inline int cuda_check(cudaError_t e, const char* what) {
@@ -409,6 +411,14 @@ struct Ctx {
     if (b->nthr > 1) swapcontext(&b->th[tid], &b->sched);
   }
   void sync_warp() const { sync(); }
+  float shfl_xor(float v, int mask) const {
+    static thread_local float lanes[1024];
+    lanes[tid] = v;
+    sync();
+    const float r = lanes[tid ^ mask];
+    sync();
+    return r;
+  }
 };
 
 inline void emu_trampoline() {

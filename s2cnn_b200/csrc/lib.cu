@@ -1,6 +1,7 @@
 // C-ABI entry points of s2cnn_b200 (see include/s2cnn_b200.h) and the host-side dispatch that
 // sequences the kernels.  nvcc -gencode arch=compute_100a,code=sm_100a for the product, the kernel
-// families with many instantiations compiled beside it from parts.cu (-DS2C_SPLIT); one translation unit
+// families with many instantiations compiled beside it from parts.cu (-DS2C_SPLIT), the operators for sequences
+// from sequence.cu; one translation unit
 // with g++ -x c++ -DS2C_EMUL for the host-emulation build used by the CPU tests.
 #include "../../include/s2cnn_b200.h"
 
@@ -32,6 +33,9 @@
 #include "so3_mm_tc.h"
 #include "misc_kernels.h"
 #include "project_kernels.h"
+#ifdef S2C_EMUL
+#include "sequence.h"
+#endif
 
 namespace s2c {
 thread_local long g_launch_count = 0;

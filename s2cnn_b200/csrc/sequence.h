@@ -1,0 +1,305 @@
+// C-ABI entry points of the operators for sequences of signals (the last section of include/s2cnn_b200.h): checks and the
+// choice of kernels.  Compiled from sequence.cu beside lib.cu; part of lib.cu's translation unit in the host-emulation build.
+#pragma once
+
+#include "../../include/s2cnn_b200.h"
+
+#include <algorithm>
+#include <cmath>
+
+#include "attention_kernels.h"
+#include "dropout_kernels.h"
+#include "layer_norm_kernels.h"
+
+namespace s2c {
+
+#define S2C_SEQ_TRY(expr)            \
+  do {                               \
+    int rc__ = (expr);               \
+    if (rc__ != S2C_OK) return rc__; \
+  } while (0)
+
+inline int seq_check_type(const char* who, int dtype) {
+  return dtype == kSeqF32 || dtype == kSeqBf16 ? S2C_OK : fail(S2C_ERR_BAD_ARG, std::string(who) + ": dtype is 0 (float32) or 1 (bfloat16)");
+}
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// ---- layer norm --------------------------------------------------------------------------------------------------------
+// A row takes the fewest threads that hold it in at most 32 registers each: neighbouring lanes up to 1024 columns, a block
+// of 128 up to 4096 and of 512 beyond.
+constexpr int kNormMaxCols = 16384;
+template <class F>
+int norm_by_cols(int cols, F f) {
+#define S2C_NORM(T, EPT) return f(std::integral_constant<int, T>(), std::integral_constant<int, EPT>())
+  if (cols <= 32) S2C_NORM(4, 8);
+  if (cols <= 128) S2C_NORM(16, 8);
+  if (cols <= 256) S2C_NORM(32, 8);
+  if (cols <= 512) S2C_NORM(32, 16);
+  if (cols <= 1024) S2C_NORM(32, 32);
+  if (cols <= 2048) S2C_NORM(128, 16);
+  if (cols <= 4096) S2C_NORM(128, 32);
+  if (cols <= 8192) S2C_NORM(512, 16);
+  S2C_NORM(512, 32);
+#undef S2C_NORM
+}
+inline int norm_bwd_blocks(long rows, int cols) {
+  return norm_by_cols(cols, [&](auto t, auto ept) {
+    using K = LayerNormBwd<float, decltype(t)::value, decltype(ept)::value, 1>;
+    return (int)std::min<long>((rows + K::kTeams - 1) / K::kTeams, (long)dev_sm_count() * K::kBlocks);
+  });
+}
+template <class T>
+int norm_forward(LayerNormParams p, stream_t st) {
+  const bool vec = p.cols % kVec<T> == 0;
+  p.wide = vec && aligned16(p.x) && aligned16(p.y) && aligned16(p.w) && aligned16(p.b);
+  return norm_by_cols(p.cols, [&](auto t, auto ept) {
+    constexpr int TT = decltype(t)::value, E = decltype(ept)::value;
+    using V = LayerNormFwd<T, TT, E, kVec<T>>;
+    using S = LayerNormFwd<T, TT, E, 1>;
+    const long blocks = std::min<long>((p.rows + V::kTeams - 1) / V::kTeams, 8L * dev_sm_count() * V::kBlocks);
+    return vec ? seq_launch<V>("layer_norm", blocks, V::smem(), st, p) : seq_launch<S>("layer_norm", blocks, S::smem(), st, p);
+  });
+}
+template <class T>
+int norm_backward(LayerNormParams p, void* dw, void* db, stream_t st) {
+  const int blocks = norm_bwd_blocks(p.rows, p.cols);
+  const bool vec = p.cols % kVec<T> == 0;
+  p.wide = vec && aligned16(p.x) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.w);
+  S2C_SEQ_TRY(norm_by_cols(p.cols, [&](auto t, auto ept) {
+    constexpr int TT = decltype(t)::value, E = decltype(ept)::value;
+    using V = LayerNormBwd<T, TT, E, kVec<T>>;
+    using S = LayerNormBwd<T, TT, E, 1>;
+    return vec ? seq_launch<V>("layer_norm_backward", blocks, V::smem(), st, p)
+               : seq_launch<S>("layer_norm_backward", blocks, S::smem(), st, p);
+  }));
+  if (!p.part) return S2C_OK;
+  LayerNormSumParams s;
+  s.part = p.part; s.dw = dw; s.db = db; s.blocks = blocks; s.cols = p.cols;
+  return seq_launch<LayerNormSum<T>>("layer_norm_sums", (2L * p.cols + 31) / 32, 256 * sizeof(float), st, s);
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------------
+constexpr int kAttnMaxDim = 128, kAttnMaxReach = 2048, kAttnMaxBuckets = 1024;
+inline int attn_check(const char* who, const s2c_attention_desc* d) {
+  const std::string w = std::string(who) + ": ";
+  if (!d) return fail(S2C_ERR_BAD_ARG, w + "no description");
+  S2C_SEQ_TRY(seq_check_type(who, d->dtype));
+  if (d->batch < 0 || d->lq < 0 || d->lk < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads || d->dim < 1)
+    return fail(S2C_ERR_BAD_ARG, w + "bad sizes (the query heads are a multiple of the key heads)");
+  if (d->dim > kAttnMaxDim) return fail(S2C_ERR_UNSUPPORTED, w + "at most 128 values per head");
+  if (std::max(d->lq, d->lk) > (1 << 28)) return fail(S2C_ERR_UNSUPPORTED, w + "at most 2^28 positions");
+  if ((long)d->batch * d->heads > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, w + "too many heads");
+  if (d->bucket_of && (d->n_buckets < 1 || d->reach < 0)) return fail(S2C_ERR_BAD_ARG, w + "bad buckets");
+  if (d->bucket_of && (d->n_buckets > kAttnMaxBuckets || d->reach > kAttnMaxReach))
+    return fail(S2C_ERR_UNSUPPORTED, w + "at most 1024 buckets and relative positions up to 2048");
+  if (!(std::fabs(d->scale) <= FLT_MAX)) return fail(S2C_ERR_BAD_ARG, w + "the scale is not finite");
+  return S2C_OK;
+}
+inline AttnParams attn_params(const s2c_attention_desc* d, const void* q, const void* k, const void* v, const void* bias) {
+  AttnParams p = {};
+  p.q = q; p.k = k; p.v = v; p.bias = d->bucket_of ? bias : nullptr;
+  p.bucket_of = d->bucket_of; p.start = d->q_starts; p.q_len = d->q_lengths; p.kv_len = d->kv_lengths;
+  for (int i = 0; i < 3; ++i) { p.qs[i] = d->q_stride[i]; p.ks[i] = d->k_stride[i]; p.vs[i] = d->v_stride[i]; }
+  p.batch = d->batch; p.lq = d->lq; p.lk = d->lk; p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->dim;
+  p.group = d->heads / d->kv_heads;
+  p.causal = d->causal != 0; p.scale = d->scale; p.start_all = d->q_start;
+  p.reach = p.bias ? d->reach : 0; p.n_buckets = p.bias ? d->n_buckets : 0;
+  p.splits = 1;
+  return p;
+}
+template <class T, class F>
+int attn_by_dim(int dim, F f) {
+  if (dim <= 16) return f(std::integral_constant<int, 16>());
+  if (dim <= 32) return f(std::integral_constant<int, 32>());
+  if (dim <= 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+inline int attn_padded(int dim) { return dim <= 16 ? 16 : dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
+inline size_t attn_align(size_t n) { return (n + 255) / 256 * 256; }
+// What the backward pass needs beside the output: the statistics of the rows, and in bfloat16 what the rounding of the output
+// left.  delta = dO . O is one error for a whole row of dS, which the bias gradient sums over all rows: with the rounded output
+// its relative error is 3.1e-3 (8 x 1000 positions, 8 heads of 64), with the rest 1.9e-3, which is its own rounding.
+inline size_t attn_stats_bytes(const AttnParams& p) { return attn_align((size_t)p.batch * p.heads * p.lq * sizeof(float2)); }
+inline size_t attn_saved_bytes(const AttnParams& p, int dtype) {
+  return attn_stats_bytes(p) + (dtype == kSeqBf16 ? (size_t)p.batch * p.lq * p.heads * p.dim * 2 : 0);
+}
+inline void attn_set_saved(AttnParams& p, int dtype, void* saved) {
+  if (!saved) return;
+  p.stats = static_cast<float2*>(saved);
+  if (dtype == kSeqBf16) p.out_lo = static_cast<char*>(saved) + attn_stats_bytes(p);
+}
+
+// Few rows per key head: the keys are split so that every SM has two blocks' worth of them.
+inline bool attn_few_rows(const AttnParams& p) { return (long)p.lq * p.group <= kAttnRows; }
+inline void attn_split(AttnParams& p) {
+  const long blocks = std::max(1L, (long)p.batch * p.kv_heads), tiles = std::max(1, (p.lk + kAttnRowKeys - 1) / kAttnRowKeys);
+  const long want = std::min(tiles, std::max(1L, 2L * dev_sm_count() / blocks)), per = (tiles + want - 1) / want;
+  p.chunk = (int)per * kAttnRowKeys;
+  p.splits = (int)((tiles + per - 1) / per);
+}
+inline size_t attn_split_bytes(const AttnParams& p) {
+  return p.splits > 1 ? (size_t)p.batch * p.kv_heads * p.splits * p.lq * p.group * (attn_padded(p.dim) + 2) * sizeof(float) : 0;
+}
+inline size_t attn_forward_bytes(AttnParams p) {
+  if (!attn_few_rows(p)) return 0;
+  attn_split(p);
+  return attn_split_bytes(p);
+}
+template <class T>
+int attn_forward(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
+  if (p.batch == 0 || p.lq == 0) return S2C_OK;
+  if (attn_few_rows(p)) {
+    attn_split(p);
+    if (attn_split_bytes(p) > ws_bytes || (p.splits > 1 && !ws)) return fail(S2C_ERR_WORKSPACE, "s2c_attention: workspace too small");
+    p.part = static_cast<float*>(ws);
+    return attn_by_dim<T>(p.dim, [&](auto d) {
+      constexpr int DP = decltype(d)::value;
+      using K = AttnRows<T, DP>;
+      using J = AttnJoin<T, DP>;
+      S2C_SEQ_TRY(seq_launch<K>("attention_rows", (long)p.batch * p.kv_heads * p.splits, K::smem(p), st, p));
+      if (p.splits == 1) return (int)S2C_OK;
+      const long rows = (long)p.batch * p.kv_heads * p.lq * p.group, per = J::kThreads / DP;
+      return seq_launch<J>("attention_join", (rows + per - 1) / per, 0, st, p);
+    });
+  }
+  p.tiles = (p.lq + kAttnTile - 1) / kAttnTile;
+  return attn_by_dim<T>(p.dim, [&](auto d) {
+    using K = AttnForward<T, decltype(d)::value>;
+    return seq_launch<K>("attention", (long)p.batch * p.heads * p.tiles, K::smem(p), st, p);
+  });
+}
+
+inline size_t attn_delta_bytes(const AttnParams& p) { return attn_align((size_t)p.batch * p.heads * p.lq * sizeof(float)); }
+inline size_t attn_backward_bytes(const AttnParams& p, bool with_bias) {
+  const size_t tiles = (p.lq + kAttnTile - 1) / kAttnTile;
+  return attn_delta_bytes(p) + (with_bias ? (size_t)p.batch * tiles * p.heads * p.n_buckets * sizeof(float) : 0);
+}
+template <class T>
+int attn_backward(AttnParams p, void* dbias, void* ws, size_t ws_bytes, stream_t st) {
+  if (attn_backward_bytes(p, dbias != nullptr) > ws_bytes || (ws_bytes && !ws))
+    return fail(S2C_ERR_WORKSPACE, "s2c_attention_backward: workspace too small");
+  p.delta = static_cast<float*>(ws);
+  p.dbias_part = dbias ? reinterpret_cast<float*>(static_cast<char*>(ws) + attn_delta_bytes(p)) : nullptr;
+  S2C_SEQ_TRY(attn_by_dim<T>(p.dim, [&](auto d) {
+    constexpr int DP = decltype(d)::value;
+    using Q = AttnGradQ<T, DP>;
+    using KV = AttnGradKV<T, DP>;
+    p.tiles = (p.lq + kAttnTile - 1) / kAttnTile;
+    S2C_SEQ_TRY(seq_launch<Q>("attention_grad_q", (long)p.batch * p.heads * p.tiles, Q::smem(p), st, p));
+    AttnParams kv = p;
+    kv.tiles = (p.lk + kAttnTile - 1) / kAttnTile;
+    return seq_launch<KV>("attention_grad_kv", (long)p.batch * p.kv_heads * kv.tiles, KV::smem(kv), st, kv);
+  }));
+  if (!dbias) return S2C_OK;
+  AttnBiasSumParams s;
+  s.part = p.dbias_part; s.out = dbias; s.parts = p.batch * p.tiles; s.heads = p.heads; s.n_buckets = p.n_buckets;
+  return seq_launch<AttnBiasSum<T>>("attention_bias_sums", ((long)p.heads * p.n_buckets + 7) / 8, 256 * sizeof(float), st, s);
+}
+
+}  // namespace s2c
+
+using namespace s2c;
+
+extern "C" {
+
+int s2c_layer_norm(int dtype, const void* x, const void* weight, const void* bias, void* y, float* stats, long rows, int cols,
+                   float eps, void* stream) {
+  S2C_SEQ_TRY(seq_check_type("s2c_layer_norm", dtype));
+  if (rows < 0 || cols < 1 || (rows > 0 && (!x || !y)) || !(eps >= 0.f)) return fail(S2C_ERR_BAD_ARG, "s2c_layer_norm: bad argument");
+  if (cols > kNormMaxCols) return fail(S2C_ERR_UNSUPPORTED, "s2c_layer_norm: at most 16384 columns");
+  LayerNormParams p = {};
+  p.x = x; p.w = weight; p.b = bias; p.y = y; p.stats = stats; p.rows = rows; p.cols = cols; p.eps = eps;
+  return dtype == kSeqF32 ? norm_forward<float>(p, (stream_t)stream) : norm_forward<bf16>(p, (stream_t)stream);
+}
+
+size_t s2c_layer_norm_backward_workspace(long rows, int cols) {
+  if (rows < 1 || cols < 1 || cols > kNormMaxCols) return 0;
+  return (size_t)norm_bwd_blocks(rows, cols) * 2 * cols * sizeof(float);
+}
+
+int s2c_layer_norm_backward(int dtype, const void* x, const void* weight, const float* stats, const void* dy, void* dx, void* dweight,
+                            void* dbias, long rows, int cols, void* workspace, size_t workspace_bytes, void* stream) {
+  S2C_SEQ_TRY(seq_check_type("s2c_layer_norm_backward", dtype));
+  if (rows < 0 || cols < 1 || (rows > 0 && (!x || !dy || !stats))) return fail(S2C_ERR_BAD_ARG, "s2c_layer_norm_backward: bad argument");
+  if (cols > kNormMaxCols) return fail(S2C_ERR_UNSUPPORTED, "s2c_layer_norm_backward: at most 16384 columns");
+  const bool sums = dweight || dbias;
+  const size_t need = sums ? s2c_layer_norm_backward_workspace(rows, cols) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return fail(S2C_ERR_WORKSPACE, "s2c_layer_norm_backward: workspace too small");
+  LayerNormParams p = {};
+  static float none;           // (no rows: the sums are written as zeros, nothing is read)
+  p.x = x; p.w = weight; p.dy = dy; p.dx = dx; p.stats = const_cast<float*>(stats); p.rows = rows; p.cols = cols;
+  p.part = !sums ? nullptr : need ? static_cast<float*>(workspace) : &none;
+  return dtype == kSeqF32 ? norm_backward<float>(p, dweight, dbias, (stream_t)stream) : norm_backward<bf16>(p, dweight, dbias, (stream_t)stream);
+}
+
+int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long n, double probability, unsigned long long seed,
+                unsigned long long step, void* stream) {
+  S2C_SEQ_TRY(seq_check_type("s2c_dropout", dtype));
+  if (n < 0 || (n > 0 && (!x || !out)) || !(probability >= 0. && probability < 1.)) return fail(S2C_ERR_BAD_ARG, "s2c_dropout: bad argument");
+  DropoutParams p = {};
+  p.x = x; p.residual = residual; p.out = out; p.n = n;
+  p.threshold = (unsigned)std::floor(probability * 4294967296.);
+  p.scale = (float)(1. / (1. - probability));
+  for (int i = 0; i < 2; ++i) {
+    p.key[i] = (unsigned)(seed >> (32 * i));
+    p.step[i] = (unsigned)(step >> (32 * i));
+  }
+  const bool vec = aligned16(x) && aligned16(residual) && aligned16(out);
+  auto go = [&](auto k) {
+    using K = typename decltype(k)::type;
+    const long blocks = (n + (long)K::kThreads * K::kStep - 1) / ((long)K::kThreads * K::kStep);
+    return seq_launch<K>("dropout", std::min<long>(blocks, 32L * dev_sm_count()), 0, (stream_t)stream, p);
+  };
+  struct A { using type = Dropout<float, true>; };
+  struct B { using type = Dropout<float, false>; };
+  struct C { using type = Dropout<bf16, true>; };
+  struct D { using type = Dropout<bf16, false>; };
+  return dtype == kSeqF32 ? (vec ? go(A()) : go(B())) : (vec ? go(C()) : go(D()));
+}
+
+size_t s2c_attention_workspace(const s2c_attention_desc* d) {
+  if (attn_check("s2c_attention_workspace", d) != S2C_OK) return 0;
+  return attn_forward_bytes(attn_params(d, nullptr, nullptr, nullptr, nullptr));
+}
+
+size_t s2c_attention_saved_bytes(const s2c_attention_desc* d) {
+  if (attn_check("s2c_attention_saved_bytes", d) != S2C_OK) return 0;
+  return attn_saved_bytes(attn_params(d, nullptr, nullptr, nullptr, nullptr), d->dtype);
+}
+
+int s2c_attention(const s2c_attention_desc* d, const void* q, const void* k, const void* v, const void* bias, void* out, void* saved,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  S2C_SEQ_TRY(attn_check("s2c_attention", d));
+  const bool some = d->batch > 0 && d->lq > 0;
+  if (some && (!q || !out || (d->lk > 0 && (!k || !v)))) return fail(S2C_ERR_BAD_ARG, "s2c_attention: a pointer is missing");
+  if ((bias != nullptr) != (d->bucket_of != nullptr)) return fail(S2C_ERR_BAD_ARG, "s2c_attention: a bias needs its buckets, and buckets a bias");
+  AttnParams p = attn_params(d, q, k, v, bias);
+  p.out = out;
+  attn_set_saved(p, d->dtype, saved);
+  return d->dtype == kSeqF32 ? attn_forward<float>(p, workspace, workspace_bytes, (stream_t)stream)
+                             : attn_forward<bf16>(p, workspace, workspace_bytes, (stream_t)stream);
+}
+
+size_t s2c_attention_backward_workspace(const s2c_attention_desc* d) {
+  if (attn_check("s2c_attention_backward_workspace", d) != S2C_OK) return 0;
+  AttnParams p = attn_params(d, nullptr, nullptr, nullptr, d->bucket_of);
+  return attn_backward_bytes(p, d->bucket_of != nullptr);
+}
+
+int s2c_attention_backward(const s2c_attention_desc* d, const void* q, const void* k, const void* v, const void* bias, const void* out,
+                           const void* saved, const void* dout, void* dq, void* dk, void* dv, void* dbias, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  S2C_SEQ_TRY(attn_check("s2c_attention_backward", d));
+  if (d->batch > 0 && d->lq > 0 && (!q || !out || !saved || !dout || !dq)) return fail(S2C_ERR_BAD_ARG, "s2c_attention_backward: a pointer is missing");
+  if (d->batch > 0 && d->lk > 0 && (!k || !v || !dk || !dv)) return fail(S2C_ERR_BAD_ARG, "s2c_attention_backward: a pointer is missing");
+  if ((bias != nullptr) != (d->bucket_of != nullptr) || (dbias && !bias))
+    return fail(S2C_ERR_BAD_ARG, "s2c_attention_backward: a bias needs its buckets, and buckets a bias");
+  AttnParams p = attn_params(d, q, k, v, bias);
+  p.o = out; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
+  attn_set_saved(p, d->dtype, const_cast<void*>(saved));
+  return d->dtype == kSeqF32 ? attn_backward<float>(p, dbias, workspace, workspace_bytes, (stream_t)stream)
+                             : attn_backward<bf16>(p, dbias, workspace, workspace_bytes, (stream_t)stream);
+}
+
+}  // extern "C"

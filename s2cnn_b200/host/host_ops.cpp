@@ -82,7 +82,9 @@ long s2_bandwidth(long nspec) {
   X(s2_conv_synthesis_workspace) X(s2_conv_synthesis) X(s2_conv_real_synthesis_workspace) X(s2_conv_real_synthesis) X(s2_conv_real_relu_so3_rfft) X(so3_ifft) X(s2_fft_workspace) X(s2_fft)    \
   X(s2_ifft) X(so3_mm) X(so3_mm_gradx_ws) X(so3_mm_gradx_workspace) X(so3_mm_grady_ws) X(so3_mm_grady_workspace) X(so3_mm_real) X(so3_mm_real_workspace) X(so3_mm_tc_status) X(s2_mm) X(s2_mm_gradx) \
   X(s2_mm_grady) X(s2_mm_real_gradx) X(s2_mm_real_grady) X(rft_forward) X(rft_forward_t) X(rft_forward_scaled) X(rft_backward_scaled) X(rft_backward_workspace) X(so3_integrate)                  \
-  X(so3_integrate_backward) X(so3_rotate_spectrum) X(project_on_sphere)
+  X(so3_integrate_backward) X(so3_rotate_spectrum) X(project_on_sphere)                            \
+  X(attention_workspace) X(attention_saved_bytes) X(attention) X(attention_backward_workspace) X(attention_backward)        \
+  X(layer_norm) X(layer_norm_backward_workspace) X(layer_norm_backward) X(dropout)
 
 struct Ops {
 #define X(name) decltype(&::s2c_##name) name##_ = nullptr;
@@ -111,12 +113,15 @@ struct Ops {
   // result and nothing that fills it) nor forward-mode differentiation sees: refused here.  The
   // differentiable ops are recorded by a tracer as one node each, see S2C_TRACED.
   void prep(const Tensor& t) const {
+    prep_any(t);
+    if (t.scalar_type() != at::kFloat)
+      raise(PyExc_TypeError, std::string("s2cnn_b200 kernels are float32 only, got ") + c10::toString(t.scalar_type()));
+  }
+  void prep_any(const Tensor& t) const {
     if (tracing())
       raise(PyExc_RuntimeError, "s2cnn_b200: torch.jit.trace cannot record this op (the differentiable layers and transforms can be traced)");
     if (t._fw_grad(0).defined())
       raise(PyExc_NotImplementedError, "s2cnn_b200 ops do not implement forward-mode automatic differentiation (no jvp)");
-    if (t.scalar_type() != at::kFloat)
-      raise(PyExc_TypeError, std::string("s2cnn_b200 kernels are float32 only, got ") + c10::toString(t.scalar_type()));
     if (t.is_cuda() != is_cuda)
       raise_s2c("s2cnn_b200: tensor on " + t.device().str() + " but the loaded library is the " +
                 (is_cuda ? "CUDA" : "emulation") + " build - the product path runs on CUDA only");
@@ -630,6 +635,147 @@ struct Ops {
     S2C_CALL(project_on_sphere, cptr(verts), (int)verts.size(0), faces.const_data_ptr<int>(), (int)faces.size(0), cptr(grid), (int)grid.size(0), ptr(out), c.stream);
     return out;
   }
+
+  // -- sequences of signals: float32 or bfloat16, one type per call -----------------------------------
+  int prep_seq(const Tensor& t) const {
+    prep_any(t);
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16)
+      raise(PyExc_TypeError, std::string("s2cnn_b200: float32 or bfloat16 expected, got ") + c10::toString(t.scalar_type()));
+    return t.scalar_type() == at::kBFloat16;
+  }
+  void prep_like(const Tensor& t, const Tensor& first, const char* what) const {
+    prep_any(t);
+    if (t.scalar_type() != first.scalar_type())
+      raise(PyExc_TypeError, std::string(what) + ": " + c10::toString(t.scalar_type()) + " beside " + c10::toString(first.scalar_type()));
+    check(t.device() == first.device(), "s2cnn_b200: tensors on different devices");
+  }
+  const int* int_ptr(const Tensor& t, const Tensor& first, int64_t n, const char* what) const {
+    if (!t.defined()) return nullptr;
+    if (t.scalar_type() != at::kInt || t.device() != first.device())
+      raise(PyExc_TypeError, std::string(what) + ": an int32 tensor on the device of the queries");
+    if (t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
+      raise(PyExc_AssertionError, std::string(what) + ": " + std::to_string(n) + " consecutive values expected");
+    return t.const_data_ptr<int>();
+  }
+  static const void* vptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+  static void* vmut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+  static Tensor unit_stride(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+  struct AttnArgs {      // undefined tensors: not given
+    Tensor q, k, v, bias, buckets, starts, q_lengths, kv_lengths;
+    bool causal = false;
+    double scale = 0;
+    int64_t q_start = 0;
+  };
+  s2c_attention_desc attention_desc(AttnArgs& a) const {
+    const int dtype = prep_seq(a.q);
+    prep_like(a.k, a.q, "attention: keys");
+    prep_like(a.v, a.q, "attention: values");
+    check(a.q.dim() == 4 && a.k.dim() == 4, "attention: [batch, length, heads, dim] operands");
+    check(a.k.sizes() == a.v.sizes(), "attention: keys and values differ in shape");
+    check(a.q.size(0) == a.k.size(0) && a.q.size(3) == a.k.size(3), "attention: queries and keys differ in batch or dim");
+    check(a.k.size(2) > 0 && a.q.size(2) > 0 && a.q.size(2) % a.k.size(2) == 0, "attention: the query heads are a multiple of the key heads");
+    check(a.bias.defined() == a.buckets.defined(), "attention: bias and buckets come together");
+    check(std::abs(a.q_start) <= 0x7fffffff, "attention: q_start is out of range");
+    for (int i = 0; i < 4; ++i) check(a.q.size(i) <= 0x7fffffff && a.k.size(i) <= 0x7fffffff, "attention: too large");
+    s2c_attention_desc d = {};
+    d.dtype = dtype;
+    d.batch = (int)a.q.size(0); d.lq = (int)a.q.size(1); d.heads = (int)a.q.size(2); d.dim = (int)a.q.size(3);
+    d.lk = (int)a.k.size(1); d.kv_heads = (int)a.k.size(2);
+    a.q = unit_stride(a.q);
+    a.k = unit_stride(a.k);
+    a.v = unit_stride(a.v);
+    for (int i = 0; i < 3; ++i) { d.q_stride[i] = a.q.stride(i); d.k_stride[i] = a.k.stride(i); d.v_stride[i] = a.v.stride(i); }
+    d.causal = a.causal;
+    d.scale = (float)a.scale;
+    d.q_start = (int)a.q_start;
+    d.q_starts = int_ptr(a.starts, a.q, d.batch, "attention: q_start");
+    d.q_lengths = int_ptr(a.q_lengths, a.q, d.batch, "attention: q_lengths");
+    d.kv_lengths = int_ptr(a.kv_lengths, a.q, d.batch, "attention: kv_lengths");
+    if (a.bias.defined()) {
+      prep_like(a.bias, a.q, "attention: bias");
+      check(a.bias.dim() == 2 && a.bias.size(1) == d.heads && a.bias.size(0) >= 1, "attention: bias [buckets, heads]");
+      check(a.buckets.dim() == 1 && a.buckets.size(0) % 2 == 1, "attention: buckets of the positions -reach ... reach");
+      a.bias = a.bias.contiguous();
+      d.bucket_of = int_ptr(a.buckets, a.q, a.buckets.size(0), "attention: buckets");
+      d.n_buckets = (int)a.bias.size(0);
+      d.reach = (int)(a.buckets.size(0) / 2);
+    }
+    return d;
+  }
+  std::tuple<Tensor, Tensor> attention(AttnArgs a, bool want_saved) const {
+    const s2c_attention_desc d = attention_desc(a);
+    Tensor out = at::empty({d.batch, d.lq, d.heads, d.dim}, a.q.options()), saved;
+    if (want_saved) saved = at::empty({(int64_t)attention_saved_bytes_(&d)}, a.q.options().dtype(at::kByte));
+    Ctx c(*this, a.q);
+    const Scratch ws(attention_workspace_(&d), a.q);
+    S2C_CALL(attention, &d, vptr(a.q), vptr(a.k), vptr(a.v), vptr(a.bias), vmut(out), vmut(saved), ws.p, ws.n, c.stream);
+    return {out, saved};
+  }
+  // dq, dk, dv, dbias
+  std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(AttnArgs a, const Tensor& out, const Tensor& saved, const Tensor& dout_,
+                                                                bool want_bias) const {
+    const s2c_attention_desc d = attention_desc(a);
+    const Tensor dout = dout_.contiguous();
+    Tensor dq = at::empty({d.batch, d.lq, d.heads, d.dim}, a.q.options()), dk = at::empty({d.batch, d.lk, d.kv_heads, d.dim}, a.q.options()),
+           dv = at::empty_like(dk), dbias;
+    if (want_bias) dbias = at::empty_like(a.bias);
+    Ctx c(*this, a.q);
+    const Scratch ws(attention_backward_workspace_(&d), a.q);
+    S2C_CALL(attention_backward, &d, vptr(a.q), vptr(a.k), vptr(a.v), vptr(a.bias), vptr(out), vptr(saved),
+             vptr(dout), vmut(dq), vmut(dk), vmut(dv), vmut(dbias), ws.p, ws.n, c.stream);
+    return {dq, dk, dv, dbias};
+  }
+
+  long norm_shape(const Tensor& x, const Tensor& w, const Tensor& b) const {
+    check(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 0x7fffffff, "layer_norm: at least one axis, of at least one value");
+    for (const Tensor& t : {w, b})
+      if (t.defined()) {
+        prep_like(t, x, "layer_norm: weight and bias");
+        check(t.dim() == 1 && t.size(0) == x.size(-1), "layer_norm: weight and bias have the last axis's length");
+      }
+    return x.numel() / x.size(-1);
+  }
+  std::tuple<Tensor, Tensor> layer_norm(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps, bool want_stats) const {
+    const int dtype = prep_seq(x_);
+    const long rows = norm_shape(x_, w_, b_);
+    check(eps >= 0, "layer_norm: eps is negative");
+    const Tensor x = x_.contiguous(), w = w_.defined() ? w_.contiguous() : w_, b = b_.defined() ? b_.contiguous() : b_;
+    Tensor y = at::empty_like(x), stats;
+    if (want_stats) stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
+    Ctx c(*this, x);
+    S2C_CALL(layer_norm, dtype, vptr(x), vptr(w), vptr(b), vmut(y), static_cast<float*>(vmut(stats)), rows, (int)x.size(-1), (float)eps, c.stream);
+    return {y, stats};
+  }
+  std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& x_, const Tensor& w_, const Tensor& stats, const Tensor& dy_, bool want_x,
+                                                         bool want_w, bool want_b) const {
+    const int dtype = prep_seq(x_);
+    const Tensor x = x_.contiguous(), w = w_.defined() ? w_.contiguous() : w_, dy = dy_.contiguous();
+    const long cols = x.size(-1), rows = x.numel() / cols;
+    Tensor dx, dw, db;
+    if (want_x) dx = at::empty_like(x);
+    if (want_w) dw = at::empty({cols}, x.options());
+    if (want_b) db = at::empty({cols}, x.options());
+    Ctx c(*this, x);
+    const Scratch ws(want_w || want_b ? layer_norm_backward_workspace_(rows, (int)cols) : 0, x);
+    S2C_CALL(layer_norm_backward, dtype, vptr(x), vptr(w), static_cast<const float*>(vptr(stats)), vptr(dy), vmut(dx), vmut(dw), vmut(db),
+             rows, (int)cols, ws.p, ws.n, c.stream);
+    return {dx, dw, db};
+  }
+
+  Tensor dropout(const Tensor& x_, const Tensor& residual_, double p, uint64_t seed, uint64_t step) const {
+    const int dtype = prep_seq(x_);
+    check(p >= 0 && p < 1, "dropout: 0 <= p < 1");
+    if (residual_.defined()) {
+      prep_like(residual_, x_, "dropout: residual");
+      check(residual_.sizes() == x_.sizes(), "dropout: x and residual differ in shape");
+    }
+    const Tensor x = x_.contiguous(), residual = residual_.defined() ? residual_.contiguous() : residual_;
+    Tensor out = at::empty_like(x);
+    Ctx c(*this, x);
+    S2C_CALL(dropout, dtype, vptr(x), vptr(residual), vmut(out), (long)x.numel(), p, (unsigned long long)seed, (unsigned long long)step, c.stream);
+    return out;
+  }
 };
 
 // ---- autograd rules -------------------------------------------------------------------------------
@@ -820,6 +966,73 @@ struct RotateSpectrum : torch::autograd::Function<RotateSpectrum> {
   }
 };
 
+// ---- sequences of signals ---------------------------------------------------------------------------
+Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
+struct Attention : torch::autograd::Function<Attention> {
+  static Tensor forward(AutogradContext* ctx, int64_t ops, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias_, const OptTensor& buckets_,
+                        const OptTensor& starts_, const OptTensor& q_lengths_, const OptTensor& kv_lengths_, bool causal, double scale, int64_t q_start) {
+    keep_ops(ctx, ops);
+    const Tensor bias = or_none(bias_), buckets = or_none(buckets_), starts = or_none(starts_), q_lengths = or_none(q_lengths_), kv_lengths = or_none(kv_lengths_);
+    Tensor out, saved;
+    std::tie(out, saved) = reinterpret_cast<Ops*>(ops)->attention({q, k, v, bias, buckets, starts, q_lengths, kv_lengths, causal, scale, q_start}, true);
+    ctx->save_for_backward({q, k, v, bias, buckets, starts, q_lengths, kv_lengths, out, saved});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["q_start"] = q_start;
+    return out;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    const auto s = ctx->get_saved_variables();
+    Tensor dq, dk, dv, dbias;
+    std::tie(dq, dk, dv, dbias) = ops_of(ctx)->attention_backward(
+        {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["q_start"].toInt()},
+        s[8], s[9], g[0], s[3].defined() && ctx->needs_input_grad(3));
+    return {Variable(), dq, dk, dv, dbias, Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
+  }
+};
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, int64_t ops, const Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps) {
+    keep_ops(ctx, ops);
+    const Tensor w = or_none(w_), b = or_none(b_);
+    ctx->saved_data["w"] = w.defined();
+    ctx->saved_data["b"] = b.defined();
+    Tensor y, stats;
+    std::tie(y, stats) = reinterpret_cast<Ops*>(ops)->layer_norm(x, w, b, eps, true);
+    ctx->save_for_backward({x, w, stats});
+    return y;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    const auto s = ctx->get_saved_variables();
+    Tensor dx, dw, db;
+    const bool has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["b"].toBool();   // (inputs not given have no index)
+    std::tie(dx, dw, db) = ops_of(ctx)->layer_norm_backward(s[0], s[1], s[2], g[0], ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
+                                                            has_b && ctx->needs_input_grad(has_w ? 2 : 1));
+    return {Variable(), dx, dw, db, Variable()};
+  }
+};
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor forward(AutogradContext* ctx, int64_t ops, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t step) {
+    keep_ops(ctx, ops);
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["step"] = step;
+    return reinterpret_cast<Ops*>(ops)->dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step);
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    Tensor dx;
+    if (ctx->needs_input_grad(0))
+      dx = ops_of(ctx)->dropout(g[0], Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["step"].toInt());
+    return {Variable(), dx, ctx->saved_data["residual"].toBool() ? g[0] : Variable(), Variable(), Variable(), Variable()};
+  }
+};
+bool wants_any(std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
 // Under torch.jit.trace an op runs as a Python autograd function (ops._traced), which the tracer records as one
 // node that calls the op again.
 template <class... A>
@@ -886,6 +1099,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("so3_rotate_spectrum", &Ops::so3_rotate_spectrum, "U"_a, "x"_a, "b"_a, "adjoint"_a = false, nogil)
       .def("project_on_sphere", &Ops::project_on_sphere, "verts"_a, "faces"_a, "grid"_a, nogil)
       // -- the same ops with their autograd rules
+      .def("ag_attention", [](Ops& o, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias, const OptTensor& buckets,
+                              const OptTensor& starts, const OptTensor& q_lengths, const OptTensor& kv_lengths, bool causal, double scale, int64_t q_start) {
+            S2C_TRACED("ag_attention", q, k, v, bias, buckets, starts, q_lengths, kv_lengths, causal, scale, q_start);
+            if (wants_any({q, k, v, or_none(bias)}))
+              return Attention::apply(id(o), q, k, v, bias, buckets, starts, q_lengths, kv_lengths, causal, scale, q_start);
+            return std::get<0>(o.attention({q, k, v, or_none(bias), or_none(buckets), or_none(starts), or_none(q_lengths), or_none(kv_lengths), causal, scale, q_start}, false));
+          }, "q"_a, "k"_a, "v"_a, "bias"_a, "buckets"_a, "starts"_a, "q_lengths"_a, "kv_lengths"_a, "causal"_a, "scale"_a, "q_start"_a, nogil)
+      .def("ag_layer_norm", [](Ops& o, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+            S2C_TRACED("ag_layer_norm", x, w, b, eps);
+            if (wants_any({x, or_none(w), or_none(b)})) return LayerNorm::apply(id(o), x, w, b, eps);
+            return std::get<0>(o.layer_norm(x, or_none(w), or_none(b), eps, false));
+          }, "x"_a, "weight"_a, "bias"_a, "eps"_a, nogil)
+      .def("ag_dropout", [](Ops& o, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t step) {
+            S2C_TRACED("ag_dropout", x, residual, p, seed, step);
+            if (wants_any({x, or_none(residual)})) return Dropout::apply(id(o), x, residual, p, seed, step);
+            return o.dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step);
+          }, "x"_a, "residual"_a, "p"_a, "seed"_a, "step"_a, nogil)
       .def("ag_s2_fft_real", [](Ops& o, const Tensor& x, std::optional<int64_t> b) {
             S2C_TRACED("ag_s2_fft_real", x, b);
             return wants_grad(x) ? S2FftReal::apply(id(o), x, b_arg(b)) : o.s2_fft(x, false, b, true);
