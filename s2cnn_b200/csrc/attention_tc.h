@@ -1,0 +1,220 @@
+// What the attention kernels on the 5th-generation tensor cores (tcgen05.mma, accumulators in TMEM) share.
+//
+// Operand tiles lie in shared memory as rows of 64 bfloat16 (128 bytes), in blocks of 64 columns, the 16-byte pieces of row r
+// exchanged by r % 8 (the 128-byte swizzle): for a product along the columns such a tile is a "K-major" operand, for a product
+// along the rows an "MN-major" one, so that keys serve both for the scores and for the gradient of the queries from one copy.
+// They are filled with 16-byte cp.async, which writes zeros in place of rows beyond the lengths: what lies there is never read.
+// Weights and score gradients pass from the threads to the tensor core through tensor memory, as its left operand.
+#pragma once
+
+#include "attention_kernels.h"
+
+#ifndef S2C_EMUL
+
+#include <stdint.h>
+
+namespace s2c {
+
+struct AttnTcParams {
+  AttnParams a;        // q, k, v (and dout): 16-byte aligned, strides multiples of 8 elements
+  long gs[3];          // strides of dout
+  int chunks;          // 16-byte pieces of a row that hold values
+  int units, pairs;    // query tiles of 128 per (batch entry, key head), and blocks of one or two of them
+  int per_block;       // query tiles of a block: 1 or 2
+};
+
+__device__ __forceinline__ uint32_t tcx_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void tcx_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tcx_addr(bar)), "r"(count));
+}
+__device__ __forceinline__ void tcx_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tcx_addr(bar)) : "memory");
+}
+// Bounded: false where the phase is not over after some tenths of a second.
+__device__ __forceinline__ bool tcx_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = tcx_addr(bar);
+  for (int spin = 0; spin < (1 << 22); ++spin) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (spin > 256) __nanosleep(40);
+  }
+  return false;
+}
+// the same by a whole warp, which goes on together
+__device__ __forceinline__ bool tcx_wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tcx_wait(bar, parity)) != 0; }
+
+__device__ __forceinline__ bool tcx_elect() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+  return pred != 0;
+}
+__device__ __forceinline__ void tcx_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tcx_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tcx_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcx_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+template <int COLS>
+__device__ __forceinline__ void tcx_alloc(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tcx_addr(slot)), "r"(COLS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+template <int COLS>
+__device__ __forceinline__ void tcx_free(uint32_t base) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(COLS) : "memory");
+}
+
+// Shared-memory descriptor of a swizzled tile: 8 rows of 128 bytes are 1024 bytes from the next 8.  `block`: bytes from one
+// block of 64 columns to the next (an MN-major operand wider than 64; a K-major one steps through its blocks by address).
+__device__ __forceinline__ uint64_t tcx_desc(uint32_t addr, uint32_t block) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor: D float32, A and B bfloat16, 128 rows, n columns; `b_mn`: B is MN-major.
+__device__ __forceinline__ uint32_t tcx_idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void tcx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// left operand in tensor memory
+__device__ __forceinline__ void tcx_mma_t(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+constexpr uint32_t kTcxTile = 128 * 128;      // bytes of 128 rows of 64 columns
+// D (128 x 128) = A B^T over 16 `steps` columns, both operands K-major tiles of 128 rows
+__device__ __forceinline__ void tcx_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+  const uint64_t da = tcx_desc(a, 0), db = tcx_desc(b, 0);
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    if (s >= steps) break;
+    const uint64_t at = (uint64_t)(((s / 4) * kTcxTile + (s % 4) * 32) >> 4);
+    tcx_mma(d, da + at, db + at, idesc, s > 0);
+  }
+}
+// D (128 x n) += A B, A 128 x 128 in tensor memory, B 128 rows of n columns (MN-major)
+__device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  const uint64_t db = tcx_desc(b, kTcxTile);
+#pragma unroll
+  for (int s = 0; s < 8; ++s) tcx_mma_t(d, a + 8 * s, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
+}
+
+// 32 columns of a lane's row; the values are there after tcx_ld_wait
+__device__ __forceinline__ void tcx_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// (the registers pass through, so that nothing reads them earlier)
+__device__ __forceinline__ void tcx_ld_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tcx_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tcx_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// rows [r0, r0 + 128) of one head into a swizzled tile, by `n` threads of which this is number t: `chunks` pieces of a row of
+// values, zeros beyond them up to a whole step of 16 columns and in rows from `end` on
+__device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, long row_stride, int r0, int end, int chunks, int t, int n) {
+  const int steps = (chunks + 1) / 2 * 2;
+  for (int e = t; e < 128 * steps; e += n) {
+    const int r = e / steps, c = e - r * steps;
+    const bool on = r0 + r < end && c < chunks;
+    const bf16* from = on ? src + (long)(r0 + r) * row_stride + 8 * c : src;
+    const uint32_t to = dst + (c / 8) * kTcxTile + r * 128 + (((c % 8) ^ (r % 8)) << 4);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+  }
+}
+// all of this thread's copies have landed and are seen by the tensor core
+__device__ __forceinline__ void tcx_loaded() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// The bias by relative position, in units of ln 2, with its last values repeated 256 positions beyond the reach on either side:
+// a tile that lies partly within the reach reads it without clamping.  At tab[d + reach + 256].
+constexpr int kTcxMargin = 256;
+__device__ __forceinline__ int tcx_tab_floats(int reach) { return 2 * reach + 2 * kTcxMargin + 1; }
+__device__ __forceinline__ void tcx_bias_table(const AttnParams& p, int head, float* tab, int t, int n, bool wide) {
+  for (int e = t; e < tcx_tab_floats(p.reach); e += n) {
+    const int at = attn_clamp(e - kTcxMargin, 0, 2 * p.reach);
+    float v = 0.f;
+    if (p.bias) {
+      const int which = p.bucket_of[at];
+      if (which >= 0 && which < p.n_buckets) {
+        const long i = (long)which * p.heads + head;
+        v = attn_bias_units(wide ? static_cast<const float*>(p.bias)[i] : widen(static_cast<const bf16*>(p.bias)[i]));
+      }
+    }
+    tab[e] = v;
+  }
+}
+__device__ __forceinline__ float2 tcx_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// `n` values of a row (a multiple of 8), as bfloat16 and, for `lo`, what the rounding left
+__device__ __forceinline__ void tcx_put_row(bf16* out, bf16* lo, const float* v, int n, int dim, int c0, bool wide) {
+  if (wide) {                                // rows of whole 16-byte pieces
+#pragma unroll
+    for (int c = 0; c < n; c += 8) {
+      if (c0 + c >= dim) break;
+      uint4 u;
+      u.x = pack_bf16(v[c], v[c + 1]);
+      u.y = pack_bf16(v[c + 2], v[c + 3]);
+      u.z = pack_bf16(v[c + 4], v[c + 5]);
+      u.w = pack_bf16(v[c + 6], v[c + 7]);
+      *reinterpret_cast<uint4*>(out + c0 + c) = u;
+      if (lo) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          r[i] = pack_bf16(v[c + 2 * i] - as_float(w[i] << 16), v[c + 2 * i + 1] - as_float(w[i] & 0xffff0000u));
+        *reinterpret_cast<uint4*>(lo + c0 + c) = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < n; ++c)
+      if (c0 + c < dim) narrow_with_rest(out + c0 + c, lo ? lo + c0 + c : nullptr, v[c]);
+  }
+}
+
+}  // namespace s2c
+#endif  // S2C_EMUL

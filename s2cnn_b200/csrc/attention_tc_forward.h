@@ -1,0 +1,280 @@
+// Attention, forward, bfloat16, on the tensor cores.
+//
+// A block takes one or two tiles of 128 queries that read the same keys: neighbouring tiles of a head, or the same tile of
+// heads that share a key head.  Roles (12 warps, the last of them idle):
+//   * warps 0 - 3 and 4 - 7, one group per query tile: thread = row = tensor-memory lane.  A group takes the finished scores of
+//     a key tile from tensor memory, adds the bias, finds the running maximum, writes the weights 2^(x - m), rounded to
+//     bfloat16, over the scores (half of their columns) and keeps the sum of the unrounded ones;
+//   * warp 8 issues the products: scores of a tile, and weights times values into the tile's output in tensor memory;
+//   * warps 9 and 10 load keys and values, two tiles ahead of each.
+// A group's thread holds 128 scores; its registers come from the third warpgroup (launched with 168 each: 8 x 208 + 4 x 88 =
+// 12 x 168).
+// While one group is at its exponentials the tensor core works for the other one.  The output is rescaled only where the
+// maximum of a row has grown by more than 8 (in units of ln 2) since it was last fixed: weights then reach 2^8 at most, which
+// costs no precision, and after the first tiles rescaling all but ends.
+// Weights in bfloat16: a relative 2^-9 on each of the many terms of an output that is itself rounded to bfloat16.
+#pragma once
+
+#include "attention_tc.h"
+
+#ifndef S2C_EMUL
+
+namespace s2c {
+
+constexpr int kTcfThreads = 12 * 32;
+constexpr float kTcfGrow = 8.f;
+
+struct TcfBars {
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
+  uint32_t tmem;
+};
+
+inline size_t tcf_smem(int blocks, int per_block, int reach) {       // blocks of 64 columns
+  return 1024 + (size_t)(per_block + 4) * blocks * kTcxTile + (size_t)per_block * (2 * reach + 2 * kTcxMargin + 1) * sizeof(float) + sizeof(TcfBars) + 16;
+}
+
+template <int NC>
+__global__ void __launch_bounds__(kTcfThreads, 1) attn_tc_forward(const AttnTcParams pp) {
+  extern __shared__ float4 s2c_dyn_smem[];
+  const AttnParams& p = pp.a;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  constexpr uint32_t kRows = NC * kTcxTile;                          // bytes of a tile of 128 rows
+  const uint32_t base = (tcx_addr(s2c_dyn_smem) + 1023u) & ~1023u;
+  unsigned char* const smem = reinterpret_cast<unsigned char*>(s2c_dyn_smem) + (base - tcx_addr(s2c_dyn_smem));
+  const int tiles = pp.per_block + 4;
+  float* const tab = reinterpret_cast<float*>(smem + (size_t)tiles * kRows);
+  TcfBars* const bars = reinterpret_cast<TcfBars*>((reinterpret_cast<uintptr_t>(tab + pp.per_block * tcx_tab_floats(p.reach)) + 15) & ~(uintptr_t)15);
+  const uint32_t q_at = base, k_at = base + pp.per_block * kRows, v_at = k_at + 2 * kRows;
+
+  // the longest rows (the last queries under `causal`) first
+  const int heads_all = p.batch * p.kv_heads;
+  const int pair = pp.pairs - 1 - (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, hk = bh % p.kv_heads, b = bh / p.kv_heads;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tcx_init(&bars->q_full[i], 128);
+      tcx_init(&bars->s_full[i], 1);
+      tcx_init(&bars->p_full[i], 4);
+      tcx_init(&bars->pv_done[i], 1);
+      tcx_init(&bars->k_full[i], 1);
+      tcx_init(&bars->k_empty[i], 1);
+      tcx_init(&bars->v_full[i], 1);
+      tcx_init(&bars->v_empty[i], 1);
+    }
+    tcx_init(&bars->drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  stream_order_wait();
+  const AttnSeq s = attn_seq(p, b);
+  // unit = tile * group + (head within its group): first row, head and key tiles of this block's query tiles
+  int i0[2], head[2], keys[2], n[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int unit = pair * pp.per_block + u;
+    const bool on = u < pp.per_block && unit < pp.units;
+    i0[u] = on ? unit / p.group * 128 : p.lq;
+    head[u] = hk * p.group + (on ? unit % p.group : 0);
+    keys[u] = i0[u] < s.qlen ? attn_keys(p, s, min(i0[u] + 128, s.qlen)) : 0;
+    n[u] = (keys[u] + 127) / 128;
+  }
+  const int n_all = max(n[0], n[1]), keys_all = max(keys[0], keys[1]);
+  if (warp == 8) {
+    __syncwarp();
+    tcx_alloc<512>(&bars->tmem);
+  }
+  for (int u = 0; u < pp.per_block; ++u) tcx_bias_table(p, head[u], tab + u * tcx_tab_floats(p.reach), tid, kTcfThreads, false);
+  tcx_before_sync();
+  __syncthreads();
+  tcx_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
+  stream_order_next();
+  // tensor memory: scores (and weights) of either tile, then their outputs
+  const uint32_t t_scores = tmem, t_out = tmem + 256;
+  bool ok = true;
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp == 8) {
+    const int steps = (pp.chunks + 1) / 2;
+    const uint32_t is = tcx_idesc(128, false), io = tcx_idesc(16 * steps, true);
+    for (int u = 0; u < 2 && ok; ++u)
+      if (n[u]) ok = tcx_wait_warp(&bars->q_full[u], 0);
+    if (ok && n_all) ok = tcx_wait_warp(&bars->k_full[0], 0);
+    if (ok && n_all && tcx_elect()) {
+      for (int u = 0; u < 2; ++u)
+        if (n[u]) {
+          tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at, is, steps);
+          tcx_commit(&bars->s_full[u]);
+        }
+      tcx_commit(&bars->k_empty[0]);
+    }
+    __syncwarp();
+    for (int j = 0; j < n_all && ok; ++j) {
+      const int sv = j & 1, sk = (j + 1) & 1;
+      const uint32_t par = (j >> 1) & 1;
+      bool have_v = false, have_k = false;
+      for (int u = 0; u < 2 && ok; ++u) {
+        if (j >= n[u]) continue;
+        ok = tcx_wait_warp(&bars->p_full[u], j & 1);
+        if (ok && !have_v) ok = have_v = tcx_wait_warp(&bars->v_full[sv], par);
+        if (!ok) break;
+        tcx_after_sync();
+        if (tcx_elect()) {
+          tcx_combine(t_out + 128 * u, t_scores + 128 * u, v_at + sv * kRows, io, j > 0);
+          tcx_commit(&bars->pv_done[u]);
+        }
+        __syncwarp();
+        if (j + 1 < n[u]) {
+          if (!have_k) ok = have_k = tcx_wait_warp(&bars->k_full[sk], ((j + 1) >> 1) & 1);
+          if (!ok) break;
+          if (tcx_elect()) {                 // in order behind the product that reads the weights from the same columns
+            tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at + sk * kRows, is, steps);
+            tcx_commit(&bars->s_full[u]);
+          }
+          __syncwarp();
+        }
+      }
+      if (ok && tcx_elect()) {
+        tcx_commit(&bars->v_empty[sv]);
+        if (j + 1 < n_all) tcx_commit(&bars->k_empty[sk]);
+      }
+      __syncwarp();
+    }
+    // nothing may be in flight when tensor memory is given back
+    if (tcx_elect()) tcx_commit(&bars->drained);
+    __syncwarp();
+    ok = tcx_wait_warp(&bars->drained, 0) && ok;
+  } else if (warp == 9 || warp == 10) {
+    const bool is_k = warp == 9;
+    const bf16* src = static_cast<const bf16*>(is_k ? p.k : p.v) + b * (is_k ? p.ks[0] : p.vs[0]) + hk * (is_k ? p.ks[2] : p.vs[2]);
+    const long stride = is_k ? p.ks[1] : p.vs[1];
+    uint64_t *full = is_k ? bars->k_full : bars->v_full, *empty = is_k ? bars->k_empty : bars->v_empty;
+    const uint32_t at = is_k ? k_at : v_at;
+    for (int j = 0; j < n_all && ok; ++j) {
+      const int slot = j & 1;
+      if (j >= 2) ok = tcx_wait_warp(&empty[slot], (j / 2 - 1) & 1);
+      if (!ok) break;
+      tcx_load_rows(at + slot * kRows, src, stride, 128 * j, keys_all, pp.chunks, lane, 32);
+      tcx_loaded();
+      __syncwarp();
+      if (lane == 0) tcx_arrive(&full[slot]);
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int u = warp >> 2, row = 32 * (warp & 3) + lane;
+    if (u < pp.per_block && i0[u] < p.lq) {
+      const int i = i0[u] + row, h = head[u];
+      if (n[u]) {
+        tcx_load_rows(q_at + u * kRows, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0[u], s.qlen, pp.chunks, tid & 127, 128);
+        tcx_loaded();
+        tcx_arrive(&bars->q_full[u]);
+      }
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+      const uint32_t ts = t_scores + 128 * u + lanes, to = t_out + 128 * u + lanes;
+      const float* tb = tab + u * tcx_tab_floats(p.reach);
+      const float scale = p.scale * kLog2e, far_before = tb[0], far_behind = tb[2 * p.reach + 2 * kTcxMargin];
+      float m = kNoScore, l = 0.f;
+      for (int j = 0; j < n[u]; ++j) {
+        const int j0 = 128 * j, d0 = j0 - i0[u] - s.start;            // relative position of the tile's first key to its first query
+        if (!(ok = tcx_wait_warp(&bars->s_full[u], j & 1))) break;
+        tcx_after_sync();
+        uint32_t raw[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tcx_ld32(ts + c, raw + c);
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tcx_ld_wait(raw + c);
+        float* x = reinterpret_cast<float*>(raw);
+        if (d0 + 127 > -p.reach && d0 - 127 < p.reach && p.reach > 0) {
+          const float* near = tb + (d0 - row + p.reach + kTcxMargin);
+#pragma unroll
+          for (int c = 0; c < 128; ++c) x[c] = fmaf(x[c], scale, near[c]);
+        } else {
+          const float far = d0 > 0 ? far_behind : far_before;
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) {
+            const float2 y = fma2(make_float2(x[c], x[c + 1]), make_float2(scale, scale), make_float2(far, far));
+            x[c] = y.x;
+            x[c + 1] = y.y;
+          }
+        }
+        if (j0 + 128 > keys[u] || (p.causal && d0 + 127 > 0)) {       // some pairs of the tile are not seen
+          const int lim = p.causal ? min(keys[u] - j0, row - d0 + 1) : keys[u] - j0;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) x[c] = c < lim ? x[c] : kNoScore;
+        }
+        float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int c = 4; c < 128; c += 4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[c + e]);
+        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (__any_sync(0xffffffffu, now > m + kTcfGrow)) {
+          const float fresh = now > m + kTcfGrow ? now : m;
+          if (j > 0) {
+            const float f = fresh == m ? 1.f : exp2_fast(m - fresh);
+            if (!(ok = tcx_wait_warp(&bars->pv_done[u], (j - 1) & 1))) break;
+            tcx_after_sync();
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < 64 * NC; c += 32) {
+              uint32_t o[32];
+              tcx_ld32(to + c, o);
+              tcx_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = as_bits(as_float(o[e]) * f);
+              tcx_st32(to + c, o);
+            }
+          }
+          m = fresh;
+        }
+        const float off = m == kNoScore ? 0.f : -m;
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t w[64];
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          float2 y = tcx_add2(make_float2(x[c], x[c + 1]), make_float2(off, off));
+          y.x = exp2_fast(y.x);
+          y.y = exp2_fast(y.y);
+          sum[(c / 2) & 1] = tcx_add2(sum[(c / 2) & 1], y);
+          w[c / 2] = pack_bf16(y.x, y.y);
+        }
+        tcx_st32(ts, w);
+        tcx_st32(ts + 32, w + 32);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tcx_st_wait();
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) tcx_arrive(&bars->p_full[u]);
+      }
+      // ---- the output row
+      if (i >= s.qlen) l = 0.f;
+      const float2 st = attn_stats(m, l);
+      if (ok && n[u]) ok = tcx_wait_warp(&bars->pv_done[u], (n[u] - 1) & 1);
+      tcx_after_sync();
+      const long at = (((long)b * p.lq + i) * p.heads + h) * p.dim;
+      bf16* out = static_cast<bf16*>(p.out) + at;
+      bf16* lo = p.out_lo ? static_cast<bf16*>(p.out_lo) + at : nullptr;
+      const bool wide = p.dim % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+#pragma unroll
+      for (int c = 0; c < 64 * NC; c += 32) {
+        uint32_t o[32];
+        if (n[u]) {
+          tcx_ld32(to + c, o);
+          tcx_ld_wait(o);
+        }
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = !ok ? bulk_nan() : l == 0.f ? 0.f : as_float(o[e]) * st.y;
+        if (i < p.lq) tcx_put_row(out, lo, v, 32, p.dim, c, wide);
+      }
+      if (p.stats && i < p.lq) p.stats[((long)b * p.heads + h) * p.lq + i] = st;
+    }
+  }
+  tcx_before_sync();
+  __syncthreads();
+  if (warp == 8) tcx_free<512>(tmem);
+}
+
+}  // namespace s2c
+#endif  // S2C_EMUL

@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "attention_kernels.h"
+#include "attention_tc_forward.h"
 #include "dropout_kernels.h"
 #include "layer_norm_kernels.h"
 
@@ -146,6 +147,25 @@ inline size_t attn_forward_bytes(AttnParams p) {
   attn_split(p);
   return attn_split_bytes(p);
 }
+#ifndef S2C_EMUL
+// Rows that the tensor-core kernels can fetch in 16-byte pieces.
+inline bool attn_pieces(const void* x, const long (&stride)[3], int dim) {
+  return aligned16(x) && dim % 8 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 && stride[2] % 8 == 0;
+}
+inline int attn_tc_forward_launch(const AttnParams& p, stream_t st) {
+  AttnTcParams t = {};
+  t.a = p;
+  t.chunks = p.dim / 8;
+  t.units = (p.lq + 127) / 128 * p.group;
+  const long heads = (long)p.batch * p.kv_heads;
+  const int nc = p.dim > 64 ? 2 : 1;
+  t.per_block = heads * ((t.units + 1) / 2) >= dev_sm_count() && tcf_smem(nc, 2, p.reach) <= (size_t)dev_smem_limit() ? 2 : 1;
+  t.pairs = (t.units + t.per_block - 1) / t.per_block;
+  const size_t smem = tcf_smem(nc, t.per_block, p.reach);
+  return nc == 1 ? launch_impl<attn_tc_forward<1>>("attention_tc", heads * t.pairs, kTcfThreads, smem, st, t)
+                 : launch_impl<attn_tc_forward<2>>("attention_tc", heads * t.pairs, kTcfThreads, smem, st, t);
+}
+#endif
 template <class T>
 int attn_forward(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
   if (p.batch == 0 || p.lq == 0) return S2C_OK;
@@ -163,6 +183,10 @@ int attn_forward(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
       return seq_launch<J>("attention_join", (rows + per - 1) / per, 0, st, p);
     });
   }
+#ifndef S2C_EMUL
+  if (sizeof(T) == 2 && p.lk > 0 && attn_pieces(p.q, p.qs, p.dim) && attn_pieces(p.k, p.ks, p.dim) && attn_pieces(p.v, p.vs, p.dim))
+    return attn_tc_forward_launch(p, st);
+#endif
   p.tiles = (p.lq + kAttnTile - 1) / kAttnTile;
   return attn_by_dim<T>(p.dim, [&](auto d) {
     using K = AttnForward<T, decltype(d)::value>;
