@@ -145,16 +145,30 @@ __device__ __forceinline__ void tcx_st32(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tcx_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// rows [r0, r0 + 128) of one head into a swizzled tile, by `n` threads of which this is number t: `chunks` pieces of a row of
-// values, zeros beyond them up to a whole step of 16 columns and in rows from `end` on
-__device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, long row_stride, int r0, int end, int chunks, int t, int n) {
-  const int steps = (chunks + 1) / 2 * 2;
-  for (int e = t; e < 128 * steps; e += n) {
-    const int r = e / steps, c = e - r * steps;
-    const bool on = r0 + r < end && c < chunks;
-    const bf16* from = on ? src + (long)(r0 + r) * row_stride + 8 * c : src;
-    const uint32_t to = dst + (c / 8) * kTcxTile + r * 128 + (((c % 8) ^ (r % 8)) << 4);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+// rows [r0, r0 + 128) of one head into a swizzled tile, by N threads of which this is number t: `chunks` pieces of a row of
+// values, zeros beyond them up to a whole step of 16 columns and in rows from `end` on.  A thread has the same piece of every
+// N / 8-th row, so that a copy costs it an addition and a comparison: one warp keeps up with the tensor core.
+template <int NC, int N>
+__device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, long row_stride, int r0, int end, int chunks, int t) {
+  const int c = t % 8, r = t / 8, left = end - r0 - r;               // rows of this thread that hold values: it * N / 8 < left
+  const long step = (long)(N / 8) * row_stride;
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+    const int cc = 8 * b + c;
+    if (cc >= (chunks + 1) / 2 * 2) break;
+    const bool in = cc < chunks;
+    const bf16* from = src + (long)(r0 + r) * row_stride + 8 * cc;
+    const uint32_t to = dst + b * kTcxTile + r * 128;
+    // (N = 32: rows r and r + 4 in turn, more threads: r % 8 stays)
+    const uint32_t even = (uint32_t)((c ^ (r % 8)) << 4), odd = (uint32_t)((c ^ ((r + N / 8) % 8)) << 4);
+#pragma unroll 8
+    for (int it = 0; it < 1024 / N; ++it) {
+      const bool on = in && it * (N / 8) < left;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + it * (16 * N) + (it % 2 ? odd : even)), "l"(on ? from : src),
+                   "r"(on ? 16 : 0)
+                   : "memory");
+      from += step;
+    }
   }
 }
 // all of this thread's copies have landed and are seen by the tensor core

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kTcfThreads, 1) attn_tc_forward(const AttnTcPa
       const int slot = j & 1;
       if (j >= 2) ok = tcx_wait_warp(&empty[slot], (j / 2 - 1) & 1);
       if (!ok) break;
-      tcx_load_rows(at + slot * kRows, src, stride, 128 * j, keys_all, pp.chunks, lane, 32);
+      tcx_load_rows<NC, 32>(at + slot * kRows, src, stride, 128 * j, keys_all, pp.chunks, lane);
       tcx_loaded();
       __syncwarp();
       if (lane == 0) tcx_arrive(&full[slot]);
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kTcfThreads, 1) attn_tc_forward(const AttnTcPa
     if (u < pp.per_block && i0[u] < p.lq) {
       const int i = i0[u] + row, h = head[u];
       if (n[u]) {
-        tcx_load_rows(q_at + u * kRows, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0[u], s.qlen, pp.chunks, tid & 127, 128);
+        tcx_load_rows<NC, 128>(q_at + u * kRows, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0[u], s.qlen, pp.chunks, tid & 127);
         tcx_loaded();
         tcx_arrive(&bars->q_full[u]);
       }
