@@ -23,6 +23,18 @@ struct AttnTcParams {
   int per_block;       // query tiles of a block: 1 or 2
 };
 
+// A tensor-core kernel as a struct: kThreads and run(p, smem), which lets the next kernel's blocks in itself.
+template <class Impl>
+__global__ void __launch_bounds__(Impl::kThreads, 1) attn_tc_kernel(const AttnTcParams p) {
+  extern __shared__ float4 s2c_dyn_smem[];
+  stream_order_wait();
+  Impl::run(p, s2c_dyn_smem);
+}
+template <class Impl>
+inline int attn_tc_launch(const char* name, long grid, size_t smem, stream_t st, const AttnTcParams& p) {
+  return launch_impl<attn_tc_kernel<Impl>>(name, grid, Impl::kThreads, smem, st, p);
+}
+
 __device__ __forceinline__ uint32_t tcx_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ void tcx_init(uint64_t* bar, int count) {
@@ -105,11 +117,13 @@ __device__ __forceinline__ void tcx_scores(uint32_t d, uint32_t a, uint32_t b, u
     tcx_mma(d, da + at, db + at, idesc, s > 0);
   }
 }
-// D (128 x n) += A B, A 128 x 128 in tensor memory, B 128 rows of n columns (MN-major)
-__device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+// D (128 x n) += A B, A 128 x 128 in tensor memory (its second 64 columns `half` behind the first), B 128 rows of n columns
+// (MN-major)
+__device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t half = 32) {
   const uint64_t db = tcx_desc(b, kTcxTile);
 #pragma unroll
-  for (int s = 0; s < 8; ++s) tcx_mma_t(d, a + 8 * s, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
+  for (int s = 0; s < 8; ++s)
+    tcx_mma_t(d, a + (s / 4) * half + (s % 4) * 8, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
 }
 
 // 32 columns of a lane's row; the values are there after tcx_ld_wait

@@ -34,8 +34,9 @@ inline size_t tcf_smem(int blocks, int per_block, int reach) {       // blocks o
 }
 
 template <int NC>
-__global__ void __launch_bounds__(kTcfThreads, 1) attn_tc_forward(const AttnTcParams pp) {
-  extern __shared__ float4 s2c_dyn_smem[];
+struct AttnTcForward {
+static constexpr int kThreads = kTcfThreads;
+static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_dyn_smem) {
   const AttnParams& p = pp.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   constexpr uint32_t kRows = NC * kTcxTile;                          // bytes of a tile of 128 rows
@@ -64,7 +65,6 @@ __global__ void __launch_bounds__(kTcfThreads, 1) attn_tc_forward(const AttnTcPa
     tcx_init(&bars->drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  stream_order_wait();
   const AttnSeq s = attn_seq(p, b);
   // unit = tile * group + (head within its group): first row, head and key tiles of this block's query tiles
   int i0[2], head[2], keys[2], n[2];
@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(kTcfThreads, 1) attn_tc_forward(const AttnTcPa
   __syncthreads();
   if (warp == 8) tcx_free<512>(tmem);
 }
+};
 
 }  // namespace s2c
 #endif  // S2C_EMUL

@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "attention_kernels.h"
+#include "attention_tc_backward.h"
 #include "attention_tc_forward.h"
 #include "dropout_kernels.h"
 #include "layer_norm_kernels.h"
@@ -162,8 +163,8 @@ inline int attn_tc_forward_launch(const AttnParams& p, stream_t st) {
   t.per_block = heads * ((t.units + 1) / 2) >= dev_sm_count() && tcf_smem(nc, 2, p.reach) <= (size_t)dev_smem_limit() ? 2 : 1;
   t.pairs = (t.units + t.per_block - 1) / t.per_block;
   const size_t smem = tcf_smem(nc, t.per_block, p.reach);
-  return nc == 1 ? launch_impl<attn_tc_forward<1>>("attention_tc", heads * t.pairs, kTcfThreads, smem, st, t)
-                 : launch_impl<attn_tc_forward<2>>("attention_tc", heads * t.pairs, kTcfThreads, smem, st, t);
+  return nc == 1 ? attn_tc_launch<AttnTcForward<1>>("attention_tc", heads * t.pairs, smem, st, t)
+                 : attn_tc_launch<AttnTcForward<2>>("attention_tc", heads * t.pairs, smem, st, t);
 }
 #endif
 template <class T>
@@ -205,7 +206,30 @@ int attn_backward(AttnParams p, void* dbias, void* ws, size_t ws_bytes, stream_t
     return fail(S2C_ERR_WORKSPACE, "s2c_attention_backward: workspace too small");
   p.delta = static_cast<float*>(ws);
   p.dbias_part = dbias ? reinterpret_cast<float*>(static_cast<char*>(ws) + attn_delta_bytes(p)) : nullptr;
-  S2C_SEQ_TRY(attn_by_dim<T>(p.dim, [&](auto d) {
+  bool done = false;
+#ifndef S2C_EMUL
+  const long gs[3] = {(long)p.lq * p.heads * p.dim, (long)p.heads * p.dim, p.dim};
+  const int nc = p.dim > 64 ? 2 : 1;
+  done = sizeof(T) == 2 && p.batch > 0 && p.lq > 0 && p.lk > 0 && attn_pieces(p.q, p.qs, p.dim) && attn_pieces(p.k, p.ks, p.dim) &&
+         attn_pieces(p.v, p.vs, p.dim) && attn_pieces(p.dout, gs, p.dim) && aligned16(p.o) &&
+         std::max(tcb_q_smem(nc, p.reach, dbias), tcb_kv_smem(nc, p.reach)) <= (size_t)dev_smem_limit();
+  if (done) {
+    AttnTcParams t = {};
+    for (int i = 0; i < 3; ++i) t.gs[i] = gs[i];
+    t.chunks = p.dim / 8;
+    p.tiles = (p.lq + 127) / 128;
+    t.a = p;
+    const long q_blocks = (long)p.batch * p.heads * p.tiles;
+    const size_t q_smem = tcb_q_smem(nc, p.reach, dbias), kv_smem = tcb_kv_smem(nc, p.reach);
+    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradQ<1>>("attention_tc_grad_q", q_blocks, q_smem, st, t)
+                        : attn_tc_launch<AttnTcGradQ<2>>("attention_tc_grad_q", q_blocks, q_smem, st, t));
+    t.a.tiles = (p.lk + 127) / 128;
+    const long kv_blocks = (long)p.batch * p.kv_heads * t.a.tiles;
+    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradKV<1>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t)
+                        : attn_tc_launch<AttnTcGradKV<2>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t));
+  }
+#endif
+  if (!done) S2C_SEQ_TRY(attn_by_dim<T>(p.dim, [&](auto d) {
     constexpr int DP = decltype(d)::value;
     using Q = AttnGradQ<T, DP>;
     using KV = AttnGradKV<T, DP>;
