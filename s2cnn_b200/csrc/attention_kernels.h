@@ -29,7 +29,7 @@ struct AttnParams {
   float2* stats;                  // [batch][heads][lq]: m, 1 / l (+inf, 0 where a row sees nothing); forward: null where nobody needs it
   float* delta;                   // [batch][heads][lq]
   float* dbias_part;              // [batch][q tiles][heads][n_buckets], null where not asked for
-  float* part;                    // split keys: see AttnRows
+  float* part;                    // split keys: see AttnFew
   const int *bucket_of, *start, *q_len, *kv_len;
   long qs[3], ks[3], vs[3];       // elements from one batch entry, position, head to the next
   int batch, lq, lk, heads, kv_heads, dim, group;
@@ -457,149 +457,6 @@ struct AttnGradKV {
     const long out = ((long)b * p.lk * p.kv_heads + hk) * p.dim, row = (long)p.kv_heads * p.dim;
     Tile::store(static_cast<T*>(p.dk) + out, (T*)nullptr, row, j0, p.lk, p.dim, ty, tx, dk);
     Tile::store(static_cast<T*>(p.dv) + out, (T*)nullptr, row, j0, p.lk, p.dim, ty, tx, dv);
-  }
-};
-
-// ---- few queries (one new position of a recording): the keys are split -------------------------------------------------------
-// The queries of all heads that share a key head make up to 16 rows.  A block takes `chunk` keys: thread t has key t of each
-// 128-key tile in the scores and column t % DP of the output, keys and values pass through shared memory, each read once for all
-// rows.  With one split the result is written; else each split leaves its running maximum, sum and output (not divided), and
-// AttnJoin adds them in order.
-constexpr int kAttnRows = 16, kAttnRowKeys = 128;
-
-template <class T, int DP>
-struct AttnRows {
-  using Params = AttnParams;
-  static constexpr int kThreads = 128, kBlocks = 1;
-  static constexpr int kPitch = DP + 1;                               // a thread reads its own row
-  static constexpr int kSlices = kThreads / DP;                       // threads of one output column take every kSlices-th key
-  static_assert(kThreads % DP == 0, "columns");
-  static size_t smem(const Params& p) {
-    const int rows = p.lq * p.group;
-    return (kAttnRowKeys * kPitch + rows * (DP + kAttnRowKeys + 4) + p.group * (2 * p.reach + 1)) * sizeof(float);
-  }
-  // of one split of one (batch entry, key head): rows x (DP values, maximum, sum)
-  static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
-    const int rows = p.lq * p.group, t = ctx.tid;
-    float* kt = reinterpret_cast<float*>(smem);                       // [128][kPitch]: keys, then values
-    float *qt = kt + kAttnRowKeys * kPitch, *w = qt + rows * DP, *red = w + rows * kAttnRowKeys, *tab = red + 4 * rows;
-    const int split = ctx.bid % p.splits, bh = ctx.bid / p.splits, hk = bh % p.kv_heads, b = bh / p.kv_heads;
-    const AttnSeq s = attn_seq(p, b);
-    const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
-    const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
-    for (int g = 0; g < p.group; ++g) attn_bias_table<T>(ctx, p, hk * p.group + g, tab + g * (2 * p.reach + 1));
-    for (int e = t; e < rows * DP; e += kThreads) {                   // row = i * group + g
-      const int r = e / DP, d = e % DP, i = r / p.group, h = hk * p.group + r % p.group;
-      qt[e] = i < s.qlen && d < p.dim ? widen(static_cast<const T*>(p.q)[b * p.qs[0] + i * p.qs[1] + h * p.qs[2] + d]) * (p.scale * kLog2e) : 0.f;
-    }
-    const int keys = attn_keys(p, s, s.qlen), j_end = keys < (split + 1) * p.chunk ? keys : (split + 1) * p.chunk;
-    const int col = t % DP, slice = t / DP;
-    float m[kAttnRows], l[kAttnRows], acc[kAttnRows];
-#pragma unroll
-    for (int r = 0; r < kAttnRows; ++r) { m[r] = kNoScore; l[r] = 0.f; acc[r] = 0.f; }
-    for (int j0 = split * p.chunk; j0 < j_end; j0 += kAttnRowKeys) {
-      ctx.sync();
-      for (int e = t; e < kAttnRowKeys * DP; e += kThreads) {
-        const int j = e / DP, d = e % DP;
-        kt[j * kPitch + d] = j0 + j < j_end && d < p.dim ? widen(k[(long)(j0 + j) * p.ks[1] + d]) : 0.f;
-      }
-      ctx.sync();
-      const int j = j0 + t;
-#pragma unroll
-      for (int r = 0; r < kAttnRows; ++r) {
-        if (r >= rows) break;
-        const int i = r / p.group, d = j - i - s.start;
-        float x = 0.f;
-        for (int c = 0; c < DP; ++c) x = fmaf(kt[t * kPitch + c], qt[r * DP + c], x);
-        x += tab[(r % p.group) * (2 * p.reach + 1) + attn_clamp(d, -p.reach, p.reach) + p.reach];
-        const bool seen = j < j_end && i < s.qlen && (!p.causal || d <= 0);
-        w[r * kAttnRowKeys + t] = seen ? x : kNoScore;
-        const float top = lanes_max<32>(ctx, seen ? x : kNoScore);
-        if (t % 32 == 0) red[4 * r + t / 32] = top;
-      }
-      ctx.sync();
-      // values in the place of the keys; weights in the place of the scores
-      for (int e = t; e < kAttnRowKeys * DP; e += kThreads) {
-        const int jj = e / DP, d = e % DP;
-        kt[jj * kPitch + d] = j0 + jj < j_end && d < p.dim ? widen(v[(long)(j0 + jj) * p.vs[1] + d]) : 0.f;
-      }
-#pragma unroll
-      for (int r = 0; r < kAttnRows; ++r) {
-        if (r >= rows) break;
-        float top = m[r];
-        for (int e = 0; e < 4; ++e) top = red[4 * r + e] > top ? red[4 * r + e] : top;
-        const float base = top == kNoScore ? 0.f : top;
-        const float old = exp2_fast(m[r] - base);
-        const float x = exp2_fast(w[r * kAttnRowKeys + t] - base);
-        w[r * kAttnRowKeys + t] = x;
-        l[r] = l[r] * old + x;                                         // (this thread's keys)
-        acc[r] *= old;
-        m[r] = top;
-      }
-      ctx.sync();
-      for (int jj = slice; jj < kAttnRowKeys; jj += kSlices) {
-        const float y = kt[jj * kPitch + col];
-#pragma unroll
-        for (int r = 0; r < kAttnRows; ++r)
-          if (r < rows) acc[r] = fmaf(w[r * kAttnRowKeys + jj], y, acc[r]);
-      }
-    }
-    // sums over the threads: of l over all, of acc over the slices of a column
-#pragma unroll
-    for (int r = 0; r < kAttnRows; ++r) {
-      if (r >= rows) break;
-      ctx.sync();
-      const float sum = lanes_sum<32>(ctx, l[r]);
-      if (t % 32 == 0) red[4 * r + t / 32] = sum;
-      kt[t] = acc[r];
-      ctx.sync();
-      const float all = (red[4 * r] + red[4 * r + 1]) + (red[4 * r + 2] + red[4 * r + 3]);
-      if (t >= DP) continue;
-      float o = 0.f;
-      for (int e = 0; e < kSlices; ++e) o += kt[e * DP + t];
-      if (p.splits == 1) {
-        const int i = r / p.group, h = hk * p.group + r % p.group;
-        if (t < p.dim) {
-          const long at = (((long)b * p.lq + i) * p.heads + h) * p.dim + t;
-          narrow_with_rest(static_cast<T*>(p.out) + at, p.out_lo ? static_cast<T*>(p.out_lo) + at : nullptr, o * attn_stats(m[r], all).y);
-        }
-        if (p.stats && t == 0) p.stats[((long)b * p.heads + h) * p.lq + i] = attn_stats(m[r], all);
-      } else {
-        float* part = p.part + ((long)ctx.bid * rows + r) * (DP + 2);
-        part[t] = o;
-        if (t == 0) { part[DP] = m[r]; part[DP + 1] = all; }
-      }
-    }
-  }
-};
-
-// joins the splits of AttnRows: a block of DP threads per row
-template <class T, int DP>
-struct AttnJoin {
-  using Params = AttnParams;
-  static constexpr int kThreads = 128, kBlocks = 4;
-  static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char*) {
-    const int rows = p.lq * p.group, per = kThreads / DP, t = ctx.tid % DP;
-    const long at = (long)ctx.bid * per + ctx.tid / DP;
-    if (at >= (long)p.batch * p.kv_heads * rows) return;
-    const int r = (int)(at % rows), bh = (int)(at / rows), hk = bh % p.kv_heads, b = bh / p.kv_heads;
-    const float* part = p.part + ((long)bh * p.splits * rows + r) * (DP + 2);
-    const long step = (long)rows * (DP + 2);
-    float m = kNoScore;
-    for (int e = 0; e < p.splits; ++e) m = part[e * step + DP] > m ? part[e * step + DP] : m;
-    const float base = m == kNoScore ? 0.f : m;
-    float o = 0.f, l = 0.f;
-    for (int e = 0; e < p.splits; ++e) {
-      const float f = exp2_fast(part[e * step + DP] - base);
-      l = fmaf(part[e * step + DP + 1], f, l);
-      o = fmaf(part[e * step + t], f, o);
-    }
-    const int i = r / p.group, h = hk * p.group + r % p.group;
-    if (t < p.dim) {
-      const long at = (((long)b * p.lq + i) * p.heads + h) * p.dim + t;
-      narrow_with_rest(static_cast<T*>(p.out) + at, p.out_lo ? static_cast<T*>(p.out_lo) + at : nullptr, o * attn_stats(m, l).y);
-    }
-    if (p.stats && t == 0) p.stats[((long)b * p.heads + h) * p.lq + i] = attn_stats(m, l);
   }
 };
 

@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "attention_few.h"
 #include "attention_kernels.h"
 #include "attention_tc_backward.h"
 #include "attention_tc_forward.h"
@@ -132,21 +133,69 @@ inline void attn_set_saved(AttnParams& p, int dtype, void* saved) {
   if (dtype == kSeqBf16) p.out_lo = static_cast<char*>(saved) + attn_stats_bytes(p);
 }
 
-// Few rows per key head: the keys are split so that every SM has two blocks' worth of them.
-inline bool attn_few_rows(const AttnParams& p) { return (long)p.lq * p.group <= kAttnRows; }
+#ifndef S2C_EMUL
+// Few rows per key head: chunks of keys, six blocks per SM of them where there are as many keys (lengths differ: what is short
+// ends early), at least 256 keys each.
+inline bool attn_few_rows(const AttnParams& p) { return (long)p.lq * p.group <= kFewRows; }
 inline void attn_split(AttnParams& p) {
-  const long blocks = std::max(1L, (long)p.batch * p.kv_heads), tiles = std::max(1, (p.lk + kAttnRowKeys - 1) / kAttnRowKeys);
-  const long want = std::min(tiles, std::max(1L, 2L * dev_sm_count() / blocks)), per = (tiles + want - 1) / want;
-  p.chunk = (int)per * kAttnRowKeys;
-  p.splits = (int)((tiles + per - 1) / per);
+  const long blocks = std::max(1L, (long)p.batch * p.kv_heads), pieces = std::max(1, (p.lk + 255) / 256);
+  const long want = std::min(pieces, std::max(1L, 6L * dev_sm_count() / blocks)), per = (pieces + want - 1) / want;
+  p.chunk = (int)per * 256;
+  p.splits = (int)((pieces + per - 1) / per);
 }
 inline size_t attn_split_bytes(const AttnParams& p) {
   return p.splits > 1 ? (size_t)p.batch * p.kv_heads * p.splits * p.lq * p.group * (attn_padded(p.dim) + 2) * sizeof(float) : 0;
 }
-inline size_t attn_forward_bytes(AttnParams p) {
-  if (!attn_few_rows(p)) return 0;
+// the largest pieces that rows of k and v can be copied in
+template <class T>
+int attn_few_piece(const AttnParams& p) {
+  auto fits = [&](int bytes) {
+    const long n = bytes / (long)sizeof(T);
+    bool ok = reinterpret_cast<uintptr_t>(p.k) % bytes == 0 && reinterpret_cast<uintptr_t>(p.v) % bytes == 0 && p.dim % n == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && p.ks[i] % n == 0 && p.vs[i] % n == 0;
+    return ok;
+  };
+  return fits(16) ? 16 : fits(4) ? 4 : 2;
+}
+// (the bias tables of all heads of a group have to lie beside the tiles: not with 16 heads and a reach of 2048)
+template <class T>
+bool attn_few_fits(const AttnParams& p) {
+  return attn_few_rows(p) && attn_by_dim<T>(p.dim, [&](auto d) {
+    return (int)(AttnFew<T, decltype(d)::value, 4>::smem(p) <= (size_t)dev_smem_limit());
+  });
+}
+template <class T>
+int attn_few(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
   attn_split(p);
-  return attn_split_bytes(p);
+  if (attn_split_bytes(p) > ws_bytes || (p.splits > 1 && !ws)) return fail(S2C_ERR_WORKSPACE, "s2c_attention: workspace too small");
+  p.part = static_cast<float*>(ws);
+  const int piece = attn_few_piece<T>(p);
+  return attn_by_dim<T>(p.dim, [&](auto d) {
+    constexpr int DP = decltype(d)::value;
+    const long grid = (long)p.batch * p.kv_heads * p.splits;
+    auto go = [&](auto k) {
+      using K = typename decltype(k)::type;
+      return seq_launch<K>("attention_few", grid, K::smem(p), st, p);
+    };
+    struct A { using type = AttnFew<T, DP, 16>; };
+    struct B { using type = AttnFew<T, DP, 4>; };
+    struct C { using type = AttnFew<T, DP, sizeof(T) == 2 ? 2 : 4>; };
+    S2C_SEQ_TRY(piece == 16 ? go(A()) : piece == 4 ? go(B()) : go(C()));
+    if (p.splits == 1) return (int)S2C_OK;
+    using J = AttnJoin<T, DP>;
+    const long rows = (long)p.batch * p.kv_heads * p.lq * p.group, per = J::kThreads / DP;
+    return seq_launch<J>("attention_join", (rows + per - 1) / per, 0, st, p);
+  });
+}
+#endif
+inline size_t attn_forward_bytes(AttnParams p) {
+#ifndef S2C_EMUL
+  if (attn_few_rows(p)) {
+    attn_split(p);
+    return attn_split_bytes(p);
+  }
+#endif
+  return 0;
 }
 #ifndef S2C_EMUL
 // Rows that the tensor-core kernels can fetch in 16-byte pieces.
@@ -170,21 +219,8 @@ inline int attn_tc_forward_launch(const AttnParams& p, stream_t st) {
 template <class T>
 int attn_forward(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
   if (p.batch == 0 || p.lq == 0) return S2C_OK;
-  if (attn_few_rows(p)) {
-    attn_split(p);
-    if (attn_split_bytes(p) > ws_bytes || (p.splits > 1 && !ws)) return fail(S2C_ERR_WORKSPACE, "s2c_attention: workspace too small");
-    p.part = static_cast<float*>(ws);
-    return attn_by_dim<T>(p.dim, [&](auto d) {
-      constexpr int DP = decltype(d)::value;
-      using K = AttnRows<T, DP>;
-      using J = AttnJoin<T, DP>;
-      S2C_SEQ_TRY(seq_launch<K>("attention_rows", (long)p.batch * p.kv_heads * p.splits, K::smem(p), st, p));
-      if (p.splits == 1) return (int)S2C_OK;
-      const long rows = (long)p.batch * p.kv_heads * p.lq * p.group, per = J::kThreads / DP;
-      return seq_launch<J>("attention_join", (rows + per - 1) / per, 0, st, p);
-    });
-  }
 #ifndef S2C_EMUL
+  if (attn_few_fits<T>(p)) return attn_few<T>(p, ws, ws_bytes, st);
   if (sizeof(T) == 2 && p.lk > 0 && attn_pieces(p.q, p.qs, p.dim) && attn_pieces(p.k, p.ks, p.dim) && attn_pieces(p.v, p.vs, p.dim))
     return attn_tc_forward_launch(p, st);
 #endif

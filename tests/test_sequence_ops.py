@@ -130,6 +130,10 @@ def test_attention_and_gradients(backend, case, dtype):
 
 
 LARGE = [
+    (2, 1, 1500, 16, 1, 128, (32, 128), {"causal": True, "q_start": [1400, 37]}),          # one query, all heads on one key head
+    (3, 2, 777, 10, 2, 25, (32, 64), {"kv_lengths": [777, 0, 513]}),                       # rows of 50 bytes
+    (1, 4, 2000, 8, 2, 34, (16, 30), {"causal": True, "q_start": 1996}),                   # rows of 68 bytes
+    (1, 1, 600, 16, 1, 128, (32, 2048), {}),                                               # bias tables beyond the shared memory
     (2, 128, 128, 2, 2, 64, (32, 128), {}),
     (1, 257, 257, 2, 2, 128, (32, 30), {"causal": True}),
     (2, 400, 400, 4, 2, 64, (32, 128), {"kv_lengths": [400, 133], "q_lengths": [400, 133], "causal": True}),
