@@ -385,10 +385,13 @@ int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long 
  *   s2c_debug_plane_chunk(signals): signals per chunk of the large-bandwidth path (1 .. 32 at b = 64, 256 at b = 32); 0
  *     restores the default: equal chunks of at most 32 / 256, or of what the workspace holds.
  *   s2c_debug_cluster(mode): 2b <= 32: 1 the cluster kernels, 2 the kernels whose blocks walk beta, 3 the
- *     plane kernels (where they exist and a workspace is given); 0 restores the choice by batch size. */
+ *     plane kernels (where they exist and a workspace is given); 0 restores the choice by batch size.
+ *   s2c_debug_attention(mode): attention of more than 16 rows per key head: 1 never on the tensor cores, 2 always (where
+ *     the biases fit beside the tiles); 0 restores the choice by size. */
 void s2c_debug_force_general_path(int level);
 void s2c_debug_plane_chunk(int signals);
 void s2c_debug_cluster(int mode);
+void s2c_debug_attention(int mode);
 
 #ifdef __cplusplus
 }

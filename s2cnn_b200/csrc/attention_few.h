@@ -54,7 +54,7 @@ struct FewLayout {
   static constexpr int kKeyPitch = sizeof(T) == 2 ? (DP + 8) * 2 : (DP + 4) * 4;
   static constexpr int kValuePitch = sizeof(T) == 2 ? (DP + 8) * 2 : (DP + 8) * 4;
   static constexpr int kStage = kFewKeys * (kKeyPitch + kValuePitch);
-  static constexpr int kStages = sizeof(T) == 2 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kWarp = kStage * kStages;
 };
 
@@ -63,27 +63,41 @@ template <class T, int DP, int PIECE>
 struct AttnFew {
   using Params = AttnParams;
   using L = FewLayout<T, DP>;
-  static constexpr int kThreads = 32 * kFewWarps, kBlocks = 1;
+  static constexpr int kThreads = 32 * kFewWarps, kBlocks = 2;
   static constexpr int kNt = DP / 8;                                 // output tiles of 8 columns
   static constexpr int kKs = sizeof(T) == 2 ? DP / 16 : DP / 8;      // steps of the scores' products
   static size_t smem(const Params& p) {
     const size_t tiles = (size_t)kFewWarps * L::kWarp, join = (size_t)kFewWarps * kFewRows * (DP + 2) * sizeof(float);
     return std::max(tiles, join) + (size_t)p.group * (2 * p.reach + 1) * sizeof(float);
   }
-  static __device__ __forceinline__ void copy_rows(unsigned char* dst, int pitch, const T* src, long stride, int j0, int end, int dim, int lane) {
+  // `left` rows that hold values (16: a whole tile), zeros behind them.  Where 32 lanes take whole rows a lane's copies are at
+  // constant distances.
+  static __device__ __forceinline__ void copy_rows(unsigned char* dst, int pitch, const T* src, long stride, int left, int dim, int lane) {
     constexpr int kPer = DP * (int)sizeof(T) / PIECE, kElems = PIECE / (int)sizeof(T);     // pieces of a row, values of a piece
-#pragma unroll 4
-    for (int e = lane; e < kFewKeys * kPer; e += 32) {
-      const int r = e / kPer, c = e % kPer;
-      const bool on = j0 + r < end && c * kElems < dim;
-      const T* from = on ? src + (long)(j0 + r) * stride + c * kElems : src;
-      unsigned char* to = dst + r * pitch + c * PIECE;
+    auto piece = [&](unsigned char* to, const T* from, bool on) {
       if constexpr (PIECE == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from), "r"(on ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(on ? from : src), "r"(on ? 16 : 0) : "memory");
       else if constexpr (PIECE == 4)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from), "r"(on ? 4 : 0) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(on ? from : src), "r"(on ? 4 : 0) : "memory");
       else
         *reinterpret_cast<unsigned short*>(to) = on ? reinterpret_cast<const unsigned short*>(from)[0] : (unsigned short)0;
+    };
+    if constexpr (kPer <= 32) {
+      constexpr int kRowsAtOnce = 32 / kPer;
+      const int r = lane / kPer, c = lane % kPer;
+      const T* from = src + r * stride + c * kElems;
+      unsigned char* to = dst + r * pitch + c * PIECE;
+      const bool in = c * kElems < dim;
+#pragma unroll
+      for (int it = 0; it < kFewKeys / kRowsAtOnce; ++it) {
+        piece(to + it * kRowsAtOnce * pitch, from, in && it * kRowsAtOnce + r < left);
+        from += kRowsAtOnce * stride;
+      }
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < kFewKeys; ++r)
+#pragma unroll
+        for (int c = lane; c < kPer; c += 32) piece(dst + r * pitch + c * PIECE, src + r * stride + c * kElems, r < left && c * kElems < dim);
     }
   }
   static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
@@ -99,8 +113,9 @@ struct AttnFew {
     const int n = j_lo < j_end ? (j_end - j_lo + kFewKeys - 1) / kFewKeys : 0;         // tiles of the block; this warp: warp, warp + 4 ...
     auto fetch = [&](int t, int stage) {
       if (t < n) {
-        copy_rows(mine + stage * L::kStage, L::kKeyPitch, k, p.ks[1], j_lo + t * kFewKeys, j_end, p.dim, lane);
-        copy_rows(mine + stage * L::kStage + kFewKeys * L::kKeyPitch, L::kValuePitch, v, p.vs[1], j_lo + t * kFewKeys, j_end, p.dim, lane);
+        const int j0 = j_lo + t * kFewKeys;
+        copy_rows(mine + stage * L::kStage, L::kKeyPitch, k + j0 * p.ks[1], p.ks[1], j_end - j0, p.dim, lane);
+        copy_rows(mine + stage * L::kStage + kFewKeys * L::kKeyPitch, L::kValuePitch, v + j0 * p.vs[1], p.vs[1], j_end - j0, p.dim, lane);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -161,16 +176,21 @@ struct AttnFew {
           few_mma(x[1], q_hi[ks], r[2], r[3]);
         }
       } else {
+        float y[2][2][4] = {};
 #pragma unroll
         for (int ks = 0; ks < kKs; ++ks)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float* row = reinterpret_cast<const float*>(kt + (8 * h + lane / 4) * L::kKeyPitch) + 8 * ks + lane % 4;
             const FewSplit b0 = few_split(row[0]), b1 = few_split(row[4]);
-            few_mma_tf32(x[h], q_lo[ks], b0.hi, b1.hi);
-            few_mma_tf32(x[h], q_hi[ks], b0.lo, b1.lo);
+            few_mma_tf32(y[0][h], q_lo[ks], b0.hi, b1.hi);            // three chains side by side, each a third as long
+            few_mma_tf32(y[1][h], q_hi[ks], b0.lo, b1.lo);
             few_mma_tf32(x[h], q_hi[ks], b0.hi, b1.hi);
           }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[h][e] += y[0][h][e] + y[1][h][e];
       }
       // ---- weights
       float top[2] = {kNoScore, kNoScore};

@@ -21,6 +21,7 @@ struct AttnTcParams {
   int chunks;          // 16-byte pieces of a row that hold values
   int units, pairs;    // query tiles of 128 per (batch entry, key head), and blocks of one or two of them
   int per_block;       // query tiles of a block: 1 or 2
+  long q_split, k_split, v_split, g_split;     // float32: elements from one part of an operand to the next (attention_tc3.h)
 };
 
 // A tensor-core kernel as a struct: kThreads and run(p, smem), which lets the next kernel's blocks in itself.
@@ -159,10 +160,10 @@ __device__ __forceinline__ void tcx_st32(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tcx_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// rows [r0, r0 + 128) of one head into a swizzled tile, by N threads of which this is number t: `chunks` pieces of a row of
+// rows [r0, r0 + ROWS) of one head into a swizzled tile, by N threads of which this is number t: `chunks` pieces of a row of
 // values, zeros beyond them up to a whole step of 16 columns and in rows from `end` on.  A thread has the same piece of every
 // N / 8-th row, so that a copy costs it an addition and a comparison: one warp keeps up with the tensor core.
-template <int NC, int N>
+template <int NC, int N, int ROWS = 128>
 __device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, long row_stride, int r0, int end, int chunks, int t) {
   const int c = t % 8, r = t / 8, left = end - r0 - r;               // rows of this thread that hold values: it * N / 8 < left
   const long step = (long)(N / 8) * row_stride;
@@ -172,11 +173,11 @@ __device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, lon
     if (cc >= (chunks + 1) / 2 * 2) break;
     const bool in = cc < chunks;
     const bf16* from = src + (long)(r0 + r) * row_stride + 8 * cc;
-    const uint32_t to = dst + b * kTcxTile + r * 128;
+    const uint32_t to = dst + b * (ROWS * 128) + r * 128;
     // (N = 32: rows r and r + 4 in turn, more threads: r % 8 stays)
     const uint32_t even = (uint32_t)((c ^ (r % 8)) << 4), odd = (uint32_t)((c ^ ((r + N / 8) % 8)) << 4);
 #pragma unroll 8
-    for (int it = 0; it < 1024 / N; ++it) {
+    for (int it = 0; it < ROWS * 8 / N; ++it) {
       const bool on = in && it * (N / 8) < left;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + it * (16 * N) + (it % 2 ? odd : even)), "l"(on ? from : src),
                    "r"(on ? 16 : 0)

@@ -5,11 +5,13 @@
 #include "../../include/s2cnn_b200.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "attention_few.h"
 #include "attention_kernels.h"
 #include "attention_tc_backward.h"
+#include "attention_tc3.h"
 #include "attention_tc_forward.h"
 #include "dropout_kernels.h"
 #include "layer_norm_kernels.h"
@@ -188,41 +190,128 @@ int attn_few(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
   });
 }
 #endif
-inline size_t attn_forward_bytes(AttnParams p) {
 #ifndef S2C_EMUL
-  if (attn_few_rows(p)) {
-    attn_split(p);
-    return attn_split_bytes(p);
+// ---- tensor-core kernels: which calls they take, and the packed copies they need
+// Rows that they can fetch in 16-byte pieces, as far as sizes and strides tell: others are packed first, as float32 always is.
+// (Bases that are not aligned to 16 bytes, with rows that would be: not on the tensor cores.  A workspace query does not see
+// them; the Python functions copy such a tensor.)
+inline bool attn_pieces(const long (&stride)[3], int dim) { return dim % 8 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 && stride[2] % 8 == 0; }
+inline bool attn_packs(const AttnParams& p, int size) {
+  return size == 4 || !(attn_pieces(p.qs, p.dim) && attn_pieces(p.ks, p.dim) && attn_pieces(p.vs, p.dim));
+}
+static std::atomic<int> g_attention{0};      // test switch: 0 by size, 1 never the tensor-core kernels, 2 always
+
+// Packed copies of q, k, v (and dout) in a workspace: three parts of float32, one of bfloat16.
+struct AttnPacked {
+  int tensors = 0, chunks = 0;
+  size_t at[4], bytes = 0;
+  long part[4];
+};
+inline AttnPacked attn_packed(const AttnParams& p, int size, int tensors) {
+  AttnPacked k;
+  k.tensors = tensors;
+  k.chunks = (p.dim + 7) / 8;
+  for (int t = 0; t < tensors; ++t) {
+    const bool of_q = t == 0 || t == 3;
+    k.part[t] = (long)p.batch * (of_q ? p.lq : p.lk) * (of_q ? p.heads : p.kv_heads) * 8 * k.chunks;
+    k.at[t] = k.bytes;
+    k.bytes += attn_align((size_t)k.part[t] * sizeof(bf16) * (size == 4 ? 3 : 1));
   }
-#endif
-  return 0;
+  return k;
 }
-#ifndef S2C_EMUL
-// Rows that the tensor-core kernels can fetch in 16-byte pieces.
-inline bool attn_pieces(const void* x, const long (&stride)[3], int dim) {
-  return aligned16(x) && dim % 8 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 && stride[2] % 8 == 0;
+// launches the copies into `ws` and turns t's operands to them
+template <class T>
+int attn_pack(AttnTcParams& t, const AttnPacked& k, char* ws, stream_t st) {
+  AttnParams& p = t.a;
+  AttnPackParams c = {};
+  const void* src[4] = {p.q, p.k, p.v, p.dout};
+  const long* stride[4] = {p.qs, p.ks, p.vs, t.gs};
+  long most = 0;
+  c.tensors = k.tensors; c.batch = p.batch; c.dim = p.dim; c.chunks = k.chunks;
+  for (int i = 0; i < k.tensors; ++i) {
+    const bool of_q = i == 0 || i == 3;
+    c.src[i] = src[i];
+    c.dst[i] = reinterpret_cast<bf16*>(ws + k.at[i]);
+    for (int e = 0; e < 3; ++e) c.stride[i][e] = stride[i][e];
+    c.part[i] = k.part[i];
+    c.len[i] = of_q ? p.lq : p.lk;
+    c.heads[i] = of_q ? p.heads : p.kv_heads;
+    most = std::max(most, k.part[i] / 8);
+  }
+  S2C_SEQ_TRY(seq_launch<AttnPack<T>>("attention_pack", std::min<long>((most + 255) / 256, 8L * dev_sm_count()), 0, st, c));
+  const long row = 8L * k.chunks;
+  auto turn = [&](const void*& x, long* s, long& part, int i) {
+    x = c.dst[i];
+    s[0] = row * c.len[i] * c.heads[i];
+    s[1] = row;
+    s[2] = row * c.len[i];
+    part = k.part[i];
+  };
+  turn(p.q, p.qs, t.q_split, 0);
+  turn(p.k, p.ks, t.k_split, 1);
+  turn(p.v, p.vs, t.v_split, 2);
+  if (k.tensors > 3) turn(p.dout, t.gs, t.g_split, 3);
+  t.chunks = k.chunks;
+  return S2C_OK;
 }
-inline int attn_tc_forward_launch(const AttnParams& p, stream_t st) {
+// The forward pass: worth it from this many scores on (see attn_tc_worth).
+inline bool attn_tc_worth(const AttnParams& p, bool packed) {
+  const int mode = g_attention.load(std::memory_order_relaxed);
+  if (p.batch < 1 || p.lq < 1 || p.lk < 1 || mode == 1) return false;
+  if (mode == 2) return true;
+  return !packed || (long)p.lq * p.lk >= 128 * 128;
+}
+template <class T>
+bool attn_forward_tc(const AttnParams& p) {
+  const bool packed = attn_packs(p, sizeof(T));
+  if (!packed && !(aligned16(p.q) && aligned16(p.k) && aligned16(p.v))) return false;
+  const size_t smem = sizeof(T) == 4 ? (p.dim > 64 ? AttnTc3Forward<2>::smem(p.reach) : AttnTc3Forward<1>::smem(p.reach)) : tcf_smem(p.dim > 64 ? 2 : 1, 1, p.reach);
+  return attn_tc_worth(p, packed) && smem <= (size_t)dev_smem_limit();
+}
+template <class T>
+int attn_tc_forward_launch(const AttnParams& p, char* ws, size_t ws_bytes, stream_t st) {
   AttnTcParams t = {};
   t.a = p;
   t.chunks = p.dim / 8;
-  t.units = (p.lq + 127) / 128 * p.group;
-  const long heads = (long)p.batch * p.kv_heads;
+  if (attn_packs(p, sizeof(T))) {
+    const AttnPacked k = attn_packed(p, sizeof(T), 3);
+    if (k.bytes > ws_bytes || !ws) return fail(S2C_ERR_WORKSPACE, "s2c_attention: workspace too small");
+    S2C_SEQ_TRY(attn_pack<T>(t, k, ws, st));
+  }
   const int nc = p.dim > 64 ? 2 : 1;
-  t.per_block = heads * ((t.units + 1) / 2) >= dev_sm_count() && tcf_smem(nc, 2, p.reach) <= (size_t)dev_smem_limit() ? 2 : 1;
-  t.pairs = (t.units + t.per_block - 1) / t.per_block;
-  const size_t smem = tcf_smem(nc, t.per_block, p.reach);
-  return nc == 1 ? attn_tc_launch<AttnTcForward<1>>("attention_tc", heads * t.pairs, smem, st, t)
-                 : attn_tc_launch<AttnTcForward<2>>("attention_tc", heads * t.pairs, smem, st, t);
+  if constexpr (sizeof(T) == 4) {
+    t.a.tiles = (p.lq + 127) / 128;
+    const long blocks = (long)p.batch * p.heads * t.a.tiles;
+    return nc == 1 ? attn_tc_launch<AttnTc3Forward<1>>("attention_tc3", blocks, AttnTc3Forward<1>::smem(p.reach), st, t)
+                   : attn_tc_launch<AttnTc3Forward<2>>("attention_tc3", blocks, AttnTc3Forward<2>::smem(p.reach), st, t);
+  } else {
+    t.units = (p.lq + 127) / 128 * p.group;
+    const long heads = (long)p.batch * p.kv_heads;
+    t.per_block = heads * ((t.units + 1) / 2) >= dev_sm_count() && tcf_smem(nc, 2, p.reach) <= (size_t)dev_smem_limit() ? 2 : 1;
+    t.pairs = (t.units + t.per_block - 1) / t.per_block;
+    const size_t smem = tcf_smem(nc, t.per_block, p.reach);
+    return nc == 1 ? attn_tc_launch<AttnTcForward<1>>("attention_tc", heads * t.pairs, smem, st, t)
+                   : attn_tc_launch<AttnTcForward<2>>("attention_tc", heads * t.pairs, smem, st, t);
+  }
 }
 #endif
+template <class T>
+size_t attn_forward_bytes(AttnParams p) {
+#ifndef S2C_EMUL
+  if (attn_few_rows(p)) {
+    attn_split(p);
+    if (attn_few_fits<T>(p)) return attn_split_bytes(p);
+  }
+  if (attn_packs(p, sizeof(T)) && attn_forward_tc<T>(p)) return attn_packed(p, sizeof(T), 3).bytes;
+#endif
+  return 0;
+}
 template <class T>
 int attn_forward(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
   if (p.batch == 0 || p.lq == 0) return S2C_OK;
 #ifndef S2C_EMUL
   if (attn_few_fits<T>(p)) return attn_few<T>(p, ws, ws_bytes, st);
-  if (sizeof(T) == 2 && p.lk > 0 && attn_pieces(p.q, p.qs, p.dim) && attn_pieces(p.k, p.ks, p.dim) && attn_pieces(p.v, p.vs, p.dim))
-    return attn_tc_forward_launch(p, st);
+  if (attn_forward_tc<T>(p)) return attn_tc_forward_launch<T>(p, static_cast<char*>(ws), ws_bytes, st);
 #endif
   p.tiles = (p.lq + kAttnTile - 1) / kAttnTile;
   return attn_by_dim<T>(p.dim, [&](auto d) {
@@ -246,8 +335,7 @@ int attn_backward(AttnParams p, void* dbias, void* ws, size_t ws_bytes, stream_t
 #ifndef S2C_EMUL
   const long gs[3] = {(long)p.lq * p.heads * p.dim, (long)p.heads * p.dim, p.dim};
   const int nc = p.dim > 64 ? 2 : 1;
-  done = sizeof(T) == 2 && p.batch > 0 && p.lq > 0 && p.lk > 0 && attn_pieces(p.q, p.qs, p.dim) && attn_pieces(p.k, p.ks, p.dim) &&
-         attn_pieces(p.v, p.vs, p.dim) && attn_pieces(p.dout, gs, p.dim) && aligned16(p.o) &&
+  done = sizeof(T) == 2 && attn_tc_worth(p, false) && !attn_packs(p, 2) && p.dim % 8 == 0 && aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout) && aligned16(p.o) &&
          std::max(tcb_q_smem(nc, p.reach, dbias), tcb_kv_smem(nc, p.reach)) <= (size_t)dev_smem_limit();
   if (done) {
     AttnTcParams t = {};
@@ -344,7 +432,8 @@ int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long 
 
 size_t s2c_attention_workspace(const s2c_attention_desc* d) {
   if (attn_check("s2c_attention_workspace", d) != S2C_OK) return 0;
-  return attn_forward_bytes(attn_params(d, nullptr, nullptr, nullptr, nullptr));
+  const AttnParams p = attn_params(d, nullptr, nullptr, nullptr, d->bucket_of);
+  return d->dtype == kSeqF32 ? attn_forward_bytes<float>(p) : attn_forward_bytes<bf16>(p);
 }
 
 size_t s2c_attention_saved_bytes(const s2c_attention_desc* d) {
@@ -384,6 +473,15 @@ int s2c_attention_backward(const s2c_attention_desc* d, const void* q, const voi
   attn_set_saved(p, d->dtype, const_cast<void*>(saved));
   return d->dtype == kSeqF32 ? attn_backward<float>(p, dbias, workspace, workspace_bytes, (stream_t)stream)
                              : attn_backward<bf16>(p, dbias, workspace, workspace_bytes, (stream_t)stream);
+}
+
+// test hook, see the header
+void s2c_debug_attention(int mode) {
+#ifndef S2C_EMUL
+  g_attention = mode;
+#else
+  (void)mode;
+#endif
 }
 
 }  // extern "C"

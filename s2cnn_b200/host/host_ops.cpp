@@ -659,7 +659,11 @@ struct Ops {
   }
   static const void* vptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
   static void* vmut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-  static Tensor unit_stride(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+  // consecutive values in the last axis, from a 16-byte boundary on
+  static Tensor unit_stride(const Tensor& t) {
+    if (t.size(-1) > 1 && t.stride(-1) != 1) return t.contiguous();
+    return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 ? t.clone(at::MemoryFormat::Contiguous) : t;
+  }
 
   struct AttnArgs {      // undefined tensors: not given
     Tensor q, k, v, bias, buckets, starts, q_lengths, kv_lengths;
