@@ -18,6 +18,7 @@ namespace s2c {
 struct AttnTcParams {
   AttnParams a;        // q, k, v (and dout): 16-byte aligned, strides multiples of 8 elements
   long gs[3];          // strides of dout
+  const void* grad;    // dout as the caller gave it, laid out as the output
   int chunks;          // 16-byte pieces of a row that hold values
   int units, pairs;    // query tiles of 128 per (batch entry, key head), and blocks of one or two of them
   int per_block;       // query tiles of a block: 1 or 2

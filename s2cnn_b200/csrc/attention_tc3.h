@@ -371,5 +371,570 @@ struct AttnTc3Forward {
   }
 };
 
+// ---- gradient of the queries, heads of at most 64 values -----------------------------------------------------------------------
+// As AttnTcGradQ, with key tiles of 64: warps 0 - 3 take the first 32 keys of a tile, warps 4 - 7 the others; the gradient of a
+// tile's keys is added to registers, half of its columns per group.
+constexpr int kTc3Diag = 2 * 48;
+struct Tc3QBars {
+  uint64_t in_full, s_full[2], dp_full, ds_full, dq_done, k_full[3], k_empty[3], v_full, v_empty, drained;
+  uint32_t tmem;
+};
+struct AttnTc3GradQ {
+  static constexpr int kThreads = kTc3Threads, KT = 64, HALF = 32;
+  static constexpr uint32_t kQ = 3 * 128 * 128, kK = 3 * KT * 128;
+  static size_t smem(int reach, bool bias_grad) {
+    return 1024 + 2 * kQ + 4 * (size_t)kK + (2 * reach + 2 * kTcxMargin + 1 + 512 + (bias_grad ? 2 * 8 * kTc3Diag + 2 * reach + 1 : 0)) * sizeof(float) +
+           sizeof(Tc3QBars) + 16;
+  }
+  static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) {
+    const AttnParams& p = pp.a;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t base = (tcx_addr(dyn) + 1023u) & ~1023u;
+    unsigned char* const smem = reinterpret_cast<unsigned char*>(dyn) + (base - tcx_addr(dyn));
+    float* const red = reinterpret_cast<float*>(smem + 2 * kQ + 4 * kK);   // [512]
+    float* const tab = red + 512;
+    float* const diag = tab + tcx_tab_floats(p.reach);                     // [2][8][kTc3Diag], then a slot per relative position
+    float* const slot = diag + (p.dbias_part ? 2 * 8 * kTc3Diag : 0);
+    Tc3QBars* const bars = reinterpret_cast<Tc3QBars*>((reinterpret_cast<uintptr_t>(slot + (p.dbias_part ? 2 * p.reach + 1 : 0)) + 15) & ~(uintptr_t)15);
+    const uint32_t q_at = base, g_at = base + kQ, k_at = base + 2 * kQ, v_at = k_at + 3 * kK;
+    const int heads_all = p.batch * p.heads;
+    const int tile = p.tiles - 1 - (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, h = bh % p.heads, b = bh / p.heads, hk = h / p.group;
+    if (tid == 0) {
+      tcx_init(&bars->in_full, 256);
+      for (int i = 0; i < 2; ++i) tcx_init(&bars->s_full[i], 1);
+      tcx_init(&bars->dp_full, 1);
+      tcx_init(&bars->ds_full, 8);
+      tcx_init(&bars->dq_done, 1);
+      for (int i = 0; i < 3; ++i) {
+        tcx_init(&bars->k_full[i], 1);
+        tcx_init(&bars->k_empty[i], 1);
+      }
+      tcx_init(&bars->v_full, 1);
+      tcx_init(&bars->v_empty, 1);
+      tcx_init(&bars->drained, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const AttnSeq s = attn_seq(p, b);
+    const int i0 = 128 * tile;
+    const int keys = i0 < s.qlen ? attn_keys(p, s, min(i0 + 128, s.qlen)) : 0, n = (keys + KT - 1) / KT;
+    if (warp == 8) {
+      __syncwarp();
+      tcx_alloc<512>(&bars->tmem);
+    }
+    tcx_bias_table(p, h, tab, tid, kTc3Threads, true);
+    if (p.dbias_part)
+      for (int e = tid; e <= 2 * p.reach; e += kTc3Threads) slot[e] = 0.f;
+    tcx_before_sync();
+    __syncthreads();
+    tcx_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
+    stream_order_next();
+    const uint32_t t_s = tmem, t_dp = tmem + 128, t_ds = tmem + 192, t_dq = tmem + 288;
+    bool ok = true;
+
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if (warp == 8 && n) {
+        const int steps = (pp.chunks + 1) / 2;
+        const uint32_t is = tcx_idesc(KT, false), io = tcx_idesc(16 * steps, true);
+        auto scores = [&](int j) {
+          if (!(ok = tcx_wait_warp(&bars->k_full[j % 3], (j / 3) & 1))) return;
+          if (tcx_elect()) {
+            tc3_scores<1, 128, KT>(t_s + KT * (j & 1), q_at, k_at + (j % 3) * kK, is, steps);
+            tcx_commit(&bars->s_full[j & 1]);
+          }
+          __syncwarp();
+        };
+        auto products = [&](int j) {
+          if (!(ok = tcx_wait_warp(&bars->v_full, j & 1))) return;
+          if (tcx_elect()) {
+            tc3_scores<1, 128, KT>(t_dp, g_at, v_at, is, steps);
+            tcx_commit(&bars->dp_full);
+            tcx_commit(&bars->v_empty);
+          }
+          __syncwarp();
+        };
+        ok = tcx_wait_warp(&bars->in_full, 0);
+        if (ok) scores(0);
+        if (ok) products(0);
+        if (ok && n > 1) scores(1);
+        for (int j = 0; j < n && ok; ++j) {
+          if (!(ok = tcx_wait_warp(&bars->ds_full, j & 1))) break;
+          tcx_after_sync();
+          if (j + 1 < n) products(j + 1);
+          if (!ok) break;
+          if (tcx_elect()) {
+            tc3_combine<1, KT, KT>(t_dq, t_ds, k_at + (j % 3) * kK, io);
+            tcx_commit(&bars->dq_done);
+            tcx_commit(&bars->k_empty[j % 3]);
+          }
+          __syncwarp();
+          if (j + 2 < n) scores(j + 2);
+        }
+        if (tcx_elect()) tcx_commit(&bars->drained);
+        __syncwarp();
+        ok = tcx_wait_warp(&bars->drained, 0) && ok;
+      } else if (warp == 9) {
+        const bf16* src = static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+        for (int j = 0; j < n && ok; ++j) {
+          if (j >= 3) ok = tcx_wait_warp(&bars->k_empty[j % 3], (j / 3 - 1) & 1);
+          if (!ok) break;
+          tc3_load<1, 32, KT>(k_at + (j % 3) * kK, src, pp.k_split, p.ks[1], KT * j, keys, pp.chunks, lane);
+          tcx_loaded();
+          __syncwarp();
+          if (lane == 0) tcx_arrive(&bars->k_full[j % 3]);
+        }
+      } else if (warp == 10) {
+        const bf16* src = static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2];
+        for (int j = 0; j < n && ok; ++j) {
+          if (j >= 1) ok = tcx_wait_warp(&bars->v_empty, (j - 1) & 1);
+          if (!ok) break;
+          tc3_load<1, 32, KT>(v_at, src, pp.v_split, p.vs[1], KT * j, keys, pp.chunks, lane);
+          tcx_loaded();
+          __syncwarp();
+          if (lane == 0) tcx_arrive(&bars->v_full);
+        }
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      const int half = warp >> 2, row = 32 * (warp & 3) + lane, i = i0 + row;
+      const long at = (((long)b * p.lq + i) * p.heads + h) * p.dim;
+      if (n) {
+        tc3_load<1, 256, 128>(q_at, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], pp.q_split, p.qs[1], i0, s.qlen, pp.chunks, tid);
+        tc3_load<1, 256, 128>(g_at, static_cast<const bf16*>(p.dout) + b * pp.gs[0] + h * pp.gs[2], pp.g_split, pp.gs[1], i0, s.qlen, pp.chunks, tid);
+        tcx_loaded();
+        tcx_arrive(&bars->in_full);
+      }
+      float delta = 0.f;                                                   // dO . O, every second value per thread
+      if (i < s.qlen) {
+        const float *g = static_cast<const float*>(pp.grad) + at, *o = static_cast<const float*>(p.o) + at;
+        for (int c = half; c < p.dim; c += 2) delta = fmaf(g[c], o[c], delta);
+      }
+      red[tid] = delta;
+      tc3_sync();
+      delta = red[row] + red[128 + row];
+      const float2 st = i < s.qlen ? p.stats[((long)b * p.heads + h) * p.lq + i] : make_float2(INFINITY, 0.f);
+      if (half == 0 && i < p.lq) p.delta[((long)b * p.heads + h) * p.lq + i] = delta;
+      const float inv = st.y;
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+      const float scale = p.scale * kLog2e, tab_before = tab[0], tab_behind = tab[2 * p.reach + 2 * kTcxMargin];
+      float far_before = 0.f, far_behind = 0.f, acc[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = 0.f;
+      auto drain = [&](int j) {
+        if (ok) ok = tcx_wait_warp(&bars->dq_done, j & 1);
+        tcx_after_sync();
+        uint32_t o[32];
+        tcx_ld32(t_dq + 32 * half + lanes, o);
+        tcx_ld_wait(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) acc[e] += as_float(o[e]);
+      };
+      int turn = 0;
+      for (int j = 0; j < n; ++j) {
+        const int j0 = KT * j, d0 = j0 - i0 - s.start;
+        const bool close = d0 + KT - 1 > -p.reach && d0 - 127 < p.reach && p.reach > 0;
+        if (ok) ok = tcx_wait_warp(&bars->s_full[j & 1], (j >> 1) & 1);
+        tcx_after_sync();
+        uint32_t raw[32], grad[32];
+        tcx_ld32(t_s + KT * (j & 1) + HALF * half + lanes, raw);
+        tcx_ld_wait(raw);
+        float* x = reinterpret_cast<float*>(raw);
+        if (close) {
+          const float* near = tab + (d0 + HALF * half - row + p.reach + kTcxMargin);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = fmaf(x[c], scale, near[c]) - st.x;
+        } else {
+          const float far = d0 > 0 ? tab_behind : tab_before;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = fmaf(x[c], scale, far) - st.x;
+        }
+        const bool edge = j0 + KT > keys || (p.causal && d0 + KT - 1 > 0);
+        const int lim = (p.causal ? min(keys - j0, row - d0 + 1) : keys - j0) - HALF * half;
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = c < lim ? x[c] : kNoScore;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = exp2_fast(x[c]) * inv;
+        if (ok) ok = tcx_wait_warp(&bars->dp_full, j & 1);
+        tcx_after_sync();
+        tcx_ld32(t_dp + HALF * half + lanes, grad);
+        tcx_ld_wait(grad);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] *= as_float(grad[c]) - delta;
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = c < lim ? x[c] : 0.f;
+        }
+        if (j > 0) drain(j - 1);                                           // (the columns of dS have been read, too)
+        tc3_put<32>(t_ds + 16 * half + lanes, 32, x);
+        tcx_st_wait();
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) tcx_arrive(&bars->ds_full);
+        if (!p.dbias_part) continue;
+        if (close) {
+          float* mine = diag + (8 * turn + warp) * kTc3Diag;
+          float run[2] = {0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) run[k] += x[16 * k + c];
+            if (c == 15) break;
+            if (lane == 31) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) mine[48 * k + c] = run[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              run[k] = __shfl_up_sync(0xffffffffu, run[k], 1);
+              run[k] = lane == 0 ? 0.f : run[k];
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) mine[48 * k + 46 - lane] = run[k];
+          tc3_sync();
+          if (tid < 127 + KT) {
+            const int off = tid - 127, d = d0 + off;
+            float sum = 0.f;
+#pragma unroll
+            for (int wv = 0; wv < 8; ++wv)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int e = off + 32 * (wv & 3) - HALF * (wv >> 2) - 16 * k + 31;
+                if (e >= 0 && e < 47) sum += diag[(8 * turn + wv) * kTc3Diag + 48 * k + e];
+              }
+            if (d <= -p.reach) far_before += sum;
+            else if (d >= p.reach) far_behind += sum;
+            else slot[d + p.reach] += sum;
+          }
+          turn ^= 1;
+        } else {
+          float sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sum[c & 1] += x[c];
+          if (d0 > 0) far_behind += sum[0] + sum[1];
+          else far_before += sum[0] + sum[1];
+        }
+      }
+      if (n) drain(n - 1);
+      if (ok && n) ok = tcx_wait_warp(&bars->drained, 0);
+      const bool wide = p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % 16 == 0;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = ok ? acc[c] * p.scale : bulk_nan();
+      if (i < p.lq) tc3_store_row(static_cast<float*>(p.dq) + at, acc, 32, p.dim, 32 * half, wide);
+      if (p.dbias_part) {
+        tc3_sync();
+        red[tid] = far_before;
+        red[256 + tid] = far_behind;
+        tc3_sync();
+        if (warp < 2) {
+          float sum = 0.f;
+          for (int e = lane; e < 256; e += 32) sum += red[256 * warp + e];
+#pragma unroll
+          for (int m = 16; m >= 1; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+          if (lane == 0) red[256 * warp] = sum;
+        }
+        tc3_sync();
+        if (tid == 0) {
+          slot[0] = red[0];
+          if (p.reach > 0) slot[2 * p.reach] = red[256];
+          else slot[0] += red[256];
+        }
+        tc3_sync();
+        float* part = p.dbias_part + (((long)b * p.tiles + tile) * p.heads + h) * p.n_buckets;
+        for (int which = tid; which < p.n_buckets; which += 256) {
+          float sum = 0.f;
+          for (int e = 0; e <= 2 * p.reach; ++e)
+            if (p.bucket_of[e] == which) sum += slot[e];
+          part[which] = ok ? sum : bulk_nan();
+        }
+      }
+    }
+    tcx_before_sync();
+    __syncthreads();
+    if (warp == 8) tcx_free<512>(tmem);
+  }
+};
+
+// ---- gradients of keys and values, heads of at most 64 values ------------------------------------------------------------------
+// As AttnTcGradKV, with query tiles of 64; the products of a tile are added to registers, half of the columns of either gradient
+// per group.
+struct Tc3KvBars {
+  uint64_t in_full, s_full, s_read, dp_full, dp_read, p_full, ds_full, dv_done, dk_done, q_full[2], q_empty[2], g_full[2], g_empty[2], r_full[2],
+      r_empty[2], drained;
+  uint32_t tmem;
+};
+struct AttnTc3GradKV {
+  static constexpr int kThreads = kTc3Threads, QT = 64, HALF = 32;
+  static constexpr uint32_t kK = 3 * 128 * 128, kQ = 3 * QT * 128;
+  static size_t smem(int reach) {
+    return 1024 + 2 * kK + 4 * (size_t)kQ + (2 * 3 * QT + 2 * reach + 2 * kTcxMargin + 1) * sizeof(float) + sizeof(Tc3KvBars) + 16;
+  }
+  static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) {
+    const AttnParams& p = pp.a;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t base = (tcx_addr(dyn) + 1023u) & ~1023u;
+    unsigned char* const smem = reinterpret_cast<unsigned char*>(dyn) + (base - tcx_addr(dyn));
+    float* const stat = reinterpret_cast<float*>(smem + 2 * kK + 4 * kQ);             // [2][3][QT]: m, 1 / l, delta
+    float* const tab = stat + 2 * 3 * QT;
+    Tc3KvBars* const bars = reinterpret_cast<Tc3KvBars*>((reinterpret_cast<uintptr_t>(tab + tcx_tab_floats(p.reach)) + 15) & ~(uintptr_t)15);
+    const uint32_t k_at = base, v_at = base + kK, q_at = base + 2 * kK, g_at = q_at + 2 * kQ;
+    const int heads_all = p.batch * p.kv_heads;
+    const int tile = (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, hk = bh % p.kv_heads, b = bh / p.kv_heads;
+    if (tid == 0) {
+      tcx_init(&bars->in_full, 256);
+      tcx_init(&bars->s_full, 1);
+      tcx_init(&bars->s_read, 8);
+      tcx_init(&bars->dp_full, 1);
+      tcx_init(&bars->dp_read, 8);
+      tcx_init(&bars->p_full, 8);
+      tcx_init(&bars->ds_full, 8);
+      tcx_init(&bars->dv_done, 1);
+      tcx_init(&bars->dk_done, 1);
+      for (int i = 0; i < 2; ++i) {
+        tcx_init(&bars->q_full[i], 1);
+        tcx_init(&bars->q_empty[i], 1);
+        tcx_init(&bars->g_full[i], 1);
+        tcx_init(&bars->g_empty[i], 1);
+        tcx_init(&bars->r_full[i], 1);
+        tcx_init(&bars->r_empty[i], 8);
+      }
+      tcx_init(&bars->drained, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const AttnSeq s = attn_seq(p, b);
+    const int j0 = 128 * tile, keys = attn_keys(p, s, s.qlen);
+    const int first = j0 < keys ? attn_first_query(p, s, j0) / QT : 0;
+    const int per_head = j0 < keys ? (s.qlen + QT - 1) / QT - first : 0, n = per_head > 0 ? per_head * p.group : 0;
+    if (warp == 8) {
+      __syncwarp();
+      tcx_alloc<512>(&bars->tmem);
+    }
+    tcx_before_sync();
+    __syncthreads();
+    tcx_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
+    stream_order_next();
+    const uint32_t t_s = tmem, t_dp = tmem + 64, t_p = tmem + 128, t_ds = tmem + 224, t_dv = tmem + 320, t_dk = tmem + 384;
+    bool ok = true;
+
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      if (warp == 8 && n) {
+        const int steps = (pp.chunks + 1) / 2;
+        const uint32_t is = tcx_idesc(QT, false), io = tcx_idesc(16 * steps, true);
+        auto scores = [&](int t) {
+          if (!(ok = tcx_wait_warp(&bars->q_full[t & 1], (t >> 1) & 1))) return;
+          if (tcx_elect()) {
+            tc3_scores<1, 128, QT>(t_s, k_at, q_at + (t & 1) * kQ, is, steps);
+            tcx_commit(&bars->s_full);
+          }
+          __syncwarp();
+        };
+        auto products = [&](int t) {
+          if (!(ok = tcx_wait_warp(&bars->g_full[t & 1], (t >> 1) & 1))) return;
+          if (tcx_elect()) {
+            tc3_scores<1, 128, QT>(t_dp, v_at, g_at + (t & 1) * kQ, is, steps);
+            tcx_commit(&bars->dp_full);
+          }
+          __syncwarp();
+        };
+        ok = tcx_wait_warp(&bars->in_full, 0);
+        if (ok) scores(0);
+        if (ok) products(0);
+        for (int t = 0; t < n && ok; ++t) {
+          if (t + 1 < n) {
+            if (!(ok = tcx_wait_warp(&bars->s_read, t & 1))) break;
+            tcx_after_sync();
+            scores(t + 1);
+          }
+          if (!ok || !(ok = tcx_wait_warp(&bars->p_full, t & 1))) break;
+          tcx_after_sync();
+          if (tcx_elect()) {
+            tc3_combine<1, QT, QT>(t_dv, t_p, g_at + (t & 1) * kQ, io);
+            tcx_commit(&bars->dv_done);
+            tcx_commit(&bars->g_empty[t & 1]);
+          }
+          __syncwarp();
+          if (t + 1 < n) {
+            if (!(ok = tcx_wait_warp(&bars->dp_read, t & 1))) break;
+            tcx_after_sync();
+            products(t + 1);
+          }
+          if (!ok || !(ok = tcx_wait_warp(&bars->ds_full, t & 1))) break;
+          tcx_after_sync();
+          if (tcx_elect()) {
+            tc3_combine<1, QT, QT>(t_dk, t_ds, q_at + (t & 1) * kQ, io);
+            tcx_commit(&bars->dk_done);
+            tcx_commit(&bars->q_empty[t & 1]);
+          }
+          __syncwarp();
+        }
+        if (tcx_elect()) tcx_commit(&bars->drained);
+        __syncwarp();
+        ok = tcx_wait_warp(&bars->drained, 0) && ok;
+      } else if (warp == 9 || warp == 10) {
+        const bool is_q = warp == 9;
+        uint64_t *full = is_q ? bars->q_full : bars->g_full, *empty = is_q ? bars->q_empty : bars->g_empty;
+        const uint32_t to = is_q ? q_at : g_at;
+        const long by_head = is_q ? p.qs[2] : pp.gs[2], stride = is_q ? p.qs[1] : pp.gs[1], part = is_q ? pp.q_split : pp.g_split;
+        const bf16* src = static_cast<const bf16*>(is_q ? p.q : p.dout) + b * (is_q ? p.qs[0] : pp.gs[0]) + hk * p.group * by_head;
+        int g = 0, it = first;
+        for (int t = 0; t < n && ok; ++t) {
+          if (t >= 2) ok = tcx_wait_warp(&empty[t & 1], (t / 2 - 1) & 1);
+          if (!ok) break;
+          tc3_load<1, 32, QT>(to + (t & 1) * kQ, src + g * by_head, part, stride, QT * it, s.qlen, pp.chunks, lane);
+          tcx_loaded();
+          __syncwarp();
+          if (lane == 0) tcx_arrive(&full[t & 1]);
+          if (++it == first + per_head) { it = first; ++g; }
+        }
+      } else if (warp == 11) {
+        int g = 0, it = first;
+        for (int t = 0; t < n && ok; ++t) {
+          if (t >= 2) ok = tcx_wait_warp(&bars->r_empty[t & 1], (t / 2 - 1) & 1);
+          if (!ok) break;
+          const long row0 = ((long)b * p.heads + hk * p.group + g) * p.lq;
+          float* to = stat + (t & 1) * 3 * QT;
+#pragma unroll
+          for (int e = lane; e < QT; e += 32) {
+            const int i = QT * it + e;
+            const float2 st = i < s.qlen ? p.stats[row0 + i] : make_float2(INFINITY, 0.f);
+            to[e] = st.x;
+            to[QT + e] = st.y;
+            to[2 * QT + e] = i < s.qlen ? p.delta[row0 + i] : 0.f;
+          }
+          __syncwarp();
+          if (lane == 0) tcx_arrive(&bars->r_full[t & 1]);
+          if (++it == first + per_head) { it = first; ++g; }
+        }
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+      const int half = warp >> 2, row = 32 * (warp & 3) + lane, j = j0 + row;
+      if (n) {
+        tc3_load<1, 256, 128>(k_at, static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2], pp.k_split, p.ks[1], j0, keys, pp.chunks, tid);
+        tc3_load<1, 256, 128>(v_at, static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2], pp.v_split, p.vs[1], j0, keys, pp.chunks, tid);
+        tcx_loaded();
+        tcx_arrive(&bars->in_full);
+      }
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+      const float scale = p.scale * kLog2e;
+      float dv[32], dk[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) dv[c] = dk[c] = 0.f;
+      auto drain = [&](uint64_t* bar, uint32_t from, int t, float (&acc)[32]) {
+        if (ok) ok = tcx_wait_warp(bar, t & 1);
+        tcx_after_sync();
+        uint32_t o[32];
+        tcx_ld32(from + 32 * half + lanes, o);
+        tcx_ld_wait(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) acc[e] += as_float(o[e]);
+      };
+      int g = -1, it = first + per_head;
+      for (int t = 0; t < n; ++t) {
+        if (it == first + per_head) {
+          it = first;
+          ++g;
+          tc3_sync();
+          tcx_bias_table(p, hk * p.group + g, tab, tid, 256, true);
+          tc3_sync();
+        }
+        const int i0 = QT * it, d0 = j0 - i0 - s.start;                    // relative position of row 0 to query 0
+        const float* sm = stat + (t & 1) * 3 * QT + HALF * half;
+        if (ok) ok = tcx_wait_warp(&bars->r_full[t & 1], (t >> 1) & 1);
+        if (ok) ok = tcx_wait_warp(&bars->s_full, t & 1);
+        tcx_after_sync();
+        uint32_t raw[32], grad[32];
+        tcx_ld32(t_s + HALF * half + lanes, raw);
+        tcx_ld_wait(raw);
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) tcx_arrive(&bars->s_read);
+        float* x = reinterpret_cast<float*>(raw);
+        if (d0 + 127 > -p.reach && d0 - (QT - 1) < p.reach && p.reach > 0) {
+          const float* near = tab + (d0 + row - HALF * half + p.reach + kTcxMargin);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = fmaf(x[c], scale, near[-c]);
+        } else {
+          const float far = d0 > 0 ? tab[2 * p.reach + 2 * kTcxMargin] : tab[0];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = fmaf(x[c], scale, far);
+        }
+        const bool edge = j0 + 128 > keys || (p.causal && d0 + 127 > 0);
+        const int low = j >= keys ? 128 : (p.causal ? d0 + row : 0) - HALF * half;
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = c >= low ? x[c] : kNoScore;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(sm + c), f = *reinterpret_cast<const float4*>(sm + QT + c);
+          x[c] = exp2_fast(x[c] - m.x) * f.x;
+          x[c + 1] = exp2_fast(x[c + 1] - m.y) * f.y;
+          x[c + 2] = exp2_fast(x[c + 2] - m.z) * f.z;
+          x[c + 3] = exp2_fast(x[c + 3] - m.w) * f.w;
+        }
+        if (t > 0) drain(&bars->dv_done, t_dv, t - 1, dv);
+        tc3_put<32>(t_p + 16 * half + lanes, 32, x);
+        tcx_st_wait();
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) tcx_arrive(&bars->p_full);
+        if (ok) ok = tcx_wait_warp(&bars->dp_full, t & 1);
+        tcx_after_sync();
+        tcx_ld32(t_dp + HALF * half + lanes, grad);
+        tcx_ld_wait(grad);
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) tcx_arrive(&bars->dp_read);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(sm + 2 * QT + c);
+          x[c] *= as_float(grad[c]) - f.x;
+          x[c + 1] *= as_float(grad[c + 1]) - f.y;
+          x[c + 2] *= as_float(grad[c + 2]) - f.z;
+          x[c + 3] *= as_float(grad[c + 3]) - f.w;
+        }
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = c >= low ? x[c] : 0.f;
+        }
+        if (t > 0) drain(&bars->dk_done, t_dk, t - 1, dk);
+        tc3_put<32>(t_ds + 16 * half + lanes, 32, x);
+        tcx_st_wait();
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          tcx_arrive(&bars->ds_full);
+          tcx_arrive(&bars->r_empty[t & 1]);
+        }
+        ++it;
+      }
+      if (n) {
+        drain(&bars->dv_done, t_dv, n - 1, dv);
+        drain(&bars->dk_done, t_dk, n - 1, dk);
+        if (ok) ok = tcx_wait_warp(&bars->drained, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        dv[c] = ok ? dv[c] : bulk_nan();
+        dk[c] = ok ? dk[c] * p.scale : bulk_nan();
+      }
+      const long at = (((long)b * p.lk + j) * p.kv_heads + hk) * p.dim;
+      if (j < p.lk) {
+        tc3_store_row(static_cast<float*>(p.dv) + at, dv, 32, p.dim, 32 * half, p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dv) % 16 == 0);
+        tc3_store_row(static_cast<float*>(p.dk) + at, dk, 32, p.dim, 32 * half, p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % 16 == 0);
+      }
+    }
+    tcx_before_sync();
+    __syncthreads();
+    if (warp == 8) tcx_free<512>(tmem);
+  }
+};
+
 }  // namespace s2c
 #endif  // S2C_EMUL

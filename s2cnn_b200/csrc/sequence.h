@@ -321,37 +321,70 @@ int attn_forward(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
 }
 
 inline size_t attn_delta_bytes(const AttnParams& p) { return attn_align((size_t)p.batch * p.heads * p.lq * sizeof(float)); }
-inline size_t attn_backward_bytes(const AttnParams& p, bool with_bias) {
+inline size_t attn_parts_bytes(const AttnParams& p, bool with_bias) {
   const size_t tiles = (p.lq + kAttnTile - 1) / kAttnTile;
-  return attn_delta_bytes(p) + (with_bias ? (size_t)p.batch * tiles * p.heads * p.n_buckets * sizeof(float) : 0);
+  return with_bias ? attn_align((size_t)p.batch * tiles * p.heads * p.n_buckets * sizeof(float)) : 0;
+}
+#ifndef S2C_EMUL
+// (float32 heads of more than 64 values: the parts of queries and gradients alone would fill the shared memory)
+template <class T>
+bool attn_backward_tc(const AttnParams& p, bool with_bias) {
+  const bool packed = attn_packs(p, sizeof(T));
+  if (!packed && !(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout) && aligned16(p.o))) return false;
+  if (sizeof(T) == 4 && p.dim > 64) return false;
+  const int nc = p.dim > 64 ? 2 : 1;
+  const size_t q = sizeof(T) == 4 ? AttnTc3GradQ::smem(p.reach, with_bias) : tcb_q_smem(nc, p.reach, with_bias);
+  const size_t kv = sizeof(T) == 4 ? AttnTc3GradKV::smem(p.reach) : tcb_kv_smem(nc, p.reach);
+  return attn_tc_worth(p, packed) && std::max(q, kv) <= (size_t)dev_smem_limit();
+}
+template <class T>
+int attn_tc_backward_launch(AttnParams& p, char* packs, stream_t st) {
+  AttnTcParams t = {};
+  t.gs[0] = (long)p.lq * p.heads * p.dim;
+  t.gs[1] = (long)p.heads * p.dim;
+  t.gs[2] = p.dim;
+  t.grad = p.dout;
+  t.chunks = p.dim / 8;
+  p.tiles = (p.lq + 127) / 128;
+  t.a = p;
+  if (attn_packs(p, sizeof(T))) S2C_SEQ_TRY(attn_pack<T>(t, attn_packed(p, sizeof(T), 4), packs, st));
+  const int nc = p.dim > 64 ? 2 : 1;
+  const bool bias_grad = p.dbias_part != nullptr;
+  const long q_blocks = (long)p.batch * p.heads * p.tiles, kv_tiles = (p.lk + 127) / 128, kv_blocks = (long)p.batch * p.kv_heads * kv_tiles;
+  if constexpr (sizeof(T) == 4) {
+    S2C_SEQ_TRY(attn_tc_launch<AttnTc3GradQ>("attention_tc3_grad_q", q_blocks, AttnTc3GradQ::smem(p.reach, bias_grad), st, t));
+    t.a.tiles = (int)kv_tiles;
+    return attn_tc_launch<AttnTc3GradKV>("attention_tc3_grad_kv", kv_blocks, AttnTc3GradKV::smem(p.reach), st, t);
+  } else {
+    const size_t q_smem = tcb_q_smem(nc, p.reach, bias_grad), kv_smem = tcb_kv_smem(nc, p.reach);
+    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradQ<1>>("attention_tc_grad_q", q_blocks, q_smem, st, t)
+                        : attn_tc_launch<AttnTcGradQ<2>>("attention_tc_grad_q", q_blocks, q_smem, st, t));
+    t.a.tiles = (int)kv_tiles;
+    return nc == 1 ? attn_tc_launch<AttnTcGradKV<1>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t)
+                   : attn_tc_launch<AttnTcGradKV<2>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t);
+  }
+}
+#endif
+// (asked without pointers: then as if all were aligned)
+template <class T>
+size_t attn_backward_bytes(const AttnParams& p, bool with_bias) {
+  size_t n = attn_delta_bytes(p) + attn_parts_bytes(p, with_bias);
+#ifndef S2C_EMUL
+  if (attn_packs(p, sizeof(T)) && attn_backward_tc<T>(p, with_bias)) n += attn_packed(p, sizeof(T), 4).bytes;
+#endif
+  return n;
 }
 template <class T>
 int attn_backward(AttnParams p, void* dbias, void* ws, size_t ws_bytes, stream_t st) {
-  if (attn_backward_bytes(p, dbias != nullptr) > ws_bytes || (ws_bytes && !ws))
-    return fail(S2C_ERR_WORKSPACE, "s2c_attention_backward: workspace too small");
-  p.delta = static_cast<float*>(ws);
-  p.dbias_part = dbias ? reinterpret_cast<float*>(static_cast<char*>(ws) + attn_delta_bytes(p)) : nullptr;
+  const size_t need = attn_backward_bytes<T>(p, dbias != nullptr);
+  if (need > ws_bytes || (need && !ws)) return fail(S2C_ERR_WORKSPACE, "s2c_attention_backward: workspace too small");
+  char* const at = static_cast<char*>(ws);
+  p.delta = reinterpret_cast<float*>(at);
+  p.dbias_part = dbias ? reinterpret_cast<float*>(at + attn_delta_bytes(p)) : nullptr;
   bool done = false;
 #ifndef S2C_EMUL
-  const long gs[3] = {(long)p.lq * p.heads * p.dim, (long)p.heads * p.dim, p.dim};
-  const int nc = p.dim > 64 ? 2 : 1;
-  done = sizeof(T) == 2 && attn_tc_worth(p, false) && !attn_packs(p, 2) && p.dim % 8 == 0 && aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout) && aligned16(p.o) &&
-         std::max(tcb_q_smem(nc, p.reach, dbias), tcb_kv_smem(nc, p.reach)) <= (size_t)dev_smem_limit();
-  if (done) {
-    AttnTcParams t = {};
-    for (int i = 0; i < 3; ++i) t.gs[i] = gs[i];
-    t.chunks = p.dim / 8;
-    p.tiles = (p.lq + 127) / 128;
-    t.a = p;
-    const long q_blocks = (long)p.batch * p.heads * p.tiles;
-    const size_t q_smem = tcb_q_smem(nc, p.reach, dbias), kv_smem = tcb_kv_smem(nc, p.reach);
-    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradQ<1>>("attention_tc_grad_q", q_blocks, q_smem, st, t)
-                        : attn_tc_launch<AttnTcGradQ<2>>("attention_tc_grad_q", q_blocks, q_smem, st, t));
-    t.a.tiles = (p.lk + 127) / 128;
-    const long kv_blocks = (long)p.batch * p.kv_heads * t.a.tiles;
-    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradKV<1>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t)
-                        : attn_tc_launch<AttnTcGradKV<2>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t));
-  }
+  done = attn_backward_tc<T>(p, dbias != nullptr);
+  if (done) S2C_SEQ_TRY(attn_tc_backward_launch<T>(p, at + attn_delta_bytes(p) + attn_parts_bytes(p, dbias != nullptr), st));
 #endif
   if (!done) S2C_SEQ_TRY(attn_by_dim<T>(p.dim, [&](auto d) {
     constexpr int DP = decltype(d)::value;
@@ -457,7 +490,9 @@ int s2c_attention(const s2c_attention_desc* d, const void* q, const void* k, con
 size_t s2c_attention_backward_workspace(const s2c_attention_desc* d) {
   if (attn_check("s2c_attention_backward_workspace", d) != S2C_OK) return 0;
   AttnParams p = attn_params(d, nullptr, nullptr, nullptr, d->bucket_of);
-  return attn_backward_bytes(p, d->bucket_of != nullptr);
+  // (whether the gradient of a bias is wanted is not known here)
+  auto bytes = [&](bool with_bias) { return d->dtype == kSeqF32 ? attn_backward_bytes<float>(p, with_bias) : attn_backward_bytes<bf16>(p, with_bias); };
+  return std::max(bytes(d->bucket_of != nullptr), bytes(false));
 }
 
 int s2c_attention_backward(const s2c_attention_desc* d, const void* q, const void* k, const void* v, const void* bias, const void* out,
