@@ -290,8 +290,11 @@ int attn_tc_forward_launch(const AttnParams& p, char* ws, size_t ws_bytes, strea
     t.per_block = heads * ((t.units + 1) / 2) >= dev_sm_count() && tcf_smem(nc, 2, p.reach) <= (size_t)dev_smem_limit() ? 2 : 1;
     t.pairs = (t.units + t.per_block - 1) / t.per_block;
     const size_t smem = tcf_smem(nc, t.per_block, p.reach);
-    return nc == 1 ? attn_tc_launch<AttnTcForward<1>>("attention_tc", heads * t.pairs, smem, st, t)
-                   : attn_tc_launch<AttnTcForward<2>>("attention_tc", heads * t.pairs, smem, st, t);
+    if (p.bias && p.stats)        // a bias gradient may follow
+      return nc == 1 ? attn_tc_launch<AttnTcForward<1, true>>("attention_tc", heads * t.pairs, smem, st, t)
+                     : attn_tc_launch<AttnTcForward<2, true>>("attention_tc", heads * t.pairs, smem, st, t);
+    return nc == 1 ? attn_tc_launch<AttnTcForward<1, false>>("attention_tc", heads * t.pairs, smem, st, t)
+                   : attn_tc_launch<AttnTcForward<2, false>>("attention_tc", heads * t.pairs, smem, st, t);
   }
 }
 #endif

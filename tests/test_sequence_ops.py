@@ -93,7 +93,7 @@ def check_attention(dev, dtype, B, Lq, Lk, H, Hk, D, bias=None, seed=0, packed=F
     args = [t.detach().requires_grad_(True) for t in ((q, k, v) if table is None else (q, k, v, table))]
     out = S.attention(*args[:3], args[3] if table is not None else None, buckets, **kw)
     grads = torch.autograd.grad(out, args, g)
-    assert torch.equal(out, inferred)
+    assert rel(inferred, want[0]) <= TOL[dtype]          # (where a bias gradient may follow, weights are kept more exactly)
     for name, a, b in zip(("out", "dq", "dk", "dv", "dbias"), (out,) + tuple(grads), want):
         # one key or one bucket per row makes score gradients that are zero up to rounding: measured against what their terms are
         err = (a.double().cpu() - b).norm().item() if b.norm() < 1e-3 * g.double().norm().cpu() and name in ("dq", "dk", "dbias") else None
