@@ -121,12 +121,15 @@ struct AttnFew {
     };
 #pragma unroll
     for (int i = 0; i < L::kStages - 1; ++i) fetch(warp + i * kFewWarps, i);
-    if (n)
+    // a chunk that lies before the reach of every query has one bias per head, and needs no table
+    const bool far = n && j_end - 1 - s.start <= -p.reach;
+    if (n && !far)
       for (int g = 0; g < p.group; ++g) attn_bias_table<T>(ctx, p, hk * p.group + g, tab + g * (2 * p.reach + 1));
     // fragments of the queries: rows lane / 4 and that + 8
     unsigned q_hi[kKs][4], q_lo[sizeof(T) == 2 ? 1 : kKs][4];
     int pos[2], of_tab[2];
     bool in_row[2];
+    float flat[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = lane / 4 + 8 * e, i = r / p.group;
@@ -134,6 +137,10 @@ struct AttnFew {
       pos[e] = i + s.start;
       of_tab[e] = (r < rows ? r % p.group : 0) * (2 * p.reach + 1) + p.reach;
       const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + (in_row[e] ? i * p.qs[1] + (hk * p.group + r % p.group) * p.qs[2] : 0);
+      if (far && p.bias && r < rows) {
+        const int which = p.bucket_of[0];
+        if (which >= 0 && which < p.n_buckets) flat[e] = attn_bias_units(widen(static_cast<const T*>(p.bias)[(long)which * p.heads + hk * p.group + r % p.group]));
+      }
       auto at = [&](int c) { return in_row[e] && n && c < p.dim ? widen(q[c]) : 0.f; };
 #pragma unroll
       for (int ks = 0; ks < kKs; ++ks) {
@@ -200,7 +207,8 @@ struct AttnFew {
         for (int e = 0; e < 4; ++e) {
           const int j = j_lo + t * kFewKeys + 8 * h + 2 * (lane % 4) + e % 2, d = j - pos[e / 2];
           const bool seen = j < j_end && in_row[e / 2] && (!p.causal || d <= 0);
-          x[h][e] = seen ? fmaf(x[h][e], scale, tab[of_tab[e / 2] + attn_clamp(d, -p.reach, p.reach)]) : kNoScore;
+          const float bias = far ? flat[e / 2] : tab[of_tab[e / 2] + attn_clamp(d, -p.reach, p.reach)];
+          x[h][e] = seen ? fmaf(x[h][e], scale, bias) : kNoScore;
           top[e / 2] = fmaxf(top[e / 2], x[h][e]);
         }
       float f[2], base[2];
@@ -328,31 +336,46 @@ struct AttnFew {
   }
 };
 
-// joins the splits: a row to DP threads, two runs over its parts
+// Joins the splits: a block per row.  The splits' maxima and sums come in one load per thread and turn, the outputs in loads
+// that do not wait for one another: thread t has column t % DP of every kThreads / DP-th split.
 template <class T, int DP>
 struct AttnJoin {
   using Params = AttnParams;
-  static constexpr int kThreads = 128, kBlocks = 4;
-  static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char*) {
-    const int rows = p.lq * p.group, per = kThreads / DP, t = ctx.tid % DP;
-    const long at = (long)ctx.bid * per + ctx.tid / DP;
-    if (at >= (long)p.batch * p.kv_heads * rows) return;
-    const int r = (int)(at % rows), bh = (int)(at / rows), hk = bh % p.kv_heads, b = bh / p.kv_heads;
+  static constexpr int kThreads = 128, kBlocks = 8, kSlices = kThreads / DP;
+  static size_t smem(const Params& p) { return (p.splits + kThreads + 8) * sizeof(float); }
+  static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
+    const int rows = p.lq * p.group, t = ctx.tid, lane = t % 32, warp = t / 32;
+    float *red = reinterpret_cast<float*>(smem), *outs = red + 8, *weight = outs + kThreads;
+    const int r = ctx.bid % rows, bh = ctx.bid / rows, hk = bh % p.kv_heads, b = bh / p.kv_heads;
     const AttnSeq s = attn_seq(p, b);                                  // splits beyond the keys have nothing
     const int keys = attn_keys(p, s, s.qlen), n = (keys + p.chunk - 1) / p.chunk;
     const float* part = p.part + ((long)bh * p.splits * rows + r) * (DP + 2);
     const long step = (long)rows * (DP + 2);
     float m = kNoScore;
-#pragma unroll 8
-    for (int e = 0; e < n; ++e) m = fmaxf(m, part[e * step + DP]);
+    for (int e = t; e < n; e += kThreads) m = fmaxf(m, part[e * step + DP]);
+    m = lanes_max<32>(ctx, m);
+    if (lane == 0) red[warp] = m;
+    ctx.sync();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float base = m == kNoScore ? 0.f : m;
-    float o = 0.f, l = 0.f;
-#pragma unroll 8
-    for (int e = 0; e < n; ++e) {
+    float l = 0.f;
+    for (int e = t; e < n; e += kThreads) {
       const float f = exp2_fast(part[e * step + DP] - base);
+      weight[e] = f;
       l = fmaf(part[e * step + DP + 1], f, l);
-      o = fmaf(part[e * step + t], f, o);
     }
+    l = lanes_sum<32>(ctx, l);
+    if (lane == 0) red[4 + warp] = l;
+    ctx.sync();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const int c = t % DP;
+    float o = 0.f;
+#pragma unroll 8
+    for (int e = t / DP; e < n; e += kSlices) o = fmaf(part[e * step + c], weight[e], o);
+    outs[t] = o;
+    ctx.sync();
+    if (t >= DP) return;
+    for (int e = 1; e < kSlices; ++e) o += outs[e * DP + t];
     const int i = r / p.group, h = hk * p.group + r % p.group;
     const float2 st = attn_stats(m, l);
     if (t < p.dim) {

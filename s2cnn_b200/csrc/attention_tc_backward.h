@@ -203,12 +203,12 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) 
       if (close) {
         const float* near = tab + (d0 + 64 * half - row + p.reach + kTcxMargin);
 #pragma unroll
-        for (int c = 0; c < 64; ++c) x[c] = fmaf(x[c], scale, near[c] + base_m);
+        for (int c = 0; c < 64; ++c) x[c] = fmaf(x[c], scale, near[c]) + base_m;      // (as the forward pass rounds it)
       } else {
-        const float far = (d0 > 0 ? tab_behind : tab_before) + base_m;
+        const float far = d0 > 0 ? tab_behind : tab_before;
 #pragma unroll
         for (int c = 0; c < 64; c += 2) {
-          const float2 y = fma2(make_float2(x[c], x[c + 1]), make_float2(scale, scale), make_float2(far, far));
+          const float2 y = tcx_add2(fma2(make_float2(x[c], x[c + 1]), make_float2(scale, scale), make_float2(far, far)), make_float2(base_m, base_m));
           x[c] = y.x;
           x[c + 1] = y.y;
         }
@@ -524,10 +524,10 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) 
 #pragma unroll
         for (int c = 0; c < 64; c += 4) {
           const float4 m = *reinterpret_cast<const float4*>(sm + c);
-          x[c] = fmaf(x[c], scale, near[-c] + m.x);
-          x[c + 1] = fmaf(x[c + 1], scale, near[-c - 1] + m.y);
-          x[c + 2] = fmaf(x[c + 2], scale, near[-c - 2] + m.z);
-          x[c + 3] = fmaf(x[c + 3], scale, near[-c - 3] + m.w);
+          x[c] = fmaf(x[c], scale, near[-c]) + m.x;
+          x[c + 1] = fmaf(x[c + 1], scale, near[-c - 1]) + m.y;
+          x[c + 2] = fmaf(x[c + 2], scale, near[-c - 2]) + m.z;
+          x[c + 3] = fmaf(x[c + 3], scale, near[-c - 3]) + m.w;
         }
       } else {
         const float far = d0 > 0 ? tab[2 * p.reach + 2 * kTcxMargin] : tab[0];
@@ -535,8 +535,8 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) 
 #pragma unroll
         for (int c = 0; c < 64; c += 4) {
           const float4 m = *reinterpret_cast<const float4*>(sm + c);
-          const float2 y = fma2(make_float2(x[c], x[c + 1]), s2, tcx_add2(make_float2(m.x, m.y), f2));
-          const float2 z = fma2(make_float2(x[c + 2], x[c + 3]), s2, tcx_add2(make_float2(m.z, m.w), f2));
+          const float2 y = tcx_add2(fma2(make_float2(x[c], x[c + 1]), s2, f2), make_float2(m.x, m.y));
+          const float2 z = tcx_add2(fma2(make_float2(x[c + 2], x[c + 3]), s2, f2), make_float2(m.z, m.w));
           x[c] = y.x; x[c + 1] = y.y; x[c + 2] = z.x; x[c + 3] = z.y;
         }
       }

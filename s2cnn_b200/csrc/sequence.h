@@ -30,25 +30,25 @@ inline int seq_check_type(const char* who, int dtype) {
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // ---- layer norm --------------------------------------------------------------------------------------------------------
-// A row takes the fewest threads that hold it in at most 32 registers each: neighbouring lanes up to 1024 columns, a block
-// of 128 up to 4096 and of 512 beyond.
+// A row takes the fewest threads that hold it, and the next one as it lies in memory, in their registers: neighbouring lanes up
+// to 1024 columns (512 of float32), a block of 128 up to 4096 (2048), of 512 beyond.
 constexpr int kNormMaxCols = 16384;
 template <class F>
-int norm_by_cols(int cols, F f) {
+int norm_by_cols(int cols, int size, F f) {
 #define S2C_NORM(T, EPT) return f(std::integral_constant<int, T>(), std::integral_constant<int, EPT>())
   if (cols <= 32) S2C_NORM(4, 8);
   if (cols <= 128) S2C_NORM(16, 8);
   if (cols <= 256) S2C_NORM(32, 8);
   if (cols <= 512) S2C_NORM(32, 16);
-  if (cols <= 1024) S2C_NORM(32, 32);
+  if (cols <= 1024 && size == 2) S2C_NORM(32, 32);
   if (cols <= 2048) S2C_NORM(128, 16);
-  if (cols <= 4096) S2C_NORM(128, 32);
+  if (cols <= 4096 && size == 2) S2C_NORM(128, 32);
   if (cols <= 8192) S2C_NORM(512, 16);
   S2C_NORM(512, 32);
 #undef S2C_NORM
 }
-inline int norm_bwd_blocks(long rows, int cols) {
-  return norm_by_cols(cols, [&](auto t, auto ept) {
+inline int norm_bwd_blocks(long rows, int cols, int size) {
+  return norm_by_cols(cols, size, [&](auto t, auto ept) {
     using K = LayerNormBwd<float, decltype(t)::value, decltype(ept)::value, 1>;
     return (int)std::min<long>((rows + K::kTeams - 1) / K::kTeams, (long)dev_sm_count() * K::kBlocks);
   });
@@ -57,20 +57,20 @@ template <class T>
 int norm_forward(LayerNormParams p, stream_t st) {
   const bool vec = p.cols % kVec<T> == 0;
   p.wide = vec && aligned16(p.x) && aligned16(p.y) && aligned16(p.w) && aligned16(p.b);
-  return norm_by_cols(p.cols, [&](auto t, auto ept) {
+  return norm_by_cols(p.cols, sizeof(T), [&](auto t, auto ept) {
     constexpr int TT = decltype(t)::value, E = decltype(ept)::value;
     using V = LayerNormFwd<T, TT, E, kVec<T>>;
     using S = LayerNormFwd<T, TT, E, 1>;
-    const long blocks = std::min<long>((p.rows + V::kTeams - 1) / V::kTeams, 8L * dev_sm_count() * V::kBlocks);
+    const long blocks = std::min<long>((p.rows + V::kTeams - 1) / V::kTeams, (long)dev_sm_count() * V::kBlocks);
     return vec ? seq_launch<V>("layer_norm", blocks, V::smem(), st, p) : seq_launch<S>("layer_norm", blocks, S::smem(), st, p);
   });
 }
 template <class T>
 int norm_backward(LayerNormParams p, void* dw, void* db, stream_t st) {
-  const int blocks = norm_bwd_blocks(p.rows, p.cols);
+  const int blocks = norm_bwd_blocks(p.rows, p.cols, sizeof(T));
   const bool vec = p.cols % kVec<T> == 0;
   p.wide = vec && aligned16(p.x) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.w);
-  S2C_SEQ_TRY(norm_by_cols(p.cols, [&](auto t, auto ept) {
+  S2C_SEQ_TRY(norm_by_cols(p.cols, sizeof(T), [&](auto t, auto ept) {
     constexpr int TT = decltype(t)::value, E = decltype(ept)::value;
     using V = LayerNormBwd<T, TT, E, kVec<T>>;
     using S = LayerNormBwd<T, TT, E, 1>;
@@ -185,8 +185,7 @@ int attn_few(AttnParams p, void* ws, size_t ws_bytes, stream_t st) {
     S2C_SEQ_TRY(piece == 16 ? go(A()) : piece == 4 ? go(B()) : go(C()));
     if (p.splits == 1) return (int)S2C_OK;
     using J = AttnJoin<T, DP>;
-    const long rows = (long)p.batch * p.kv_heads * p.lq * p.group, per = J::kThreads / DP;
-    return seq_launch<J>("attention_join", (rows + per - 1) / per, 0, st, p);
+    return seq_launch<J>("attention_join", (long)p.batch * p.kv_heads * p.lq * p.group, J::smem(p), st, p);
   });
 }
 #endif
@@ -423,7 +422,7 @@ int s2c_layer_norm(int dtype, const void* x, const void* weight, const void* bia
 
 size_t s2c_layer_norm_backward_workspace(long rows, int cols) {
   if (rows < 1 || cols < 1 || cols > kNormMaxCols) return 0;
-  return (size_t)norm_bwd_blocks(rows, cols) * 2 * cols * sizeof(float);
+  return (size_t)std::max(norm_bwd_blocks(rows, cols, 2), norm_bwd_blocks(rows, cols, 4)) * 2 * cols * sizeof(float);
 }
 
 int s2c_layer_norm_backward(int dtype, const void* x, const void* weight, const float* stats, const void* dy, void* dx, void* dweight,
