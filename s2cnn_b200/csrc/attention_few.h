@@ -1,7 +1,7 @@
 // Attention of few queries (one new position of each recording, say): the queries of all heads that share a key head make up to
 // 16 rows, and the time is that of reading the keys and values once, 4 lq dim heads / kv_heads flops for every 2 dim values.
 //
-// A block of four warps takes `chunk` keys.  A warp has tiles of 16 keys to itself: it copies them into shared memory, kFewStages
+// A block of four warps (eight for float32) takes `chunk` keys.  A warp has tiles of 16 keys (8) to itself: it copies them into shared memory, two
 // tiles ahead (the copies in flight are what the memory's rate asks for: 100 KB per SM at 128 values), and never waits for
 // another warp.  Scores and outputs are products of 16 rows on the warp-level matrix instructions, which are far from their
 // limit here; the large tiles of tcgen05 would be one eighth full.  To keep float32 exact to a few units, an operand v is split
@@ -15,7 +15,7 @@
 
 namespace s2c {
 
-constexpr int kFewRows = 16, kFewKeys = 16, kFewWarps = 4;
+constexpr int kFewRows = 16;
 
 __device__ __forceinline__ void few_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -53,7 +53,9 @@ template <class T, int DP>
 struct FewLayout {
   static constexpr int kKeyPitch = sizeof(T) == 2 ? (DP + 8) * 2 : (DP + 4) * 4;
   static constexpr int kValuePitch = sizeof(T) == 2 ? (DP + 8) * 2 : (DP + 8) * 4;
-  static constexpr int kStage = kFewKeys * (kKeyPitch + kValuePitch);
+  // float32 tiles of 8 keys, so that twice as many warps share the memory: its products take three times the instructions
+  static constexpr int kKeys = sizeof(T) == 2 ? 16 : 8, kWarps = sizeof(T) == 2 ? 4 : 8;
+  static constexpr int kStage = kKeys * (kKeyPitch + kValuePitch);
   static constexpr int kStages = 3;
   static constexpr int kWarp = kStage * kStages;
 };
@@ -63,7 +65,9 @@ template <class T, int DP, int PIECE>
 struct AttnFew {
   using Params = AttnParams;
   using L = FewLayout<T, DP>;
-  static constexpr int kThreads = 32 * kFewWarps, kBlocks = 2;
+  static constexpr int kFewKeys = L::kKeys, kFewWarps = L::kWarps;
+  static constexpr int kThreads = 32 * kFewWarps, kBlocks = DP > 64 && sizeof(T) == 4 ? 1 : 2;
+  static constexpr int kHalves = kFewKeys / 8;                       // tiles of 8 keys
   static constexpr int kNt = DP / 8;                                 // output tiles of 8 columns
   static constexpr int kKs = sizeof(T) == 2 ? DP / 16 : DP / 8;      // steps of the scores' products
   static size_t smem(const Params& p) {
@@ -110,7 +114,7 @@ struct AttnFew {
     const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[2];
     const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[2];
     unsigned char* const mine = smem + warp * L::kWarp;
-    const int n = j_lo < j_end ? (j_end - j_lo + kFewKeys - 1) / kFewKeys : 0;         // tiles of the block; this warp: warp, warp + 4 ...
+    const int n = j_lo < j_end ? (j_end - j_lo + kFewKeys - 1) / kFewKeys : 0;         // tiles of the block; this warp: every kFewWarps-th
     auto fetch = [&](int t, int stage) {
       if (t < n) {
         const int j0 = j_lo + t * kFewKeys;
@@ -172,7 +176,7 @@ struct AttnFew {
       __syncwarp();
       const unsigned char *kt = mine + stage * L::kStage, *vt = kt + kFewKeys * L::kKeyPitch;
       // ---- scores: two tiles of 8 keys
-      float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float x[kHalves][4] = {};
       if constexpr (sizeof(T) == 2) {
         const unsigned addr = (unsigned)__cvta_generic_to_shared(kt) + (lane % 8 + (lane / 16) * 8) * L::kKeyPitch + ((lane / 8) % 2) * 16;
 #pragma unroll
@@ -183,11 +187,11 @@ struct AttnFew {
           few_mma(x[1], q_hi[ks], r[2], r[3]);
         }
       } else {
-        float y[2][2][4] = {};
+        float y[2][kHalves][4] = {};
 #pragma unroll
         for (int ks = 0; ks < kKs; ++ks)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < kHalves; ++h) {
             const float* row = reinterpret_cast<const float*>(kt + (8 * h + lane / 4) * L::kKeyPitch) + 8 * ks + lane % 4;
             const FewSplit b0 = few_split(row[0]), b1 = few_split(row[4]);
             few_mma_tf32(y[0][h], q_lo[ks], b0.hi, b1.hi);            // three chains side by side, each a third as long
@@ -195,14 +199,14 @@ struct AttnFew {
             few_mma_tf32(x[h], q_hi[ks], b0.hi, b1.hi);
           }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < kHalves; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[h][e] += y[0][h][e] + y[1][h][e];
       }
       // ---- weights
       float top[2] = {kNoScore, kNoScore};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = j_lo + t * kFewKeys + 8 * h + 2 * (lane % 4) + e % 2, d = j - pos[e / 2];
@@ -235,7 +239,7 @@ struct AttnFew {
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[h][e] = exp2_fast(x[h][e] - base[e / 2]);
@@ -245,7 +249,7 @@ struct AttnFew {
       if constexpr (sizeof(T) == 2) {
         unsigned hi[4], lo[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < kHalves; ++h)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float u = x[h][2 * e], w = x[h][2 * e + 1];
@@ -266,7 +270,7 @@ struct AttnFew {
       } else {
         // a step of 8 keys; its columns lane % 4 and that + 4 are keys 2 (lane % 4) and that + 1, as the scores lie
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kHalves; ++h) {
           unsigned hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
