@@ -119,12 +119,13 @@ __device__ __forceinline__ void tcx_scores(uint32_t d, uint32_t a, uint32_t b, u
     tcx_mma(d, da + at, db + at, idesc, s > 0);
   }
 }
-// D (128 x n) += A B, A 128 x 128 in tensor memory (its second 64 columns `half` behind the first), B 128 rows of n columns
-// (MN-major)
+// D (128 x n) += A B over 16 STEPS rows of B, A in tensor memory (its second 64 columns `half` behind the first), B rows of n
+// columns (MN-major) of a tile of 128
+template <int STEPS = 8>
 __device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t half = 32) {
   const uint64_t db = tcx_desc(b, kTcxTile);
 #pragma unroll
-  for (int s = 0; s < 8; ++s)
+  for (int s = 0; s < STEPS; ++s)
     tcx_mma_t(d, a + (s / 4) * half + (s % 4) * 8, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
 }
 
@@ -209,6 +210,11 @@ __device__ __forceinline__ void tcx_bias_table(const AttnParams& p, int head, fl
     }
     tab[e] = v;
   }
+}
+__device__ __forceinline__ float tcx_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ float2 tcx_add2(float2 a, float2 b) {
   float2 d;

@@ -25,7 +25,7 @@ constexpr int kTcfThreads = 12 * 32;
 constexpr float kTcfGrow = 8.f;
 
 struct TcfBars {
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
+  uint64_t q_full[2], s_full[2], p_full[4], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
   uint32_t tmem;
 };
 
@@ -59,7 +59,8 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
     for (int i = 0; i < 2; ++i) {
       tcx_init(&bars->q_full[i], 128);
       tcx_init(&bars->s_full[i], 1);
-      tcx_init(&bars->p_full[i], 4);
+      tcx_init(&bars->p_full[2 * i], 4);
+      tcx_init(&bars->p_full[2 * i + 1], 4);
       tcx_init(&bars->pv_done[i], 1);
       tcx_init(&bars->k_full[i], 1);
       tcx_init(&bars->k_empty[i], 1);
@@ -119,16 +120,20 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
       bool have_v = false, have_k = false;
       for (int u = 0; u < 2 && ok; ++u) {
         if (j >= n[u]) continue;
-        ok = tcx_wait_warp(&bars->p_full[u], j & 1);
-        if (ok && !have_v) ok = have_v = tcx_wait_warp(&bars->v_full[sv], par);
-        if (!ok) break;
-        tcx_after_sync();
-        if (tcx_elect()) {
-          if (FINE) tcx_combine(t_out + 128 * u, t_scores + 128 * u + 64, v_at + sv * kRows, io, j > 0);
-          tcx_combine(t_out + 128 * u, t_scores + 128 * u, v_at + sv * kRows, io, FINE || j > 0);
-          tcx_commit(&bars->pv_done[u]);
+        for (int half = 0; half < 2 && ok; ++half) {
+          ok = tcx_wait_warp(&bars->p_full[2 * u + half], j & 1);
+          if (ok && !have_v) ok = have_v = tcx_wait_warp(&bars->v_full[sv], par);
+          if (!ok) break;
+          tcx_after_sync();
+          if (tcx_elect()) {
+            const uint32_t w = t_scores + 128 * u + 32 * half, v = v_at + sv * kRows + 64 * 128 * half;
+            if (FINE) tcx_combine<4>(t_out + 128 * u, w + 64, v, io, j > 0 || half);
+            tcx_combine<4>(t_out + 128 * u, w, v, io, FINE || j > 0 || half);
+            if (half) tcx_commit(&bars->pv_done[u]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         if (j + 1 < n[u]) {
           if (!have_k) ok = have_k = tcx_wait_warp(&bars->k_full[sk], ((j + 1) >> 1) & 1);
           if (!ok) break;
@@ -190,30 +195,35 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
 #pragma unroll
         for (int c = 0; c < 128; c += 32) tcx_ld_wait(raw + c);
         float* x = reinterpret_cast<float*>(raw);
-        if (d0 + 127 > -p.reach && d0 - 127 < p.reach && p.reach > 0) {
-          const float* near = tb + (d0 - row + p.reach + kTcxMargin);
+        const bool close = d0 + 127 > -p.reach && d0 - 127 < p.reach && p.reach > 0;
+        const bool edge = j0 + 128 > keys[u] || (p.causal && d0 + 127 > 0);            // some pairs of the tile are not seen
+        const float far = d0 > 0 ? far_behind : far_before;
+        // A tile of one bias, all seen: the maximum of the raw scores tells that of the others, and scale, bias and maximum are one
+        // multiply-add.  (Not for a bias so large that the scores vanish beside it, see AttnParams::stats.)
+        const bool plain = !close && !edge && scale > 0.f && fabsf(far) < 1e30f;
+        if (!plain) {
+          if (close) {
+            const float* near = tb + (d0 - row + p.reach + kTcxMargin);
 #pragma unroll
-          for (int c = 0; c < 128; ++c) x[c] = fmaf(x[c], scale, near[c]);
-        } else {
-          const float far = d0 > 0 ? far_behind : far_before;
+            for (int c = 0; c < 128; ++c) x[c] = fmaf(x[c], scale, near[c]);
+          } else {
 #pragma unroll
-          for (int c = 0; c < 128; c += 2) {
-            const float2 y = fma2(make_float2(x[c], x[c + 1]), make_float2(scale, scale), make_float2(far, far));
-            x[c] = y.x;
-            x[c + 1] = y.y;
+            for (int c = 0; c < 128; ++c) x[c] = fmaf(x[c], scale, far);
           }
-        }
-        if (j0 + 128 > keys[u] || (p.causal && d0 + 127 > 0)) {       // some pairs of the tile are not seen
-          const int lim = p.causal ? min(keys[u] - j0, row - d0 + 1) : keys[u] - j0;
+          if (edge) {
+            const int lim = p.causal ? min(keys[u] - j0, row - d0 + 1) : keys[u] - j0;
 #pragma unroll
-          for (int c = 0; c < 128; ++c) x[c] = c < lim ? x[c] : kNoScore;
+            for (int c = 0; c < 128; ++c) x[c] = c < lim ? x[c] : kNoScore;
+          }
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 4; c < 128; c += 4)
+        for (int c = 4; c < 124; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], x[c + e]);
-        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          for (int e = 0; e < 4; ++e) top[e] = tcx_max3(top[e], x[c + e], x[c + 4 + e]);
+        float now = fmaxf(tcx_max3(top[0], top[1], top[2]), tcx_max3(top[3], x[124], x[125]));
+        now = tcx_max3(now, x[126], x[127]);
+        if (plain) now = fmaf(now, scale, far);
         if (__any_sync(0xffffffffu, now > m + kTcfGrow)) {
           const float fresh = now > m + kTcfGrow ? now : m;
           if (j > 0) {
@@ -233,29 +243,30 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
           }
           m = fresh;
         }
-        const float off = m == kNoScore ? 0.f : -m;
+        const float base = m == kNoScore ? 0.f : -m, mul = plain ? scale : 1.f, add = plain ? far + base : base;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t w[64], rest[FINE ? 64 : 1];
+        // half of the weights at a time: their product with the values begins while the others are computed
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          float2 y = tcx_add2(make_float2(x[c], x[c + 1]), make_float2(off, off));
-          y.x = exp2_fast(y.x);
-          y.y = exp2_fast(y.y);
-          sum[(c / 2) & 1] = tcx_add2(sum[(c / 2) & 1], y);
-          w[c / 2] = pack_bf16(y.x, y.y);
-          if constexpr (FINE) rest[c / 2] = pack_bf16(y.x - as_float(w[c / 2] << 16), y.y - as_float(w[c / 2] & 0xffff0000u));
-        }
-        tcx_st32(ts, w);
-        tcx_st32(ts + 32, w + 32);
-        if constexpr (FINE) {
-          tcx_st32(ts + 64, rest);
-          tcx_st32(ts + 96, rest + 32);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32], rest[FINE ? 32 : 1];
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            const int c = 64 * half + e;
+            float2 y = fma2(make_float2(x[c], x[c + 1]), make_float2(mul, mul), make_float2(add, add));
+            y.x = exp2_fast(y.x);
+            y.y = exp2_fast(y.y);
+            sum[(c / 2) & 1] = tcx_add2(sum[(c / 2) & 1], y);
+            w[e / 2] = pack_bf16(y.x, y.y);
+            if constexpr (FINE) rest[e / 2] = pack_bf16(y.x - as_float(w[e / 2] << 16), y.y - as_float(w[e / 2] & 0xffff0000u));
+          }
+          tcx_st32(ts + 32 * half, w);
+          if constexpr (FINE) tcx_st32(ts + 64 + 32 * half, rest);
+          tcx_st_wait();
+          tcx_before_sync();
+          __syncwarp();
+          if (lane == 0) tcx_arrive(&bars->p_full[2 * u + half]);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        tcx_st_wait();
-        tcx_before_sync();
-        __syncwarp();
-        if (lane == 0) tcx_arrive(&bars->p_full[u]);
       }
       // ---- the output row
       if (i >= s.qlen) l = 0.f;
