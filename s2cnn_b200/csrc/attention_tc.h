@@ -129,6 +129,34 @@ __device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, 
     tcx_mma_t(d, a + (s / 4) * half + (s % 4) * 8, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
 }
 
+// the same, A of 128 rows against B of ROWS (D 128 x ROWS)
+template <int ROWS>
+__device__ __forceinline__ void tcx_scores_of(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+  const uint64_t da = tcx_desc(a, 0), db = tcx_desc(b, 0);
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    if (s >= steps) break;
+    tcx_mma(d, da + (uint64_t)(((s / 4) * kTcxTile + (s % 4) * 32) >> 4), db + (uint64_t)(((s / 4) * (ROWS * 128) + (s % 4) * 32) >> 4), idesc, s > 0);
+  }
+}
+// and with A in tensor memory
+template <int ROWS>
+__device__ __forceinline__ void tcx_scores_t(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+  const uint64_t db = tcx_desc(b, 0);
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    if (s >= steps) break;
+    tcx_mma_t(d, a + 8 * s, db + (uint64_t)(((s / 4) * (ROWS * 128) + (s % 4) * 32) >> 4), idesc, s > 0);
+  }
+}
+// D (128 x n) += A B, A 128 x ROWS in tensor memory, B a tile of ROWS rows (MN-major)
+template <int ROWS>
+__device__ __forceinline__ void tcx_combine_of(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  const uint64_t db = tcx_desc(b, ROWS * 128);
+#pragma unroll
+  for (int s = 0; s < ROWS / 16; ++s) tcx_mma_t(d, a + 8 * s, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
+}
+
 // 32 columns of a lane's row; the values are there after tcx_ld_wait
 __device__ __forceinline__ void tcx_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -159,6 +187,23 @@ __device__ __forceinline__ void tcx_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tcx_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// 32 values of a bfloat16 row (columns c0 ... c0 + 31; zeros from `chunks` pieces on, or all of them) as a left operand
+__device__ __forceinline__ void tcx_put_operand(uint32_t taddr, const bf16* row, int c0, int chunks, bool on) {
+  uint32_t r[16];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (on && c0 / 8 + k < chunks) u = *reinterpret_cast<const uint4*>(row + c0 + 8 * k);
+    r[4 * k] = u.x; r[4 * k + 1] = u.y; r[4 * k + 2] = u.z; r[4 * k + 3] = u.w;
+  }
+  tcx_st16(taddr + c0 / 2, r);
 }
 __device__ __forceinline__ void tcx_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

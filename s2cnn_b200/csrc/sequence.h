@@ -335,8 +335,8 @@ bool attn_backward_tc(const AttnParams& p, bool with_bias) {
   if (!packed && !(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout) && aligned16(p.o))) return false;
   if (sizeof(T) == 4 && p.dim > 64) return false;
   const int nc = p.dim > 64 ? 2 : 1;
-  const size_t q = sizeof(T) == 4 ? AttnTc3GradQ::smem(p.reach, with_bias) : tcb_q_smem(nc, p.reach, with_bias);
-  const size_t kv = sizeof(T) == 4 ? AttnTc3GradKV::smem(p.reach) : tcb_kv_smem(nc, p.reach);
+  const size_t q = sizeof(T) == 4 ? AttnTc3GradQ::smem(p.reach, with_bias) : nc == 1 ? AttnTcGradQ<1>::smem(p.reach, with_bias) : AttnTcGradQ<2>::smem(p.reach, with_bias);
+  const size_t kv = sizeof(T) == 4 ? AttnTc3GradKV::smem(p.reach) : nc == 1 ? AttnTcGradKV<1>::smem(p.reach) : AttnTcGradKV<2>::smem(p.reach);
   return attn_tc_worth(p, packed) && std::max(q, kv) <= (size_t)dev_smem_limit();
 }
 template <class T>
@@ -358,12 +358,11 @@ int attn_tc_backward_launch(AttnParams& p, char* packs, stream_t st) {
     t.a.tiles = (int)kv_tiles;
     return attn_tc_launch<AttnTc3GradKV>("attention_tc3_grad_kv", kv_blocks, AttnTc3GradKV::smem(p.reach), st, t);
   } else {
-    const size_t q_smem = tcb_q_smem(nc, p.reach, bias_grad), kv_smem = tcb_kv_smem(nc, p.reach);
-    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradQ<1>>("attention_tc_grad_q", q_blocks, q_smem, st, t)
-                        : attn_tc_launch<AttnTcGradQ<2>>("attention_tc_grad_q", q_blocks, q_smem, st, t));
+    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradQ<1>>("attention_tc_grad_q", q_blocks, AttnTcGradQ<1>::smem(p.reach, bias_grad), st, t)
+                        : attn_tc_launch<AttnTcGradQ<2>>("attention_tc_grad_q", q_blocks, AttnTcGradQ<2>::smem(p.reach, bias_grad), st, t));
     t.a.tiles = (int)kv_tiles;
-    return nc == 1 ? attn_tc_launch<AttnTcGradKV<1>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t)
-                   : attn_tc_launch<AttnTcGradKV<2>>("attention_tc_grad_kv", kv_blocks, kv_smem, st, t);
+    return nc == 1 ? attn_tc_launch<AttnTcGradKV<1>>("attention_tc_grad_kv", kv_blocks, AttnTcGradKV<1>::smem(p.reach), st, t)
+                   : attn_tc_launch<AttnTcGradKV<2>>("attention_tc_grad_kv", kv_blocks, AttnTcGradKV<2>::smem(p.reach), st, t);
   }
 }
 #endif
