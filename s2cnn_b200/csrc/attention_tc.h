@@ -233,6 +233,13 @@ __device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, lon
     }
   }
 }
+// Arrives at the barrier (whose count has this thread in it) once this thread's copies so far have landed; the thread goes on.
+// Who waits for that and then issues products has tcx_seen in between.
+__device__ __forceinline__ void tcx_arrive_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tcx_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tcx_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void tcx_seen() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // all of this thread's copies have landed and are seen by the tensor core
 __device__ __forceinline__ void tcx_loaded() {
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;\n\tfence.proxy.async.shared::cta;" ::: "memory");

@@ -163,10 +163,10 @@ struct AttnTc3Forward {
       for (int i = 0; i < 2; ++i) {
         tcx_init(&bars->p_full[i], 4);
         tcx_init(&bars->pv_done[i], 1);
-        tcx_init(&bars->k_full[i], 1);
+        tcx_init(&bars->k_full[i], 32);
         tcx_init(&bars->k_empty[i], 1);
       }
-      tcx_init(&bars->v_full, 1);
+      tcx_init(&bars->v_full, 32);
       tcx_init(&bars->v_empty, 1);
       tcx_init(&bars->drained, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -192,61 +192,57 @@ struct AttnTc3Forward {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8 && n) {
-        const int steps = (pp.chunks + 1) / 2;
-        const uint32_t is = tcx_idesc(KT, false), io = tcx_idesc(16 * steps, true);
-        auto scores = [&](int j) {
-          if (!(ok = tcx_wait_warp(&bars->k_full[j % KS], (j / KS) & 1))) return;
-          if (tcx_elect()) {
+      if (warp == 8) {
+        if (n && tcx_elect()) {
+          const int steps = (pp.chunks + 1) / 2;
+          const uint32_t is = tcx_idesc(KT, false), io = tcx_idesc(16 * steps, true);
+          auto scores = [&](int j) {
+            if (!(ok = tcx_wait(&bars->k_full[j % KS], (j / KS) & 1))) return;
+            tcx_seen();
             tc3_scores<NC, 128, KT>(t_s, q_at, k_at + (j % KS) * kK, is, steps);
             tcx_commit(&bars->s_full);
             tcx_commit(&bars->k_empty[j % KS]);
-          }
-          __syncwarp();
-        };
-        ok = tcx_wait_warp(&bars->q_full, 0);
-        if (ok) scores(0);
-        for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n) {
-            if (!(ok = tcx_wait_warp(&bars->s_read, j & 1))) break;
-            tcx_after_sync();
-            scores(j + 1);
-          }
-          if (!ok || !(ok = tcx_wait_warp(&bars->v_full, j & 1))) break;
-          for (int w = 0; w < 2 && ok; ++w) {
-            if (!(ok = tcx_wait_warp(&bars->p_full[w], j & 1))) break;
-            tcx_after_sync();
-            if (tcx_elect()) {
+          };
+          ok = tcx_wait(&bars->q_full, 0);
+          if (ok) scores(0);
+          for (int j = 0; j < n && ok; ++j) {
+            if (j + 1 < n) {
+              if (!(ok = tcx_wait(&bars->s_read, j & 1))) break;
+              tcx_after_sync();
+              scores(j + 1);
+            }
+            if (!ok || !(ok = tcx_wait(&bars->v_full, j & 1))) break;
+            tcx_seen();
+            for (int w = 0; w < 2 && ok; ++w) {
+              if (!(ok = tcx_wait(&bars->p_full[w], j & 1))) break;
+              tcx_after_sync();
               tc3_combine<NC, HALF, KT>(t_o + w * kO, t_w + w * kW, v_at + w * HALF * 128, io);
               tcx_commit(&bars->pv_done[w]);
               if (w == 1) tcx_commit(&bars->v_empty);
             }
-            __syncwarp();
           }
+          tcx_commit(&bars->drained);
+          tcx_wait(&bars->drained, 0);
         }
-        if (tcx_elect()) tcx_commit(&bars->drained);
         __syncwarp();
-        ok = tcx_wait_warp(&bars->drained, 0) && ok;
       } else if (warp == 9) {
         const bf16* src = static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2];
         for (int j = 0; j < n && ok; ++j) {
           if (j >= KS) ok = tcx_wait_warp(&bars->k_empty[j % KS], (j / KS - 1) & 1);
           if (!ok) break;
           tc3_load<NC, 32, KT>(k_at + (j % KS) * kK, src, pp.k_split, p.ks[1], KT * j, keys, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->k_full[j % KS]);
+          tcx_arrive_copies(&bars->k_full[j % KS]);
         }
+        tcx_copies_done();
       } else if (warp == 10) {
         const bf16* src = static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2];
         for (int j = 0; j < n && ok; ++j) {
           if (j >= 1) ok = tcx_wait_warp(&bars->v_empty, (j - 1) & 1);
           if (!ok) break;
           tc3_load<NC, 32, KT>(v_at, src, pp.v_split, p.vs[1], KT * j, keys, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->v_full);
+          tcx_arrive_copies(&bars->v_full);
         }
+        tcx_copies_done();
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -406,10 +402,10 @@ struct AttnTc3GradQ {
       tcx_init(&bars->ds_full, 8);
       tcx_init(&bars->dq_done, 1);
       for (int i = 0; i < 3; ++i) {
-        tcx_init(&bars->k_full[i], 1);
+        tcx_init(&bars->k_full[i], 32);
         tcx_init(&bars->k_empty[i], 1);
       }
-      tcx_init(&bars->v_full, 1);
+      tcx_init(&bars->v_full, 32);
       tcx_init(&bars->v_empty, 1);
       tcx_init(&bars->drained, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -434,66 +430,59 @@ struct AttnTc3GradQ {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8 && n) {
-        const int steps = (pp.chunks + 1) / 2;
-        const uint32_t is = tcx_idesc(KT, false), io = tcx_idesc(16 * steps, true);
-        auto scores = [&](int j) {
-          if (!(ok = tcx_wait_warp(&bars->k_full[j % 3], (j / 3) & 1))) return;
-          if (tcx_elect()) {
+      if (warp == 8) {
+        if (n && tcx_elect()) {
+          const int steps = (pp.chunks + 1) / 2;
+          const uint32_t is = tcx_idesc(KT, false), io = tcx_idesc(16 * steps, true);
+          auto scores = [&](int j) {
+            if (!(ok = tcx_wait(&bars->k_full[j % 3], (j / 3) & 1))) return;
+            tcx_seen();
             tc3_scores<1, 128, KT>(t_s + KT * (j & 1), q_at, k_at + (j % 3) * kK, is, steps);
             tcx_commit(&bars->s_full[j & 1]);
-          }
-          __syncwarp();
-        };
-        auto products = [&](int j) {
-          if (!(ok = tcx_wait_warp(&bars->v_full, j & 1))) return;
-          if (tcx_elect()) {
+          };
+          auto products = [&](int j) {
+            if (!(ok = tcx_wait(&bars->v_full, j & 1))) return;
+            tcx_seen();
             tc3_scores<1, 128, KT>(t_dp, g_at, v_at, is, steps);
             tcx_commit(&bars->dp_full);
             tcx_commit(&bars->v_empty);
-          }
-          __syncwarp();
-        };
-        ok = tcx_wait_warp(&bars->in_full, 0);
-        if (ok) scores(0);
-        if (ok) products(0);
-        if (ok && n > 1) scores(1);
-        for (int j = 0; j < n && ok; ++j) {
-          if (!(ok = tcx_wait_warp(&bars->ds_full, j & 1))) break;
-          tcx_after_sync();
-          if (j + 1 < n) products(j + 1);
-          if (!ok) break;
-          if (tcx_elect()) {
+          };
+          ok = tcx_wait(&bars->in_full, 0);
+          if (ok) scores(0);
+          if (ok) products(0);
+          if (ok && n > 1) scores(1);
+          for (int j = 0; j < n && ok; ++j) {
+            if (!(ok = tcx_wait(&bars->ds_full, j & 1))) break;
+            tcx_after_sync();
+            if (j + 1 < n) products(j + 1);
+            if (!ok) break;
             tc3_combine<1, KT, KT>(t_dq, t_ds, k_at + (j % 3) * kK, io);
             tcx_commit(&bars->dq_done);
             tcx_commit(&bars->k_empty[j % 3]);
+            if (j + 2 < n) scores(j + 2);
           }
-          __syncwarp();
-          if (j + 2 < n) scores(j + 2);
+          tcx_commit(&bars->drained);
+          tcx_wait(&bars->drained, 0);
         }
-        if (tcx_elect()) tcx_commit(&bars->drained);
         __syncwarp();
-        ok = tcx_wait_warp(&bars->drained, 0) && ok;
       } else if (warp == 9) {
         const bf16* src = static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2];
         for (int j = 0; j < n && ok; ++j) {
           if (j >= 3) ok = tcx_wait_warp(&bars->k_empty[j % 3], (j / 3 - 1) & 1);
           if (!ok) break;
           tc3_load<1, 32, KT>(k_at + (j % 3) * kK, src, pp.k_split, p.ks[1], KT * j, keys, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->k_full[j % 3]);
+          tcx_arrive_copies(&bars->k_full[j % 3]);
         }
+        tcx_copies_done();
       } else if (warp == 10) {
         const bf16* src = static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2];
         for (int j = 0; j < n && ok; ++j) {
           if (j >= 1) ok = tcx_wait_warp(&bars->v_empty, (j - 1) & 1);
           if (!ok) break;
           tc3_load<1, 32, KT>(v_at, src, pp.v_split, p.vs[1], KT * j, keys, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->v_full);
+          tcx_arrive_copies(&bars->v_full);
         }
+        tcx_copies_done();
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -694,9 +683,9 @@ struct AttnTc3GradKV {
       tcx_init(&bars->dv_done, 1);
       tcx_init(&bars->dk_done, 1);
       for (int i = 0; i < 2; ++i) {
-        tcx_init(&bars->q_full[i], 1);
+        tcx_init(&bars->q_full[i], 32);
         tcx_init(&bars->q_empty[i], 1);
-        tcx_init(&bars->g_full[i], 1);
+        tcx_init(&bars->g_full[i], 32);
         tcx_init(&bars->g_empty[i], 1);
         tcx_init(&bars->r_full[i], 1);
         tcx_init(&bars->r_empty[i], 8);
@@ -722,59 +711,51 @@ struct AttnTc3GradKV {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8 && n) {
-        const int steps = (pp.chunks + 1) / 2;
-        const uint32_t is = tcx_idesc(QT, false), io = tcx_idesc(16 * steps, true);
-        auto scores = [&](int t) {
-          if (!(ok = tcx_wait_warp(&bars->q_full[t & 1], (t >> 1) & 1))) return;
-          if (tcx_elect()) {
+      if (warp == 8) {
+        if (n && tcx_elect()) {
+          const int steps = (pp.chunks + 1) / 2;
+          const uint32_t is = tcx_idesc(QT, false), io = tcx_idesc(16 * steps, true);
+          auto scores = [&](int t) {
+            if (!(ok = tcx_wait(&bars->q_full[t & 1], (t >> 1) & 1))) return;
+            tcx_seen();
             tc3_scores<1, 128, QT>(t_s, k_at, q_at + (t & 1) * kQ, is, steps);
             tcx_commit(&bars->s_full);
-          }
-          __syncwarp();
-        };
-        auto products = [&](int t) {
-          if (!(ok = tcx_wait_warp(&bars->g_full[t & 1], (t >> 1) & 1))) return;
-          if (tcx_elect()) {
+          };
+          auto products = [&](int t) {
+            if (!(ok = tcx_wait(&bars->g_full[t & 1], (t >> 1) & 1))) return;
+            tcx_seen();
             tc3_scores<1, 128, QT>(t_dp, v_at, g_at + (t & 1) * kQ, is, steps);
             tcx_commit(&bars->dp_full);
-          }
-          __syncwarp();
-        };
-        ok = tcx_wait_warp(&bars->in_full, 0);
-        if (ok) scores(0);
-        if (ok) products(0);
-        for (int t = 0; t < n && ok; ++t) {
-          if (t + 1 < n) {
-            if (!(ok = tcx_wait_warp(&bars->s_read, t & 1))) break;
+          };
+          ok = tcx_wait(&bars->in_full, 0);
+          if (ok) scores(0);
+          if (ok) products(0);
+          for (int t = 0; t < n && ok; ++t) {
+            if (t + 1 < n) {
+              if (!(ok = tcx_wait(&bars->s_read, t & 1))) break;
+              tcx_after_sync();
+              scores(t + 1);
+            }
+            if (!ok || !(ok = tcx_wait(&bars->p_full, t & 1))) break;
             tcx_after_sync();
-            scores(t + 1);
-          }
-          if (!ok || !(ok = tcx_wait_warp(&bars->p_full, t & 1))) break;
-          tcx_after_sync();
-          if (tcx_elect()) {
             tc3_combine<1, QT, QT>(t_dv, t_p, g_at + (t & 1) * kQ, io);
             tcx_commit(&bars->dv_done);
             tcx_commit(&bars->g_empty[t & 1]);
-          }
-          __syncwarp();
-          if (t + 1 < n) {
-            if (!(ok = tcx_wait_warp(&bars->dp_read, t & 1))) break;
+            if (t + 1 < n) {
+              if (!(ok = tcx_wait(&bars->dp_read, t & 1))) break;
+              tcx_after_sync();
+              products(t + 1);
+            }
+            if (!ok || !(ok = tcx_wait(&bars->ds_full, t & 1))) break;
             tcx_after_sync();
-            products(t + 1);
-          }
-          if (!ok || !(ok = tcx_wait_warp(&bars->ds_full, t & 1))) break;
-          tcx_after_sync();
-          if (tcx_elect()) {
             tc3_combine<1, QT, QT>(t_dk, t_ds, q_at + (t & 1) * kQ, io);
             tcx_commit(&bars->dk_done);
             tcx_commit(&bars->q_empty[t & 1]);
           }
-          __syncwarp();
+          tcx_commit(&bars->drained);
+          tcx_wait(&bars->drained, 0);
         }
-        if (tcx_elect()) tcx_commit(&bars->drained);
         __syncwarp();
-        ok = tcx_wait_warp(&bars->drained, 0) && ok;
       } else if (warp == 9 || warp == 10) {
         const bool is_q = warp == 9;
         uint64_t *full = is_q ? bars->q_full : bars->g_full, *empty = is_q ? bars->q_empty : bars->g_empty;
@@ -786,11 +767,10 @@ struct AttnTc3GradKV {
           if (t >= 2) ok = tcx_wait_warp(&empty[t & 1], (t / 2 - 1) & 1);
           if (!ok) break;
           tc3_load<1, 32, QT>(to + (t & 1) * kQ, src + g * by_head, part, stride, QT * it, s.qlen, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&full[t & 1]);
+          tcx_arrive_copies(&full[t & 1]);
           if (++it == first + per_head) { it = first; ++g; }
         }
+        tcx_copies_done();
       } else if (warp == 11) {
         int g = 0, it = first;
         for (int t = 0; t < n && ok; ++t) {

@@ -69,11 +69,11 @@ struct AttnTcGradQ {
         tcx_init(&bars->ds_full[i], 4);
       }
       for (int i = 0; i < KS; ++i) {
-        tcx_init(&bars->k_full[i], 1);
+        tcx_init(&bars->k_full[i], 32);
         tcx_init(&bars->k_empty[i], 1);
       }
       for (int i = 0; i < VS; ++i) {
-        tcx_init(&bars->v_full[i], 1);
+        tcx_init(&bars->v_full[i], 32);
         tcx_init(&bars->v_empty[i], 1);
       }
       tcx_init(&bars->drained, 1);
@@ -101,71 +101,64 @@ struct AttnTcGradQ {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8 && n) {
-        const int steps = (pp.chunks + 1) / 2;
-        const uint32_t is = tcx_idesc(kTcbTile, false), io = tcx_idesc(16 * steps, true);
-        auto scores = [&](int j) {
-          if (!(ok = tcx_wait_warp(&bars->k_full[j % KS], (j / KS) & 1))) return;
-          if (tcx_elect()) {
+      if (warp == 8) {
+        if (n && tcx_elect()) {                                              // one thread issues all: a warp's votes cost it 100 clocks a wait
+          const int steps = (pp.chunks + 1) / 2;
+          const uint32_t is = tcx_idesc(kTcbTile, false), io = tcx_idesc(16 * steps, true);
+          auto scores = [&](int j) {
+            if (!(ok = tcx_wait(&bars->k_full[j % KS], (j / KS) & 1))) return;
+            tcx_seen();
             tcx_scores_t<kTcbTile>(t_s + kTcbTile * (j & 1), t_q, k_at + (j % KS) * kRows, is, steps);
             tcx_commit(&bars->s_full[j & 1]);
-          }
-          __syncwarp();
-        };
-        auto products = [&](int j) {                                         // dP
-          if (!(ok = tcx_wait_warp(&bars->v_full[j % VS], (j / VS) & 1))) return;
-          if (tcx_elect()) {
+          };
+          auto products = [&](int j) {                                         // dP
+            if (!(ok = tcx_wait(&bars->v_full[j % VS], (j / VS) & 1))) return;
+            tcx_seen();
             tcx_scores_t<kTcbTile>(t_dp + kTcbTile * (j & 1), t_g, v_at + (j % VS) * kRows, is, steps);
             tcx_commit(&bars->dp_full[j & 1]);
             tcx_commit(&bars->v_empty[j % VS]);
-          }
-          __syncwarp();
-        };
-        ok = tcx_wait_warp(&bars->in_full, 0);
-        tcx_after_sync();
-        for (int j = 0; j < 2 && j < n && ok; ++j) {
-          scores(j);
-          if (ok) products(j);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const uint32_t par = (j >> 1) & 1;
-          if (j + 2 < n) {
-            if (!(ok = tcx_wait_warp(&bars->s_read[j & 1], par))) break;
-            tcx_after_sync();
-            scores(j + 2);
-          }
-          if (!ok || !(ok = tcx_wait_warp(&bars->ds_full[j & 1], par))) break;
+          };
+          ok = tcx_wait(&bars->in_full, 0);
           tcx_after_sync();
-          if (tcx_elect()) {
+          for (int j = 0; j < 2 && j < n && ok; ++j) {
+            scores(j);
+            if (ok) products(j);
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            const uint32_t par = (j >> 1) & 1;
+            if (j + 2 < n) {
+              if (!(ok = tcx_wait(&bars->s_read[j & 1], par))) break;
+              tcx_after_sync();
+              scores(j + 2);
+            }
+            if (!ok || !(ok = tcx_wait(&bars->ds_full[j & 1], par))) break;
+            tcx_after_sync();
             tcx_combine_of<kTcbTile>(t_dq, t_dp + kTcbTile * (j & 1), k_at + (j % KS) * kRows, io, j > 0);
             tcx_commit(&bars->k_empty[j % KS]);
+            if (j + 2 < n) products(j + 2);                                    // in order behind the product that reads these columns
           }
-          __syncwarp();
-          if (j + 2 < n) products(j + 2);                                    // in order behind the product that reads these columns
+          tcx_commit(&bars->drained);
+          tcx_wait(&bars->drained, 0);
         }
-        if (tcx_elect()) tcx_commit(&bars->drained);
         __syncwarp();
-        ok = tcx_wait_warp(&bars->drained, 0) && ok;
       } else if (warp == 9) {
         const bf16* src = static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2];
         for (int j = 0; j < n && ok; ++j) {
           if (j >= KS) ok = tcx_wait_warp(&bars->k_empty[j % KS], (j / KS - 1) & 1);
           if (!ok) break;
           tcx_load_rows<NC, 32, kTcbTile>(k_at + (j % KS) * kRows, src, p.ks[1], kTcbTile * j, keys, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->k_full[j % KS]);
+          tcx_arrive_copies(&bars->k_full[j % KS]);
         }
+        tcx_copies_done();
       } else if (warp == 10) {
         const bf16* src = static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2];
         for (int j = 0; j < n && ok; ++j) {
           if (j >= VS) ok = tcx_wait_warp(&bars->v_empty[j % VS], (j / VS - 1) & 1);
           if (!ok) break;
           tcx_load_rows<NC, 32, kTcbTile>(v_at + (j % VS) * kRows, src, p.vs[1], kTcbTile * j, keys, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->v_full[j % VS]);
+          tcx_arrive_copies(&bars->v_full[j % VS]);
         }
+        tcx_copies_done();
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -417,9 +410,9 @@ struct AttnTcGradKV {
         tcx_init(&bars->ds_full[i], 4);
       }
       for (int i = 0; i < QS; ++i) {
-        tcx_init(&bars->q_full[i], 1);
+        tcx_init(&bars->q_full[i], 32);
         tcx_init(&bars->q_empty[i], 1);
-        tcx_init(&bars->g_full[i], 1);
+        tcx_init(&bars->g_full[i], 32);
         tcx_init(&bars->g_empty[i], 1);
         tcx_init(&bars->r_full[i], 1);
         tcx_init(&bars->r_empty[i], 4);
@@ -445,52 +438,44 @@ struct AttnTcGradKV {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8 && n) {
-        const int steps = (pp.chunks + 1) / 2;
-        const uint32_t is = tcx_idesc(kTcbTile, false), io = tcx_idesc(16 * steps, true);
-        auto scores = [&](int t) {
-          if (!(ok = tcx_wait_warp(&bars->q_full[t % QS], (t / QS) & 1))) return;
-          if (tcx_elect()) {
+      if (warp == 8) {
+        if (n && tcx_elect()) {                                              // one thread issues all: a warp's votes cost it 100 clocks a wait
+          const int steps = (pp.chunks + 1) / 2;
+          const uint32_t is = tcx_idesc(kTcbTile, false), io = tcx_idesc(16 * steps, true);
+          auto scores = [&](int t) {
+            if (!(ok = tcx_wait(&bars->q_full[t % QS], (t / QS) & 1))) return;
+            tcx_seen();
             tcx_scores_of<kTcbTile>(t_s + kTcbTile * (t & 1), k_at, q_at + (t % QS) * kRows, is, steps);
             tcx_commit(&bars->s_full[t & 1]);
-          }
-          __syncwarp();
-        };
-        auto products = [&](int t) {
-          if (!(ok = tcx_wait_warp(&bars->g_full[t % QS], (t / QS) & 1))) return;
-          if (tcx_elect()) {
+          };
+          auto products = [&](int t) {
+            if (!(ok = tcx_wait(&bars->g_full[t % QS], (t / QS) & 1))) return;
+            tcx_seen();
             tcx_scores_of<kTcbTile>(t_dp + kTcbTile * (t & 1), v_at, g_at + (t % QS) * kRows, is, steps);
             tcx_commit(&bars->dp_full[t & 1]);
+          };
+          ok = tcx_wait(&bars->in_full, 0);
+          for (int t = 0; t < 2 && t < n && ok; ++t) {
+            scores(t);
+            if (ok) products(t);
           }
-          __syncwarp();
-        };
-        ok = tcx_wait_warp(&bars->in_full, 0);
-        for (int t = 0; t < 2 && t < n && ok; ++t) {
-          scores(t);
-          if (ok) products(t);
-        }
-        for (int t = 0; t < n && ok; ++t) {
-          const uint32_t par = (t >> 1) & 1;
-          if (!(ok = tcx_wait_warp(&bars->p_full[t & 1], par))) break;
-          tcx_after_sync();
-          if (tcx_elect()) {
+          for (int t = 0; t < n && ok; ++t) {
+            const uint32_t par = (t >> 1) & 1;
+            if (!(ok = tcx_wait(&bars->p_full[t & 1], par))) break;
+            tcx_after_sync();
             tcx_combine_of<kTcbTile>(t_dv, t_s + kTcbTile * (t & 1), g_at + (t % QS) * kRows, io, t > 0);
             tcx_commit(&bars->g_empty[t % QS]);                              // (dP^T of this tile is older)
-          }
-          __syncwarp();
-          if (t + 2 < n) scores(t + 2);
-          if (!ok || !(ok = tcx_wait_warp(&bars->ds_full[t & 1], par))) break;
-          tcx_after_sync();
-          if (tcx_elect()) {
+            if (t + 2 < n) scores(t + 2);
+            if (!ok || !(ok = tcx_wait(&bars->ds_full[t & 1], par))) break;
+            tcx_after_sync();
             tcx_combine_of<kTcbTile>(t_dk, t_dp + kTcbTile * (t & 1), q_at + (t % QS) * kRows, io, t > 0);
             tcx_commit(&bars->q_empty[t % QS]);
+            if (t + 2 < n) products(t + 2);
           }
-          __syncwarp();
-          if (t + 2 < n) products(t + 2);
+          tcx_commit(&bars->drained);
+          tcx_wait(&bars->drained, 0);
         }
-        if (tcx_elect()) tcx_commit(&bars->drained);
         __syncwarp();
-        ok = tcx_wait_warp(&bars->drained, 0) && ok;
       } else if (warp == 9 || warp == 10) {
         const bool is_q = warp == 9;
         uint64_t *full = is_q ? bars->q_full : bars->g_full, *empty = is_q ? bars->q_empty : bars->g_empty;
@@ -502,11 +487,10 @@ struct AttnTcGradKV {
           if (t >= QS) ok = tcx_wait_warp(&empty[t % QS], (t / QS - 1) & 1);
           if (!ok) break;
           tcx_load_rows<NC, 32, kTcbTile>(to + (t % QS) * kRows, src + g * by_head, stride, kTcbTile * it, s.qlen, pp.chunks, lane);
-          tcx_loaded();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&full[t % QS]);
+          tcx_arrive_copies(&full[t % QS]);
           if (++it == first + per_head) { it = first; ++g; }
         }
+        tcx_copies_done();
       } else if (warp == 11) {
         int g = 0, it = first;
         for (int t = 0; t < n && ok; ++t) {

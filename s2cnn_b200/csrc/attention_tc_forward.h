@@ -62,9 +62,9 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
       tcx_init(&bars->p_full[2 * i], 4);
       tcx_init(&bars->p_full[2 * i + 1], 4);
       tcx_init(&bars->pv_done[i], 1);
-      tcx_init(&bars->k_full[i], 1);
+      tcx_init(&bars->k_full[i], 32);
       tcx_init(&bars->k_empty[i], 1);
-      tcx_init(&bars->v_full[i], 1);
+      tcx_init(&bars->v_full[i], 32);
       tcx_init(&bars->v_empty[i], 1);
     }
     tcx_init(&bars->drained, 1);
@@ -100,60 +100,59 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 8) {
-    const int steps = (pp.chunks + 1) / 2;
-    const uint32_t is = tcx_idesc(128, false), io = tcx_idesc(16 * steps, true);
-    for (int u = 0; u < 2 && ok; ++u)
-      if (n[u]) ok = tcx_wait_warp(&bars->q_full[u], 0);
-    if (ok && n_all) ok = tcx_wait_warp(&bars->k_full[0], 0);
-    if (ok && n_all && tcx_elect()) {
-      for (int u = 0; u < 2; ++u)
-        if (n[u]) {
-          tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at, is, steps);
-          tcx_commit(&bars->s_full[u]);
-        }
-      tcx_commit(&bars->k_empty[0]);
-    }
-    __syncwarp();
-    for (int j = 0; j < n_all && ok; ++j) {
-      const int sv = j & 1, sk = (j + 1) & 1;
-      const uint32_t par = (j >> 1) & 1;
-      bool have_v = false, have_k = false;
-      for (int u = 0; u < 2 && ok; ++u) {
-        if (j >= n[u]) continue;
-        for (int half = 0; half < 2 && ok; ++half) {
-          ok = tcx_wait_warp(&bars->p_full[2 * u + half], j & 1);
-          if (ok && !have_v) ok = have_v = tcx_wait_warp(&bars->v_full[sv], par);
-          if (!ok) break;
-          tcx_after_sync();
-          if (tcx_elect()) {
+    if (tcx_elect()) {                       // one thread issues all: a warp's votes cost it 100 clocks a wait
+      const int steps = (pp.chunks + 1) / 2;
+      const uint32_t is = tcx_idesc(128, false), io = tcx_idesc(16 * steps, true);
+      for (int u = 0; u < 2 && ok; ++u)
+        if (n[u]) ok = tcx_wait(&bars->q_full[u], 0);
+      if (ok && n_all) ok = tcx_wait(&bars->k_full[0], 0);
+      tcx_seen();
+      if (ok && n_all) {
+        for (int u = 0; u < 2; ++u)
+          if (n[u]) {
+            tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at, is, steps);
+            tcx_commit(&bars->s_full[u]);
+          }
+        tcx_commit(&bars->k_empty[0]);
+      }
+      for (int j = 0; j < n_all && ok; ++j) {
+        const int sv = j & 1, sk = (j + 1) & 1;
+        bool have_v = false, have_k = false;
+        for (int u = 0; u < 2 && ok; ++u) {
+          if (j >= n[u]) continue;
+          for (int half = 0; half < 2 && ok; ++half) {
+            ok = tcx_wait(&bars->p_full[2 * u + half], j & 1);
+            if (ok && !have_v) {
+              ok = have_v = tcx_wait(&bars->v_full[sv], (j >> 1) & 1);
+              tcx_seen();
+            }
+            if (!ok) break;
+            tcx_after_sync();
             const uint32_t w = t_scores + 128 * u + 32 * half, v = v_at + sv * kRows + 64 * 128 * half;
             if (FINE) tcx_combine<4>(t_out + 128 * u, w + 64, v, io, j > 0 || half);
             tcx_combine<4>(t_out + 128 * u, w, v, io, FINE || j > 0 || half);
             if (half) tcx_commit(&bars->pv_done[u]);
           }
-          __syncwarp();
-        }
-        if (!ok) break;
-        if (j + 1 < n[u]) {
-          if (!have_k) ok = have_k = tcx_wait_warp(&bars->k_full[sk], ((j + 1) >> 1) & 1);
-          if (!ok) break;
-          if (tcx_elect()) {                 // in order behind the product that reads the weights from the same columns
+          if (ok && j + 1 < n[u]) {
+            if (!have_k) {
+              ok = have_k = tcx_wait(&bars->k_full[sk], ((j + 1) >> 1) & 1);
+              tcx_seen();
+            }
+            if (!ok) break;
+            // in order behind the product that reads the weights from the same columns
             tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at + sk * kRows, is, steps);
             tcx_commit(&bars->s_full[u]);
           }
-          __syncwarp();
+        }
+        if (ok) {
+          tcx_commit(&bars->v_empty[sv]);
+          if (j + 1 < n_all) tcx_commit(&bars->k_empty[sk]);
         }
       }
-      if (ok && tcx_elect()) {
-        tcx_commit(&bars->v_empty[sv]);
-        if (j + 1 < n_all) tcx_commit(&bars->k_empty[sk]);
-      }
-      __syncwarp();
+      tcx_commit(&bars->drained);            // nothing may be in flight when tensor memory is given back
+      tcx_wait(&bars->drained, 0);
     }
-    // nothing may be in flight when tensor memory is given back
-    if (tcx_elect()) tcx_commit(&bars->drained);
     __syncwarp();
-    ok = tcx_wait_warp(&bars->drained, 0) && ok;
   } else if (warp == 9 || warp == 10) {
     const bool is_k = warp == 9;
     const bf16* src = static_cast<const bf16*>(is_k ? p.k : p.v) + b * (is_k ? p.ks[0] : p.vs[0]) + hk * (is_k ? p.ks[2] : p.vs[2]);
@@ -165,10 +164,9 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
       if (j >= 2) ok = tcx_wait_warp(&empty[slot], (j / 2 - 1) & 1);
       if (!ok) break;
       tcx_load_rows<NC, 32>(at + slot * kRows, src, stride, 128 * j, keys_all, pp.chunks, lane);
-      tcx_loaded();
-      __syncwarp();
-      if (lane == 0) tcx_arrive(&full[slot]);
+      tcx_arrive_copies(&full[slot]);
     }
+    tcx_copies_done();
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
