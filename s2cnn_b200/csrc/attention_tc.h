@@ -45,23 +45,41 @@ __device__ __forceinline__ void tcx_init(uint64_t* bar, int count) {
 __device__ __forceinline__ void tcx_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tcx_addr(bar)) : "memory");
 }
-// Bounded: false where the phase is not over after some tenths of a second.
+__device__ __forceinline__ bool tcx_try(uint32_t addr, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Bounded: false where the phase is not over after some tenths of a second.  (The first try stands in line with the code around
+// it: a role that issues products runs through cold instructions, which come quickly only where nothing branches.)
 __device__ __forceinline__ bool tcx_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = tcx_addr(bar);
+  if (__builtin_expect(tcx_try(addr, parity), 1)) return true;
+#pragma unroll 1
   for (int spin = 0; spin < (1 << 22); ++spin) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (done) return true;
+    if (tcx_try(addr, parity)) return true;
     if (spin > 256) __nanosleep(40);
   }
   return false;
 }
+// a place in a ring of N barriers and the parity of its phase
+template <int N>
+struct TcxRing {
+  int at = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) {
+      at = 0;
+      parity ^= 1;
+    }
+  }
+};
 // the same by a whole warp, which goes on together
 __device__ __forceinline__ bool tcx_wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tcx_wait(bar, parity)) != 0; }
 
@@ -108,53 +126,57 @@ __device__ __forceinline__ void tcx_mma_t(uint32_t d, uint32_t a, uint64_t b, ui
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// four steps, each step's operands A_STEP and B_STEP (in descriptor units) behind the last ones'
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void tcx_mma4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 q, %4, 0;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t"
+      "add.s64 x, %1, %5;\n\tadd.s64 y, %2, %6;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t"
+      "add.s64 x, %1, %7;\n\tadd.s64 y, %2, %8;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t"
+      "add.s64 x, %1, %9;\n\tadd.s64 y, %2, %10;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP), "n"(2 * A_STEP), "n"(2 * B_STEP), "n"(3 * A_STEP), "n"(3 * B_STEP)
+      : "memory");
+}
+template <int B_STEP>
+__device__ __forceinline__ void tcx_mma4_t(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b32 x;\n\t.reg .b64 y;\n\tsetp.ne.b32 q, %4, 0;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t"
+      "add.s32 x, %1, 8;\n\tadd.s64 y, %2, %5;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, p;\n\t"
+      "add.s32 x, %1, 16;\n\tadd.s64 y, %2, %6;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, p;\n\t"
+      "add.s32 x, %1, 24;\n\tadd.s64 y, %2, %7;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(B_STEP), "n"(2 * B_STEP), "n"(3 * B_STEP)
+      : "memory");
+}
 constexpr uint32_t kTcxTile = 128 * 128;      // bytes of 128 rows of 64 columns
-// D (128 x 128) = A B^T over 16 `steps` columns, both operands K-major tiles of 128 rows
-__device__ __forceinline__ void tcx_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
-  const uint64_t da = tcx_desc(a, 0), db = tcx_desc(b, 0);
+// D (128 x ROWS) (+)= A B^T over NC blocks of 64 columns, both operands K-major tiles: A of A_ROWS rows, B of ROWS.  (Zeros behind
+// the values: straight-line code for every width.)
+template <int NC, int A_ROWS, int ROWS>
+__device__ __forceinline__ void tcx_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate = 0) {
 #pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    if (s >= steps) break;
-    const uint64_t at = (uint64_t)(((s / 4) * kTcxTile + (s % 4) * 32) >> 4);
-    tcx_mma(d, da + at, db + at, idesc, s > 0);
-  }
+  for (int k = 0; k < NC; ++k)
+    tcx_mma4<2, 2>(d, tcx_desc(a, 0) + (uint64_t)(k * A_ROWS * 128 >> 4), tcx_desc(b, 0) + (uint64_t)(k * ROWS * 128 >> 4), idesc, accumulate | (uint32_t)k);
 }
-// D (128 x n) += A B over 16 STEPS rows of B, A in tensor memory (its second 64 columns `half` behind the first), B rows of n
-// columns (MN-major) of a tile of 128
-template <int STEPS = 8>
-__device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t half = 32) {
-  const uint64_t db = tcx_desc(b, kTcxTile);
+// the same with A in tensor memory
+template <int NC, int ROWS>
+__device__ __forceinline__ void tcx_scores_t(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-    tcx_mma_t(d, a + (s / 4) * half + (s % 4) * 8, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
+  for (int k = 0; k < NC; ++k) tcx_mma4_t<2>(d, a + 32 * k, tcx_desc(b, 0) + (uint64_t)(k * ROWS * 128 >> 4), idesc, (uint32_t)k);
 }
-
-// the same, A of 128 rows against B of ROWS (D 128 x ROWS)
-template <int ROWS>
-__device__ __forceinline__ void tcx_scores_of(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
-  const uint64_t da = tcx_desc(a, 0), db = tcx_desc(b, 0);
-#pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    if (s >= steps) break;
-    tcx_mma(d, da + (uint64_t)(((s / 4) * kTcxTile + (s % 4) * 32) >> 4), db + (uint64_t)(((s / 4) * (ROWS * 128) + (s % 4) * 32) >> 4), idesc, s > 0);
-  }
-}
-// and with A in tensor memory
-template <int ROWS>
-__device__ __forceinline__ void tcx_scores_t(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
-  const uint64_t db = tcx_desc(b, 0);
-#pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    if (s >= steps) break;
-    tcx_mma_t(d, a + 8 * s, db + (uint64_t)(((s / 4) * (ROWS * 128) + (s % 4) * 32) >> 4), idesc, s > 0);
-  }
-}
-// D (128 x n) += A B, A 128 x ROWS in tensor memory, B a tile of ROWS rows (MN-major)
-template <int ROWS>
-__device__ __forceinline__ void tcx_combine_of(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+// D (128 x n) (+)= A B over K rows of B: A 128 x K in tensor memory, B K rows (from `b` on) of a tile of ROWS rows, MN-major
+template <int K, int ROWS>
+__device__ __forceinline__ void tcx_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
   const uint64_t db = tcx_desc(b, ROWS * 128);
 #pragma unroll
-  for (int s = 0; s < ROWS / 16; ++s) tcx_mma_t(d, a + 8 * s, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
+  for (int s = 0; s < K / 16; s += 4) {
+    if constexpr (K % 64 == 0) {
+      tcx_mma4_t<(2048 >> 4)>(d, a + 8 * s, db + (uint64_t)(s * 2048 >> 4), idesc, accumulate || s > 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < K / 16; ++e) tcx_mma_t(d, a + 8 * e, db + (uint64_t)(e * 2048 >> 4), idesc, accumulate || e > 0);
+    }
+  }
 }
 
 // 32 columns of a lane's row; the values are there after tcx_ld_wait
@@ -208,7 +230,7 @@ __device__ __forceinline__ void tcx_put_operand(uint32_t taddr, const bf16* row,
 __device__ __forceinline__ void tcx_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // rows [r0, r0 + ROWS) of one head into a swizzled tile, by N threads of which this is number t: `chunks` pieces of a row of
-// values, zeros beyond them up to a whole step of 16 columns and in rows from `end` on.  A thread has the same piece of every
+// values, zeros beyond them and in rows from `end` on.  A thread has the same piece of every
 // N / 8-th row, so that a copy costs it an addition and a comparison: one warp keeps up with the tensor core.
 template <int NC, int N, int ROWS = 128>
 __device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, long row_stride, int r0, int end, int chunks, int t) {
@@ -217,7 +239,6 @@ __device__ __forceinline__ void tcx_load_rows(uint32_t dst, const bf16* src, lon
 #pragma unroll
   for (int b = 0; b < NC; ++b) {
     const int cc = 8 * b + c;
-    if (cc >= (chunks + 1) / 2 * 2) break;
     const bool in = cc < chunks;
     const bf16* from = src + (long)(r0 + r) * row_stride + 8 * cc;
     const uint32_t to = dst + b * (ROWS * 128) + r * 128;

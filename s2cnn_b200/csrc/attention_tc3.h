@@ -62,29 +62,18 @@ struct AttnPack {
 // the six partial products, smallest first
 __device__ __forceinline__ int tc3_left(int k) { return k == 0 ? 0 : k == 1 ? 2 : k == 2 ? 1 : k == 3 ? 0 : k == 4 ? 1 : 0; }
 __device__ __forceinline__ int tc3_right(int k) { return k == 0 ? 2 : k == 1 ? 0 : k == 2 ? 1 : k == 3 ? 1 : k == 4 ? 0 : 0; }
-// D = A B^T over 16 `steps` columns: tiles of A_ROWS and B_ROWS rows, NC blocks of 64 columns, three parts of each
+// D = A B^T: tiles of A_ROWS and B_ROWS rows, NC blocks of 64 columns, three parts of each
 template <int NC, int A_ROWS, int B_ROWS>
-__device__ __forceinline__ void tc3_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+__device__ __forceinline__ void tc3_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
 #pragma unroll
-  for (int k = 0; k < 6; ++k) {
-    const uint64_t da = tcx_desc(a + tc3_left(k) * NC * A_ROWS * 128, 0), db = tcx_desc(b + tc3_right(k) * NC * B_ROWS * 128, 0);
-#pragma unroll
-    for (int s = 0; s < 4 * NC; ++s) {
-      if (s >= steps) break;
-      tcx_mma(d, da + (uint64_t)(((s / 4) * (A_ROWS * 128) + (s % 4) * 32) >> 4), db + (uint64_t)(((s / 4) * (B_ROWS * 128) + (s % 4) * 32) >> 4), idesc,
-              k > 0 || s > 0);
-    }
-  }
+  for (int k = 0; k < 6; ++k)
+    tcx_scores<NC, A_ROWS, B_ROWS>(d, a + tc3_left(k) * NC * A_ROWS * 128, b + tc3_right(k) * NC * B_ROWS * 128, idesc, k > 0);
 }
 // D = A B: A in tensor memory, 128 x K, its parts K / 2 columns apart; B: K rows (from `b` on) of a tile of B_ROWS rows, MN-major
 template <int NC, int K, int B_ROWS>
 __device__ __forceinline__ void tc3_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
 #pragma unroll
-  for (int k = 0; k < 6; ++k) {
-    const uint64_t db = tcx_desc(b + tc3_right(k) * NC * B_ROWS * 128, B_ROWS * 128);
-#pragma unroll
-    for (int s = 0; s < K / 16; ++s) tcx_mma_t(d, a + tc3_left(k) * (K / 2) + 8 * s, db + (uint64_t)(s * 2048 >> 4), idesc, k > 0 || s > 0);
-  }
+  for (int k = 0; k < 6; ++k) tcx_combine<K, B_ROWS>(d, a + tc3_left(k) * (K / 2), b + tc3_right(k) * NC * B_ROWS * 128, idesc, k > 0);
 }
 template <int NC, int N, int ROWS>
 __device__ __forceinline__ void tc3_load(uint32_t dst, const bf16* src, long part, long row_stride, int r0, int end, int chunks, int t) {
@@ -199,7 +188,7 @@ struct AttnTc3Forward {
           auto scores = [&](int j) {
             if (!(ok = tcx_wait(&bars->k_full[j % KS], (j / KS) & 1))) return;
             tcx_seen();
-            tc3_scores<NC, 128, KT>(t_s, q_at, k_at + (j % KS) * kK, is, steps);
+            tc3_scores<NC, 128, KT>(t_s, q_at, k_at + (j % KS) * kK, is);
             tcx_commit(&bars->s_full);
             tcx_commit(&bars->k_empty[j % KS]);
           };
@@ -437,13 +426,13 @@ struct AttnTc3GradQ {
           auto scores = [&](int j) {
             if (!(ok = tcx_wait(&bars->k_full[j % 3], (j / 3) & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, KT>(t_s + KT * (j & 1), q_at, k_at + (j % 3) * kK, is, steps);
+            tc3_scores<1, 128, KT>(t_s + KT * (j & 1), q_at, k_at + (j % 3) * kK, is);
             tcx_commit(&bars->s_full[j & 1]);
           };
           auto products = [&](int j) {
             if (!(ok = tcx_wait(&bars->v_full, j & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, KT>(t_dp, g_at, v_at, is, steps);
+            tc3_scores<1, 128, KT>(t_dp, g_at, v_at, is);
             tcx_commit(&bars->dp_full);
             tcx_commit(&bars->v_empty);
           };
@@ -718,13 +707,13 @@ struct AttnTc3GradKV {
           auto scores = [&](int t) {
             if (!(ok = tcx_wait(&bars->q_full[t & 1], (t >> 1) & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, QT>(t_s, k_at, q_at + (t & 1) * kQ, is, steps);
+            tc3_scores<1, 128, QT>(t_s, k_at, q_at + (t & 1) * kQ, is);
             tcx_commit(&bars->s_full);
           };
           auto products = [&](int t) {
             if (!(ok = tcx_wait(&bars->g_full[t & 1], (t >> 1) & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, QT>(t_dp, v_at, g_at + (t & 1) * kQ, is, steps);
+            tc3_scores<1, 128, QT>(t_dp, v_at, g_at + (t & 1) * kQ, is);
             tcx_commit(&bars->dp_full);
           };
           ok = tcx_wait(&bars->in_full, 0);

@@ -27,8 +27,9 @@ __device__ __forceinline__ void tcb_sync_group(int group) { asm volatile("bar.sy
 // ---- gradient of the queries -----------------------------------------------------------------------------------------------
 // A block has 128 queries of one head (thread = query = tensor-memory lane) and walks over the keys.  Queries and dO lie in
 // tensor memory as left operands for the whole time: S = Q K^T, dP = dO V^T, dQ += dS K with dS = P (dP - delta) written over dP.
-// The next scores of a group are computed as soon as it has read the last ones.  Warp 8 issues the products, warps 9 and 10
-// load keys and values.
+// The next scores of a group are computed as soon as it has read the last ones.  Warp 8 issues the scores, warp 11 dP and dQ
+// (issuing one step with its waits takes a thread some 1500 clocks, as long as two groups take for two tiles), warps 9 and 10 load
+// keys and values.
 // The bias gradient: a tile that lies beyond the reach adds to one bucket, a sum per thread.  In the others each warp adds its 32 x 64
 // values along the diagonals: a running sum moves one lane up with every column, so that it follows its diagonal; four runs
 // of 16 columns side by side cover the latency of the exchange.  The sums of a group's four warps meet in shared memory, where
@@ -76,7 +77,7 @@ struct AttnTcGradQ {
         tcx_init(&bars->v_full[i], 32);
         tcx_init(&bars->v_empty[i], 1);
       }
-      tcx_init(&bars->drained, 1);
+      tcx_init(&bars->drained, 2);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const AttnSeq s = attn_seq(p, b);
@@ -101,41 +102,42 @@ struct AttnTcGradQ {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8) {
-        if (n && tcx_elect()) {                                              // one thread issues all: a warp's votes cost it 100 clocks a wait
+      if (warp == 8 || warp == 11) {
+        if (n && tcx_elect()) {
           const int steps = (pp.chunks + 1) / 2;
           const uint32_t is = tcx_idesc(kTcbTile, false), io = tcx_idesc(16 * steps, true);
-          auto scores = [&](int j) {
-            if (!(ok = tcx_wait(&bars->k_full[j % KS], (j / KS) & 1))) return;
-            tcx_seen();
-            tcx_scores_t<kTcbTile>(t_s + kTcbTile * (j & 1), t_q, k_at + (j % KS) * kRows, is, steps);
-            tcx_commit(&bars->s_full[j & 1]);
-          };
-          auto products = [&](int j) {                                         // dP
-            if (!(ok = tcx_wait(&bars->v_full[j % VS], (j / VS) & 1))) return;
-            tcx_seen();
-            tcx_scores_t<kTcbTile>(t_dp + kTcbTile * (j & 1), t_g, v_at + (j % VS) * kRows, is, steps);
-            tcx_commit(&bars->dp_full[j & 1]);
-            tcx_commit(&bars->v_empty[j % VS]);
-          };
           ok = tcx_wait(&bars->in_full, 0);
           tcx_after_sync();
-          for (int j = 0; j < 2 && j < n && ok; ++j) {
-            scores(j);
-            if (ok) products(j);
-          }
-          for (int j = 0; j < n && ok; ++j) {
-            const uint32_t par = (j >> 1) & 1;
-            if (j + 2 < n) {
-              if (!(ok = tcx_wait(&bars->s_read[j & 1], par))) break;
+          if (warp == 8) {                                                   // the scores
+            TcxRing<KS> k;
+            for (int j = 0; j < n && ok; ++j, k.next()) {
+              if (j >= 2 && !(ok = tcx_wait(&bars->s_read[j & 1], ((j >> 1) - 1) & 1))) break;
+              if (!(ok = tcx_wait(&bars->k_full[k.at], k.parity))) break;
               tcx_after_sync();
-              scores(j + 2);
+              tcx_seen();
+              tcx_scores_t<NC, kTcbTile>(t_s + kTcbTile * (j & 1), t_q, k_at + k.at * kRows, is);
+              tcx_commit(&bars->s_full[j & 1]);
             }
-            if (!ok || !(ok = tcx_wait(&bars->ds_full[j & 1], par))) break;
-            tcx_after_sync();
-            tcx_combine_of<kTcbTile>(t_dq, t_dp + kTcbTile * (j & 1), k_at + (j % KS) * kRows, io, j > 0);
-            tcx_commit(&bars->k_empty[j % KS]);
-            if (j + 2 < n) products(j + 2);                                    // in order behind the product that reads these columns
+          } else {                                                           // dP, and the gradient
+            TcxRing<KS> k;
+            TcxRing<VS> v;
+            for (int j = -2; j < n && ok; ++j) {
+              if (j >= 0) {
+                if (!(ok = tcx_wait(&bars->ds_full[j & 1], (j >> 1) & 1))) break;
+                tcx_after_sync();
+                tcx_combine<kTcbTile, kTcbTile>(t_dq, t_dp + kTcbTile * (j & 1), k_at + k.at * kRows, io, j > 0);
+                tcx_commit(&bars->k_empty[k.at]);
+                k.next();
+              }
+              if (j + 2 < n) {                                               // in order behind the product that reads these columns
+                if (!(ok = tcx_wait(&bars->v_full[v.at], v.parity))) break;
+                tcx_seen();
+                tcx_scores_t<NC, kTcbTile>(t_dp + kTcbTile * (j & 1), t_g, v_at + v.at * kRows, is);
+                tcx_commit(&bars->dp_full[j & 1]);
+                tcx_commit(&bars->v_empty[v.at]);
+                v.next();
+              }
+            }
           }
           tcx_commit(&bars->drained);
           tcx_wait(&bars->drained, 0);
@@ -377,26 +379,26 @@ struct AttnTcGradQ {
 // A block has 128 keys of one of their heads and walks over the queries of all heads that share it.  The scores are computed
 // transposed (thread = key), so that weights and score gradients are left operands again: dV += P^T dO, dK += dS^T Q.  P^T goes
 // over the scores, dS^T over dP^T; the next scores of a group are computed while it works on dS^T, the next dP^T while it works on
-// P^T.  Warps 9 and 10 load queries and dO, warp 11 the rows' statistics.
+// P^T.  Warp 8 issues scores and dV, warp 11 dP^T and dK, warps 9 and 10 load queries and dO.
 struct TcbKvBars {
-  uint64_t in_full, s_full[2], dp_full[2], p_full[2], ds_full[2], q_full[4], q_empty[4], g_full[4], g_empty[4], r_full[4], r_empty[4], drained;
+  uint64_t in_full, s_full[2], dp_full[2], p_full[2], ds_full[2], q_full[4], q_empty[4], g_full[4], g_empty[4], drained;
   uint32_t tmem;
 };
 
 template <int NC>
 struct AttnTcGradKV {
-  static constexpr int kThreads = kTcbThreads, QS = 4;                       // tiles of queries, of dO and of statistics in turn
+  static constexpr int kThreads = kTcbThreads, QS = 4;                       // tiles of queries and of dO in turn
   static constexpr uint32_t kKeys = NC * kTcxTile, kRows = NC * kTcbTile * 128;
   static size_t smem(int reach) {
-    return 1024 + 2 * (size_t)kKeys + 2 * QS * (size_t)kRows + (QS * 3 * kTcbTile + 2 * (2 * reach + 2 * kTcxMargin + 1)) * sizeof(float) + sizeof(TcbKvBars) + 16;
+    return 1024 + 2 * (size_t)kKeys + 2 * QS * (size_t)kRows + (2 * 2 * 3 * kTcbTile + 2 * (2 * reach + 2 * kTcxMargin + 1)) * sizeof(float) + sizeof(TcbKvBars) + 16;
   }
   static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) {
     const AttnParams& p = pp.a;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t base = (tcx_addr(dyn) + 1023u) & ~1023u;
     unsigned char* const smem = reinterpret_cast<unsigned char*>(dyn) + (base - tcx_addr(dyn));
-    float* const stat = reinterpret_cast<float*>(smem + 2 * (size_t)kKeys + 2 * QS * (size_t)kRows);      // [QS][3][64]: -m, 1 / l, -delta
-    float* const tabs = stat + QS * 3 * kTcbTile;                            // the bias of its head, for either group
+    float* const stat = reinterpret_cast<float*>(smem + 2 * (size_t)kKeys + 2 * QS * (size_t)kRows);      // [group][turn][3][64]: -m, 1 / l, -delta
+    float* const tabs = stat + 2 * 2 * 3 * kTcbTile;                            // the bias of its head, for either group
     TcbKvBars* const bars = reinterpret_cast<TcbKvBars*>((reinterpret_cast<uintptr_t>(tabs + 2 * tcx_tab_floats(p.reach)) + 15) & ~(uintptr_t)15);
     const uint32_t k_at = base, v_at = base + kKeys, q_at = base + 2 * kKeys, g_at = q_at + QS * kRows;
     const int heads_all = p.batch * p.kv_heads;                              // under `causal` the first keys have the most queries
@@ -413,11 +415,9 @@ struct AttnTcGradKV {
         tcx_init(&bars->q_full[i], 32);
         tcx_init(&bars->q_empty[i], 1);
         tcx_init(&bars->g_full[i], 32);
-        tcx_init(&bars->g_empty[i], 1);
-        tcx_init(&bars->r_full[i], 1);
-        tcx_init(&bars->r_empty[i], 4);
+        tcx_init(&bars->g_empty[i], 2);
       }
-      tcx_init(&bars->drained, 1);
+      tcx_init(&bars->drained, 2);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const AttnSeq s = attn_seq(p, b);
@@ -438,39 +438,51 @@ struct AttnTcGradKV {
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 8) {
-        if (n && tcx_elect()) {                                              // one thread issues all: a warp's votes cost it 100 clocks a wait
+      if (warp == 8 || warp == 11) {
+        if (n && tcx_elect()) {
           const int steps = (pp.chunks + 1) / 2;
           const uint32_t is = tcx_idesc(kTcbTile, false), io = tcx_idesc(16 * steps, true);
-          auto scores = [&](int t) {
-            if (!(ok = tcx_wait(&bars->q_full[t % QS], (t / QS) & 1))) return;
-            tcx_seen();
-            tcx_scores_of<kTcbTile>(t_s + kTcbTile * (t & 1), k_at, q_at + (t % QS) * kRows, is, steps);
-            tcx_commit(&bars->s_full[t & 1]);
-          };
-          auto products = [&](int t) {
-            if (!(ok = tcx_wait(&bars->g_full[t % QS], (t / QS) & 1))) return;
-            tcx_seen();
-            tcx_scores_of<kTcbTile>(t_dp + kTcbTile * (t & 1), v_at, g_at + (t % QS) * kRows, is, steps);
-            tcx_commit(&bars->dp_full[t & 1]);
-          };
           ok = tcx_wait(&bars->in_full, 0);
-          for (int t = 0; t < 2 && t < n && ok; ++t) {
-            scores(t);
-            if (ok) products(t);
-          }
-          for (int t = 0; t < n && ok; ++t) {
-            const uint32_t par = (t >> 1) & 1;
-            if (!(ok = tcx_wait(&bars->p_full[t & 1], par))) break;
-            tcx_after_sync();
-            tcx_combine_of<kTcbTile>(t_dv, t_s + kTcbTile * (t & 1), g_at + (t % QS) * kRows, io, t > 0);
-            tcx_commit(&bars->g_empty[t % QS]);                              // (dP^T of this tile is older)
-            if (t + 2 < n) scores(t + 2);
-            if (!ok || !(ok = tcx_wait(&bars->ds_full[t & 1], par))) break;
-            tcx_after_sync();
-            tcx_combine_of<kTcbTile>(t_dk, t_dp + kTcbTile * (t & 1), q_at + (t % QS) * kRows, io, t > 0);
-            tcx_commit(&bars->q_empty[t % QS]);
-            if (t + 2 < n) products(t + 2);
+          TcxRing<QS> in, out;
+          if (warp == 8) {                                                   // the scores, and the gradient of the values
+            for (int t = -2; t < n && ok; ++t) {
+              if (t >= 0) {
+                if (!(ok = tcx_wait(&bars->p_full[t & 1], (t >> 1) & 1))) break;
+                if (!(ok = tcx_wait(&bars->g_full[out.at], out.parity))) break;
+                tcx_after_sync();
+                tcx_seen();
+                tcx_combine<kTcbTile, kTcbTile>(t_dv, t_s + kTcbTile * (t & 1), g_at + out.at * kRows, io, t > 0);
+                tcx_commit(&bars->g_empty[out.at]);
+                out.next();
+              }
+              if (t + 2 < n) {
+                if (!(ok = tcx_wait(&bars->q_full[in.at], in.parity))) break;
+                tcx_seen();
+                tcx_scores<NC, 128, kTcbTile>(t_s + kTcbTile * (t & 1), k_at, q_at + in.at * kRows, is);
+                tcx_commit(&bars->s_full[t & 1]);
+                in.next();
+              }
+            }
+          } else {                                                           // dP^T, and the gradient of the keys
+            for (int t = -2; t < n && ok; ++t) {
+              if (t >= 0) {
+                if (!(ok = tcx_wait(&bars->ds_full[t & 1], (t >> 1) & 1))) break;
+                if (!(ok = tcx_wait(&bars->q_full[out.at], out.parity))) break;
+                tcx_after_sync();
+                tcx_seen();
+                tcx_combine<kTcbTile, kTcbTile>(t_dk, t_dp + kTcbTile * (t & 1), q_at + out.at * kRows, io, t > 0);
+                tcx_commit(&bars->q_empty[out.at]);                          // (the scores of this tile are older)
+                out.next();
+              }
+              if (t + 2 < n) {
+                if (!(ok = tcx_wait(&bars->g_full[in.at], in.parity))) break;
+                tcx_seen();
+                tcx_scores<NC, 128, kTcbTile>(t_dp + kTcbTile * (t & 1), v_at, g_at + in.at * kRows, is);
+                tcx_commit(&bars->dp_full[t & 1]);
+                tcx_commit(&bars->g_empty[in.at]);
+                in.next();
+              }
+            }
           }
           tcx_commit(&bars->drained);
           tcx_wait(&bars->drained, 0);
@@ -491,25 +503,6 @@ struct AttnTcGradKV {
           if (++it == first + per_head) { it = first; ++g; }
         }
         tcx_copies_done();
-      } else if (warp == 11) {
-        int g = 0, it = first;
-        for (int t = 0; t < n && ok; ++t) {
-          if (t >= QS) ok = tcx_wait_warp(&bars->r_empty[t % QS], (t / QS - 1) & 1);
-          if (!ok) break;
-          const long row0 = ((long)b * p.heads + hk * p.group + g) * p.lq;
-          float* to = stat + (t % QS) * 3 * kTcbTile;
-#pragma unroll
-          for (int e = lane; e < kTcbTile; e += 32) {
-            const int i = kTcbTile * it + e;
-            const float2 st = i < s.qlen ? p.stats[row0 + i] : make_float2(INFINITY, 0.f);
-            to[e] = -st.x;
-            to[kTcbTile + e] = st.y;
-            to[2 * kTcbTile + e] = i < s.qlen ? -p.delta[row0 + i] : 0.f;
-          }
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->r_full[t % QS]);
-          if (++it == first + per_head) { it = first; ++g; }
-        }
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -525,6 +518,16 @@ struct AttnTcGradKV {
       const float scale = p.scale * kLog2e;
       float* const tab = tabs + group * tcx_tab_floats(p.reach);
       int head = -1;
+      float2 ahead = make_float2(INFINITY, 0.f);
+      float ahead_delta = 0.f;
+      auto fetch = [&](int t) {
+        if ((tid & 127) >= kTcbTile || t >= n) return;
+        const int g = t / per_head, i = kTcbTile * (first + t - g * per_head) + (tid & 63);
+        const long at = ((long)b * p.heads + hk * p.group + g) * p.lq + i;
+        ahead = i < s.qlen ? p.stats[at] : make_float2(INFINITY, 0.f);
+        ahead_delta = i < s.qlen ? p.delta[at] : 0.f;
+      };
+      fetch(group);
       for (int t = group; t < n; t += 2) {
         const uint32_t par = (t >> 1) & 1;
         const int g = t / per_head, it = first + t - g * per_head;
@@ -535,8 +538,15 @@ struct AttnTcGradKV {
           tcb_sync_group(group);
         }
         const int i0 = kTcbTile * it, d0 = j0 - i0 - s.start;
-        const float* sm = stat + (t % QS) * 3 * kTcbTile;                    // -m, 1 / l, -delta of the tile's queries
-        if (ok) ok = tcx_wait_warp(&bars->r_full[t % QS], (t / QS) & 1);
+        // -m, 1 / l, -delta of the tile's queries, fetched a tile ahead, by one thread each
+        float* const sm = stat + (2 * group + (int)par) * 3 * kTcbTile;
+        if ((tid & 127) < kTcbTile) {
+          sm[tid & 63] = -ahead.x;
+          sm[kTcbTile + (tid & 63)] = ahead.y;
+          sm[2 * kTcbTile + (tid & 63)] = -ahead_delta;
+        }
+        fetch(t + 2);
+        tcb_sync_group(group);
         if (ok) ok = tcx_wait_warp(&bars->s_full[group], par);
         tcx_after_sync();
         uint32_t raw[64];
@@ -619,10 +629,7 @@ struct AttnTcGradKV {
         tcx_st_wait();
         tcx_before_sync();
         __syncwarp();
-        if (lane == 0) {
-          tcx_arrive(&bars->ds_full[group]);
-          tcx_arrive(&bars->r_empty[t % QS]);
-        }
+        if (lane == 0) tcx_arrive(&bars->ds_full[group]);
       }
       // ---- rows of dV (warps 0 - 3) and dK (warps 4 - 7)
       if (ok && n) ok = tcx_wait_warp(&bars->drained, 0);

@@ -110,7 +110,7 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
       if (ok && n_all) {
         for (int u = 0; u < 2; ++u)
           if (n[u]) {
-            tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at, is, steps);
+            tcx_scores<NC, 128, 128>(t_scores + 128 * u, q_at + u * kRows, k_at, is);
             tcx_commit(&bars->s_full[u]);
           }
         tcx_commit(&bars->k_empty[0]);
@@ -129,8 +129,8 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
             if (!ok) break;
             tcx_after_sync();
             const uint32_t w = t_scores + 128 * u + 32 * half, v = v_at + sv * kRows + 64 * 128 * half;
-            if (FINE) tcx_combine<4>(t_out + 128 * u, w + 64, v, io, j > 0 || half);
-            tcx_combine<4>(t_out + 128 * u, w, v, io, FINE || j > 0 || half);
+            if (FINE) tcx_combine<64, 128>(t_out + 128 * u, w + 64, v, io, j > 0 || half);
+            tcx_combine<64, 128>(t_out + 128 * u, w, v, io, FINE || j > 0 || half);
             if (half) tcx_commit(&bars->pv_done[u]);
           }
           if (ok && j + 1 < n[u]) {
@@ -140,7 +140,7 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
             }
             if (!ok) break;
             // in order behind the product that reads the weights from the same columns
-            tcx_scores(t_scores + 128 * u, q_at + u * kRows, k_at + sk * kRows, is, steps);
+            tcx_scores<NC, 128, 128>(t_scores + 128 * u, q_at + u * kRows, k_at + sk * kRows, is);
             tcx_commit(&bars->s_full[u]);
           }
         }
