@@ -160,9 +160,9 @@ __device__ __forceinline__ void tcx_scores(uint32_t d, uint32_t a, uint32_t b, u
 }
 // the same with A in tensor memory
 template <int NC, int ROWS>
-__device__ __forceinline__ void tcx_scores_t(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void tcx_scores_t(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate = 0) {
 #pragma unroll
-  for (int k = 0; k < NC; ++k) tcx_mma4_t<2>(d, a + 32 * k, tcx_desc(b, 0) + (uint64_t)(k * ROWS * 128 >> 4), idesc, (uint32_t)k);
+  for (int k = 0; k < NC; ++k) tcx_mma4_t<2>(d, a + 32 * k, tcx_desc(b, 0) + (uint64_t)(k * ROWS * 128 >> 4), idesc, accumulate | (uint32_t)k);
 }
 // D (128 x n) (+)= A B over K rows of B: A 128 x K in tensor memory, B K rows (from `b` on) of a tile of ROWS rows, MN-major
 template <int K, int ROWS>

@@ -69,6 +69,12 @@ __device__ __forceinline__ void tc3_scores(uint32_t d, uint32_t a, uint32_t b, u
   for (int k = 0; k < 6; ++k)
     tcx_scores<NC, A_ROWS, B_ROWS>(d, a + tc3_left(k) * NC * A_ROWS * 128, b + tc3_right(k) * NC * B_ROWS * 128, idesc, k > 0);
 }
+// the same with the parts of A side by side in tensor memory
+template <int NC, int B_ROWS>
+__device__ __forceinline__ void tc3_scores_t(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int k = 0; k < 6; ++k) tcx_scores_t<NC, B_ROWS>(d, a + tc3_left(k) * 32 * NC, b + tc3_right(k) * NC * B_ROWS * 128, idesc, k > 0);
+}
 // D = A B: A in tensor memory, 128 x K, its parts K / 2 columns apart; B: K rows (from `b` on) of a tile of B_ROWS rows, MN-major
 template <int NC, int K, int B_ROWS>
 __device__ __forceinline__ void tc3_combine(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
@@ -356,19 +362,23 @@ struct AttnTc3Forward {
   }
 };
 
-// ---- gradient of the queries, heads of at most 64 values -----------------------------------------------------------------------
+// ---- gradient of the queries -----------------------------------------------------------------------------------------------------
 // As AttnTcGradQ, with key tiles of 64: warps 0 - 3 take the first 32 keys of a tile, warps 4 - 7 the others; the gradient of a
 // tile's keys is added to registers, half of its columns per group.
+// Heads of more than 64 values (NC = 2): the parts of queries and dO do not fit in shared memory beside those of keys and values.
+// The queries lie in tensor memory, dS goes over the scores, and there is one tile each of keys and values: a tile is then
+// finished before the next one's scores begin.
 constexpr int kTc3Diag = 2 * 48;
 struct Tc3QBars {
   uint64_t in_full, s_full[2], dp_full, ds_full, dq_done, k_full[3], k_empty[3], v_full, v_empty, drained;
   uint32_t tmem;
 };
+template <int NC>
 struct AttnTc3GradQ {
-  static constexpr int kThreads = kTc3Threads, KT = 64, HALF = 32;
-  static constexpr uint32_t kQ = 3 * 128 * 128, kK = 3 * KT * 128;
+  static constexpr int kThreads = kTc3Threads, KT = 64, HALF = 32, KS = NC == 1 ? 3 : 1;
+  static constexpr uint32_t kQ = 3 * NC * 128 * 128, kK = 3 * NC * KT * 128, kTiles = (NC == 1 ? 2 : 1) * kQ + (KS + 1) * kK;
   static size_t smem(int reach, bool bias_grad) {
-    return 1024 + 2 * kQ + 4 * (size_t)kK + (2 * reach + 2 * kTcxMargin + 1 + 512 + (bias_grad ? 2 * 8 * kTc3Diag + 2 * reach + 1 : 0)) * sizeof(float) +
+    return 1024 + (size_t)kTiles + (2 * reach + 2 * kTcxMargin + 1 + 512 + (bias_grad ? 2 * 8 * kTc3Diag + 2 * reach + 1 : 0)) * sizeof(float) +
            sizeof(Tc3QBars) + 16;
   }
   static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) {
@@ -376,12 +386,12 @@ struct AttnTc3GradQ {
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t base = (tcx_addr(dyn) + 1023u) & ~1023u;
     unsigned char* const smem = reinterpret_cast<unsigned char*>(dyn) + (base - tcx_addr(dyn));
-    float* const red = reinterpret_cast<float*>(smem + 2 * kQ + 4 * kK);   // [512]
+    float* const red = reinterpret_cast<float*>(smem + kTiles);   // [512]
     float* const tab = red + 512;
     float* const diag = tab + tcx_tab_floats(p.reach);                     // [2][8][kTc3Diag], then a slot per relative position
     float* const slot = diag + (p.dbias_part ? 2 * 8 * kTc3Diag : 0);
     Tc3QBars* const bars = reinterpret_cast<Tc3QBars*>((reinterpret_cast<uintptr_t>(slot + (p.dbias_part ? 2 * p.reach + 1 : 0)) + 15) & ~(uintptr_t)15);
-    const uint32_t q_at = base, g_at = base + kQ, k_at = base + 2 * kQ, v_at = k_at + 3 * kK;
+    const uint32_t g_at = base, k_at = base + kQ, v_at = k_at + KS * kK, q_at = v_at + kK;           // (q: NC = 1)
     const int heads_all = p.batch * p.heads;
     const int tile = p.tiles - 1 - (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, h = bh % p.heads, b = bh / p.heads, hk = h / p.group;
     if (tid == 0) {
@@ -390,7 +400,7 @@ struct AttnTc3GradQ {
       tcx_init(&bars->dp_full, 1);
       tcx_init(&bars->ds_full, 8);
       tcx_init(&bars->dq_done, 1);
-      for (int i = 0; i < 3; ++i) {
+      for (int i = 0; i < KS; ++i) {
         tcx_init(&bars->k_full[i], 32);
         tcx_init(&bars->k_empty[i], 1);
       }
@@ -414,7 +424,10 @@ struct AttnTc3GradQ {
     tcx_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
     stream_order_next();
-    const uint32_t t_s = tmem, t_dp = tmem + 128, t_ds = tmem + 192, t_dq = tmem + 288;
+    // NC = 1: two tiles of scores, products, three parts of dS, the gradient; NC = 2: three parts of the queries, scores and dS in
+    // one place, products, the gradient
+    const uint32_t t_q = tmem, t_s = NC == 1 ? tmem : tmem + 192, t_dp = NC == 1 ? tmem + 128 : tmem + 288, t_ds = NC == 1 ? tmem + 192 : t_s,
+                   t_dq = NC == 1 ? tmem + 288 : tmem + 352;
     bool ok = true;
 
     if (warp >= 8) {
@@ -424,31 +437,37 @@ struct AttnTc3GradQ {
           const int steps = (pp.chunks + 1) / 2;
           const uint32_t is = tcx_idesc(KT, false), io = tcx_idesc(16 * steps, true);
           auto scores = [&](int j) {
-            if (!(ok = tcx_wait(&bars->k_full[j % 3], (j / 3) & 1))) return;
+            if (!(ok = tcx_wait(&bars->k_full[j % KS], (j / KS) & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, KT>(t_s + KT * (j & 1), q_at, k_at + (j % 3) * kK, is);
+            if constexpr (NC == 1) tc3_scores<1, 128, KT>(t_s + KT * (j & 1), q_at, k_at + (j % KS) * kK, is);
+            else tc3_scores_t<NC, KT>(t_s, t_q, k_at, is);
             tcx_commit(&bars->s_full[j & 1]);
           };
           auto products = [&](int j) {
             if (!(ok = tcx_wait(&bars->v_full, j & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, KT>(t_dp, g_at, v_at, is);
+            tc3_scores<NC, 128, KT>(t_dp, g_at, v_at, is);
             tcx_commit(&bars->dp_full);
             tcx_commit(&bars->v_empty);
           };
           ok = tcx_wait(&bars->in_full, 0);
+          tcx_after_sync();
           if (ok) scores(0);
           if (ok) products(0);
-          if (ok && n > 1) scores(1);
+          if (NC == 1 && ok && n > 1) scores(1);
           for (int j = 0; j < n && ok; ++j) {
             if (!(ok = tcx_wait(&bars->ds_full, j & 1))) break;
             tcx_after_sync();
-            if (j + 1 < n) products(j + 1);
+            if (NC == 1 && j + 1 < n) products(j + 1);
             if (!ok) break;
-            tc3_combine<1, KT, KT>(t_dq, t_ds, k_at + (j % 3) * kK, io);
+            tc3_combine<NC, KT, KT>(t_dq, t_ds, k_at + (j % KS) * kK, io);
             tcx_commit(&bars->dq_done);
-            tcx_commit(&bars->k_empty[j % 3]);
-            if (j + 2 < n) scores(j + 2);
+            tcx_commit(&bars->k_empty[j % KS]);
+            if (NC == 1 && j + 2 < n) scores(j + 2);
+            if (NC == 2 && j + 1 < n) {
+              scores(j + 1);
+              if (ok) products(j + 1);
+            }
           }
           tcx_commit(&bars->drained);
           tcx_wait(&bars->drained, 0);
@@ -457,10 +476,10 @@ struct AttnTc3GradQ {
       } else if (warp == 9) {
         const bf16* src = static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2];
         for (int j = 0; j < n && ok; ++j) {
-          if (j >= 3) ok = tcx_wait_warp(&bars->k_empty[j % 3], (j / 3 - 1) & 1);
+          if (j >= KS) ok = tcx_wait_warp(&bars->k_empty[j % KS], (j / KS - 1) & 1);
           if (!ok) break;
-          tc3_load<1, 32, KT>(k_at + (j % 3) * kK, src, pp.k_split, p.ks[1], KT * j, keys, pp.chunks, lane);
-          tcx_arrive_copies(&bars->k_full[j % 3]);
+          tc3_load<NC, 32, KT>(k_at + (j % KS) * kK, src, pp.k_split, p.ks[1], KT * j, keys, pp.chunks, lane);
+          tcx_arrive_copies(&bars->k_full[j % KS]);
         }
         tcx_copies_done();
       } else if (warp == 10) {
@@ -468,7 +487,7 @@ struct AttnTc3GradQ {
         for (int j = 0; j < n && ok; ++j) {
           if (j >= 1) ok = tcx_wait_warp(&bars->v_empty, (j - 1) & 1);
           if (!ok) break;
-          tc3_load<1, 32, KT>(v_at, src, pp.v_split, p.vs[1], KT * j, keys, pp.chunks, lane);
+          tc3_load<NC, 32, KT>(v_at, src, pp.v_split, p.vs[1], KT * j, keys, pp.chunks, lane);
           tcx_arrive_copies(&bars->v_full);
         }
         tcx_copies_done();
@@ -478,8 +497,20 @@ struct AttnTc3GradQ {
       const int half = warp >> 2, row = 32 * (warp & 3) + lane, i = i0 + row;
       const long at = (((long)b * p.lq + i) * p.heads + h) * p.dim;
       if (n) {
-        tc3_load<1, 256, 128>(q_at, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], pp.q_split, p.qs[1], i0, s.qlen, pp.chunks, tid);
-        tc3_load<1, 256, 128>(g_at, static_cast<const bf16*>(p.dout) + b * pp.gs[0] + h * pp.gs[2], pp.g_split, pp.gs[1], i0, s.qlen, pp.chunks, tid);
+        const bf16* const q0 = static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2];
+        if constexpr (NC == 1) {
+          tc3_load<1, 256, 128>(q_at, q0, pp.q_split, p.qs[1], i0, s.qlen, pp.chunks, tid);
+        } else {
+          const bf16* const row_at = q0 + (long)(i < s.qlen ? i : 0) * p.qs[1];
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int c = 0; c < 64; c += 32)
+              tcx_put_operand(t_q + 64 * part + ((uint32_t)(32 * (warp & 3)) << 16), row_at + part * pp.q_split, 64 * half + c, pp.chunks, i < s.qlen);
+          tcx_st_wait();
+          tcx_before_sync();
+        }
+        tc3_load<NC, 256, 128>(g_at, static_cast<const bf16*>(p.dout) + b * pp.gs[0] + h * pp.gs[2], pp.g_split, pp.gs[1], i0, s.qlen, pp.chunks, tid);
         tcx_loaded();
         tcx_arrive(&bars->in_full);
       }
@@ -496,17 +527,20 @@ struct AttnTc3GradQ {
       const float inv = st.y;
       const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
       const float scale = p.scale * kLog2e, tab_before = tab[0], tab_behind = tab[2 * p.reach + 2 * kTcxMargin];
-      float far_before = 0.f, far_behind = 0.f, acc[32];
+      float far_before = 0.f, far_behind = 0.f, acc[32 * NC];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) acc[c] = 0.f;
+      for (int c = 0; c < 32 * NC; ++c) acc[c] = 0.f;
       auto drain = [&](int j) {
         if (ok) ok = tcx_wait_warp(&bars->dq_done, j & 1);
         tcx_after_sync();
-        uint32_t o[32];
-        tcx_ld32(t_dq + 32 * half + lanes, o);
-        tcx_ld_wait(o);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) acc[e] += as_float(o[e]);
+        for (int c = 0; c < 32 * NC; c += 32) {
+          uint32_t o[32];
+          tcx_ld32(t_dq + 32 * NC * half + c + lanes, o);
+          tcx_ld_wait(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[c + e] += as_float(o[e]);
+        }
       };
       int turn = 0;
       for (int j = 0; j < n; ++j) {
@@ -515,7 +549,7 @@ struct AttnTc3GradQ {
         if (ok) ok = tcx_wait_warp(&bars->s_full[j & 1], (j >> 1) & 1);
         tcx_after_sync();
         uint32_t raw[32], grad[32];
-        tcx_ld32(t_s + KT * (j & 1) + HALF * half + lanes, raw);
+        tcx_ld32(t_s + (NC == 1 ? KT * (j & 1) : 0) + HALF * half + lanes, raw);
         tcx_ld_wait(raw);
         float* x = reinterpret_cast<float*>(raw);
         if (close) {
@@ -546,6 +580,11 @@ struct AttnTc3GradQ {
           for (int c = 0; c < 32; ++c) x[c] = c < lim ? x[c] : 0.f;
         }
         if (j > 0) drain(j - 1);                                           // (the columns of dS have been read, too)
+        if (NC == 2) {                                                     // both groups have read the scores
+          tcx_before_sync();
+          tc3_sync();
+          tcx_after_sync();
+        }
         tc3_put<32>(t_ds + 16 * half + lanes, 32, x);
         tcx_st_wait();
         tcx_before_sync();
@@ -600,8 +639,8 @@ struct AttnTc3GradQ {
       if (ok && n) ok = tcx_wait_warp(&bars->drained, 0);
       const bool wide = p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % 16 == 0;
 #pragma unroll
-      for (int c = 0; c < 32; ++c) acc[c] = ok ? acc[c] * p.scale : bulk_nan();
-      if (i < p.lq) tc3_store_row(static_cast<float*>(p.dq) + at, acc, 32, p.dim, 32 * half, wide);
+      for (int c = 0; c < 32 * NC; ++c) acc[c] = ok ? acc[c] * p.scale : bulk_nan();
+      if (i < p.lq) tc3_store_row(static_cast<float*>(p.dq) + at, acc, 32 * NC, p.dim, 32 * NC * half, wide);
       if (p.dbias_part) {
         tc3_sync();
         red[tid] = far_before;
@@ -636,29 +675,32 @@ struct AttnTc3GradQ {
   }
 };
 
-// ---- gradients of keys and values, heads of at most 64 values ------------------------------------------------------------------
+// ---- gradients of keys and values ------------------------------------------------------------------------------------------------
 // As AttnTcGradKV, with query tiles of 64; the products of a tile are added to registers, half of the columns of either gradient
 // per group.
+// NC = 2: the keys lie in tensor memory, P^T and dS^T go over scores and products, both gradients pass through the same columns one
+// after the other, and there is one tile each of queries and dO.
 struct Tc3KvBars {
   uint64_t in_full, s_full, s_read, dp_full, dp_read, p_full, ds_full, dv_done, dk_done, q_full[2], q_empty[2], g_full[2], g_empty[2], r_full[2],
       r_empty[2], drained;
   uint32_t tmem;
 };
+template <int NC>
 struct AttnTc3GradKV {
-  static constexpr int kThreads = kTc3Threads, QT = 64, HALF = 32;
-  static constexpr uint32_t kK = 3 * 128 * 128, kQ = 3 * QT * 128;
+  static constexpr int kThreads = kTc3Threads, QT = 64, HALF = 32, QS = NC == 1 ? 2 : 1;
+  static constexpr uint32_t kK = 3 * NC * 128 * 128, kQ = 3 * NC * QT * 128, kTiles = (NC == 1 ? 2 : 1) * kK + 2 * QS * kQ;
   static size_t smem(int reach) {
-    return 1024 + 2 * kK + 4 * (size_t)kQ + (2 * 3 * QT + 2 * reach + 2 * kTcxMargin + 1) * sizeof(float) + sizeof(Tc3KvBars) + 16;
+    return 1024 + (size_t)kTiles + (2 * 3 * QT + 2 * reach + 2 * kTcxMargin + 1) * sizeof(float) + sizeof(Tc3KvBars) + 16;
   }
   static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* dyn) {
     const AttnParams& p = pp.a;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t base = (tcx_addr(dyn) + 1023u) & ~1023u;
     unsigned char* const smem = reinterpret_cast<unsigned char*>(dyn) + (base - tcx_addr(dyn));
-    float* const stat = reinterpret_cast<float*>(smem + 2 * kK + 4 * kQ);             // [2][3][QT]: m, 1 / l, delta
+    float* const stat = reinterpret_cast<float*>(smem + kTiles);             // [2][3][QT]: m, 1 / l, delta
     float* const tab = stat + 2 * 3 * QT;
     Tc3KvBars* const bars = reinterpret_cast<Tc3KvBars*>((reinterpret_cast<uintptr_t>(tab + tcx_tab_floats(p.reach)) + 15) & ~(uintptr_t)15);
-    const uint32_t k_at = base, v_at = base + kK, q_at = base + 2 * kK, g_at = q_at + 2 * kQ;
+    const uint32_t v_at = base, q_at = base + kK, g_at = q_at + QS * kQ, k_at = g_at + QS * kQ;      // (k: NC = 1)
     const int heads_all = p.batch * p.kv_heads;
     const int tile = (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, hk = bh % p.kv_heads, b = bh / p.kv_heads;
     if (tid == 0) {
@@ -695,7 +737,8 @@ struct AttnTc3GradKV {
     tcx_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
     stream_order_next();
-    const uint32_t t_s = tmem, t_dp = tmem + 64, t_p = tmem + 128, t_ds = tmem + 224, t_dv = tmem + 320, t_dk = tmem + 384;
+    const uint32_t t_k = tmem, t_s = NC == 1 ? tmem : tmem + 192, t_dp = NC == 1 ? tmem + 64 : tmem + 288, t_p = NC == 1 ? tmem + 128 : t_s,
+                   t_ds = NC == 1 ? tmem + 224 : t_dp, t_dv = NC == 1 ? tmem + 320 : tmem + 384, t_dk = tmem + 384;
     bool ok = true;
 
     if (warp >= 8) {
@@ -705,41 +748,47 @@ struct AttnTc3GradKV {
           const int steps = (pp.chunks + 1) / 2;
           const uint32_t is = tcx_idesc(QT, false), io = tcx_idesc(16 * steps, true);
           auto scores = [&](int t) {
-            if (!(ok = tcx_wait(&bars->q_full[t & 1], (t >> 1) & 1))) return;
+            if (!(ok = tcx_wait(&bars->q_full[t % QS], (t / QS) & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, QT>(t_s, k_at, q_at + (t & 1) * kQ, is);
+            if constexpr (NC == 1) tc3_scores<1, 128, QT>(t_s, k_at, q_at + (t % QS) * kQ, is);
+            else tc3_scores_t<NC, QT>(t_s, t_k, q_at, is);
             tcx_commit(&bars->s_full);
           };
           auto products = [&](int t) {
-            if (!(ok = tcx_wait(&bars->g_full[t & 1], (t >> 1) & 1))) return;
+            if (!(ok = tcx_wait(&bars->g_full[t % QS], (t / QS) & 1))) return;
             tcx_seen();
-            tc3_scores<1, 128, QT>(t_dp, v_at, g_at + (t & 1) * kQ, is);
+            tc3_scores<NC, 128, QT>(t_dp, v_at, g_at + (t % QS) * kQ, is);
             tcx_commit(&bars->dp_full);
           };
           ok = tcx_wait(&bars->in_full, 0);
+          tcx_after_sync();
           if (ok) scores(0);
           if (ok) products(0);
           for (int t = 0; t < n && ok; ++t) {
-            if (t + 1 < n) {
+            if (NC == 1 && t + 1 < n) {
               if (!(ok = tcx_wait(&bars->s_read, t & 1))) break;
               tcx_after_sync();
               scores(t + 1);
             }
             if (!ok || !(ok = tcx_wait(&bars->p_full, t & 1))) break;
             tcx_after_sync();
-            tc3_combine<1, QT, QT>(t_dv, t_p, g_at + (t & 1) * kQ, io);
+            tc3_combine<NC, QT, QT>(t_dv, t_p, g_at + (t % QS) * kQ, io);
             tcx_commit(&bars->dv_done);
-            tcx_commit(&bars->g_empty[t & 1]);
-            if (t + 1 < n) {
+            tcx_commit(&bars->g_empty[t % QS]);
+            if (NC == 1 && t + 1 < n) {
               if (!(ok = tcx_wait(&bars->dp_read, t & 1))) break;
               tcx_after_sync();
               products(t + 1);
             }
             if (!ok || !(ok = tcx_wait(&bars->ds_full, t & 1))) break;
             tcx_after_sync();
-            tc3_combine<1, QT, QT>(t_dk, t_ds, q_at + (t & 1) * kQ, io);
+            tc3_combine<NC, QT, QT>(t_dk, t_ds, q_at + (t % QS) * kQ, io);
             tcx_commit(&bars->dk_done);
-            tcx_commit(&bars->q_empty[t & 1]);
+            tcx_commit(&bars->q_empty[t % QS]);
+            if (NC == 2 && t + 1 < n) {
+              scores(t + 1);
+              if (ok) products(t + 1);
+            }
           }
           tcx_commit(&bars->drained);
           tcx_wait(&bars->drained, 0);
@@ -753,10 +802,10 @@ struct AttnTc3GradKV {
         const bf16* src = static_cast<const bf16*>(is_q ? p.q : p.dout) + b * (is_q ? p.qs[0] : pp.gs[0]) + hk * p.group * by_head;
         int g = 0, it = first;
         for (int t = 0; t < n && ok; ++t) {
-          if (t >= 2) ok = tcx_wait_warp(&empty[t & 1], (t / 2 - 1) & 1);
+          if (t >= QS) ok = tcx_wait_warp(&empty[t % QS], (t / QS - 1) & 1);
           if (!ok) break;
-          tc3_load<1, 32, QT>(to + (t & 1) * kQ, src + g * by_head, part, stride, QT * it, s.qlen, pp.chunks, lane);
-          tcx_arrive_copies(&full[t & 1]);
+          tc3_load<NC, 32, QT>(to + (t % QS) * kQ, src + g * by_head, part, stride, QT * it, s.qlen, pp.chunks, lane);
+          tcx_arrive_copies(&full[t % QS]);
           if (++it == first + per_head) { it = first; ++g; }
         }
         tcx_copies_done();
@@ -784,24 +833,39 @@ struct AttnTc3GradKV {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
       const int half = warp >> 2, row = 32 * (warp & 3) + lane, j = j0 + row;
       if (n) {
-        tc3_load<1, 256, 128>(k_at, static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2], pp.k_split, p.ks[1], j0, keys, pp.chunks, tid);
-        tc3_load<1, 256, 128>(v_at, static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2], pp.v_split, p.vs[1], j0, keys, pp.chunks, tid);
+        const bf16* const k0 = static_cast<const bf16*>(p.k) + b * p.ks[0] + hk * p.ks[2];
+        if constexpr (NC == 1) {
+          tc3_load<1, 256, 128>(k_at, k0, pp.k_split, p.ks[1], j0, keys, pp.chunks, tid);
+        } else {
+          const bf16* const row_at = k0 + (long)(j < keys ? j : 0) * p.ks[1];
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int c = 0; c < 64; c += 32)
+              tcx_put_operand(t_k + 64 * part + ((uint32_t)(32 * (warp & 3)) << 16), row_at + part * pp.k_split, 64 * half + c, pp.chunks, j < keys);
+          tcx_st_wait();
+          tcx_before_sync();
+        }
+        tc3_load<NC, 256, 128>(v_at, static_cast<const bf16*>(p.v) + b * p.vs[0] + hk * p.vs[2], pp.v_split, p.vs[1], j0, keys, pp.chunks, tid);
         tcx_loaded();
         tcx_arrive(&bars->in_full);
       }
       const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
       const float scale = p.scale * kLog2e;
-      float dv[32], dk[32];
+      float dv[32 * NC], dk[32 * NC];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) dv[c] = dk[c] = 0.f;
-      auto drain = [&](uint64_t* bar, uint32_t from, int t, float (&acc)[32]) {
+      for (int c = 0; c < 32 * NC; ++c) dv[c] = dk[c] = 0.f;
+      auto drain = [&](uint64_t* bar, uint32_t from, int t, float (&acc)[32 * NC]) {
         if (ok) ok = tcx_wait_warp(bar, t & 1);
         tcx_after_sync();
-        uint32_t o[32];
-        tcx_ld32(from + 32 * half + lanes, o);
-        tcx_ld_wait(o);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) acc[e] += as_float(o[e]);
+        for (int c = 0; c < 32 * NC; c += 32) {
+          uint32_t o[32];
+          tcx_ld32(from + 32 * NC * half + c + lanes, o);
+          tcx_ld_wait(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[c + e] += as_float(o[e]);
+        }
       };
       int g = -1, it = first + per_head;
       for (int t = 0; t < n; ++t) {
@@ -847,7 +911,14 @@ struct AttnTc3GradKV {
           x[c + 2] = exp2_fast(x[c + 2] - m.z) * f.z;
           x[c + 3] = exp2_fast(x[c + 3] - m.w) * f.w;
         }
-        if (t > 0) drain(&bars->dv_done, t_dv, t - 1, dv);
+        if (NC == 1) {
+          if (t > 0) drain(&bars->dv_done, t_dv, t - 1, dv);
+        } else {
+          if (t > 0) drain(&bars->dk_done, t_dk, t - 1, dk);
+          tcx_before_sync();
+          tc3_sync();                                                      // both groups have read the scores
+          tcx_after_sync();
+        }
         tc3_put<32>(t_p + 16 * half + lanes, 32, x);
         tcx_st_wait();
         tcx_before_sync();
@@ -872,7 +943,14 @@ struct AttnTc3GradKV {
 #pragma unroll
           for (int c = 0; c < 32; ++c) x[c] = c >= low ? x[c] : 0.f;
         }
-        if (t > 0) drain(&bars->dk_done, t_dk, t - 1, dk);
+        if (NC == 1) {
+          if (t > 0) drain(&bars->dk_done, t_dk, t - 1, dk);
+        } else {
+          drain(&bars->dv_done, t_dv, t, dv);
+          tcx_before_sync();
+          tc3_sync();                                                      // both have read the products
+          tcx_after_sync();
+        }
         tc3_put<32>(t_ds + 16 * half + lanes, 32, x);
         tcx_st_wait();
         tcx_before_sync();
@@ -884,19 +962,19 @@ struct AttnTc3GradKV {
         ++it;
       }
       if (n) {
-        drain(&bars->dv_done, t_dv, n - 1, dv);
+        if (NC == 1) drain(&bars->dv_done, t_dv, n - 1, dv);
         drain(&bars->dk_done, t_dk, n - 1, dk);
         if (ok) ok = tcx_wait_warp(&bars->drained, 0);
       }
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
+      for (int c = 0; c < 32 * NC; ++c) {
         dv[c] = ok ? dv[c] : bulk_nan();
         dk[c] = ok ? dk[c] * p.scale : bulk_nan();
       }
       const long at = (((long)b * p.lk + j) * p.kv_heads + hk) * p.dim;
       if (j < p.lk) {
-        tc3_store_row(static_cast<float*>(p.dv) + at, dv, 32, p.dim, 32 * half, p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dv) % 16 == 0);
-        tc3_store_row(static_cast<float*>(p.dk) + at, dk, 32, p.dim, 32 * half, p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % 16 == 0);
+        tc3_store_row(static_cast<float*>(p.dv) + at, dv, 32 * NC, p.dim, 32 * NC * half, p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dv) % 16 == 0);
+        tc3_store_row(static_cast<float*>(p.dk) + at, dk, 32 * NC, p.dim, 32 * NC * half, p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dk) % 16 == 0);
       }
     }
     tcx_before_sync();

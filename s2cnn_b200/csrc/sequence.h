@@ -328,15 +328,13 @@ inline size_t attn_parts_bytes(const AttnParams& p, bool with_bias) {
   return with_bias ? attn_align((size_t)p.batch * tiles * p.heads * p.n_buckets * sizeof(float)) : 0;
 }
 #ifndef S2C_EMUL
-// (float32 heads of more than 64 values: the parts of queries and gradients alone would fill the shared memory)
 template <class T>
 bool attn_backward_tc(const AttnParams& p, bool with_bias) {
   const bool packed = attn_packs(p, sizeof(T));
   if (!packed && !(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout) && aligned16(p.o))) return false;
-  if (sizeof(T) == 4 && p.dim > 64) return false;
   const int nc = p.dim > 64 ? 2 : 1;
-  const size_t q = sizeof(T) == 4 ? AttnTc3GradQ::smem(p.reach, with_bias) : nc == 1 ? AttnTcGradQ<1>::smem(p.reach, with_bias) : AttnTcGradQ<2>::smem(p.reach, with_bias);
-  const size_t kv = sizeof(T) == 4 ? AttnTc3GradKV::smem(p.reach) : nc == 1 ? AttnTcGradKV<1>::smem(p.reach) : AttnTcGradKV<2>::smem(p.reach);
+  const size_t q = sizeof(T) == 4 ? (nc == 1 ? AttnTc3GradQ<1>::smem(p.reach, with_bias) : AttnTc3GradQ<2>::smem(p.reach, with_bias)) : nc == 1 ? AttnTcGradQ<1>::smem(p.reach, with_bias) : AttnTcGradQ<2>::smem(p.reach, with_bias);
+  const size_t kv = sizeof(T) == 4 ? (nc == 1 ? AttnTc3GradKV<1>::smem(p.reach) : AttnTc3GradKV<2>::smem(p.reach)) : nc == 1 ? AttnTcGradKV<1>::smem(p.reach) : AttnTcGradKV<2>::smem(p.reach);
   return attn_tc_worth(p, packed) && std::max(q, kv) <= (size_t)dev_smem_limit();
 }
 template <class T>
@@ -354,9 +352,11 @@ int attn_tc_backward_launch(AttnParams& p, char* packs, stream_t st) {
   const bool bias_grad = p.dbias_part != nullptr;
   const long q_blocks = (long)p.batch * p.heads * p.tiles, kv_tiles = (p.lk + 127) / 128, kv_blocks = (long)p.batch * p.kv_heads * kv_tiles;
   if constexpr (sizeof(T) == 4) {
-    S2C_SEQ_TRY(attn_tc_launch<AttnTc3GradQ>("attention_tc3_grad_q", q_blocks, AttnTc3GradQ::smem(p.reach, bias_grad), st, t));
+    S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTc3GradQ<1>>("attention_tc3_grad_q", q_blocks, AttnTc3GradQ<1>::smem(p.reach, bias_grad), st, t)
+                        : attn_tc_launch<AttnTc3GradQ<2>>("attention_tc3_grad_q", q_blocks, AttnTc3GradQ<2>::smem(p.reach, bias_grad), st, t));
     t.a.tiles = (int)kv_tiles;
-    return attn_tc_launch<AttnTc3GradKV>("attention_tc3_grad_kv", kv_blocks, AttnTc3GradKV::smem(p.reach), st, t);
+    return nc == 1 ? attn_tc_launch<AttnTc3GradKV<1>>("attention_tc3_grad_kv", kv_blocks, AttnTc3GradKV<1>::smem(p.reach), st, t)
+                   : attn_tc_launch<AttnTc3GradKV<2>>("attention_tc3_grad_kv", kv_blocks, AttnTc3GradKV<2>::smem(p.reach), st, t);
   } else {
     S2C_SEQ_TRY(nc == 1 ? attn_tc_launch<AttnTcGradQ<1>>("attention_tc_grad_q", q_blocks, AttnTcGradQ<1>::smem(p.reach, bias_grad), st, t)
                         : attn_tc_launch<AttnTcGradQ<2>>("attention_tc_grad_q", q_blocks, AttnTcGradQ<2>::smem(p.reach, bias_grad), st, t));
