@@ -30,29 +30,28 @@ struct AttnPack {
   using Params = AttnPackParams;
   static constexpr int kThreads = 256, kBlocks = 4;
   static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char*) {
-    for (int t = 0; t < p.tensors; ++t) {
-      const long pieces = (long)p.batch * p.len[t] * p.heads[t] * p.chunks;
-      for (long e = (long)ctx.bid * kThreads + ctx.tid; e < pieces; e += (long)ctx.nblk * kThreads) {
-        // in the order of memory of the usual [batch][position][head] input
-        const int c = (int)(e % p.chunks);
-        long r = e / p.chunks;
-        const int h = (int)(r % p.heads[t]);
-        r /= p.heads[t];
-        const int i = (int)(r % p.len[t]), b = (int)(r / p.len[t]);
-        const T* from = static_cast<const T*>(p.src[t]) + b * p.stride[t][0] + i * p.stride[t][1] + h * p.stride[t][2] + 8 * c;
-        bf16* to = p.dst[t] + (((long)b * p.heads[t] + h) * p.len[t] + i) * 8 * p.chunks + 8 * c;
-        float v[8];
+    const int t = ctx.bid % p.tensors;                                     // a block has one of the tensors
+    const long pieces = (long)p.batch * p.len[t] * p.heads[t] * p.chunks;
+    for (long e = (long)(ctx.bid / p.tensors) * kThreads + ctx.tid; e < pieces; e += (long)(ctx.nblk / p.tensors) * kThreads) {
+      // in the order of memory of the usual [batch][position][head] input
+      const int c = (int)(e % p.chunks);
+      long r = e / p.chunks;
+      const int h = (int)(r % p.heads[t]);
+      r /= p.heads[t];
+      const int i = (int)(r % p.len[t]), b = (int)(r / p.len[t]);
+      const T* from = static_cast<const T*>(p.src[t]) + b * p.stride[t][0] + i * p.stride[t][1] + h * p.stride[t][2] + 8 * c;
+      bf16* to = p.dst[t] + (((long)b * p.heads[t] + h) * p.len[t] + i) * 8 * p.chunks + 8 * c;
+      float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 8 * c + k < p.dim ? widen(from[k]) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = 8 * c + k < p.dim ? widen(from[k]) : 0.f;
 #pragma unroll
-        for (int part = 0; part < (sizeof(T) == 4 ? 3 : 1); ++part) {
-          store_vec(to + part * p.part[t], v);
+      for (int part = 0; part < (sizeof(T) == 4 ? 3 : 1); ++part) {
+        store_vec(to + part * p.part[t], v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            bf16 w;
-            narrow(&w, v[k]);
-            v[k] -= widen(w);
-          }
+        for (int k = 0; k < 8; ++k) {
+          bf16 w;
+          narrow(&w, v[k]);
+          v[k] -= widen(w);
         }
       }
     }

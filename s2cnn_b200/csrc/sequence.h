@@ -237,7 +237,7 @@ int attn_pack(AttnTcParams& t, const AttnPacked& k, char* ws, stream_t st) {
     c.heads[i] = of_q ? p.heads : p.kv_heads;
     most = std::max(most, k.part[i] / 8);
   }
-  S2C_SEQ_TRY(seq_launch<AttnPack<T>>("attention_pack", std::min<long>((most + 255) / 256, 8L * dev_sm_count()), 0, st, c));
+  S2C_SEQ_TRY(seq_launch<AttnPack<T>>("attention_pack", k.tensors * std::min<long>((most + 255) / 256, 4L * dev_sm_count()), 0, st, c));
   const long row = 8L * k.chunks;
   auto turn = [&](const void*& x, long* s, long& part, int i) {
     x = c.dst[i];
@@ -253,12 +253,14 @@ int attn_pack(AttnTcParams& t, const AttnPacked& k, char* ws, stream_t st) {
   t.chunks = k.chunks;
   return S2C_OK;
 }
-// The forward pass: worth it from this many scores on (see attn_tc_worth).
+// Whether a call is worth the tensor cores.  Rows they can fetch: always (tiles of 64 on the FP32 pipes / tensor cores, forward and
+// backward: 32 x 17 positions, 4 heads of 64, 66 / 49 us; 32 x 60, 82 / 48).  Rows to be packed: from 96 x 96 scores per head on
+// (float32, 4 x 100, 4 heads of 64, packing included: 98 / 76 us; 32 x 60, 4 heads of 10: 49 / 67; 128 x 60, 8 of 32: 195 / 260).
 inline bool attn_tc_worth(const AttnParams& p, bool packed) {
   const int mode = g_attention.load(std::memory_order_relaxed);
   if (p.batch < 1 || p.lq < 1 || p.lk < 1 || mode == 1) return false;
   if (mode == 2) return true;
-  return !packed || (long)p.lq * p.lk >= 128 * 128;
+  return !packed || (long)p.lq * p.lk >= 96 * 96;
 }
 template <class T>
 bool attn_forward_tc(const AttnParams& p) {

@@ -6,14 +6,20 @@ layers.  Attribute names and ``nn.Sequential`` positions are the reference's, so
 * ``S2ConvNet_deep``      - examples/mnist/run.py:101-185 (convolutional.{0,2,...,12}, linear.{0,...,7})
 * ``Shrec17Model``        - examples/shrec17/model.py:7-48 (sequential.{0,...}, out_layer)
 
+and, without a counterpart there, ``SphereSequenceNet`` for spherical signals in order (the frames of a
+recording, the shells of a volume): the layers of ``S2ConvNet_original`` on every signal, attention over the
+sequence (``s2cnn_b200.sequence``), one answer.
+
 Every model is written with plain module calls; ``s2cnn_b200.fuse(model)`` routes the conv - ReLU
 - conv and conv - ReLU - so3_integrate chains through the fused kernels (and folds an eval-mode
 BatchNorm3d that follows a convolution into that layer's spectrum and bias).
 """
 import numpy as np
+import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .sequence import LayerNorm, SequenceBlock
 from .s2_grid import s2_equatorial_grid, s2_near_identity_grid
 from .so3_grid import so3_equatorial_grid, so3_near_identity_grid
 from .soft.s2_conv import S2Convolution
@@ -98,3 +104,37 @@ class Shrec17Model(nn.Module):
     def forward(self, x):
         x = so3_integrate(self.sequential(x))
         return F.log_softmax(self.out_layer(x), dim=1)
+
+
+class SphereSequenceNet(nn.Module):
+    """One answer about a sequence of spherical signals: S2Conv(1 -> f1, b_in -> b_l1), ReLU, SO3Conv(f1 -> f2,
+    b_l1 -> b_l2), ReLU, so3_integrate for every signal; ``layers`` SequenceBlocks over the f2 features of the
+    signals in order; layer norm, mean over the filled positions, Linear(f2 -> f_output)."""
+
+    def __init__(self, f1=20, f2=40, f_output=10, b_in=30, b_l1=10, b_l2=6, layers=2, heads=4, p=0.1, num_buckets=16, reach=30,
+                 causal=False):
+        super().__init__()
+        self.conv1 = S2Convolution(nfeature_in=1, nfeature_out=f1, b_in=b_in, b_out=b_l1, grid=s2_near_identity_grid())
+        self.conv2 = SO3Convolution(nfeature_in=f1, nfeature_out=f2, b_in=b_l1, b_out=b_l2, grid=so3_near_identity_grid())
+        self.blocks = nn.ModuleList([SequenceBlock(f2, heads, causal=causal, p=p, num_buckets=num_buckets, reach=reach)
+                                     for _ in range(layers)])
+        self.norm = LayerNorm(f2)
+        self.out_layer = nn.Linear(f2, f_output)
+
+    def features(self, x):
+        """[batch, length, 1, 2 b_in, 2 b_in] -> [batch, length, f2]"""
+        y = F.relu(self.conv2(F.relu(self.conv1(x.flatten(0, 1)))))
+        return so3_integrate(y).unflatten(0, x.shape[:2])
+
+    def forward(self, x, lengths=None):
+        """:param x: [batch, length, 1, 2 b_in, 2 b_in], sequences padded to the longest
+        :param lengths: int32 [batch], the signals of each sequence (None: all)
+        :return: [batch, f_output]"""
+        y = self.features(x)
+        for block in self.blocks:
+            y = block(y, lengths)
+        y = self.norm(y)
+        if lengths is None:
+            return self.out_layer(y.mean(1))
+        filled = torch.arange(x.size(1), device=x.device) < lengths[:, None]
+        return self.out_layer((y * filled[..., None]).sum(1) / lengths.clamp_min(1)[:, None])

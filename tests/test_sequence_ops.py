@@ -525,3 +525,69 @@ def test_block_whole_and_step_by_step(backend):
         assert not torch.equal(a, b)                       # every call a mask of its own
         a.sum().backward()
         assert all(t.grad is not None and bool(torch.isfinite(t.grad).all()) for t in m.parameters())
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+def test_network_over_sequences_of_signals(backend):
+    """What is padded changes no answer, the signals' order does, and every parameter has a gradient."""
+    with backends.active(backend) as (_, dev):
+        torch.manual_seed(14)
+        m = S.models.SphereSequenceNet(f1=2, f2=8, f_output=3, b_in=4, b_l1=3, b_l2=2, heads=2, num_buckets=8, reach=3).to(dev).eval()
+        x = torch.randn(2, 5, 1, 8, 8, device=dev)
+        lengths = torch.tensor([5, 3], dtype=torch.int32, device=dev)
+        with torch.no_grad():
+            for block in m.blocks:
+                block.bias.weight.normal_()
+            y = m(x, lengths)
+            other = x.clone()
+            other[1, 3:] = torch.randn(2, 1, 8, 8, device=dev)
+            assert torch.equal(m(other, lengths), y)
+            assert rel(m(x[1:, :3], None), y[1:]) <= 4 * TOL[F32]
+            assert rel(m(x[:1].flip(1), None), y[:1]) > 1e-3
+        m.train()
+        m(x, lengths).square().sum().backward()
+        for name, t in m.named_parameters():
+            assert t.grad is not None and bool(torch.isfinite(t.grad).all()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_either_kind_of_kernels_takes_every_size(mode, dtype):
+    """The tiles on the FP32 pipes at many tiles, the tensor cores at parts of one."""
+    lib = _lib.cuda_lib()
+    lib.s2c_debug_attention(mode)
+    try:
+        cases = SMALL[1:] if mode == 2 else LARGE[:4] + LARGE[-7:]
+        for B, Lq, Lk, H, Hk, D, bias, kw in cases:
+            check_attention("cuda", dtype, B, Lq, Lk, H, Hk, D, bias, packed=Lq == Lk, **kw)
+    finally:
+        lib.s2c_debug_attention(0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_operators_on_another_stream_and_in_a_graph(dtype):
+    """Work and scratch space follow the current stream, and a captured forward pass gives what the call gave."""
+    gen = torch.Generator().manual_seed(15)
+    q, k, v = (normal(gen, "cuda", dtype, 2, 200, n, 64) for n in (4, 2, 2))
+    table, buckets = normal(gen, "cuda", dtype, 16, 4), S.relative_buckets(16, 64, device="cuda")
+    x, w = normal(gen, "cuda", dtype, 200, 96), normal(gen, "cuda", dtype, 96)
+
+    def run():
+        return (S.attention(q, k, v, table, buckets), S.attention(q[:, :1], k, v, table, buckets), S.layer_norm(x, w, w),
+                S.dropout(x, 0.2, 9, 1, residual=x))
+
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
