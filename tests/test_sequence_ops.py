@@ -286,6 +286,29 @@ def test_few_queries_agree_with_many():
         assert rel(one, every[:, 39:]) <= 2 * TOL[dtype]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [1, 130])
+def test_offsets_beyond_32_bits(lq):
+    """Keys and values 131072 elements apart: the last of 20000 lie 2.6e9 elements behind the first."""
+    gen = torch.Generator().manual_seed(16)
+    k, v = (normal(gen, "cuda", BF16, 1, 20000, 1, 64) for _ in range(2))
+    q = normal(gen, "cuda", BF16, 1, lq, 2, 64)
+    room = torch.empty(20000, 1024, 128, dtype=BF16, device="cuda")
+    far_k, far_v = room[:, :1, :64].unsqueeze(0), room[:, 1:2, 64:].unsqueeze(0)
+    far_k.copy_(k)
+    far_v.copy_(v)
+    assert far_k.stride(1) * 19999 > 2 ** 31
+    kw = {"causal": True, "q_start": 20000 - lq}
+    assert torch.equal(S.attention(q, far_k, far_v, **kw), S.attention(q, k, v, **kw))
+    if lq > 1:
+        g = normal(gen, "cuda", BF16, 1, lq, 2, 64)
+        results = []
+        for kk, vv in ((far_k, far_v), (k, v)):
+            args = [t.detach().requires_grad_(True) for t in (q, kk, vv)]
+            results.append(torch.autograd.grad(S.attention(*args, **kw), args, g))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 # ---- layer norm ---------------------------------------------------------------------------------------------------------
 
 
