@@ -333,9 +333,10 @@ int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, 
  * over the seen j; 0 where a query sees nothing.  start, q_length and kv_length are those of the batch entry
  * (device int32 [batch]; NULL: q_start, lq, lk; lengths outside 0 .. lq / lk are clamped).  bias
  * [n_buckets][heads] and bucket_of (device int32 [2 reach + 1]; an entry outside 0 .. n_buckets - 1 means no
- * bias) come together or are both NULL.  reach <= 2048, n_buckets <= 1024.  Rows of k and v that no query sees
- * are not read.  (Under `causal`, what a tile of 128 queries sees is read by the whole tile: an infinity or NaN
- * among those values may reach its other queries.) */
+ * bias) come together or are both NULL.  reach <= 2048, n_buckets <= 1024.  Rows of k and v that no query of
+ * a block of the call sees are not read.  (Under `causal`, what one of 256 neighbouring queries sees is read for
+ * all of them: an infinity or NaN among those values may reach the others, as 0 times it.)  Rows of q and dout
+ * beyond q_length are not read either. */
 typedef struct s2c_attention_desc {
   int dtype, batch, lq, lk, heads, kv_heads, dim;
   long q_stride[3], k_stride[3], v_stride[3];      /* batch entry, position, head */

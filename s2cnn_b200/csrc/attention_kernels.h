@@ -13,7 +13,8 @@
 // is not read, whatever it holds.
 //
 // The kernels here take tiles of 64 queries x 64 keys, 16 x 16 threads with 4 x 4 scores each.  They are written for the host
-// emulation as well, and on the GPU serve the problems that are too small for the tensor-core kernels.
+// emulation as well, and on the GPU serve the problems that are too small for the tensor-core kernels.  Bound by the FP32 pipes and
+// shared memory: 2 x 4096 positions, 16 heads of 128, forward and backward, 36 ms against 7.6 on the tensor cores (float32).
 #pragma once
 
 #include <cfloat>

@@ -12,6 +12,8 @@
 // While one group is at its exponentials the tensor core works for the other one.  The output is rescaled only where the
 // maximum of a row has grown by more than 8 (in units of ln 2) since it was last fixed: weights then reach 2^8 at most, which
 // costs no precision, and after the first tiles rescaling all but ends.
+// 2 x 4096 positions, 16 heads of 128: 287 us, 958 TFLOP/s; with a bias 298, and 374 where its gradient may follow.  16 of 64: 253 us (in
+// training).  Exponentials, tensor pipe and the threads' other work each take about half of that and overlap but in part.
 // Weights in bfloat16: a relative 2^-9 on each of the many terms of an output that is itself rounded to bfloat16.
 #pragma once
 
