@@ -1,19 +1,20 @@
 // Attention, forward, bfloat16, on the tensor cores.
 //
 // A block takes one or two tiles of 128 queries that read the same keys: neighbouring tiles of a head, or the same tile of
-// heads that share a key head.  Roles (12 warps, the last of them idle):
+// heads that share a key head.  Roles (12 warps):
 //   * warps 0 - 3 and 4 - 7, one group per query tile: thread = row = tensor-memory lane.  A group takes the finished scores of
-//     a key tile from tensor memory, adds the bias, finds the running maximum, writes the weights 2^(x - m), rounded to
+//     64 keys from tensor memory, adds the bias, finds the running maximum, writes the weights 2^(x - m), rounded to
 //     bfloat16, over the scores (half of their columns) and keeps the sum of the unrounded ones;
-//   * warp 8 issues the products: scores of a tile, and weights times values into the tile's output in tensor memory;
-//   * warps 9 and 10 load keys and values, two tiles ahead of each.
-// A group's thread holds 128 scores; its registers come from the third warpgroup (launched with 168 each: 8 x 208 + 4 x 88 =
-// 12 x 168).
-// While one group is at its exponentials the tensor core works for the other one.  The output is rescaled only where the
-// maximum of a row has grown by more than 8 (in units of ln 2) since it was last fixed: weights then reach 2^8 at most, which
-// costs no precision, and after the first tiles rescaling all but ends.
-// 2 x 4096 positions, 16 heads of 128: 287 us, 958 TFLOP/s; with a bias 298, and 374 where its gradient may follow.  16 of 64: 253 us (in
-// training).  Exponentials, tensor pipe and the threads' other work each take about half of that and overlap but in part.
+//   * warps 8 and 11 issue the products of a group each: scores of a tile, and weights times values into the output in tensor memory;
+//   * warps 9 and 10 load keys and values, four tiles ahead of each.
+// A group has two buffers of scores: the next tile's are there while it is at the exponentials of this one.  (With one buffer for
+// tiles of 128 keys and one issuing thread: 2 x 4096 positions, 16 heads of 128, 287 us, now 269; of 64, in training, 253 / 229.  The
+// tiles of 64 with one issuing thread: 278 and 256.)
+// Its registers come from the third warpgroup (launched with 168 each: 8 x 208 + 4 x 88 = 12 x 168).
+// The output is rescaled only where the maximum of a row has grown by more than 8 (in units of ln 2) since it was last fixed:
+// weights then reach 2^8 at most, which costs no precision, and after the first tiles rescaling all but ends.
+// 2 x 4096 positions, 16 heads of 128: 269 us, 1022 TFLOP/s; with a bias 281, and 373 where its gradient may follow.  Bound by the
+// exponentials (16 a clock and SM: half of the time) and the tensor pipe (half of it), which overlap but in part.
 // Weights in bfloat16: a relative 2^-9 on each of the many terms of an output that is itself rounded to bfloat16.
 #pragma once
 
@@ -27,7 +28,7 @@ constexpr int kTcfThreads = 12 * 32;
 constexpr float kTcfGrow = 8.f;
 
 struct TcfBars {
-  uint64_t q_full[2], s_full[2], p_full[4], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], k_full[4], k_empty[4], v_full[4], v_empty[4], drained[2];
   uint32_t tmem;
 };
 
@@ -45,33 +46,17 @@ static constexpr int kThreads = kTcfThreads;
 static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_dyn_smem) {
   const AttnParams& p = pp.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  constexpr uint32_t kRows = NC * kTcxTile;                          // bytes of a tile of 128 rows
+  constexpr uint32_t kQ = NC * kTcxTile, kRows = kQ / 2;             // bytes of a tile of 128 queries, of 64 keys
   const uint32_t base = (tcx_addr(s2c_dyn_smem) + 1023u) & ~1023u;
   unsigned char* const smem = reinterpret_cast<unsigned char*>(s2c_dyn_smem) + (base - tcx_addr(s2c_dyn_smem));
-  const int tiles = pp.per_block + 4;
-  float* const tab = reinterpret_cast<float*>(smem + (size_t)tiles * kRows);
+    float* const tab = reinterpret_cast<float*>(smem + (size_t)(pp.per_block + 4) * kQ);
   TcfBars* const bars = reinterpret_cast<TcfBars*>((reinterpret_cast<uintptr_t>(tab + pp.per_block * tcx_tab_floats(p.reach)) + 15) & ~(uintptr_t)15);
-  const uint32_t q_at = base, k_at = base + pp.per_block * kRows, v_at = k_at + 2 * kRows;
+  const uint32_t q_at = base, k_at = base + pp.per_block * kQ, v_at = k_at + 4 * kRows;
 
   // the longest rows (the last queries under `causal`) first
   const int heads_all = p.batch * p.kv_heads;
   const int pair = pp.pairs - 1 - (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, hk = bh % p.kv_heads, b = bh / p.kv_heads;
 
-  if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      tcx_init(&bars->q_full[i], 128);
-      tcx_init(&bars->s_full[i], 1);
-      tcx_init(&bars->p_full[2 * i], 4);
-      tcx_init(&bars->p_full[2 * i + 1], 4);
-      tcx_init(&bars->pv_done[i], 1);
-      tcx_init(&bars->k_full[i], 32);
-      tcx_init(&bars->k_empty[i], 1);
-      tcx_init(&bars->v_full[i], 32);
-      tcx_init(&bars->v_empty[i], 1);
-    }
-    tcx_init(&bars->drained, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   const AttnSeq s = attn_seq(p, b);
   // unit = tile * group + (head within its group): first row, head and key tiles of this block's query tiles
   int i0[2], head[2], keys[2], n[2];
@@ -82,9 +67,28 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
     i0[u] = on ? unit / p.group * 128 : p.lq;
     head[u] = hk * p.group + (on ? unit % p.group : 0);
     keys[u] = i0[u] < s.qlen ? attn_keys(p, s, min(i0[u] + 128, s.qlen)) : 0;
-    n[u] = (keys[u] + 127) / 128;
+    n[u] = (keys[u] + 63) / 64;
   }
   const int n_all = max(n[0], n[1]), keys_all = max(keys[0], keys[1]);
+  const int users = max(1, (n[0] > 0) + (n[1] > 0));                 // issuing threads that read a tile of keys
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tcx_init(&bars->q_full[i], 128);
+      for (int e = 0; e < 2; ++e) {
+        tcx_init(&bars->s_full[i][e], 1);
+        tcx_init(&bars->p_full[i][e], 4);
+      }
+      tcx_init(&bars->pv_done[i], 1);
+      tcx_init(&bars->drained[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      tcx_init(&bars->k_full[i], 32);
+      tcx_init(&bars->k_empty[i], users);
+      tcx_init(&bars->v_full[i], 32);
+      tcx_init(&bars->v_empty[i], users);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   if (warp == 8) {
     __syncwarp();
     tcx_alloc<512>(&bars->tmem);
@@ -101,58 +105,55 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp == 8) {
-    if (tcx_elect()) {                       // one thread issues all: a warp's votes cost it 100 clocks a wait
+  if (warp == 8 || warp == 11) {
+    const int u = warp == 11;
+    if (n[u] && tcx_elect()) {               // one thread issues all of a group: a warp's votes cost it 100 clocks a wait
       const int steps = (pp.chunks + 1) / 2;
-      const uint32_t is = tcx_idesc(128, false), io = tcx_idesc(16 * steps, true);
-      for (int u = 0; u < 2 && ok; ++u)
-        if (n[u]) ok = tcx_wait(&bars->q_full[u], 0);
-      if (ok && n_all) ok = tcx_wait(&bars->k_full[0], 0);
-      tcx_seen();
-      if (ok && n_all) {
-        for (int u = 0; u < 2; ++u)
-          if (n[u]) {
-            tcx_scores<NC, 128, 128>(t_scores + 128 * u, q_at + u * kRows, k_at, is);
-            tcx_commit(&bars->s_full[u]);
-          }
-        tcx_commit(&bars->k_empty[0]);
+      const uint32_t is = tcx_idesc(64, false), io = tcx_idesc(16 * steps, true);
+      const uint32_t q = q_at + u * kQ, scores = t_scores + 128 * u, out = t_out + 128 * u;
+      ok = tcx_wait(&bars->q_full[u], 0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (!ok || j >= n_all) break;
+        ok = tcx_wait(&bars->k_full[j], 0);
+        tcx_seen();
+        if (!ok) break;
+        if (j < n[u]) {
+          tcx_scores<NC, 128, 64>(scores + 64 * j, q, k_at + j * kRows, is);
+          tcx_commit(&bars->s_full[u][j]);
+        }
+        tcx_commit(&bars->k_empty[j]);
       }
+      // (a group that is done early still waits for the tiles that the other one needs, so that their slots are given back in turn)
       for (int j = 0; j < n_all && ok; ++j) {
-        const int sv = j & 1, sk = (j + 1) & 1;
-        bool have_v = false, have_k = false;
-        for (int u = 0; u < 2 && ok; ++u) {
-          if (j >= n[u]) continue;
-          for (int half = 0; half < 2 && ok; ++half) {
-            ok = tcx_wait(&bars->p_full[2 * u + half], j & 1);
-            if (ok && !have_v) {
-              ok = have_v = tcx_wait(&bars->v_full[sv], (j >> 1) & 1);
-              tcx_seen();
-            }
-            if (!ok) break;
-            tcx_after_sync();
-            const uint32_t w = t_scores + 128 * u + 32 * half, v = v_at + sv * kRows + 64 * 128 * half;
-            if (FINE) tcx_combine<64, 128>(t_out + 128 * u, w + 64, v, io, j > 0 || half);
-            tcx_combine<64, 128>(t_out + 128 * u, w, v, io, FINE || j > 0 || half);
-            if (half) tcx_commit(&bars->pv_done[u]);
-          }
-          if (ok && j + 1 < n[u]) {
-            if (!have_k) {
-              ok = have_k = tcx_wait(&bars->k_full[sk], ((j + 1) >> 1) & 1);
-              tcx_seen();
-            }
-            if (!ok) break;
-            // in order behind the product that reads the weights from the same columns
-            tcx_scores<NC, 128, 128>(t_scores + 128 * u, q_at + u * kRows, k_at + sk * kRows, is);
-            tcx_commit(&bars->s_full[u]);
-          }
+        const int sv = j & 3, sk = (j + 2) & 3, turn = j & 1;
+        const uint32_t w = scores + 64 * turn;
+        ok = tcx_wait(&bars->v_full[sv], (j >> 2) & 1);
+        tcx_seen();
+        if (ok && j < n[u]) {
+          ok = tcx_wait(&bars->p_full[u][turn], (j >> 1) & 1);
+          if (!ok) break;
+          tcx_after_sync();
+          const uint32_t v = v_at + sv * kRows;
+          if (FINE) tcx_combine<64, 64>(out, w + 32, v, io, j > 0);
+          tcx_combine<64, 64>(out, w, v, io, FINE || j > 0);
+          tcx_commit(&bars->pv_done[u]);
         }
-        if (ok) {
-          tcx_commit(&bars->v_empty[sv]);
-          if (j + 1 < n_all) tcx_commit(&bars->k_empty[sk]);
+        if (!ok) break;
+        tcx_commit(&bars->v_empty[sv]);
+        if (j + 2 < n_all) {
+          ok = tcx_wait(&bars->k_full[sk], ((j + 2) >> 2) & 1);
+          tcx_seen();
+          if (!ok) break;
+          if (j + 2 < n[u]) {                // in order behind the product that reads the weights from the same columns
+            tcx_scores<NC, 128, 64>(w, q, k_at + sk * kRows, is);
+            tcx_commit(&bars->s_full[u][turn]);
+          }
+          tcx_commit(&bars->k_empty[sk]);
         }
       }
-      tcx_commit(&bars->drained);            // nothing may be in flight when tensor memory is given back
-      tcx_wait(&bars->drained, 0);
+      tcx_commit(&bars->drained[u]);         // nothing may be in flight when tensor memory is given back
+      tcx_wait(&bars->drained[u], 0);
     }
     __syncwarp();
   } else if (warp == 9 || warp == 10) {
@@ -162,10 +163,10 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
     uint64_t *full = is_k ? bars->k_full : bars->v_full, *empty = is_k ? bars->k_empty : bars->v_empty;
     const uint32_t at = is_k ? k_at : v_at;
     for (int j = 0; j < n_all && ok; ++j) {
-      const int slot = j & 1;
-      if (j >= 2) ok = tcx_wait_warp(&empty[slot], (j / 2 - 1) & 1);
+      const int slot = j & 3;
+      if (j >= 4) ok = tcx_wait_warp(&empty[slot], (j / 4 - 1) & 1);
       if (!ok) break;
-      tcx_load_rows<NC, 32>(at + slot * kRows, src, stride, 128 * j, keys_all, pp.chunks, lane);
+      tcx_load_rows<NC, 32, 64>(at + slot * kRows, src, stride, 64 * j, keys_all, pp.chunks, lane);
       tcx_arrive_copies(&full[slot]);
     }
     tcx_copies_done();
@@ -176,27 +177,28 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
     if (u < pp.per_block && i0[u] < p.lq) {
       const int i = i0[u] + row, h = head[u];
       if (n[u]) {
-        tcx_load_rows<NC, 128>(q_at + u * kRows, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0[u], s.qlen, pp.chunks, tid & 127);
+        tcx_load_rows<NC, 128>(q_at + u * kQ, static_cast<const bf16*>(p.q) + b * p.qs[0] + h * p.qs[2], p.qs[1], i0[u], s.qlen, pp.chunks, tid & 127);
         tcx_loaded();
         tcx_arrive(&bars->q_full[u]);
       }
       const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-      const uint32_t ts = t_scores + 128 * u + lanes, to = t_out + 128 * u + lanes;
+      const uint32_t to = t_out + 128 * u + lanes;
       const float* tb = tab + u * tcx_tab_floats(p.reach);
       const float scale = p.scale * kLog2e, far_before = tb[0], far_behind = tb[2 * p.reach + 2 * kTcxMargin];
       float m = kNoScore, l = 0.f;
       for (int j = 0; j < n[u]; ++j) {
-        const int j0 = 128 * j, d0 = j0 - i0[u] - s.start;            // relative position of the tile's first key to its first query
-        if (!(ok = tcx_wait_warp(&bars->s_full[u], j & 1))) break;
+        const int j0 = 64 * j, d0 = j0 - i0[u] - s.start;             // relative position of the tile's first key to its first query
+        const uint32_t ts = t_scores + 128 * u + 64 * (j & 1) + lanes;
+        if (!(ok = tcx_wait_warp(&bars->s_full[u][j & 1], (j >> 1) & 1))) break;
         tcx_after_sync();
-        uint32_t raw[128];
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) tcx_ld32(ts + c, raw + c);
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) tcx_ld_wait(raw + c);
+        uint32_t raw[64];
+        tcx_ld32(ts, raw);
+        tcx_ld32(ts + 32, raw + 32);
+        tcx_ld_wait(raw);
+        tcx_ld_wait(raw + 32);
         float* x = reinterpret_cast<float*>(raw);
-        const bool close = d0 + 127 > -p.reach && d0 - 127 < p.reach && p.reach > 0;
-        const bool edge = j0 + 128 > keys[u] || (p.causal && d0 + 127 > 0);            // some pairs of the tile are not seen
+        const bool close = d0 + 63 > -p.reach && d0 - 127 < p.reach && p.reach > 0;
+        const bool edge = j0 + 64 > keys[u] || (p.causal && d0 + 63 > 0);            // some pairs of the tile are not seen
         const float far = d0 > 0 ? far_behind : far_before;
         // A tile of one bias, all seen: the maximum of the raw scores tells that of the others, and scale, bias and maximum are one
         // multiply-add.  (Not for a bias so large that the scores vanish beside it, see AttnParams::stats.)
@@ -205,24 +207,24 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
           if (close) {
             const float* near = tb + (d0 - row + p.reach + kTcxMargin);
 #pragma unroll
-            for (int c = 0; c < 128; ++c) x[c] = fmaf(x[c], scale, near[c]);
+            for (int c = 0; c < 64; ++c) x[c] = fmaf(x[c], scale, near[c]);
           } else {
 #pragma unroll
-            for (int c = 0; c < 128; ++c) x[c] = fmaf(x[c], scale, far);
+            for (int c = 0; c < 64; ++c) x[c] = fmaf(x[c], scale, far);
           }
           if (edge) {
             const int lim = p.causal ? min(keys[u] - j0, row - d0 + 1) : keys[u] - j0;
 #pragma unroll
-            for (int c = 0; c < 128; ++c) x[c] = c < lim ? x[c] : kNoScore;
+            for (int c = 0; c < 64; ++c) x[c] = c < lim ? x[c] : kNoScore;
           }
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 4; c < 124; c += 8)
+        for (int c = 4; c < 60; c += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top[e] = tcx_max3(top[e], x[c + e], x[c + 4 + e]);
-        float now = fmaxf(tcx_max3(top[0], top[1], top[2]), tcx_max3(top[3], x[124], x[125]));
-        now = tcx_max3(now, x[126], x[127]);
+        float now = fmaxf(tcx_max3(top[0], top[1], top[2]), tcx_max3(top[3], x[60], x[61]));
+        now = tcx_max3(now, x[62], x[63]);
         if (plain) now = fmaf(now, scale, far);
         if (__any_sync(0xffffffffu, now > m + kTcfGrow)) {
           const float fresh = now > m + kTcfGrow ? now : m;
@@ -245,27 +247,22 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
         }
         const float base = m == kNoScore ? 0.f : -m, mul = plain ? scale : 1.f, add = plain ? far + base : base;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // half of the weights at a time: their product with the values begins while the others are computed
+        uint32_t w[32], rest[FINE ? 32 : 1];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[32], rest[FINE ? 32 : 1];
-#pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const int c = 64 * half + e;
-            float2 y = fma2(make_float2(x[c], x[c + 1]), make_float2(mul, mul), make_float2(add, add));
-            y.x = exp2_fast(y.x);
-            y.y = exp2_fast(y.y);
-            sum[(c / 2) & 1] = tcx_add2(sum[(c / 2) & 1], y);
-            w[e / 2] = pack_bf16(y.x, y.y);
-            if constexpr (FINE) rest[e / 2] = pack_bf16(y.x - as_float(w[e / 2] << 16), y.y - as_float(w[e / 2] & 0xffff0000u));
-          }
-          tcx_st32(ts + 32 * half, w);
-          if constexpr (FINE) tcx_st32(ts + 64 + 32 * half, rest);
-          tcx_st_wait();
-          tcx_before_sync();
-          __syncwarp();
-          if (lane == 0) tcx_arrive(&bars->p_full[2 * u + half]);
+        for (int c = 0; c < 64; c += 2) {
+          float2 y = fma2(make_float2(x[c], x[c + 1]), make_float2(mul, mul), make_float2(add, add));
+          y.x = exp2_fast(y.x);
+          y.y = exp2_fast(y.y);
+          sum[(c / 2) & 1] = tcx_add2(sum[(c / 2) & 1], y);
+          w[c / 2] = pack_bf16(y.x, y.y);
+          if constexpr (FINE) rest[c / 2] = pack_bf16(y.x - as_float(w[c / 2] << 16), y.y - as_float(w[c / 2] & 0xffff0000u));
         }
+        tcx_st32(ts, w);
+        if constexpr (FINE) tcx_st32(ts + 32, rest);
+        tcx_st_wait();
+        tcx_before_sync();
+        __syncwarp();
+        if (lane == 0) tcx_arrive(&bars->p_full[u][j & 1]);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       // ---- the output row
