@@ -22,6 +22,7 @@ struct AttnTcParams {
   int chunks;          // 16-byte pieces of a row that hold values
   int units, pairs;    // query tiles of 128 per (batch entry, key head), and blocks of one or two of them
   int per_block;       // query tiles of a block: 1 or 2
+  int whole;           // forward: blocks from this one on take one tile of a pair each
   long q_split, k_split, v_split, g_split;     // float32: elements from one part of an operand to the next (attention_tc3.h)
 };
 

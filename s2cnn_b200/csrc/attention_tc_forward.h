@@ -27,8 +27,10 @@ namespace s2c {
 constexpr int kTcfThreads = 12 * 32;
 constexpr float kTcfGrow = 8.f;
 
+// pv_done: products with the values of even and odd tiles.  (The scores of tile j tell a group that the product of j - 2 is done: on one
+// barrier for all, whose waits tell two neighbouring phases apart and no more, the one of j - 2 could pass for that of j.)
 struct TcfBars {
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], k_full[4], k_empty[4], v_full[4], v_empty[4], drained[2];
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], k_full[4], k_empty[4], v_full[4], v_empty[4], drained[2];
   uint32_t tmem;
 };
 
@@ -55,15 +57,17 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
 
   // the longest rows (the last queries under `causal`) first
   const int heads_all = p.batch * p.kv_heads;
-  const int pair = pp.pairs - 1 - (int)blockIdx.x / heads_all, bh = (int)blockIdx.x % heads_all, hk = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int cut = max(0, (int)blockIdx.x - pp.whole), at = (int)blockIdx.x - (cut + 1) / 2;
+  const bool single = (int)blockIdx.x >= pp.whole;
+  const int pair = pp.pairs - 1 - at / heads_all, bh = at % heads_all, hk = bh % p.kv_heads, b = bh / p.kv_heads;
 
   const AttnSeq s = attn_seq(p, b);
   // unit = tile * group + (head within its group): first row, head and key tiles of this block's query tiles
   int i0[2], head[2], keys[2], n[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int unit = pair * pp.per_block + u;
-    const bool on = u < pp.per_block && unit < pp.units;
+    const int unit = pair * pp.per_block + u + (single ? cut & 1 : 0);
+    const bool on = u < (single ? 1 : pp.per_block) && unit < pp.units;
     i0[u] = on ? unit / p.group * 128 : p.lq;
     head[u] = hk * p.group + (on ? unit % p.group : 0);
     keys[u] = i0[u] < s.qlen ? attn_keys(p, s, min(i0[u] + 128, s.qlen)) : 0;
@@ -77,8 +81,8 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
       for (int e = 0; e < 2; ++e) {
         tcx_init(&bars->s_full[i][e], 1);
         tcx_init(&bars->p_full[i][e], 4);
+        tcx_init(&bars->pv_done[i][e], 1);
       }
-      tcx_init(&bars->pv_done[i], 1);
       tcx_init(&bars->drained[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
@@ -137,7 +141,7 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
           const uint32_t v = v_at + sv * kRows;
           if (FINE) tcx_combine<64, 64>(out, w + 32, v, io, j > 0);
           tcx_combine<64, 64>(out, w, v, io, FINE || j > 0);
-          tcx_commit(&bars->pv_done[u]);
+          tcx_commit(&bars->pv_done[u][turn]);
         }
         if (!ok) break;
         tcx_commit(&bars->v_empty[sv]);
@@ -230,7 +234,7 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
           const float fresh = now > m + kTcfGrow ? now : m;
           if (j > 0) {
             const float f = fresh == m ? 1.f : exp2_fast(m - fresh);
-            if (!(ok = tcx_wait_warp(&bars->pv_done[u], (j - 1) & 1))) break;
+            if (!(ok = tcx_wait_warp(&bars->pv_done[u][(j - 1) & 1], ((j - 1) >> 1) & 1))) break;
             tcx_after_sync();
             l *= f;
 #pragma unroll
@@ -268,7 +272,7 @@ static __device__ __forceinline__ void run(const AttnTcParams& pp, float4* s2c_d
       // ---- the output row
       if (i >= s.qlen) l = 0.f;
       const float2 st = attn_stats(m, l);
-      if (ok && n[u]) ok = tcx_wait_warp(&bars->pv_done[u], (n[u] - 1) & 1);
+      if (ok && n[u]) ok = tcx_wait_warp(&bars->pv_done[u][(n[u] - 1) & 1], ((n[u] - 1) >> 1) & 1);
       tcx_after_sync();
       const long at = (((long)b * p.lq + i) * p.heads + h) * p.dim;
       bf16* out = static_cast<bf16*>(p.out) + at;

@@ -275,6 +275,40 @@ def test_attention_gradients_are_reproducible():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("case", [(8, 1000, 8, 8, 64, True), (8, 1000, 8, 8, 64, False), (5, 1000, 8, 8, 128, True), (4, 1100, 8, 8, 64, False),
+                                  (13, 333, 8, 4, 128, True), (40, 64, 8, 2, 64, True), (38, 130, 4, 4, 32, False)],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_attention_of_several_waves(case, dtype):
+    """More blocks than run at once, with a last wave of any size: against whole matrices in 64 bits, and the same in every call."""
+    B, L, H, Hk, D, causal = case
+    gen = torch.Generator().manual_seed(17)
+    q, k, v = (normal(gen, "cuda", dtype, B, L, n, D) for n in (H, Hk, Hk))
+    table, g = normal(gen, "cuda", dtype, 32, H) * 2, normal(gen, "cuda", dtype, B, L, H, D)
+    buckets = S.relative_buckets(32, 128, device="cuda")
+    args = [t.requires_grad_(True) for t in (q, k, v, table)]
+    ref = [t.detach().double().requires_grad_(True) for t in args]
+    rel_pos = torch.arange(L, device="cuda") - torch.arange(L, device="cuda")[:, None]
+    which = buckets.long()[rel_pos.clamp(-128, 128) + 128]
+    scores = torch.einsum("bihd,bjhd->bhij", ref[0], ref[1].repeat_interleave(H // Hk, 2)) / math.sqrt(D) + ref[3][which].permute(2, 0, 1)
+    if causal:
+        scores = scores.masked_fill(rel_pos > 0, -math.inf)
+    want = torch.einsum("bhij,bjhd->bihd", torch.softmax(scores, -1), ref[2].repeat_interleave(H // Hk, 2))
+    want = (want.detach(),) + torch.autograd.grad(want, ref, g.double())
+    del scores
+    first = None
+    for _ in range(4):
+        with torch.no_grad():
+            inferred = S.attention(*args, buckets, causal=causal)
+        out = S.attention(*args, buckets, causal=causal)
+        now = (inferred, out) + torch.autograd.grad(out, args, g)
+        for name, a, b in zip(("inferred", "out", "dq", "dk", "dv", "dbias"), now, want[:1] + want):
+            assert rel(a, b) <= TOL[dtype], (name, rel(a, b))
+        first = first or now
+        assert all(torch.equal(a, b) for a, b in zip(first, now))
+
+
+@pytest.mark.gpu
 def test_few_queries_agree_with_many():
     """One query of a long cache, split over the keys, beside the same query among others."""
     gen = torch.Generator().manual_seed(8)
