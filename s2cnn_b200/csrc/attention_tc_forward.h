@@ -13,8 +13,9 @@
 // Its registers come from the third warpgroup (launched with 168 each: 8 x 208 + 4 x 88 = 12 x 168).
 // The output is rescaled only where the maximum of a row has grown by more than 8 (in units of ln 2) since it was last fixed:
 // weights then reach 2^8 at most, which costs no precision, and after the first tiles rescaling all but ends.
-// 2 x 4096 positions, 16 heads of 128: 269 us, 1022 TFLOP/s; with a bias 281, and 373 where its gradient may follow.  Bound by the
-// exponentials (16 a clock and SM: half of the time) and the tensor pipe (half of it), which overlap but in part.
+// 2 x 4096 positions, 16 heads of 128: 257 us, 1071 TFLOP/s (the last wave halved); with a bias 264, and 340 where its gradient may
+// follow.  Bound by the exponentials (16 a clock and SM: 60 % of the time) and the tensor pipe (66 % of the measured peak), which
+// overlap but in part.  A quarter of the exponentials as polynomials on the FP32 pipes gave nothing (260 us).
 // Weights in bfloat16: a relative 2^-9 on each of the many terms of an output that is itself rounded to bfloat16.
 #pragma once
 
