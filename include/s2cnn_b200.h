@@ -374,6 +374,10 @@ int s2c_layer_norm_backward(int dtype, const void* x, const void* weight, const 
  * gradient of out without a residual. */
 int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long n, double probability,
                 unsigned long long seed, unsigned long long step, void* stream);
+/* The same with seed and step in device memory, numbers = {seed, step}, read when the kernel runs: a captured call takes
+ * what is there at each replay. */
+int s2c_dropout_numbers(int dtype, const void* x, const void* residual, void* out, long n, double probability,
+                        const unsigned long long* numbers, void* stream);
 
 /* ---- test hooks (not part of the drop-in surface; no counterpart in the reference) ------------ */
 /* Path selection for the test-suite, so that every kernel variant can be compared with the oracle

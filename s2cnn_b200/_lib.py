@@ -106,6 +106,7 @@ _SIGNATURES = {
     "s2c_layer_norm_backward_workspace": (c_size_t, [c_long, c_int]),
     "s2c_layer_norm_backward": (c_int, [c_int] + [_P] * 7 + [c_long, c_int, _P, c_size_t, _P]),
     "s2c_dropout": (c_int, [c_int, _P, _P, _P, c_long, c_double, c_ulonglong, c_ulonglong, _P]),
+    "s2c_dropout_numbers": (c_int, [c_int, _P, _P, _P, c_long, c_double, _P, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

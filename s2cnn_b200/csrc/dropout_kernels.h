@@ -21,6 +21,7 @@ struct DropoutParams {
   unsigned threshold;     // floor(p 2^32): a word below it drops its element
   float scale;            // 1 / (1 - p)
   unsigned key[2], step[2];
+  const unsigned long long* numbers;   // seed and step in memory, null: those above
 };
 
 S2C_D void philox7(unsigned long long block, const unsigned (&key)[2], const unsigned (&step)[2], unsigned (&w)[4]) {
@@ -49,12 +50,19 @@ struct Dropout {
     const T* res = static_cast<const T*>(p.residual);
     T* out = static_cast<T*>(p.out);
     const long stride = (long)ctx.nblk * ctx.nthr * kStep;
+    unsigned key[2] = {p.key[0], p.key[1]}, step[2] = {p.step[0], p.step[1]};
+    if (p.numbers) {
+      key[0] = (unsigned)p.numbers[0];
+      key[1] = (unsigned)(p.numbers[0] >> 32);
+      step[0] = (unsigned)p.numbers[1];
+      step[1] = (unsigned)(p.numbers[1] >> 32);
+    }
     for (long i = ((long)ctx.bid * ctx.nthr + ctx.tid) * kStep; i < p.n; i += stride) {
       unsigned w[kStep];
 #pragma unroll
       for (int b = 0; b < kStep / 4; ++b) {
         unsigned four[4];
-        philox7((unsigned long long)(i / 4 + b), p.key, p.step, four);
+        philox7((unsigned long long)(i / 4 + b), key, step, four);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * b + e] = four[e];
       }

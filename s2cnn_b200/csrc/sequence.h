@@ -83,6 +83,26 @@ int norm_backward(LayerNormParams p, void* dw, void* db, stream_t st) {
   return seq_launch<LayerNormSum<T>>("layer_norm_sums", (2L * p.cols + 31) / 32, 256 * sizeof(float), st, s);
 }
 
+// ---- dropout -----------------------------------------------------------------------------------------------------------
+inline int dropout(const char* who, int dtype, DropoutParams p, const void* x, const void* residual, void* out, long n, double probability, stream_t st) {
+  S2C_SEQ_TRY(seq_check_type(who, dtype));
+  if (n < 0 || (n > 0 && (!x || !out)) || !(probability >= 0. && probability < 1.)) return fail(S2C_ERR_BAD_ARG, std::string(who) + ": bad argument");
+  p.x = x; p.residual = residual; p.out = out; p.n = n;
+  p.threshold = (unsigned)std::floor(probability * 4294967296.);
+  p.scale = (float)(1. / (1. - probability));
+  const bool vec = aligned16(x) && aligned16(residual) && aligned16(out);
+  auto go = [&](auto k) {
+    using K = typename decltype(k)::type;
+    const long blocks = (n + (long)K::kThreads * K::kStep - 1) / ((long)K::kThreads * K::kStep);
+    return seq_launch<K>("dropout", std::min<long>(blocks, 32L * dev_sm_count()), 0, st, p);
+  };
+  struct A { using type = Dropout<float, true>; };
+  struct B { using type = Dropout<float, false>; };
+  struct C { using type = Dropout<bf16, true>; };
+  struct D { using type = Dropout<bf16, false>; };
+  return dtype == kSeqF32 ? (vec ? go(A()) : go(B())) : (vec ? go(C()) : go(D()));
+}
+
 // ---- attention ---------------------------------------------------------------------------------------------------------
 constexpr int kAttnMaxDim = 128, kAttnMaxReach = 2048, kAttnMaxBuckets = 1024;
 inline int attn_check(const char* who, const s2c_attention_desc* d) {
@@ -449,27 +469,20 @@ int s2c_layer_norm_backward(int dtype, const void* x, const void* weight, const 
 
 int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long n, double probability, unsigned long long seed,
                 unsigned long long step, void* stream) {
-  S2C_SEQ_TRY(seq_check_type("s2c_dropout", dtype));
-  if (n < 0 || (n > 0 && (!x || !out)) || !(probability >= 0. && probability < 1.)) return fail(S2C_ERR_BAD_ARG, "s2c_dropout: bad argument");
   DropoutParams p = {};
-  p.x = x; p.residual = residual; p.out = out; p.n = n;
-  p.threshold = (unsigned)std::floor(probability * 4294967296.);
-  p.scale = (float)(1. / (1. - probability));
   for (int i = 0; i < 2; ++i) {
     p.key[i] = (unsigned)(seed >> (32 * i));
     p.step[i] = (unsigned)(step >> (32 * i));
   }
-  const bool vec = aligned16(x) && aligned16(residual) && aligned16(out);
-  auto go = [&](auto k) {
-    using K = typename decltype(k)::type;
-    const long blocks = (n + (long)K::kThreads * K::kStep - 1) / ((long)K::kThreads * K::kStep);
-    return seq_launch<K>("dropout", std::min<long>(blocks, 32L * dev_sm_count()), 0, (stream_t)stream, p);
-  };
-  struct A { using type = Dropout<float, true>; };
-  struct B { using type = Dropout<float, false>; };
-  struct C { using type = Dropout<bf16, true>; };
-  struct D { using type = Dropout<bf16, false>; };
-  return dtype == kSeqF32 ? (vec ? go(A()) : go(B())) : (vec ? go(C()) : go(D()));
+  return dropout("s2c_dropout", dtype, p, x, residual, out, n, probability, (stream_t)stream);
+}
+
+int s2c_dropout_numbers(int dtype, const void* x, const void* residual, void* out, long n, double probability,
+                        const unsigned long long* numbers, void* stream) {
+  if (!numbers || reinterpret_cast<uintptr_t>(numbers) % 8) return fail(S2C_ERR_BAD_ARG, "s2c_dropout_numbers: no seed and step, or not aligned to their type");
+  DropoutParams p = {};
+  p.numbers = numbers;
+  return dropout("s2c_dropout_numbers", dtype, p, x, residual, out, n, probability, (stream_t)stream);
 }
 
 size_t s2c_attention_workspace(const s2c_attention_desc* d) {

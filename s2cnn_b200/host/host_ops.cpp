@@ -84,7 +84,7 @@ long s2_bandwidth(long nspec) {
   X(s2_mm_grady) X(s2_mm_real_gradx) X(s2_mm_real_grady) X(rft_forward) X(rft_forward_t) X(rft_forward_scaled) X(rft_backward_scaled) X(rft_backward_workspace) X(so3_integrate)                  \
   X(so3_integrate_backward) X(so3_rotate_spectrum) X(project_on_sphere)                            \
   X(attention_workspace) X(attention_saved_bytes) X(attention) X(attention_backward_workspace) X(attention_backward)        \
-  X(layer_norm) X(layer_norm_backward_workspace) X(layer_norm_backward) X(dropout)
+  X(layer_norm) X(layer_norm_backward_workspace) X(layer_norm_backward) X(dropout) X(dropout_numbers)
 
 struct Ops {
 #define X(name) decltype(&::s2c_##name) name##_ = nullptr;
@@ -767,17 +767,26 @@ struct Ops {
     return {dx, dw, db};
   }
 
-  Tensor dropout(const Tensor& x_, const Tensor& residual_, double p, uint64_t seed, uint64_t step) const {
+  // numbers: int64 {seed, step} on the device of x, in place of the two (undefined: not given)
+  Tensor dropout(const Tensor& x_, const Tensor& residual_, double p, uint64_t seed, uint64_t step, const Tensor& numbers) const {
     const int dtype = prep_seq(x_);
     check(p >= 0 && p < 1, "dropout: 0 <= p < 1");
     if (residual_.defined()) {
       prep_like(residual_, x_, "dropout: residual");
       check(residual_.sizes() == x_.sizes(), "dropout: x and residual differ in shape");
     }
+    if (numbers.defined()) {
+      if (numbers.scalar_type() != at::kLong || numbers.device() != x_.device())
+        raise(PyExc_TypeError, "dropout: seed and step as an int64 tensor on the device of x");
+      check(numbers.dim() == 1 && numbers.size(0) == 2 && numbers.is_contiguous(), "dropout: two consecutive numbers, seed and step");
+    }
     const Tensor x = x_.contiguous(), residual = residual_.defined() ? residual_.contiguous() : residual_;
     Tensor out = at::empty_like(x);
     Ctx c(*this, x);
-    S2C_CALL(dropout, dtype, vptr(x), vptr(residual), vmut(out), (long)x.numel(), p, (unsigned long long)seed, (unsigned long long)step, c.stream);
+    if (numbers.defined())
+      S2C_CALL(dropout_numbers, dtype, vptr(x), vptr(residual), vmut(out), (long)x.numel(), p, static_cast<const unsigned long long*>(vptr(numbers)), c.stream);
+    else
+      S2C_CALL(dropout, dtype, vptr(x), vptr(residual), vmut(out), (long)x.numel(), p, (unsigned long long)seed, (unsigned long long)step, c.stream);
     return out;
   }
 };
@@ -1015,19 +1024,22 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 struct Dropout : torch::autograd::Function<Dropout> {
-  static Tensor forward(AutogradContext* ctx, int64_t ops, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t step) {
+  static Tensor forward(AutogradContext* ctx, int64_t ops, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t step,
+                        const OptTensor& numbers) {
     keep_ops(ctx, ops);
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["p"] = p;
     ctx->saved_data["seed"] = seed;
     ctx->saved_data["step"] = step;
-    return reinterpret_cast<Ops*>(ops)->dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step);
+    ctx->save_for_backward({or_none(numbers)});
+    return reinterpret_cast<Ops*>(ops)->dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step, or_none(numbers));
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list g) {
     Tensor dx;
     if (ctx->needs_input_grad(0))
-      dx = ops_of(ctx)->dropout(g[0], Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["step"].toInt());
-    return {Variable(), dx, ctx->saved_data["residual"].toBool() ? g[0] : Variable(), Variable(), Variable(), Variable()};
+      dx = ops_of(ctx)->dropout(g[0], Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["step"].toInt(),
+                                ctx->get_saved_variables()[0]);
+    return {Variable(), dx, ctx->saved_data["residual"].toBool() ? g[0] : Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
 bool wants_any(std::initializer_list<Tensor> ts) {
@@ -1115,11 +1127,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             if (wants_any({x, or_none(w), or_none(b)})) return LayerNorm::apply(id(o), x, w, b, eps);
             return std::get<0>(o.layer_norm(x, or_none(w), or_none(b), eps, false));
           }, "x"_a, "weight"_a, "bias"_a, "eps"_a, nogil)
-      .def("ag_dropout", [](Ops& o, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t step) {
-            S2C_TRACED("ag_dropout", x, residual, p, seed, step);
-            if (wants_any({x, or_none(residual)})) return Dropout::apply(id(o), x, residual, p, seed, step);
-            return o.dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step);
-          }, "x"_a, "residual"_a, "p"_a, "seed"_a, "step"_a, nogil)
+      .def("ag_dropout", [](Ops& o, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t step, const OptTensor& numbers) {
+            S2C_TRACED("ag_dropout", x, residual, p, seed, step, numbers);
+            if (wants_any({x, or_none(residual)})) return Dropout::apply(id(o), x, residual, p, seed, step, numbers);
+            return o.dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step, or_none(numbers));
+          }, "x"_a, "residual"_a, "p"_a, "seed"_a, "step"_a, "numbers"_a, nogil)
       .def("ag_s2_fft_real", [](Ops& o, const Tensor& x, std::optional<int64_t> b) {
             S2C_TRACED("ag_s2_fft_real", x, b);
             return wants_grad(x) ? S2FftReal::apply(id(o), x, b_arg(b)) : o.s2_fft(x, false, b, true);

@@ -70,10 +70,14 @@ def dropout(x, p, seed, step=0, residual=None):
 
     The mask is a function of (seed, step, index of the element): the same for the same numbers, never
     stored, computed again for the gradient.  Give every place in a model a ``seed`` and every call a ``step``
-    of its own (both below 2^63).
+    of its own (both below 2^63).  Numbers are part of a captured or recorded call; ``seed`` may instead be an
+    int64 tensor of the two on the device of x, which the kernel reads when it runs.
     """
+    if isinstance(seed, torch.Tensor):
+        assert step == 0, "dropout: the tensor holds the step, too"
+        return cuda_ops().ag_dropout(x, residual, float(p), 0, 0, seed)
     assert 0 <= seed < 1 << 63 and 0 <= step < 1 << 63
-    return cuda_ops().ag_dropout(x, residual, float(p), int(seed), int(step))
+    return cuda_ops().ag_dropout(x, residual, float(p), int(seed), int(step), None)
 
 
 class RelativeBias(nn.Module):
@@ -100,21 +104,20 @@ class LayerNorm(nn.Module):
 
 
 class Dropout(nn.Module):
-    """``dropout`` with a seed drawn at construction (from torch's generator) and a step that counts the calls
-    in training mode; in evaluation ``residual + x``."""
+    """``dropout`` with a seed and a step that every call in training mode draws from torch's generator of the device of
+    x; in evaluation ``residual + x``.  So a call that activation checkpointing repeats has the mask of the first one (it
+    restores the generator), a saved state of the generator brings the masks back, and a captured call has a new mask
+    in every replay."""
 
     def __init__(self, p):
         super().__init__()
         assert 0 <= p < 1
         self.p = p
-        self.seed = int(torch.randint(1 << 62, ()))
-        self.step = 0
 
     def forward(self, x, residual=None):
         if not self.training or self.p == 0:
             return x if residual is None else residual + x
-        self.step += 1
-        return dropout(x, self.p, self.seed, self.step, residual)
+        return dropout(x, self.p, torch.randint(1 << 62, (2,), device=x.device), residual=residual)
 
 
 class SequenceBlock(nn.Module):
