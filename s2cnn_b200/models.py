@@ -128,13 +128,15 @@ class SphereSequenceNet(nn.Module):
 
     def forward(self, x, lengths=None):
         """:param x: [batch, length, 1, 2 b_in, 2 b_in], sequences padded to the longest
-        :param lengths: int32 [batch], the signals of each sequence (None: all)
+        :param lengths: int32 [batch], the signals of each sequence (None: all); the others are not looked at
         :return: [batch, f_output]"""
+        if lengths is not None:
+            padded = (torch.arange(x.size(1), device=x.device) >= lengths[:, None])[..., None]
+            x = x.masked_fill(padded[..., None, None], 0)       # (a NaN times 0 would be one in the parameters' gradients)
         y = self.features(x)
         for block in self.blocks:
             y = block(y, lengths)
         y = self.norm(y)
         if lengths is None:
             return self.out_layer(y.mean(1))
-        filled = torch.arange(x.size(1), device=x.device) < lengths[:, None]
-        return self.out_layer((y * filled[..., None]).sum(1) / lengths.clamp_min(1)[:, None])
+        return self.out_layer(y.masked_fill(padded, 0).sum(1) / lengths.clamp_min(1)[:, None])
