@@ -332,7 +332,7 @@ struct AttnFew {
       if (p.splits == 1) {
         const float2 st = attn_stats(top, sum);
         const long to = (((long)b * p.lq + i) * p.heads + h) * p.dim + c;
-        if (c < p.dim) narrow_with_rest(static_cast<T*>(p.out) + to, p.out_lo ? static_cast<T*>(p.out_lo) + to : nullptr, o * st.y);
+        if (c < p.dim) narrow_with_rest(static_cast<T*>(p.out) + to, p.out_lo ? static_cast<T*>(p.out_lo) + to : nullptr, st.y == 0.f ? 0.f : o * st.y);
         if (p.stats && c == 0) p.stats[((long)b * p.heads + h) * p.lq + i] = st;
       } else {
         float* part = p.part + ((long)ctx.bid * rows + r) * (DP + 2);
@@ -387,7 +387,7 @@ struct AttnJoin {
     const float2 st = attn_stats(m, l);
     if (t < p.dim) {
       const long to = (((long)b * p.lq + i) * p.heads + h) * p.dim + t;
-      narrow_with_rest(static_cast<T*>(p.out) + to, p.out_lo ? static_cast<T*>(p.out_lo) + to : nullptr, o * st.y);
+      narrow_with_rest(static_cast<T*>(p.out) + to, p.out_lo ? static_cast<T*>(p.out_lo) + to : nullptr, st.y == 0.f ? 0.f : o * st.y);
     }
     if (p.stats && t == 0) p.stats[((long)b * p.heads + h) * p.lq + i] = st;
   }

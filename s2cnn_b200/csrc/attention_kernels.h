@@ -240,7 +240,7 @@ struct AttnForward {
       const float sum = lanes_sum<16>(ctx, l[r]);
       const float inv = attn_stats(m[r], sum).y;
 #pragma unroll
-      for (int c = 0; c < Tile::kCols; ++c) acc[r][c] *= inv;
+      for (int c = 0; c < Tile::kCols; ++c) acc[r][c] = inv == 0.f ? 0.f : acc[r][c] * inv;      // (0 times a NaN that others see)
       const int i = i0 + 4 * ty + r;
       if (p.stats && tx == 0 && i < p.lq) p.stats[(long)bh * p.lq + i] = attn_stats(m[r], sum);
     }
@@ -334,7 +334,7 @@ struct AttnGradQ {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < Tile::kCols; ++c) acc[r][c] *= p.scale;
+      for (int c = 0; c < Tile::kCols; ++c) acc[r][c] = inv[4 * ty + r] == 0.f ? 0.f : acc[r][c] * p.scale;
     Tile::store(static_cast<T*>(p.dq) + row0, (T*)nullptr, row_stride, i0, p.lq, p.dim, ty, tx, acc);
     if (!p.dbias_part) return;
     ctx.sync();

@@ -341,7 +341,7 @@ struct AttnTcGradQ {
         }
         float v[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = !ok ? bulk_nan() : n ? as_float(o[e]) * p.scale : 0.f;
+        for (int e = 0; e < 32; ++e) v[e] = !ok ? bulk_nan() : n && inv != 0.f ? as_float(o[e]) * p.scale : 0.f;      // (inv 0: sees nothing)
         if (i < p.lq) tcx_put_row(static_cast<bf16*>(p.dq) + at, nullptr, v, 32, p.dim, c, wide);
       }
       if (p.dbias_part) {

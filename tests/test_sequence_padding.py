@@ -30,3 +30,23 @@ def test_padded_signals_change_no_answer_and_no_gradient(backend, value):
             results.append([y.detach(), leaf.grad] + [p.grad.clone() for p in m.parameters()])
         for a, b in zip(*results):
             assert bool(torch.isfinite(b).all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lq", [2, 70])
+def test_a_query_that_sees_nothing_gives_zero_beside_others(backend, dtype, lq):
+    """Where other queries of the block see an infinity or a NaN, one that sees no key still gives 0, and no gradient of its own."""
+    with backends.active(backend) as (_, dev):
+        gen = torch.Generator().manual_seed(31)
+        q, k, v, g = (torch.randn(2, n, 2, 24, generator=gen).to(dtype).to(dev) for n in (lq, 200, 200, lq))
+        k[:, 0, :, 3], v[:, 0, :, 5], v[:, 0, :, 6] = math.nan, math.inf, math.nan
+        ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        for kw, seen in (({"q_lengths": ints(1, 0)}, [1, 0]), ({"causal": True, "q_start": ints(1 - lq, -lq)}, [-1, 0])):
+            args = [t.clone().requires_grad_(True) for t in (q, k, v)]
+            out = S.attention(*args, **kw)
+            dq, = torch.autograd.grad(out, args[:1], g)
+            for b in range(2):
+                rest = slice(seen[b], None) if seen[b] >= 0 else slice(0, seen[b])
+                assert not out[b, rest].any() and not dq[b, rest].any()
+                assert not seen[b] or bool(torch.isnan(out[b, 0 if seen[b] > 0 else -1, :, 6]).all())
