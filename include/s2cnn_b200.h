@@ -348,7 +348,7 @@ typedef struct s2c_attention_desc {
   int n_buckets, reach;
 } s2c_attention_desc;
 /* out [batch][lq][heads][dim].  saved (NULL: no backward pass follows): s2c_attention_saved_bytes() bytes that
- * s2c_attention_backward reads, 16-byte aligned. */
+ * s2c_attention_backward reads.  saved and the workspaces start on 16-byte boundaries. */
 size_t s2c_attention_workspace(const s2c_attention_desc* desc);
 size_t s2c_attention_saved_bytes(const s2c_attention_desc* desc);
 int s2c_attention(const s2c_attention_desc* desc, const void* q, const void* k, const void* v, const void* bias, void* out,

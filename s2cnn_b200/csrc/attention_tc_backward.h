@@ -188,7 +188,7 @@ struct AttnTcGradQ {
       float delta = 0.f;
       if (in) {
         const bf16 *o = static_cast<const bf16*>(p.o) + at, *lo = static_cast<const bf16*>(p.out_lo) + at;
-        if (p.dim % 8 == 0) {
+        if (p.dim % 8 == 0 && reinterpret_cast<uintptr_t>(p.o) % 16 == 0) {     // (rows of dO and of the rest are fetched in pieces anyway)
           for (int c = 8 * group; c < p.dim; c += 16) {
             float x[8], y[8], z[8];
             load_vec(g_row + c, x);

@@ -120,6 +120,10 @@ inline int attn_check(const char* who, const s2c_attention_desc* d) {
   if (!(std::fabs(d->scale) <= FLT_MAX)) return fail(S2C_ERR_BAD_ARG, w + "the scale is not finite");
   return S2C_OK;
 }
+// what the library lays out itself; the caller's arrays need no more alignment than their type
+inline int attn_check_own(const char* who, const void* saved, const void* workspace) {
+  return aligned16(saved) && aligned16(workspace) ? S2C_OK : fail(S2C_ERR_BAD_ARG, std::string(who) + ": saved and workspace start on 16-byte boundaries");
+}
 inline AttnParams attn_params(const s2c_attention_desc* d, const void* q, const void* k, const void* v, const void* bias) {
   AttnParams p = {};
   p.q = q; p.k = k; p.v = v; p.bias = d->bucket_of ? bias : nullptr;
@@ -359,7 +363,7 @@ inline size_t attn_parts_bytes(const AttnParams& p, bool with_bias) {
 template <class T>
 bool attn_backward_tc(const AttnParams& p, bool with_bias) {
   const bool packed = attn_packs(p, sizeof(T));
-  if (!packed && !(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout) && aligned16(p.o))) return false;
+  if (!packed && !(aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.dout))) return false;
   const int nc = p.dim > 64 ? 2 : 1;
   const size_t q = sizeof(T) == 4 ? (nc == 1 ? AttnTc3GradQ<1>::smem(p.reach, with_bias) : AttnTc3GradQ<2>::smem(p.reach, with_bias)) : nc == 1 ? AttnTcGradQ<1>::smem(p.reach, with_bias) : AttnTcGradQ<2>::smem(p.reach, with_bias);
   const size_t kv = sizeof(T) == 4 ? (nc == 1 ? AttnTc3GradKV<1>::smem(p.reach) : AttnTc3GradKV<2>::smem(p.reach)) : nc == 1 ? AttnTcGradKV<1>::smem(p.reach) : AttnTcGradKV<2>::smem(p.reach);
@@ -503,6 +507,7 @@ int s2c_attention(const s2c_attention_desc* d, const void* q, const void* k, con
   if (some && (!q || !out || (d->lk > 0 && (!k || !v)))) return fail(S2C_ERR_BAD_ARG, "s2c_attention: a pointer is missing");
   if ((bias != nullptr) != (d->bucket_of != nullptr)) return fail(S2C_ERR_BAD_ARG, "s2c_attention: a bias needs its buckets, and buckets a bias");
   AttnParams p = attn_params(d, q, k, v, bias);
+  S2C_SEQ_TRY(attn_check_own("s2c_attention", saved, workspace));
   p.out = out;
   attn_set_saved(p, d->dtype, saved);
   return d->dtype == kSeqF32 ? attn_forward<float>(p, workspace, workspace_bytes, (stream_t)stream)
@@ -526,6 +531,7 @@ int s2c_attention_backward(const s2c_attention_desc* d, const void* q, const voi
   if ((bias != nullptr) != (d->bucket_of != nullptr) || (dbias && !bias))
     return fail(S2C_ERR_BAD_ARG, "s2c_attention_backward: a bias needs its buckets, and buckets a bias");
   AttnParams p = attn_params(d, q, k, v, bias);
+  S2C_SEQ_TRY(attn_check_own("s2c_attention_backward", saved, workspace));
   p.o = out; p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
   attn_set_saved(p, d->dtype, const_cast<void*>(saved));
   return d->dtype == kSeqF32 ? attn_backward<float>(p, dbias, workspace, workspace_bytes, (stream_t)stream)
