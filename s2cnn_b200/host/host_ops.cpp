@@ -720,7 +720,7 @@ struct Ops {
   std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(AttnArgs a, const Tensor& out, const Tensor& saved, const Tensor& dout_,
                                                                 bool want_bias) const {
     const s2c_attention_desc d = attention_desc(a);
-    const Tensor dout = dout_.contiguous();
+    const Tensor dout = unit_stride(dout_.contiguous());
     Tensor dq = at::empty({d.batch, d.lq, d.heads, d.dim}, a.q.options()), dk = at::empty({d.batch, d.lk, d.kv_heads, d.dim}, a.q.options()),
            dv = at::empty_like(dk), dbias;
     if (want_bias) dbias = at::empty_like(a.bias);

@@ -98,3 +98,16 @@ def test_saved_and_workspace_are_aligned(backend):
             with pytest.raises(_lib.S2cError, match="status 1"):
                 ops.lib.call("s2c_attention_backward", p, q.data_ptr(), k.data_ptr(), v.data_ptr(), None, out.data_ptr(), saved, g.data_ptr(), out.data_ptr(),
                              k.data_ptr(), v.data_ptr(), None, ws, 1 << 21, stream_of(dev))
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_off_a_boundary_takes_the_same_kernels(backend, dtype):
+    """What comes back for dout is the same to the last bit wherever dout lies."""
+    with backends.active(backend) as (_, dev):
+        q, k, v, g = operands(dev, dtype, 1, 130, 140, 2, 64, 0)
+        args = [t.requires_grad_(True) for t in (q, k, v)]
+        off = off_by(g, 1)
+        assert off.is_contiguous() and off.data_ptr() % 16
+        a, b = (torch.autograd.grad(S.attention(*args), args, t) for t in (g, off))
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
