@@ -20,7 +20,9 @@
 namespace s2c {
 
 // ---- rows of a tensor of any strides, packed: [part][batch][head][position][8 chunks], zeros behind the values -----------------
+// Only rows that some query sees, and queries that are filled: nothing reads the places of the others.
 struct AttnPackParams {
+  AttnParams a;            // lengths and positions
   const void* src[4];
   bf16* dst[4];
   long stride[4][3];       // batch entry, position, head
@@ -42,6 +44,8 @@ struct AttnPack {
       const int h = (int)(r % p.heads[t]);
       r /= p.heads[t];
       const int i = (int)(r % p.len[t]), b = (int)(r / p.len[t]);
+      const AttnSeq s = attn_seq(p.a, b);
+      if (i >= (t == 0 || t == 3 ? s.qlen : attn_keys(p.a, s, s.qlen))) continue;
       const T* from = static_cast<const T*>(p.src[t]) + b * p.stride[t][0] + i * p.stride[t][1] + h * p.stride[t][2] + 8 * c;
       bf16* to = p.dst[t] + (((long)b * p.heads[t] + h) * p.len[t] + i) * 8 * p.chunks + 8 * c;
       float v[8];

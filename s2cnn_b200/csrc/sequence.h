@@ -250,6 +250,7 @@ int attn_pack(AttnTcParams& t, const AttnPacked& k, char* ws, stream_t st) {
   const void* src[4] = {p.q, p.k, p.v, p.dout};
   const long* stride[4] = {p.qs, p.ks, p.vs, t.gs};
   long most = 0;
+  c.a = p;
   c.tensors = k.tensors; c.batch = p.batch; c.dim = p.dim; c.chunks = k.chunks;
   for (int i = 0; i < k.tensors; ++i) {
     const bool of_q = i == 0 || i == 3;

@@ -111,3 +111,35 @@ def test_gradient_off_a_boundary_takes_the_same_kernels(backend, dtype):
         assert off.is_contiguous() and off.data_ptr() % 16
         a, b = (torch.autograd.grad(S.attention(*args), args, t) for t in (g, off))
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_rows_that_nobody_sees_are_not_packed(dtype, causal):
+    """A workspace keeps what it held where the packed copies of rows beyond the lengths, and of keys behind all queries, would
+    be: [tensor][part][batch][head][position][values], each tensor from a 256-byte boundary on."""
+    ops, dev = backends.get("cuda")
+    B, Lq, Lk, H, D = 3, 130, 300, 2, 20
+    q, k, v, g = operands(dev, dtype, B, Lq, Lk, H, D, 0)
+    q_lengths, kv_lengths = [130, 0, 70], [200, 300, 40]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    starts = i32([-60, 0, 10])
+    keep = i32(q_lengths), i32(kv_lengths)
+    _, ws, back = call(ops, dev, q, k, v, g, q_lengths=keep[0], kv_lengths=keep[1], q_starts=starts, causal=causal)
+    keys = [min(n, max(0, s + m)) if causal else n for n, m, s in zip(kv_lengths, q_lengths, [-60, 0, 10])]
+
+    def untouched(rows, lengths):
+        t = torch.zeros((3 if dtype == F32 else 1, B, H, rows, 24 * 2), dtype=torch.bool)
+        for b, n in enumerate(lengths):
+            t[:, b, :, n:] = True
+        t = t.flatten()
+        return torch.cat((t, torch.zeros(-len(t) % 256, dtype=torch.bool)))
+
+    parts = [untouched(Lq, q_lengths), untouched(Lk, keys), untouched(Lk, keys), untouched(Lq, q_lengths)]
+    for space, of in ((ws, parts[:3]), (back, parts)):
+        mask = torch.cat(of)
+        assert len(mask) <= len(space)
+        mask = torch.cat((torch.zeros(len(space) - len(mask), dtype=torch.bool), mask))
+        assert mask.any() and bool((space.cpu()[mask] == 0x5A).all())
+        assert bool((space.cpu()[~mask] != 0x5A).any())
