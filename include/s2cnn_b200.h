@@ -323,7 +323,8 @@ int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, 
  * buckets of the relative position, layer norm, dropout, each with its gradient (no counterpart in the
  * reference).  `dtype` is the type of every value array of a call: 0 float32, 1 bfloat16; arithmetic
  * and sums are float32 for both.  These arrays need no more alignment than their type.  Results and
- * gradients are the same to the last bit in every call on the same inputs.
+ * gradients are the same to the last bit in every call on the same inputs, whether a backward pass is
+ * prepared or not (of attention: with the same bias_grad).
  *
  * A call of s2c_attention, q [batch][lq][heads][dim], k and v [batch][lk][kv_heads][dim], any strides
  * (in elements, of the first three axes; the last is contiguous), dim <= 128, heads a multiple of
@@ -346,6 +347,8 @@ typedef struct s2c_attention_desc {
   const int *q_starts, *q_lengths, *kv_lengths;
   const int* bucket_of;
   int n_buckets, reach;
+  int bias_grad;       /* dbias will be asked for: bfloat16 weights keep their rounding in a second product, for a dbias whose error is
+                        * that of its own rounding (see attention_tc_forward.h); costs the forward pass up to 30 % */
 } s2c_attention_desc;
 /* out [batch][lq][heads][dim].  saved (NULL: no backward pass follows): s2c_attention_saved_bytes() bytes that
  * s2c_attention_backward reads.  saved and the workspaces start on 16-byte boundaries. */

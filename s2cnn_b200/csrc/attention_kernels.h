@@ -34,7 +34,7 @@ struct AttnParams {
   const int *bucket_of, *start, *q_len, *kv_len;
   long qs[3], ks[3], vs[3];       // elements from one batch entry, position, head to the next
   int batch, lq, lk, heads, kv_heads, dim, group;
-  int causal, start_all, reach, n_buckets;
+  int causal, start_all, reach, n_buckets, bias_grad;
   float scale;
   int tiles, splits, chunk;       // tiles of the blocked axis; splits of the keys, of `chunk` keys each
 };

@@ -13,8 +13,8 @@
 // Its registers come from the third warpgroup (launched with 168 each: 8 x 208 + 4 x 88 = 12 x 168).
 // The output is rescaled only where the maximum of a row has grown by more than 8 (in units of ln 2) since it was last fixed:
 // weights then reach 2^8 at most, which costs no precision, and after the first tiles rescaling all but ends.
-// 2 x 4096 positions, 16 heads of 128: 257 us, 1071 TFLOP/s (the last wave halved); with a bias 264, and 340 where its gradient may
-// follow.  Bound by the exponentials (16 a clock and SM: 60 % of the time) and the tensor pipe (66 % of the measured peak), which
+// 2 x 4096 positions, 16 heads of 128: 257 us, 1071 TFLOP/s (the last wave halved); with a bias 264, and 340 where its gradient is
+// asked for.  Bound by the exponentials (16 a clock and SM: 60 % of the time) and the tensor pipe (66 % of the measured peak), which
 // overlap but in part.  A quarter of the exponentials as polynomials on the FP32 pipes gave nothing (260 us).
 // Weights in bfloat16: a relative 2^-9 on each of the many terms of an output that is itself rounded to bfloat16.
 #pragma once
@@ -39,8 +39,8 @@ inline size_t tcf_smem(int blocks, int per_block, int reach) {       // blocks o
   return 1024 + (size_t)(per_block + 4) * blocks * kTcxTile + (size_t)per_block * (2 * reach + 2 * kTcxMargin + 1) * sizeof(float) + sizeof(TcfBars) + 16;
 }
 
-// FINE: the weights' rounding goes into a second product, in the other half of the scores' columns.  For the bias gradient: it sums
-// dS = P (dP - delta) over all rows, delta = dO . O is one number for a whole row, and an output whose weights were rounded
+// FINE, where a bias gradient will be asked for: the weights' rounding goes into a second product, in the other half of the
+// scores' columns.  That gradient sums dS = P (dP - delta) over all rows, delta = dO . O is one number for a whole row, and an output whose weights were rounded
 // gives it an error that does not average out (relative error of the bias gradient, 2 x 4096 positions, 16 heads of 128:
 // 2.4e-3 without, against 1.7e-3 of its own rounding).
 template <int NC, bool FINE>

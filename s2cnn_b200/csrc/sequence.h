@@ -132,7 +132,7 @@ inline AttnParams attn_params(const s2c_attention_desc* d, const void* q, const 
   p.batch = d->batch; p.lq = d->lq; p.lk = d->lk; p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->dim;
   p.group = d->heads / d->kv_heads;
   p.causal = d->causal != 0; p.scale = d->scale; p.start_all = d->q_start;
-  p.reach = p.bias ? d->reach : 0; p.n_buckets = p.bias ? d->n_buckets : 0;
+  p.reach = p.bias ? d->reach : 0; p.n_buckets = p.bias ? d->n_buckets : 0; p.bias_grad = p.bias && d->bias_grad;
   p.splits = 1;
   return p;
 }
@@ -322,7 +322,7 @@ int attn_tc_forward_launch(const AttnParams& p, char* ws, size_t ws_bytes, strea
     t.whole = (int)(halve ? blocks - rest : blocks);
     const long grid = blocks + (halve ? rest : 0);
     const size_t smem = tcf_smem(nc, t.per_block, p.reach);
-    if (p.bias && p.stats)        // a bias gradient may follow
+    if (p.bias_grad)
       return nc == 1 ? attn_tc_launch<AttnTcForward<1, true>>("attention_tc", grid, smem, st, t)
                      : attn_tc_launch<AttnTcForward<2, true>>("attention_tc", grid, smem, st, t);
     return nc == 1 ? attn_tc_launch<AttnTcForward<1, false>>("attention_tc", grid, smem, st, t)

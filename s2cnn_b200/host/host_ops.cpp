@@ -670,6 +670,7 @@ struct Ops {
     bool causal = false;
     double scale = 0;
     int64_t q_start = 0;
+    bool bias_grad = false;
   };
   s2c_attention_desc attention_desc(AttnArgs& a) const {
     const int dtype = prep_seq(a.q);
@@ -693,6 +694,7 @@ struct Ops {
     d.causal = a.causal;
     d.scale = (float)a.scale;
     d.q_start = (int)a.q_start;
+    d.bias_grad = a.bias_grad;
     d.q_starts = int_ptr(a.starts, a.q, d.batch, "attention: q_start");
     d.q_lengths = int_ptr(a.q_lengths, a.q, d.batch, "attention: q_lengths");
     d.kv_lengths = int_ptr(a.kv_lengths, a.q, d.batch, "attention: kv_lengths");
@@ -987,7 +989,8 @@ struct Attention : torch::autograd::Function<Attention> {
     keep_ops(ctx, ops);
     const Tensor bias = or_none(bias_), buckets = or_none(buckets_), starts = or_none(starts_), q_lengths = or_none(q_lengths_), kv_lengths = or_none(kv_lengths_);
     Tensor out, saved;
-    std::tie(out, saved) = reinterpret_cast<Ops*>(ops)->attention({q, k, v, bias, buckets, starts, q_lengths, kv_lengths, causal, scale, q_start}, true);
+    std::tie(out, saved) = reinterpret_cast<Ops*>(ops)->attention({q, k, v, bias, buckets, starts, q_lengths, kv_lengths, causal, scale, q_start,
+                                                                          bias.defined() && bias.requires_grad()}, true);
     ctx->save_for_backward({q, k, v, bias, buckets, starts, q_lengths, kv_lengths, out, saved});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;

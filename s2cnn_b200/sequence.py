@@ -9,7 +9,9 @@ sphere) and an answer about all of them.
 
 and the modules built on them, ``RelativeBias``, ``LayerNorm``, ``Dropout`` and ``SequenceBlock``.  The
 reference has no counterpart.  Tensors are float32 or bfloat16 (one type per call; all arithmetic and sums
-are float32); results and gradients are the same to the last bit in every call on the same inputs.
+are float32); results and gradients are the same to the last bit in every call on the same inputs, recorded for
+gradients or not (but for the output of bfloat16 attention where the gradient of a bias is wanted: its weights are
+kept more exactly then).
 """
 import math
 

@@ -19,7 +19,7 @@ class Desc(ctypes.Structure):
                 [(n, ctypes.c_long * 3) for n in ("q_stride", "k_stride", "v_stride")] +
                 [("causal", ctypes.c_int), ("scale", ctypes.c_float), ("q_start", ctypes.c_int)] +
                 [(n, ctypes.c_void_p) for n in ("q_starts", "q_lengths", "kv_lengths", "bucket_of")] +
-                [(n, ctypes.c_int) for n in ("n_buckets", "reach")])
+                [(n, ctypes.c_int) for n in ("n_buckets", "reach", "bias_grad")])
 
 
 def describe(q, k, v, **kw):
@@ -143,3 +143,17 @@ def test_rows_that_nobody_sees_are_not_packed(dtype, causal):
         mask = torch.cat((torch.zeros(len(space) - len(mask), dtype=torch.bool), mask))
         assert mask.any() and bool((space.cpu()[mask] == 0x5A).all())
         assert bool((space.cpu()[~mask] != 0x5A).any())
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lq", [3, 200])
+def test_output_is_the_same_recorded_or_not(backend, dtype, lq):
+    """To the last bit, where the bias itself wants no gradient."""
+    with backends.active(backend) as (_, dev):
+        q, k, v, _ = operands(dev, dtype, 2, lq, 200, 2, 64, 0)
+        table, buckets = torch.randn(16, 2, generator=torch.Generator().manual_seed(41)).to(dtype).to(dev), S.relative_buckets(16, 30, device=dev)
+        plain = S.attention(q, k, v, table, buckets)
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        recorded = S.attention(*leaves, table, buckets)
+        assert recorded.requires_grad and torch.equal(plain, recorded)
