@@ -15,6 +15,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <atomic>
@@ -982,7 +984,23 @@ struct RotateSpectrum : torch::autograd::Function<RotateSpectrum> {
 };
 
 // ---- sequences of signals ---------------------------------------------------------------------------
+bool wants_any(std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
 Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
+// Gradients that a kernel computed from `inputs`, in a backward pass that is recorded itself (create_graph): a second derivative
+// through them is refused when it is asked for, instead of missing from a sum.
+void refuse_second(const char* what, const tensor_list& inputs, std::initializer_list<Tensor*> grads) {
+  if (!at::GradMode::is_enabled()) return;
+  const std::shared_ptr<torch::autograd::Node> refusal(
+      new torch::autograd::Error(std::string("s2cnn_b200: ") + what + " has no second derivative", torch::autograd::collect_next_edges(inputs)),
+      torch::autograd::deleteNode);
+  for (Tensor* g : grads)
+    if (g->defined()) torch::autograd::set_history(*g, refusal);
+}
 struct Attention : torch::autograd::Function<Attention> {
   static Tensor forward(AutogradContext* ctx, int64_t ops, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias_, const OptTensor& buckets_,
                         const OptTensor& starts_, const OptTensor& q_lengths_, const OptTensor& kv_lengths_, bool causal, double scale, int64_t q_start) {
@@ -1003,6 +1021,7 @@ struct Attention : torch::autograd::Function<Attention> {
     std::tie(dq, dk, dv, dbias) = ops_of(ctx)->attention_backward(
         {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["q_start"].toInt()},
         s[8], s[9], g[0], s[3].defined() && ctx->needs_input_grad(3));
+    refuse_second("attention", {s[0], s[1], s[2], s[3], g[0]}, {&dq, &dk, &dv, &dbias});
     return {Variable(), dq, dk, dv, dbias, Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
@@ -1023,6 +1042,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const bool has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["b"].toBool();   // (inputs not given have no index)
     std::tie(dx, dw, db) = ops_of(ctx)->layer_norm_backward(s[0], s[1], s[2], g[0], ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1),
                                                             has_b && ctx->needs_input_grad(has_w ? 2 : 1));
+    refuse_second("layer norm", {s[0], s[1], g[0]}, {&dx, &dw, &db});
     return {Variable(), dx, dw, db, Variable()};
   }
 };
@@ -1039,19 +1059,17 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list g) {
     Tensor dx;
-    if (ctx->needs_input_grad(0))
-      dx = ops_of(ctx)->dropout(g[0], Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["step"].toInt(),
-                                ctx->get_saved_variables()[0]);
+    if (ctx->needs_input_grad(0)) {
+      const double p = ctx->saved_data["p"].toDouble();
+      const int64_t ops = ctx->saved_data["ops"].toInt(), seed = ctx->saved_data["seed"].toInt(), step = ctx->saved_data["step"].toInt();
+      const Tensor numbers = ctx->get_saved_variables()[0];
+      // (linear: its own derivative again)
+      dx = wants_any({g[0]}) ? Dropout::apply(ops, g[0], OptTensor(), p, seed, step, numbers.defined() ? OptTensor(numbers) : OptTensor())
+                             : ops_of(ctx)->dropout(g[0], Tensor(), p, (uint64_t)seed, (uint64_t)step, numbers);
+    }
     return {Variable(), dx, ctx->saved_data["residual"].toBool() ? g[0] : Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
-bool wants_any(std::initializer_list<Tensor> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor& t : ts)
-    if (t.defined() && t.requires_grad()) return true;
-  return false;
-}
-
 // Under torch.jit.trace an op runs as a Python autograd function (ops._traced), which the tracer records as one
 // node that calls the op again.
 template <class... A>
