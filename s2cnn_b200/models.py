@@ -109,7 +109,8 @@ class Shrec17Model(nn.Module):
 class SphereSequenceNet(nn.Module):
     """One answer about a sequence of spherical signals: S2Conv(1 -> f1, b_in -> b_l1), ReLU, SO3Conv(f1 -> f2,
     b_l1 -> b_l2), ReLU, so3_integrate for every signal; ``layers`` SequenceBlocks over the f2 features of the
-    signals in order; layer norm, mean over the filled positions, Linear(f2 -> f_output)."""
+    signals in order; layer norm, mean over the filled positions, Linear(f2 -> f_output).  The spherical layers are float32;
+    ``net.blocks.to(torch.bfloat16)`` or ``torch.autocast`` has the blocks in bfloat16."""
 
     def __init__(self, f1=20, f2=40, f_output=10, b_in=30, b_l1=10, b_l2=6, layers=2, heads=4, p=0.1, num_buckets=16, reach=30,
                  causal=False):

@@ -93,7 +93,7 @@ class RelativeBias(nn.Module):
 
 
 class LayerNorm(nn.Module):
-    """``layer_norm`` with a learned weight and bias (parameter names as in torch)."""
+    """``layer_norm`` with a learned weight and bias (parameter names as in torch), in the type of these."""
 
     def __init__(self, features, eps=1e-5):
         super().__init__()
@@ -102,7 +102,7 @@ class LayerNorm(nn.Module):
         self.bias = Parameter(torch.zeros(features))
 
     def forward(self, x):
-        return layer_norm(x, self.weight, self.bias, self.eps)
+        return layer_norm(x.to(self.weight.dtype), self.weight, self.bias, self.eps)
 
 
 class Dropout(nn.Module):
@@ -130,6 +130,9 @@ class SequenceBlock(nn.Module):
     ``step(x, keys, values, filled)`` takes new positions [batch, new, features] of sequences whose first
     ``filled`` (int32 [batch]) keys and values are kept in ``keys``, ``values`` [batch, room, kv_heads, dim]:
     it writes the new ones behind them and answers for the new positions.
+
+    With its parameters in bfloat16, or under ``torch.autocast`` to bfloat16 (``keys`` and ``values`` bfloat16 then), the products and
+    attention run in that type; what goes around them keeps the type of x.
     """
 
     def __init__(self, features, heads, kv_heads=None, causal=False, p=0.1, num_buckets=32, reach=128, hidden=None):
@@ -149,12 +152,12 @@ class SequenceBlock(nn.Module):
         return self.project(self.norm1(x)).unflatten(-1, (-1, self.dim)).split((self.heads, self.kv_heads, self.kv_heads), dim=2)
 
     def _rest(self, x, a):
-        x = self.drop1(self.out(a.flatten(2)), residual=x)
-        return self.drop2(self.mlp(self.norm2(x)), residual=x)
+        x = self.drop1(self.out(a.flatten(2)).to(x.dtype), residual=x)
+        return self.drop2(self.mlp(self.norm2(x)).to(x.dtype), residual=x)
 
     def forward(self, x, lengths=None):
         q, k, v = self._projected(x)
-        a = attention(q, k, v, self.bias.weight, self.bias.buckets, causal=self.causal, q_lengths=lengths, kv_lengths=lengths)
+        a = attention(q, k, v, self.bias.weight.to(q.dtype), self.bias.buckets, causal=self.causal, q_lengths=lengths, kv_lengths=lengths)
         return self._rest(x, a)
 
     def step(self, x, keys, values, filled):
@@ -162,6 +165,6 @@ class SequenceBlock(nn.Module):
         at = filled.long()[:, None] + torch.arange(x.size(1), device=x.device)
         which = torch.arange(x.size(0), device=x.device)[:, None]
         keys[which, at], values[which, at] = k, v
-        a = attention(q, keys, values, self.bias.weight, self.bias.buckets, causal=self.causal, q_start=filled,
+        a = attention(q, keys, values, self.bias.weight.to(q.dtype), self.bias.buckets, causal=self.causal, q_start=filled,
                       kv_lengths=filled + x.size(1))
         return self._rest(x, a)
