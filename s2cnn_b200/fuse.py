@@ -3,8 +3,8 @@
 Models built on the reference look like examples/mnist/run.py:55-98 - convolution modules,
 ``F.relu`` between them, ``so3_integrate`` before the linear head - either as a hand-written
 ``forward`` or as an ``nn.Sequential``.  Written that way every layer boundary is a tensor in
-memory.  ``fuse`` traces the model once (``torch.fx``; the convolution modules are leaves,
-``so3_integrate`` is recorded as one call), finds the chains below and rewrites them into the
+memory.  ``fuse`` traces the model once (``torch.fx``; the convolution modules and those on sequences are
+leaves, ``so3_integrate``, ``attention``, ``layer_norm`` and ``dropout`` are recorded as one call each), finds the chains below and rewrites them into the
 keyword arguments of this package's modules that select the fused kernels; everything else in the
 model is left as traced.  The result computes the same function.
 
@@ -28,11 +28,13 @@ import torch
 import torch.fx
 import torch.nn.functional as F
 
+from .sequence import Dropout, LayerNorm, SequenceBlock, attention, dropout, layer_norm
 from .soft.s2_conv import S2Convolution
 from .soft.so3_conv import SO3Convolution, SO3Shortcut
 from .soft.so3_integrate import so3_integrate, so3_relu_integrate
 
-_LEAVES = (S2Convolution, SO3Convolution, SO3Shortcut)
+_LEAVES = (S2Convolution, SO3Convolution, SO3Shortcut, SequenceBlock, LayerNorm, Dropout)
+_CALLS = (so3_integrate, so3_relu_integrate, attention, layer_norm, dropout)
 _RELU_FUNCTIONS = (torch.relu, F.relu, torch.nn.functional.relu, torch.relu_)
 
 
@@ -53,7 +55,7 @@ class _RecordedCalls:
     @staticmethod
     def _stand_in(fn):
         def call(*args, **kwargs):
-            for a in args:
+            for a in (*args, *kwargs.values()):
                 if isinstance(a, torch.fx.Proxy):
                     return a.tracer.create_proxy("call_function", fn, args, kwargs)
             return fn(*args, **kwargs)
@@ -129,7 +131,7 @@ def fuse(model):
     """Returns a ``torch.fx.GraphModule`` sharing ``model``'s parameters in which the chains listed
     in the module docstring run through the fused kernels.  ``model`` itself is not modified."""
     tracer = _Tracer()
-    with _RecordedCalls(so3_integrate, so3_relu_integrate):
+    with _RecordedCalls(*_CALLS):
         graph = tracer.trace(model)
     modules = dict(model.named_modules())
     # eval-mode BatchNorm3d right after a convolution: fold it into the layer

@@ -16,6 +16,7 @@ BatchNorm3d that follows a convolution into that layer's spectrum and bias).
 """
 import numpy as np
 import torch
+import torch.fx
 import torch.nn as nn
 import torch.nn.functional as F
 
@@ -106,6 +107,23 @@ class Shrec17Model(nn.Module):
         return F.log_softmax(self.out_layer(x), dim=1)
 
 
+def _zero_padded(x, lengths):
+    """x [batch, length, ...], zeros at the positions beyond the lengths (None: all are filled)"""
+    if lengths is None:
+        return x
+    padded = torch.arange(x.size(1), device=x.device) >= lengths[:, None]
+    return x.masked_fill(padded.view(padded.shape + (1,) * (x.dim() - 2)), 0)
+
+
+def _mean_filled(y, lengths):
+    """[batch, length, features] -> [batch, features], the mean over the filled positions"""
+    return y.mean(1) if lengths is None else _zero_padded(y, lengths).sum(1) / lengths.clamp_min(1)[:, None]
+
+
+torch.fx.wrap("_zero_padded")      # ``fuse`` records a call of either: lengths may be given to the fused network or not
+torch.fx.wrap("_mean_filled")
+
+
 class SphereSequenceNet(nn.Module):
     """One answer about a sequence of spherical signals: S2Conv(1 -> f1, b_in -> b_l1), ReLU, SO3Conv(f1 -> f2,
     b_l1 -> b_l2), ReLU, so3_integrate for every signal; ``layers`` SequenceBlocks over the f2 features of the
@@ -131,13 +149,7 @@ class SphereSequenceNet(nn.Module):
         """:param x: [batch, length, 1, 2 b_in, 2 b_in], sequences padded to the longest
         :param lengths: int32 [batch], the signals of each sequence (None: all); the others are not looked at
         :return: [batch, f_output]"""
-        if lengths is not None:
-            padded = (torch.arange(x.size(1), device=x.device) >= lengths[:, None])[..., None]
-            x = x.masked_fill(padded[..., None, None], 0)       # (a NaN times 0 would be one in the parameters' gradients)
-        y = self.features(x)
+        y = self.features(_zero_padded(x, lengths))             # (a NaN times 0 would be one in the parameters' gradients)
         for block in self.blocks:
             y = block(y, lengths)
-        y = self.norm(y)
-        if lengths is None:
-            return self.out_layer(y.mean(1))
-        return self.out_layer(y.masked_fill(padded, 0).sum(1) / lengths.clamp_min(1)[:, None])
+        return self.out_layer(_mean_filled(self.norm(y), lengths))
