@@ -129,7 +129,8 @@ class SequenceBlock(nn.Module):
     ``forward(x, lengths)`` takes whole sequences, padded to the longest (``lengths`` int32 [batch]).
     ``step(x, keys, values, filled)`` takes new positions [batch, new, features] of sequences whose first
     ``filled`` (int32 [batch]) keys and values are kept in ``keys``, ``values`` [batch, room, kv_heads, dim]:
-    it writes the new ones behind them and answers for the new positions.
+    it writes the new ones behind them and answers for the new positions.  A sequence whose room they exceed gives NaN (the
+    numbers stay on the device), and the last of its keys and values are lost.
 
     With its parameters in bfloat16, or under ``torch.autocast`` to bfloat16 (``keys`` and ``values`` bfloat16 then), the products and
     attention run in that type; what goes around them keeps the type of x.
@@ -162,9 +163,11 @@ class SequenceBlock(nn.Module):
 
     def step(self, x, keys, values, filled):
         q, k, v = self._projected(x)
-        at = filled.long()[:, None] + torch.arange(x.size(1), device=x.device)
+        assert x.size(1) <= keys.size(1), "step: more new positions than there is room"
+        first = filled.clamp(0, keys.size(1) - x.size(1))
+        at = first.long()[:, None] + torch.arange(x.size(1), device=x.device)
         which = torch.arange(x.size(0), device=x.device)[:, None]
         keys[which, at], values[which, at] = k, v
         a = attention(q, keys, values, self.bias.weight.to(q.dtype), self.bias.buckets, causal=self.causal, q_start=filled,
                       kv_lengths=filled + x.size(1))
-        return self._rest(x, a)
+        return self._rest(x, a.masked_fill((first != filled)[:, None, None, None], math.nan))
