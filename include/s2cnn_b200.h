@@ -337,7 +337,11 @@ int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, 
  * bias) come together or are both NULL.  reach <= 2048, n_buckets <= 1024.  Rows of k and v that no query of
  * a block of the call sees are not read.  (Under `causal`, what one of 256 neighbouring queries sees is read for
  * all of them: an infinity or NaN among those values may reach the others, as 0 times it.)  Rows of q and dout
- * beyond q_length are not read either. */
+ * beyond q_length are not read either.
+ * An infinity or NaN that is seen makes its column of out (of v) or its rows (of q, k) infinite or NaN, which of the two
+ * depends on the size of the call (operands are split into parts for the tensor cores); a score of -infinity that is no
+ * mask may thus be NaN, too.  Sums over the keys are formed before they are divided, with weights of up to 2^8: finite values
+ * beyond 2^119 / lk may overflow in them. */
 typedef struct s2c_attention_desc {
   int dtype, batch, lq, lk, heads, kv_heads, dim;
   long q_stride[3], k_stride[3], v_stride[3];      /* batch entry, position, head */

@@ -53,6 +53,9 @@ def attention(q, k, v, bias=None, buckets=None, causal=False, scale=None, q_star
     :param q_lengths, kv_lengths: int32 [batch], the queries and keys that are filled; what is beyond them
         is not looked at.  A query that sees no key gives 0 and no gradient
     :return: [batch, queries, heads, dim]
+
+    An infinity or NaN that a query sees makes its column (in v) or the query's whole row (in q, k) infinite or NaN;
+    which of the two depends on the size of the call.
     """
     starts = None
     if isinstance(q_start, torch.Tensor):
