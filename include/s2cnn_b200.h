@@ -321,8 +321,11 @@ int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, 
 /* ---- sequences of signals ------------------------------------------------------------------- */
 /* Operators of a model over signals in order (frames, shells, rings): attention with a learned bias by
  * buckets of the relative position, layer norm, dropout, each with its gradient (no counterpart in the
- * reference).  `dtype` is the type of every value array of a call: 0 float32, 1 bfloat16; arithmetic
- * and sums are float32 for both.  These arrays need no more alignment than their type.  Results and
+ * reference).  `dtype` is the type of every value array of a call: 0 float32, 1 bfloat16.  Sums, the
+ * statistics of softmax and norm and what is computed element by element are float32 for both; bfloat16
+ * attention on the tensor cores (more than 16 query rows per key head) takes weights, and in the backward pass
+ * weights and score gradients, into its products rounded to bfloat16: a result is off by 2.4e-3 (2-norm) instead
+ * of the 1.7e-3 of its own rounding.  These arrays need no more alignment than their type.  Results and
  * gradients are the same to the last bit in every call on the same inputs, whether a backward pass is
  * prepared or not (of attention: with the same bias_grad).
  *

@@ -1,8 +1,9 @@
 // What the kernels for sequences of signals (attention, layer norm, dropout) share: the two element types, wide accesses,
 // base-2 exponentials and the launcher of a kernel written as a struct.
 //
-// All arithmetic is in float32; a bfloat16 input is widened exactly when it is read and a result rounded once, to nearest
-// even, when it is written.
+// Sums and what is computed element by element are float32; a bfloat16 input is widened exactly when it is read and a result
+// rounded once, to nearest even, when it is written.  (The bfloat16 attention kernels on the tensor cores also round the left operands of
+// their second products, weights and score gradients: see there.)
 #pragma once
 
 #include "backend.h"
