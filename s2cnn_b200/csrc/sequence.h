@@ -183,7 +183,9 @@ int attn_few_piece(const AttnParams& p) {
   };
   return fits(16) ? 16 : fits(4) ? 4 : 2;
 }
-// (the bias tables of all heads of a group have to lie beside the tiles: not with 16 heads and a reach of 2048)
+// The bias tables of all heads of a group have to lie beside the tiles.  Heads of more than 64 values, float32: not from a reach of 208
+// on with 16 heads per key head, 416 with 8, 832 with 4, 1664 with 2; bfloat16 and smaller heads have more room (bfloat16, 128 values, 16
+// heads: up to 999).  Such calls take the tiles of 64 or 128 queries.
 template <class T>
 bool attn_few_fits(const AttnParams& p) {
   return attn_few_rows(p) && attn_by_dim<T>(p.dim, [&](auto d) {
