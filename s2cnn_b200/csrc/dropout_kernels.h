@@ -5,8 +5,9 @@
 // round takes the four words (a, b, c, d) to (hi(M1 c) ^ b ^ k0, lo(M1 c), hi(M0 a) ^ d ^ k1, lo(M0 a)) and adds a Weyl
 // constant to either half of the key.  Seven rounds are the fewest that the paper found to pass all of BigCrush.
 // The gradient is the same kernel on the gradient of y, without a residual: the mask follows from the index alone, whatever
-// the shape of the launch.  Bound by memory (the generator takes some 60 instructions for 4 elements): 16384 x 1024 bfloat16 with a
-// residual 24 us, 4.2 TB/s, without 21.
+// the shape of the launch.  Bound by the loads on their way, not by their bytes: a thread has one 16-byte piece of each input in
+// flight, and the generator (some 60 instructions for 4 elements) between one piece and the next.  16384 x 1024 with a residual and
+// without, in calls among others: bfloat16 22 and 17 us (4.5 and 3.9 TB/s), float32 36 and 30 us (5.6 and 4.5).
 #pragma once
 
 #include "seq_common.h"

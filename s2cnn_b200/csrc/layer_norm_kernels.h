@@ -31,7 +31,8 @@ struct LayerNormParams {
 // T threads per row (4 ... 32 neighbouring lanes, or the whole block), each with EPT elements in pieces of VEC consecutive ones.
 // A row's raw pieces are loaded one turn ahead where they fit in 16 registers (and the team is not a block of 512), and weight
 // and bias are kept from turn to turn: what a warp has on its way is then two rows of 2 KB.  Bound by memory: 16384 x 1024
-// bfloat16, forward and backward, 34 and 54 us without, 14 and 23 with (4.9 and 4.5 TB/s; 5 more for the sums of the blocks).
+// bfloat16, forward and backward, 34 and 54 us without, 14 and 23 with (4.9 and 4.5 TB/s; 5 more for the sums of the blocks);
+// float32, a block of 128 per row whose sums are barriers, 39 and some 53 us (3.5 and 3.8 TB/s).
 template <class T_, int T, int EPT, int VEC>
 struct LayerNormTeam {
   static constexpr int kThreads = T <= 32 ? 256 : T, kTeams = kThreads / T;
