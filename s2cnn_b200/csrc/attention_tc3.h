@@ -644,8 +644,9 @@ struct AttnTc3GradQ {
       if (n) drain(n - 1);
       if (ok && n) ok = tcx_wait_warp(&bars->drained, 0);
       const bool wide = p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(p.dq) % 16 == 0;
+      const bool sees = i < s.qlen && p.stats[((long)b * p.heads + h) * p.lq + i].y != 0.f;      // (read again, see AttnTcGradQ)
 #pragma unroll
-      for (int c = 0; c < 32 * NC; ++c) acc[c] = !ok ? bulk_nan() : inv == 0.f ? 0.f : acc[c] * p.scale;
+      for (int c = 0; c < 32 * NC; ++c) acc[c] = !ok ? bulk_nan() : sees ? acc[c] * p.scale : 0.f;
       if (i < p.lq) tc3_store_row(static_cast<float*>(p.dq) + at, acc, 32 * NC, p.dim, 32 * NC * half, wide);
       if (p.dbias_part) {
         tc3_sync();
