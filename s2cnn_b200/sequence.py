@@ -107,7 +107,9 @@ class LayerNorm(nn.Module):
         self.bias = Parameter(torch.zeros(features))
 
     def forward(self, x):
-        return layer_norm(x.to(self.weight.dtype), self.weight, self.bias, self.eps)
+        if x.dtype in (torch.float32, torch.bfloat16):          # (others are refused)
+            x = x.to(self.weight.dtype)
+        return layer_norm(x, self.weight, self.bias, self.eps)
 
 
 class Dropout(nn.Module):

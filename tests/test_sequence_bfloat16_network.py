@@ -72,3 +72,12 @@ def test_network_with_bfloat16_blocks(backend):
         m(x, lengths).square().sum().backward()
         for name, p in m.named_parameters():
             assert p.grad is not None and p.grad.dtype == p.dtype and bool(torch.isfinite(p.grad).all()), name
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+def test_other_types_are_refused(backend):
+    with backends.active(backend) as (_, dev):
+        for m in (S.LayerNorm(32).to(dev), S.SequenceBlock(32, 4).to(dev)):
+            for dtype in (torch.float16, torch.float64, torch.int32):
+                with pytest.raises(TypeError):
+                    m(torch.ones(2, 5, 32, dtype=dtype, device=dev))
