@@ -323,8 +323,8 @@ int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, 
  * buckets of the relative position, layer norm, dropout, each with its gradient (no counterpart in the
  * reference).  `dtype` is the type of every value array of a call: 0 float32, 1 bfloat16.  Sums, the
  * statistics of softmax and norm and what is computed element by element are float32 for both; bfloat16
- * attention on the tensor cores (more than 16 query rows per key head) takes weights, and in the backward pass
- * weights and score gradients, into its products rounded to bfloat16: a result is off by 2.4e-3 (2-norm) instead
+ * attention on the tensor cores (forward of more than 16 query rows per key head, every backward pass) takes
+ * weights, and in the backward pass weights and score gradients, into its products rounded to bfloat16: a result is off by 2.4e-3 (2-norm) instead
  * of the 1.7e-3 of its own rounding.  These arrays need no more alignment than their type.  Results and
  * gradients are the same to the last bit in every call on the same inputs, whether a backward pass is
  * prepared or not (of attention: with the same bias_grad).
@@ -339,7 +339,8 @@ int s2c_project_on_sphere(const float* verts, int nv, const int* faces, int nf, 
  * [n_buckets][heads] and bucket_of (device int32 [2 reach + 1]; an entry outside 0 .. n_buckets - 1 means no
  * bias) come together or are both NULL.  reach <= 2048, n_buckets <= 1024.  Rows of k and v that no query of
  * a block of the call sees are not read.  (Under `causal`, what one of 256 neighbouring queries sees is read for
- * all of them: an infinity or NaN among those values may reach the others, as 0 times it.)  Rows of q and dout
+ * all of them: an infinity or NaN among those values, or in the q or dout of one that sees no key, may reach the results of the
+ * others, as 0 times it; the output of a query that sees no key is 0 all the same.)  Rows of q and dout
  * beyond q_length are not read either.
  * An infinity or NaN that is seen makes its column of out (of v) or its rows (of q, k) infinite or NaN, which of the two
  * depends on the size of the call (operands are split into parts for the tensor cores); a score of -infinity that is no

@@ -9,9 +9,9 @@ sphere) and an answer about all of them.
 
 and the modules built on them, ``RelativeBias``, ``LayerNorm``, ``Dropout`` and ``SequenceBlock``.  The
 reference has no counterpart.  Tensors are float32 or bfloat16 (one type per call).  Sums, the statistics of
-softmax and norm and what is computed element by element are float32; bfloat16 attention of more than 16 query
-rows per key head takes its weights, and in the backward pass weights and score gradients, into the products
-rounded to bfloat16 (results are off by 2.4e-3 in the 2-norm, of which their own rounding is 1.7e-3).  Results and
+softmax and norm and what is computed element by element are float32; bfloat16 attention takes its weights (of more
+than 16 query rows per key head), and in the backward pass weights and score gradients, into the products rounded
+to bfloat16 (results are off by 2.4e-3 in the 2-norm, of which their own rounding is 1.7e-3).  Results and
 gradients are the same to the last bit in every call on the same inputs, recorded for gradients or not (but for
 the output of bfloat16 attention where the gradient of a bias is wanted: its weights are kept more exactly then).
 """
