@@ -390,6 +390,58 @@ int s2c_dropout(int dtype, const void* x, const void* residual, void* out, long 
 int s2c_dropout_numbers(int dtype, const void* x, const void* residual, void* out, long n, double probability,
                         const unsigned long long* numbers, void* stream);
 
+/* Heads of queries and keys, q [batch][length][heads][dim], k and v [batch][length][kv_heads][dim], any strides (in elements, of the
+ * first three axes; the last is contiguous), dim <= 128: normed (norm != 0) head by head and turned by their position,
+ *   z = x / sqrt(mean(x^2) + eps) * weight   (weight [dim], NULL: 1;  norm == 0: z = x)
+ *   y_a = magnitude (z_a cos t - z_b sin t),  y_b = magnitude (z_a sin t + z_b cos t),  t = position * frequencies[pair]
+ * for the pairs (a, b) = (i, i + pairs), or (2 i, 2 i + 1) where interleaved != 0, i < pairs; the values from 2 pairs on are not
+ * turned.  frequencies: device float64 [pairs], radians per position; angles are computed modulo whole turns in 64 bits, so that far
+ * positions lose nothing.  The position of row i of batch entry n is start + i, positions[n] + i, or, where each != 0,
+ * positions[n * length + i] (device int32).  Arrays need no more alignment than their type. */
+typedef struct s2c_head_desc {
+  int dtype, batch, length, heads, kv_heads, dim;
+  long q_stride[3], k_stride[3], v_stride[3];      /* batch entry, position, head */
+  const double* frequencies;
+  int pairs, interleaved;
+  float magnitude;
+  int norm;
+  float eps;
+  int start, each;
+  const int *positions;
+  const int *lengths;                              /* s2c_norm_rotate_store: device int32 [batch], the rows that are filled; NULL: all */
+} s2c_head_desc;
+/* q_out, k_out: contiguous; q or k NULL: none of it. */
+int s2c_norm_rotate(const s2c_head_desc* desc, const void* q, const void* k, const void* q_weight, const void* k_weight, void* q_out, void* k_out,
+                    void* stream);
+/* Gradients of q and k (contiguous), and of the weights, from those of q_out and k_out (contiguous); NULL: not wanted.  The
+ * workspace is needed for the weights' (heads or kv_heads 0: no queries, no keys). */
+size_t s2c_norm_rotate_backward_workspace(const s2c_head_desc* desc);
+int s2c_norm_rotate_backward(const s2c_head_desc* desc, const void* q, const void* k, const void* q_weight, const void* k_weight, const void* dq_out,
+                             const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Kept keys and values in pages of one pool: keys and values [count][page][kv_heads][dim], any strides (in elements, of the first three
+ * axes).  table (device int32 [batch][columns]): position j of sequence n lies in page table[n][j / page], at j % page.  page is a
+ * power of two, at least 8.  An entry outside 0 .. count - 1 is no page: what would be written there is left out, and reads as NaN. */
+typedef struct s2c_page_desc {
+  const int* table;
+  int columns, count, page;
+  long key_stride[3], value_stride[3];             /* page, position, head */
+} s2c_page_desc;
+/* s2c_norm_rotate with the keys, and v as it is, written to the pages of their positions (rows beyond `lengths` are neither read nor
+ * written).  q_out is 0 beyond `lengths`, and NaN where the position has no page (it lies beyond the table, or the entry is none).  q
+ * NULL: keys and values alone.  Two rows with one place (two sequences that share the page): which of them it holds is not said. */
+int s2c_norm_rotate_store(const s2c_head_desc* desc, const s2c_page_desc* pages, const void* q, const void* k, const void* v, const void* q_weight,
+                          const void* k_weight, void* q_out, void* keys, void* values, void* stream);
+/* s2c_attention on keys and values in pages, without a backward pass; lk, k_stride and v_stride of the description are not used:
+ * there are columns * page positions. */
+size_t s2c_paged_attention_workspace(const s2c_attention_desc* desc, const s2c_page_desc* pages);
+int s2c_paged_attention(const s2c_attention_desc* desc, const s2c_page_desc* pages, const void* q, const void* keys, const void* values,
+                        const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream);
+/* Page target[i] becomes a copy of page source[i] (device int32, i < n; entries outside 0 .. count - 1 are left out), of page_bytes
+ * each, page_stride bytes apart.  A target that is the source or target of another i holds a mixture. */
+int s2c_copy_pages(void* storage, long page_stride, long page_bytes, int count, const int* source, const int* target, long n, void* stream);
+
 /* ---- test hooks (not part of the drop-in surface; no counterpart in the reference) ------------ */
 /* Path selection for the test-suite, so that every kernel variant can be compared with the oracle
  * at the same sizes.  The switches are process-wide atomics read once per call by the dispatcher;

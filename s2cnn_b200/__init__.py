@@ -13,8 +13,9 @@ from .s2_mm import s2_mm
 from .so3_mm import so3_mm
 from .soft import (S2Convolution, SO3Convolution, SO3Shortcut, so3_integrate, so3_relu_integrate,
                    so3_rotation)
-from .sequence import (attention, layer_norm, dropout, relative_buckets, RelativeBias, LayerNorm, Dropout,
-                       SequenceBlock)
+from .sequence import (attention, layer_norm, dropout, relative_buckets, norm_rotate, rotary_frequencies, RelativeBias,
+                       LayerNorm, Dropout, SequenceBlock)
+from .pages import norm_rotate_store, paged_attention, copy_pages, PagedCache
 from .fuse import fuse
 from . import models, projection
 from .tables import set_table_cache_dir
@@ -25,6 +26,6 @@ __all__ = [
     "so3_rotation",
     "S2Convolution", "SO3Convolution", "SO3Shortcut", "so3_integrate", "so3_relu_integrate",
     "attention", "layer_norm", "dropout", "relative_buckets", "RelativeBias", "LayerNorm", "Dropout",
-    "SequenceBlock",
+    "SequenceBlock", "norm_rotate", "rotary_frequencies", "norm_rotate_store", "paged_attention", "copy_pages", "PagedCache",
     "fuse", "models", "projection", "set_table_cache_dir",
 ]

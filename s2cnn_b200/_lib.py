@@ -107,6 +107,13 @@ _SIGNATURES = {
     "s2c_layer_norm_backward": (c_int, [c_int] + [_P] * 7 + [c_long, c_int, _P, c_size_t, _P]),
     "s2c_dropout": (c_int, [c_int, _P, _P, _P, c_long, c_double, c_ulonglong, c_ulonglong, _P]),
     "s2c_dropout_numbers": (c_int, [c_int, _P, _P, _P, c_long, c_double, _P, _P]),
+    "s2c_norm_rotate": (c_int, [_P] * 8),
+    "s2c_norm_rotate_backward_workspace": (c_size_t, [_P]),
+    "s2c_norm_rotate_backward": (c_int, [_P] * 12 + [c_size_t, _P]),
+    "s2c_norm_rotate_store": (c_int, [_P] * 11),
+    "s2c_paged_attention_workspace": (c_size_t, [_P, _P]),
+    "s2c_paged_attention": (c_int, [_P] * 8 + [c_size_t, _P]),
+    "s2c_copy_pages": (c_int, [_P, c_long, c_long, c_int, _P, _P, c_long, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

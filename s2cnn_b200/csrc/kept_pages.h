@@ -1,0 +1,92 @@
+// Keys and values in pages: where a position lies, pages copied within their pool, and keys and values brought from their pages into one
+// array for the kernels of whole tiles.
+#pragma once
+
+#include "seq_common.h"
+
+namespace s2c {
+
+constexpr int kPageLeast = 8;
+struct PageTable {
+  const int* table = nullptr;     // [batch][columns]: the page of positions [c page, (c + 1) page)
+  void* array[2] = {};            // keys, values
+  int columns = 0, count = 0, page = 1;     // pages of the pool; positions of a page, a power of two
+  // page * `page` + place in the page of position `at` of sequence b; false: it has none
+  S2C_D bool at(int b, long at, long& slot) const {
+    if (at < 0 || at >= (long)columns * page) return false;
+    const int which = table[(long)b * columns + at / page];
+    slot = (long)which * page + at % page;
+    return which >= 0 && which < count;
+  }
+};
+
+// ---- pages copied within their pool -----------------------------------------------------------------------------------
+struct PageCopyParams {
+  char* base;
+  long stride, bytes;             // from one page to the next; of a page
+  const int *source, *target;
+  long n, chunks;                 // copies; pieces of kChunk bytes of each
+  int count;
+};
+// P: bytes of one access.  A block copies kChunk bytes at a time, all loads before the stores.
+template <int P>
+struct PageCopy {
+  using Params = PageCopyParams;
+  struct alignas(P) Piece {
+    unsigned char b[P];
+  };
+  static constexpr int kThreads = 256, kBlocks = 4, kAhead = P == 16 ? 4 : 8;
+  static constexpr long kChunk = (long)kThreads * kAhead * P;
+  static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char*) {
+    for (long u = ctx.bid; u < p.n * p.chunks; u += ctx.nblk) {
+      const long i = u / p.chunks, at = u % p.chunks * kChunk + (long)ctx.tid * P;
+      const int from = p.source[i], to = p.target[i];
+      if (from < 0 || from >= p.count || to < 0 || to >= p.count) continue;
+      const char* x = p.base + from * p.stride + at;
+      char* y = p.base + to * p.stride + at;
+      Piece v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (at + (long)k * kThreads * P < p.bytes) v[k] = *reinterpret_cast<const Piece*>(x + (long)k * kThreads * P);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (at + (long)k * kThreads * P < p.bytes) *reinterpret_cast<Piece*>(y + (long)k * kThreads * P) = v[k];
+    }
+  }
+};
+
+// ---- keys and values of every sequence, one after another --------------------------------------------------------------
+struct PageGatherParams {
+  PageTable pages;
+  void* out[2];                   // [batch][length][heads][dim]
+  long stride[2][3];              // page, position, head
+  const int *q_len, *kv_len, *start;
+  int batch, length, heads, dim, lq, causal, start_all;
+};
+// A warp takes the rows of one position; NaN where its page is none.  Rows that no query sees are left as they are.
+template <class T>
+struct PageGather {
+  using Params = PageGatherParams;
+  static constexpr int kThreads = 256, kBlocks = 4;
+  static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char*) {
+    const long warps = (long)ctx.nblk * (kThreads / 32), rows = (long)p.batch * p.length;
+    const int lane = ctx.tid % 32, width = p.heads * p.dim;
+    for (long r = (long)ctx.bid * (kThreads / 32) + ctx.tid / 32; r < rows; r += warps) {
+      const int b = (int)(r / p.length), j = (int)(r % p.length);
+      if (p.kv_len && j >= p.kv_len[b]) continue;
+      if (p.causal && j > (long)(p.start ? p.start[b] : p.start_all) + (p.q_len ? p.q_len[b] : p.lq) - 1) continue;
+      long slot = 0;
+      const bool there = p.pages.at(b, j, slot);
+      for (int which = 0; which < 2; ++which) {
+        const T* from = static_cast<const T*>(p.pages.array[which]) + (there ? slot / p.pages.page * p.stride[which][0] + slot % p.pages.page * p.stride[which][1] : 0);
+        T* to = static_cast<T*>(p.out[which]) + r * width;
+        for (int e = lane; e < width; e += 32) {
+          if (there) to[e] = from[e / p.dim * p.stride[which][2] + e % p.dim];
+          else narrow(to + e, as_float(0x7fffffffu));
+        }
+      }
+    }
+  }
+};
+
+}  // namespace s2c

@@ -4,7 +4,7 @@ Models built on the reference look like examples/mnist/run.py:55-98 - convolutio
 ``F.relu`` between them, ``so3_integrate`` before the linear head - either as a hand-written
 ``forward`` or as an ``nn.Sequential``.  Written that way every layer boundary is a tensor in
 memory.  ``fuse`` traces the model once (``torch.fx``; the convolution modules and those on sequences are
-leaves, ``so3_integrate``, ``attention``, ``layer_norm`` and ``dropout`` are recorded as one call each), finds the chains below and rewrites them into the
+leaves, ``so3_integrate``, ``attention``, ``layer_norm``, ``dropout`` and ``norm_rotate`` are recorded as one call each), finds the chains below and rewrites them into the
 keyword arguments of this package's modules that select the fused kernels; everything else in the
 model is left as traced.  The result computes the same function.
 
@@ -28,13 +28,13 @@ import torch
 import torch.fx
 import torch.nn.functional as F
 
-from .sequence import Dropout, LayerNorm, SequenceBlock, attention, dropout, layer_norm
+from .sequence import Dropout, LayerNorm, SequenceBlock, attention, dropout, layer_norm, norm_rotate
 from .soft.s2_conv import S2Convolution
 from .soft.so3_conv import SO3Convolution, SO3Shortcut
 from .soft.so3_integrate import so3_integrate, so3_relu_integrate
 
 _LEAVES = (S2Convolution, SO3Convolution, SO3Shortcut, SequenceBlock, LayerNorm, Dropout)
-_CALLS = (so3_integrate, so3_relu_integrate, attention, layer_norm, dropout)
+_CALLS = (so3_integrate, so3_relu_integrate, attention, layer_norm, dropout, norm_rotate)
 _RELU_FUNCTIONS = (torch.relu, F.relu, torch.nn.functional.relu, torch.relu_)
 
 

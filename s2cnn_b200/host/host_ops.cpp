@@ -86,7 +86,9 @@ long s2_bandwidth(long nspec) {
   X(s2_mm_grady) X(s2_mm_real_gradx) X(s2_mm_real_grady) X(rft_forward) X(rft_forward_t) X(rft_forward_scaled) X(rft_backward_scaled) X(rft_backward_workspace) X(so3_integrate)                  \
   X(so3_integrate_backward) X(so3_rotate_spectrum) X(project_on_sphere)                            \
   X(attention_workspace) X(attention_saved_bytes) X(attention) X(attention_backward_workspace) X(attention_backward)        \
-  X(layer_norm) X(layer_norm_backward_workspace) X(layer_norm_backward) X(dropout) X(dropout_numbers)
+  X(layer_norm) X(layer_norm_backward_workspace) X(layer_norm_backward) X(dropout) X(dropout_numbers)                      \
+  X(norm_rotate) X(norm_rotate_backward_workspace) X(norm_rotate_backward) X(norm_rotate_store)                            \
+  X(paged_attention_workspace) X(paged_attention) X(copy_pages)
 
 struct Ops {
 #define X(name) decltype(&::s2c_##name) name##_ = nullptr;
@@ -793,6 +795,180 @@ struct Ops {
       S2C_CALL(dropout, dtype, vptr(x), vptr(residual), vmut(out), (long)x.numel(), p, (unsigned long long)seed, (unsigned long long)step, c.stream);
     return out;
   }
+  // -- heads turned by their position ---------------------------------------------------------------------
+  struct HeadArgs {      // undefined tensors: not given
+    Tensor q, k, frequencies, q_weight, k_weight, positions;
+    double eps = -1;     // negative: no norm
+    int64_t start = 0;
+    bool interleaved = false;
+    double magnitude = 1;
+    Tensor v, lengths;
+  };
+  // consecutive values in the last axis
+  static Tensor unit_last(const Tensor& t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
+  s2c_head_desc head_desc(HeadArgs& a, const char* who) const {
+    const std::string w = std::string(who) + ": ";
+    auto want = [&](bool ok, const char* what) { check(ok, (w + what).c_str()); };
+    const Tensor& any = a.q.defined() ? a.q : a.k;
+    want(any.defined(), "neither queries nor keys");
+    s2c_head_desc d = {};
+    d.dtype = prep_seq(any);
+    want(any.dim() == 4, "[batch, length, heads, dim] operands");
+    for (Tensor* t : {&a.q, &a.k, &a.v}) {
+      if (!t->defined()) continue;
+      prep_like(*t, any, who);
+      want(t->dim() == 4 && t->size(0) == any.size(0) && t->size(1) == any.size(1) && t->size(3) == any.size(3), "operands differ in batch, length or dim");
+      for (int i = 0; i < 4; ++i) want(t->size(i) <= 0x7fffffff, "too large");
+      want(t->size(3) >= 1, "heads without values");
+      *t = unit_last(*t);
+    }
+    d.batch = (int)any.size(0); d.length = (int)any.size(1); d.dim = (int)any.size(3);
+    d.heads = a.q.defined() ? (int)a.q.size(2) : 0;
+    d.kv_heads = a.k.defined() ? (int)a.k.size(2) : 0;
+    if (a.v.defined()) want(a.k.defined() && a.v.size(2) == d.kv_heads, "keys and values differ in shape");
+    for (int i = 0; i < 3; ++i) {
+      if (a.q.defined()) d.q_stride[i] = a.q.stride(i);
+      if (a.k.defined()) d.k_stride[i] = a.k.stride(i);
+      if (a.v.defined()) d.v_stride[i] = a.v.stride(i);
+    }
+    if (a.frequencies.defined()) {
+      if (a.frequencies.scalar_type() != at::kDouble || a.frequencies.device() != any.device())
+        raise(PyExc_TypeError, w + "frequencies are a float64 tensor on the device of the heads");
+      want(a.frequencies.dim() == 1 && 2 * a.frequencies.size(0) <= d.dim, "a frequency for each pair of values, at most dim / 2");
+      a.frequencies = a.frequencies.contiguous();
+      d.pairs = (int)a.frequencies.size(0);
+      d.frequencies = d.pairs ? a.frequencies.const_data_ptr<double>() : nullptr;
+    }
+    d.interleaved = a.interleaved;
+    want(std::isfinite(a.magnitude), "the magnitude is not finite");
+    d.magnitude = (float)a.magnitude;
+    d.norm = a.eps >= 0;
+    want(!std::isnan(a.eps) && a.eps != -HUGE_VAL, "eps is no number");
+    d.eps = (float)(d.norm ? a.eps : 0);
+    for (Tensor* t : {&a.q_weight, &a.k_weight}) {
+      if (!t->defined()) continue;
+      prep_like(*t, any, (w + "weights").c_str());
+      want(d.norm, "weights belong to a norm: eps is missing");
+      want(t->dim() == 1 && t->size(0) == d.dim, "a weight for each value of a head");
+      *t = t->contiguous();
+    }
+    want(std::abs(a.start) <= 0x7fffffff, "positions are out of range");
+    d.start = (int)a.start;
+    if (a.positions.defined()) {
+      if (a.positions.scalar_type() != at::kInt || a.positions.device() != any.device())
+        raise(PyExc_TypeError, w + "positions are a number or an int32 tensor on the device of the heads");
+      d.each = a.positions.dim() == 2;
+      want((d.each || a.positions.dim() == 1) && a.positions.size(0) == d.batch && (!d.each || a.positions.size(1) == d.length),
+           "positions [batch] of the first ones, or [batch, length]");
+      a.positions = a.positions.contiguous();
+      d.positions = a.positions.const_data_ptr<int>();
+    }
+    d.lengths = int_ptr(a.lengths, any, d.batch, (w + "lengths").c_str());
+    return d;
+  }
+  std::tuple<Tensor, Tensor> norm_rotate(HeadArgs a) const {
+    const s2c_head_desc d = head_desc(a, "norm_rotate");
+    const Tensor& any = a.q.defined() ? a.q : a.k;
+    Tensor q, k;
+    if (a.q.defined()) q = at::empty(a.q.sizes(), any.options());
+    if (a.k.defined()) k = at::empty(a.k.sizes(), any.options());
+    Ctx c(*this, any);
+    S2C_CALL(norm_rotate, &d, vptr(a.q), vptr(a.k), vptr(a.q_weight), vptr(a.k_weight), vmut(q), vmut(k), c.stream);
+    return {q, k};
+  }
+  // dq, dk and the gradients of the weights
+  std::tuple<Tensor, Tensor, Tensor, Tensor> norm_rotate_backward(HeadArgs a, const Tensor& gq_, const Tensor& gk_, bool want_q, bool want_k, bool want_wq,
+                                                                  bool want_wk) const {
+    const s2c_head_desc d = head_desc(a, "norm_rotate");
+    const Tensor& any = a.q.defined() ? a.q : a.k;
+    const Tensor gq = a.q.defined() ? gq_.contiguous() : Tensor(), gk = a.k.defined() ? gk_.contiguous() : Tensor();
+    Tensor dq, dk, dwq, dwk;
+    if (a.q.defined() && want_q) dq = at::empty(a.q.sizes(), any.options());
+    if (a.k.defined() && want_k) dk = at::empty(a.k.sizes(), any.options());
+    if (want_wq) dwq = at::empty({d.dim}, any.options());
+    if (want_wk) dwk = at::empty({d.dim}, any.options());
+    Ctx c(*this, any);
+    const Scratch ws(want_wq || want_wk ? norm_rotate_backward_workspace_(&d) : 0, any);
+    S2C_CALL(norm_rotate_backward, &d, vptr(a.q), vptr(a.k), vptr(a.q_weight), vptr(a.k_weight), vptr(gq), vptr(gk), vmut(dq), vmut(dk), vmut(dwq), vmut(dwk),
+             ws.p, ws.n, c.stream);
+    return {dq, dk, dwq, dwk};
+  }
+
+  // -- kept keys in pages ---------------------------------------------------------------------------------
+  s2c_page_desc page_desc(const Tensor& like, const Tensor& keys, const Tensor& values, const Tensor& pages, int64_t batch, const char* who) const {
+    const std::string w = std::string(who) + ": ";
+    auto want = [&](bool ok, const char* what) { check(ok, (w + what).c_str()); };
+    prep_like(keys, like, (w + "keys").c_str());
+    prep_like(values, like, (w + "values").c_str());
+    want(keys.dim() == 4 && keys.sizes() == values.sizes(), "keys and values [pages, positions of a page, kv_heads, dim]");
+    want(keys.size(3) == like.size(3), "heads of another dim than those in the pages");
+    want(keys.size(3) <= 1 || (keys.stride(3) == 1 && values.stride(3) == 1), "keys and values with a contiguous last axis");
+    if (pages.scalar_type() != at::kInt || pages.device() != like.device()) raise(PyExc_TypeError, w + "pages are an int32 tensor on the device of the keys");
+    want(pages.dim() == 2 && pages.size(0) == batch && pages.is_contiguous(), "pages [batch, columns], contiguous");
+    s2c_page_desc d = {};
+    d.table = static_cast<const int*>(vptr(pages));
+    if (!d.table) d.table = &no_pages;               // (an empty table)
+    const int64_t page = keys.size(1);
+    want(page >= 8 && (page & (page - 1)) == 0, "the positions of a page are a power of two, at least 8");
+    want(pages.size(1) <= (1 << 28) / page && keys.size(0) <= 0x7fffffff / page, "at most 2^28 positions in a sequence and 2^31 in a pool");
+    d.columns = (int)pages.size(1); d.count = (int)keys.size(0); d.page = (int)page;
+    for (int i = 0; i < 3; ++i) { d.key_stride[i] = keys.stride(i); d.value_stride[i] = values.stride(i); }
+    return d;
+  }
+  inline static const int no_pages = -1;
+  static void refuse_grad(const char* who, std::initializer_list<Tensor> ts) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor& t : ts)
+      if (t.defined() && t.requires_grad()) raise(PyExc_RuntimeError, std::string("s2cnn_b200: ") + who + " has no gradient (call it under torch.no_grad)");
+  }
+  Tensor norm_rotate_store(HeadArgs a, const Tensor& keys, const Tensor& values, const Tensor& pages) const {
+    refuse_grad("norm_rotate_store", {a.q, a.k, a.v, a.q_weight, a.k_weight, keys, values});
+    const s2c_head_desc d = head_desc(a, "norm_rotate_store");
+    const s2c_page_desc p = page_desc(a.k, keys, values, pages, d.batch, "norm_rotate_store");
+    check(keys.size(2) == d.kv_heads, "norm_rotate_store: other key heads than those in the pages");
+    for (int i = 0; i < 4; ++i)
+      for (const Tensor& t : {keys, values}) check(t.size(i) <= 1 || t.stride(i) != 0, "norm_rotate_store: pages that overlap cannot be written");
+    Tensor q;
+    if (a.q.defined()) q = at::empty(a.q.sizes(), a.q.options());
+    Ctx c(*this, a.k);
+    S2C_CALL(norm_rotate_store, &d, &p, vptr(a.q), vptr(a.k), vptr(a.v), vptr(a.q_weight), vptr(a.k_weight), vmut(q), vmut(keys), vmut(values), c.stream);
+    wrote(keys);
+    wrote(values);
+    return q;
+  }
+  // an array written in place: its saved uses are out of date
+  static void wrote(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+  Tensor paged_attention(AttnArgs a, const Tensor& keys, const Tensor& values, const Tensor& pages) const {
+    refuse_grad("paged_attention", {a.q, keys, values, a.bias});
+    prep_seq(a.q);
+    check(a.q.dim() == 4, "paged_attention: queries [batch, length, heads, dim]");
+    const s2c_page_desc p = page_desc(a.q, keys, values, pages, a.q.size(0), "paged_attention");
+    a.k = keys.new_empty({a.q.size(0), 0, keys.size(2), keys.size(3)});       // (the checks of attention; the pages are read instead)
+    a.v = a.k;
+    const s2c_attention_desc d = attention_desc(a);
+    Tensor out = at::empty({d.batch, d.lq, d.heads, d.dim}, a.q.options());
+    Ctx c(*this, a.q);
+    const Scratch ws(paged_attention_workspace_(&d, &p), a.q);
+    S2C_CALL(paged_attention, &d, &p, vptr(a.q), vptr(keys), vptr(values), vptr(a.bias), vmut(out), ws.p, ws.n, c.stream);
+    return out;
+  }
+  void copy_pages(const Tensor& storage, const Tensor& source, const Tensor& target) const {
+    refuse_grad("copy_pages", {storage});
+    prep_any(storage);
+    check(storage.dim() >= 2 && storage.size(0) <= 0x7fffffff, "copy_pages: storage [pages, ...]");
+    const int* from = int_ptr(source, storage, source.numel(), "copy_pages: source");
+    const int* to = int_ptr(target, storage, source.numel(), "copy_pages: target");
+    const int64_t bytes = storage.numel() ? storage.numel() / storage.size(0) * storage.element_size() : 0;
+    if (storage.numel()) {
+      check(storage.select(0, 0).is_contiguous(), "copy_pages: each page is contiguous");
+      check(storage.size(0) == 1 || storage.stride(0) * storage.element_size() >= bytes, "copy_pages: pages overlap");
+    }
+    Ctx c(*this, storage);
+    S2C_CALL(copy_pages, vmut(storage), (long)(storage.stride(0) * storage.element_size()), (long)bytes, (int)storage.size(0), from, to, (long)source.numel(), c.stream);
+    wrote(storage);
+  }
 };
 
 // ---- autograd rules -------------------------------------------------------------------------------
@@ -1070,13 +1246,44 @@ struct Dropout : torch::autograd::Function<Dropout> {
     return {Variable(), dx, ctx->saved_data["residual"].toBool() ? g[0] : Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
+struct NormRotate : torch::autograd::Function<NormRotate> {
+  static tensor_list forward(AutogradContext* ctx, int64_t ops, const OptTensor& q_, const OptTensor& k_, const OptTensor& f_, const OptTensor& wq_,
+                             const OptTensor& wk_, const OptTensor& positions_, double eps, int64_t start, bool interleaved, double magnitude) {
+    keep_ops(ctx, ops);
+    const Tensor q = or_none(q_), k = or_none(k_), f = or_none(f_), wq = or_none(wq_), wk = or_none(wk_), positions = or_none(positions_);
+    const auto out = reinterpret_cast<Ops*>(ops)->norm_rotate({q, k, f, wq, wk, positions, eps, start, interleaved, magnitude});
+    ctx->save_for_backward({q, k, f, wq, wk, positions});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    tensor_list given;
+    if (q.defined()) given.push_back(std::get<0>(out));
+    if (k.defined()) given.push_back(std::get<1>(out));
+    return given;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    const auto s = ctx->get_saved_variables();
+    // (inputs not given have no index)
+    size_t at = 0;
+    bool needed[6];
+    for (int i = 0; i < 6; ++i) needed[i] = s[i].defined() && ctx->needs_input_grad(at++);
+    const Tensor gq = s[0].defined() ? g[0] : Tensor(), gk = s[1].defined() ? g[s[0].defined() ? 1 : 0] : Tensor();
+    Tensor dq, dk, dwq, dwk;
+    std::tie(dq, dk, dwq, dwk) = ops_of(ctx)->norm_rotate_backward(
+        {s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble(), ctx->saved_data["start"].toInt(), ctx->saved_data["interleaved"].toBool(),
+         ctx->saved_data["magnitude"].toDouble()}, gq, gk, needed[0], needed[1], needed[3], needed[4]);
+    refuse_second("norm_rotate", {s[0], s[1], s[3], s[4], gq, gk}, {&dq, &dk, &dwq, &dwk});
+    return {Variable(), dq, dk, Variable(), dwq, dwk, Variable(), Variable(), Variable(), Variable(), Variable()};
+  }
+};
 // Under torch.jit.trace an op runs as a Python autograd function (ops._traced), which the tracer records as one
 // node that calls the op again.
-template <class... A>
-Tensor traced(Ops& o, const char* name, const A&... args) {
+template <class R = Tensor, class... A>
+R traced(Ops& o, const char* name, const A&... args) {
   pybind11::gil_scoped_acquire gil;
   const pybind11::handle fn(g_traced);
-  return fn(pybind11::cast(&o, pybind11::return_value_policy::reference), name, args...).template cast<Tensor>();
+  return fn(pybind11::cast(&o, pybind11::return_value_policy::reference), name, args...).template cast<R>();
 }
 #define S2C_TRACED(name, ...) \
   if (tracing()) return traced(o, name, __VA_ARGS__)
@@ -1153,6 +1360,31 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             if (wants_any({x, or_none(residual)})) return Dropout::apply(id(o), x, residual, p, seed, step, numbers);
             return o.dropout(x, or_none(residual), p, (uint64_t)seed, (uint64_t)step, or_none(numbers));
           }, "x"_a, "residual"_a, "p"_a, "seed"_a, "step"_a, "numbers"_a, nogil)
+      .def("ag_norm_rotate", [](Ops& o, const OptTensor& q, const OptTensor& k, const OptTensor& f, const OptTensor& wq, const OptTensor& wk,
+                                const OptTensor& positions, double eps, int64_t start, bool interleaved, double magnitude) -> tensor_list {
+            if (tracing()) return traced<tensor_list>(o, "ag_norm_rotate", q, k, f, wq, wk, positions, eps, start, interleaved, magnitude);
+            if (wants_any({or_none(q), or_none(k), or_none(wq), or_none(wk)}))
+              return NormRotate::apply(id(o), q, k, f, wq, wk, positions, eps, start, interleaved, magnitude);
+            const auto out = o.norm_rotate({or_none(q), or_none(k), or_none(f), or_none(wq), or_none(wk), or_none(positions), eps, start, interleaved, magnitude});
+            tensor_list given;
+            if (q) given.push_back(std::get<0>(out));
+            if (k) given.push_back(std::get<1>(out));
+            return given;
+          }, "q"_a, "k"_a, "frequencies"_a, "q_weight"_a, "k_weight"_a, "positions"_a, "eps"_a, "start"_a, "interleaved"_a, "magnitude"_a, nogil)
+      .def("norm_rotate_store", [](Ops& o, const OptTensor& q, const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values, const Tensor& pages,
+                                   const OptTensor& f, const OptTensor& wq, const OptTensor& wk, const OptTensor& positions, const OptTensor& lengths, double eps,
+                                   int64_t start, bool interleaved, double magnitude) -> OptTensor {
+            const Tensor out = o.norm_rotate_store({or_none(q), k, or_none(f), or_none(wq), or_none(wk), or_none(positions), eps, start, interleaved, magnitude, v,
+                                                    or_none(lengths)}, keys, values, pages);
+            return out.defined() ? OptTensor(out) : std::nullopt;
+          }, "q"_a, "k"_a, "v"_a, "keys"_a, "values"_a, "pages"_a, "frequencies"_a, "q_weight"_a, "k_weight"_a, "positions"_a, "lengths"_a, "eps"_a, "start"_a,
+          "interleaved"_a, "magnitude"_a, nogil)
+      .def("paged_attention", [](Ops& o, const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& pages, const OptTensor& bias, const OptTensor& buckets,
+                                 const OptTensor& starts, const OptTensor& q_lengths, const OptTensor& kv_lengths, bool causal, double scale, int64_t q_start) {
+            return o.paged_attention({q, Tensor(), Tensor(), or_none(bias), or_none(buckets), or_none(starts), or_none(q_lengths), or_none(kv_lengths), causal, scale,
+                                      q_start}, keys, values, pages);
+          }, "q"_a, "keys"_a, "values"_a, "pages"_a, "bias"_a, "buckets"_a, "starts"_a, "q_lengths"_a, "kv_lengths"_a, "causal"_a, "scale"_a, "q_start"_a, nogil)
+      .def("copy_pages", &Ops::copy_pages, "storage"_a, "source"_a, "target"_a, nogil)
       .def("ag_s2_fft_real", [](Ops& o, const Tensor& x, std::optional<int64_t> b) {
             S2C_TRACED("ag_s2_fft_real", x, b);
             return wants_grad(x) ? S2FftReal::apply(id(o), x, b_arg(b)) : o.s2_fft(x, false, b, true);

@@ -128,14 +128,16 @@ class SphereSequenceNet(nn.Module):
     """One answer about a sequence of spherical signals: S2Conv(1 -> f1, b_in -> b_l1), ReLU, SO3Conv(f1 -> f2,
     b_l1 -> b_l2), ReLU, so3_integrate for every signal; ``layers`` SequenceBlocks over the f2 features of the
     signals in order; layer norm, mean over the filled positions, Linear(f2 -> f_output).  The spherical layers are float32;
-    ``net.blocks.to(torch.bfloat16)`` or ``torch.autocast`` has the blocks in bfloat16."""
+    ``net.blocks.to(torch.bfloat16)`` or ``torch.autocast`` has the blocks in bfloat16.  ``rotary`` and ``head_norm``: positions by rotation, see
+    ``SequenceBlock``."""
 
     def __init__(self, f1=20, f2=40, f_output=10, b_in=30, b_l1=10, b_l2=6, layers=2, heads=4, p=0.1, num_buckets=16, reach=30,
-                 causal=False):
+                 causal=False, rotary=None, head_norm=False):
         super().__init__()
         self.conv1 = S2Convolution(nfeature_in=1, nfeature_out=f1, b_in=b_in, b_out=b_l1, grid=s2_near_identity_grid())
         self.conv2 = SO3Convolution(nfeature_in=f1, nfeature_out=f2, b_in=b_l1, b_out=b_l2, grid=so3_near_identity_grid())
-        self.blocks = nn.ModuleList([SequenceBlock(f2, heads, causal=causal, p=p, num_buckets=num_buckets, reach=reach)
+        self.blocks = nn.ModuleList([SequenceBlock(f2, heads, causal=causal, p=p, num_buckets=num_buckets, reach=reach, rotary=rotary,
+                                                   head_norm=head_norm)
                                      for _ in range(layers)])
         self.norm = LayerNorm(f2)
         self.out_layer = nn.Linear(f2, f_output)

@@ -49,21 +49,24 @@ class _Traced(torch.autograd.Function):
         ctx.op, ctx.others = op, [None if isinstance(a, torch.Tensor) else a for a in args]
         ctx.save_for_backward(*[a if isinstance(a, torch.Tensor) else None for a in args])
         with _lib.host_module().InsideTracedOp():
-            return op(*args)
+            out = op(*args)
+        return tuple(out) if isinstance(out, list) else out
 
     @staticmethod
-    def backward(ctx, grad):
+    def backward(ctx, *grad):
         args = [o if t is None else t.detach().requires_grad_(need) for t, o, need in
                 zip(ctx.saved_tensors, ctx.others, ctx.needs_input_grad[1:])]
         with torch.enable_grad():
             out = ctx.op(*args)
         wanted = [a for a, need in zip(args, ctx.needs_input_grad[1:]) if need]
+        out, grad = zip(*[(o, g) for o, g in zip(out if isinstance(out, (tuple, list)) else (out,), grad) if o.requires_grad])
         grads = iter(torch.autograd.grad(out, wanted, grad, allow_unused=True))
         return (None,) + tuple(next(grads) if need else None for need in ctx.needs_input_grad[1:])
 
 
 def _traced(native, name, *args):
-    return _Traced.apply(getattr(native, name), *args)
+    out = _Traced.apply(getattr(native, name), *args)
+    return list(out) if isinstance(out, tuple) else out
 
 
 class Ops:
