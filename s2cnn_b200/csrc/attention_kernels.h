@@ -17,8 +17,11 @@
 // shared memory: 2 x 4096 positions, 16 heads of 128, forward and backward, 36 ms against 7.6 on the tensor cores (float32).
 #pragma once
 
+#include <algorithm>
 #include <cfloat>
+#include <cmath>
 
+#include "../../include/s2cnn_b200.h"
 #include "seq_common.h"
 
 namespace s2c {
@@ -38,6 +41,24 @@ struct AttnParams {
   float scale;
   int tiles, splits, chunk;       // tiles of the blocked axis; splits of the keys, of `chunk` keys each
 };
+
+// what every call of attention has to fulfil
+constexpr int kAttnMaxDim = 128, kAttnMaxReach = 2048, kAttnMaxBuckets = 1024;
+inline int attn_check(const char* who, const s2c_attention_desc* d) {
+  const std::string w = std::string(who) + ": ";
+  if (!d) return fail(S2C_ERR_BAD_ARG, w + "no description");
+  S2C_SEQ_TRY(seq_check_type(who, d->dtype));
+  if (d->batch < 0 || d->lq < 0 || d->lk < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads || d->dim < 1)
+    return fail(S2C_ERR_BAD_ARG, w + "bad sizes (the query heads are a multiple of the key heads)");
+  if (d->dim > kAttnMaxDim) return fail(S2C_ERR_UNSUPPORTED, w + "at most 128 values per head");
+  if (std::max(d->lq, d->lk) > (1 << 28)) return fail(S2C_ERR_UNSUPPORTED, w + "at most 2^28 positions");
+  if ((long)d->batch * d->heads > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, w + "too many heads");
+  if (d->bucket_of && (d->n_buckets < 1 || d->reach < 0)) return fail(S2C_ERR_BAD_ARG, w + "bad buckets");
+  if (d->bucket_of && (d->n_buckets > kAttnMaxBuckets || d->reach > kAttnMaxReach))
+    return fail(S2C_ERR_UNSUPPORTED, w + "at most 1024 buckets and relative positions up to 2048");
+  if (!(std::fabs(d->scale) <= FLT_MAX)) return fail(S2C_ERR_BAD_ARG, w + "the scale is not finite");
+  return S2C_OK;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoScore = -INFINITY;

@@ -1,0 +1,558 @@
+// Attention of few queries over keys and values in pages: the queries of all heads that share a key head make up to 8 or 16 rows of a
+// block (more: several row blocks), and the time is that of reading the keys and values once.
+//
+// Keys and values never pass through shared memory.  Products are transposed, S^T = K Q^T and O^T = V^T P^T, on the warp-level matrix
+// instructions, with keys and values as left operands of 16 rows straight from the registers that they were loaded into.  A sum
+// over the values of a head may run in any order that both operands share, and rows of O^T may be any values of a head: so a lane
+// loads 16 consecutive bytes of a row and takes them as the operand's elements that it is to hold, and rows 8 positions apart as
+// its other half.  For V^T the halves of two words are exchanged (neighbouring positions have to share a register); the weights
+// change from rows to columns by one movement within the warp.  The eight columns are the queries: with at most eight no row is wasted.
+//
+// Keys of the next tile are asked for as soon as the scores of this one are done, its values as soon as the outputs are: a warp has
+// up to 8 KB (float32 16) on its way and waits for nobody.  The page of every eighth position comes a tile earlier, by one load per warp.
+//
+// Work is dealt in steps of (4 warps x tile) positions of one item (sequence, key head, row block), an equal share to each block as
+// the lengths on the device give it: a block finds where its share begins by adding up the sequences' steps.  Items that lie in
+// several blocks leave partial results, joined by a second kernel in the order of the blocks.
+//
+// bfloat16 queries and keys are multiplied as they are; the weights enter the second product as two bfloat16 parts, float32 operands
+// as two TF32 parts of which the product of the smaller ones is left out, so that a result's rounding is its own.
+#pragma once
+
+#include "attention_few.h"
+#include "kept_pages.h"
+
+#ifndef S2C_EMUL
+
+namespace s2c {
+
+struct PagedParams {
+  AttnParams a;              // k, v are not used
+  PageTable pages;
+  long ks[3], vs[3];         // page, position, head
+  int row_blocks;
+  float* part;               // [2 blocks][rows][DP + 2]: slot 2 c: an item that began before block c; 2 c + 1: one that goes on behind it
+  int4* split;               // [min(items, blocks)]: item, first block, blocks of an item that is joined; 0 blocks: none
+};
+
+__device__ __forceinline__ unsigned paged_movmatrix(unsigned v) {
+  unsigned r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void paged_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void paged_mma_tf32(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// N consecutive values of a row from value c on: there where on > 0 and c < dim, NaN where on < 0, zeros otherwise.  WIDE: rows lie on
+// boundaries of N values (a piece that the row ends in is still read value by value).
+template <class T, int N, bool WIDE>
+__device__ __forceinline__ void paged_load(unsigned (&w)[N * sizeof(T) / 4], const T* row, int c, int dim, int on) {
+  constexpr int kWords = N * sizeof(T) / 4;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) w[i] = on < 0 ? 0x7fffffffu : 0u;
+  if (WIDE) {
+    const int whole = on > 0 && c + N <= dim;
+    if constexpr (kWords == 4)
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                   : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(row + c), "r"(whole) : "memory");
+    else
+      asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t@p ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}"
+                   : "+r"(w[0]), "+r"(w[1]) : "l"(row + c), "r"(whole) : "memory");
+    if (dim % N == 0 || whole || on <= 0 || c >= dim) return;
+  }
+  if (on <= 0) return;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    if (c + e >= dim) break;
+    if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const unsigned*>(row)[c + e];
+    else w[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[c + e] << (16 * (e % 2));
+  }
+}
+
+// DP: values of a head, rounded up to 32, 64 or 128; NT: row blocks of 8 NT rows
+template <class T, int DP, int NT>
+struct PagedShape {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kWarps = 4, kThreads = 32 * kWarps, kRows = 8 * NT;
+  static constexpr int kTiles = kHalf ? 128 / DP : DP == 128 ? 1 : 64 / DP;     // of 16 positions, for a warp's step
+  static constexpr int kKeys = 16 * kTiles, kStep = kWarps * kKeys;
+  static constexpr int kQk = kHalf ? DP / 32 : DP / 16;                       // a row's chunks of four 16-byte pieces
+  static constexpr int kVd = kHalf && DP > 32 ? 8 : 4, kVc = DP / (8 * kVd);   // a lane's consecutive values of a row of V, chunks
+  static constexpr int kOut = DP / 16;                                        // tiles of 16 rows of O^T
+  static constexpr size_t kQuery = (size_t)kQk * NT * 32 * 16 * (kHalf ? 1 : 2), kJoin = (size_t)kWarps * kRows * (DP + 2) * 4;
+  // where value `m` (0: of the upper eight rows) of tile t of a lane lies in a head
+  static __device__ __forceinline__ int value(int t, int lane) { return t / (kVd / 2) * 8 * kVd + lane / 4 * kVd + 2 * (t % (kVd / 2)); }
+};
+
+// keys of a sequence that some query sees, and the steps of its items: at least one, which writes the zeros of a sequence without keys
+__device__ __forceinline__ int paged_steps(const AttnParams& a, int b, int step) {
+  const AttnSeq s = attn_seq(a, b);
+  const int n = (attn_keys(a, s, s.qlen) + step - 1) / step;
+  return n > 0 ? n : 1;
+}
+
+template <class T, int DP, int NT, bool WIDE>
+struct PagedAttention {
+  using Params = PagedParams;
+  using H = PagedShape<T, DP, NT>;
+  static constexpr int kThreads = H::kThreads;
+  static constexpr int kBlocks = H::kHalf ? (NT == 1 ? 3 : 2) : 2;
+  static size_t smem() { return H::kQuery + H::kJoin + 64; }
+
+  struct Tile {
+    unsigned k[H::kTiles][2][H::kQk][4];
+    unsigned v[H::kTiles][4][H::kVc][H::kVd * sizeof(T) / 4];
+  };
+
+  static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
+    const AttnParams& a = p.a;
+    const int lane = ctx.tid % 32, warp = ctx.tid / 32;
+    uint4* const query = reinterpret_cast<uint4*>(smem);
+    float* const join = reinterpret_cast<float*>(smem + H::kQuery);
+    long* const find = reinterpret_cast<long*>(smem + H::kQuery + H::kJoin);      // [0 .. 3] the warps' sums, [4], [5] where the share begins
+    const int per_batch = a.kv_heads * p.row_blocks;                              // items of a sequence
+
+    // ---- this block's share: steps [lo, hi) of all
+    const int mine = (a.batch + kThreads - 1) / kThreads;
+    long sum = 0;
+    for (int i = 0; i < mine; ++i)
+      if (ctx.tid * mine + i < a.batch) sum += paged_steps(a, ctx.tid * mine + i, H::kStep);
+    long before = sum;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      const long o = __shfl_up_sync(0xffffffffu, before, m);
+      if (lane >= m) before += o;
+    }
+    if (lane == 31) find[warp] = before;
+    ctx.sync();
+    long all = 0;
+    for (int w = 0; w < H::kWarps; ++w) {
+      if (w == warp) before += all;
+      all += find[w];
+    }
+    before -= sum;
+    const long total = all * per_batch, blocks = min((long)ctx.nblk, total);
+    const bool by_item = (long)a.batch * per_batch <= ctx.nblk;                   // as the host counts the splits
+    if (ctx.bid >= blocks) {
+      if (!by_item && ctx.tid == 0) p.split[ctx.bid] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    const long lo = ctx.bid * total / blocks, hi = (ctx.bid + 1) * total / blocks;
+    if (before * per_batch <= lo && lo < (before + sum) * per_batch) {
+      int b = ctx.tid * mine;
+      for (;; ++b) {
+        const int n = paged_steps(a, b, H::kStep);
+        if (lo < (before + n) * per_batch) break;
+        before += n;
+      }
+      find[4] = b;
+      find[5] = lo - before * per_batch;
+    }
+    ctx.sync();
+    int b = (int)find[4];
+    int n = paged_steps(a, b, H::kStep);
+    int within = (int)(find[5] / n), s0 = (int)(find[5] % n);
+    bool joined = false;
+    for (long at = lo; at < hi;) {
+      const int s1 = (int)min((long)n, s0 + (hi - at));
+      const int hk = within / p.row_blocks, rb = within % p.row_blocks, item = b * per_batch + within;
+      const bool whole = s0 == 0 && s1 == n;
+      float* part = whole ? nullptr : p.part + (2L * ctx.bid + (s0 == 0 ? 1 : 0)) * H::kRows * (DP + 2);
+      piece(ctx, p, query, join, b, hk, rb, s0, s1, part);
+      if (ctx.tid == 0) {
+        if (by_item) {
+          if (whole) p.split[item] = make_int4(0, 0, 0, 0);
+        }
+        if (!whole && s0 == 0) {
+          const long last = ((at + n) * blocks - 1) / total;
+          p.split[by_item ? item : ctx.bid] = make_int4(item, ctx.bid, (int)(last - ctx.bid) + 1, 0);
+          joined = true;
+        }
+      }
+      at += s1 - s0;
+      s0 = 0;
+      if (at < hi && ++within == per_batch) {
+        within = 0;
+        n = paged_steps(a, ++b, H::kStep);
+      }
+    }
+    if (!by_item && !joined && ctx.tid == 0) p.split[ctx.bid] = make_int4(0, 0, 0, 0);
+  }
+
+  // steps [s0, s1) of one item; to `part`, or to the output where that is null
+  static __device__ __forceinline__ void piece(const Ctx& ctx, const Params& p, uint4* query, float* join, int b, int hk, int rb, int s0, int s1, float* part) {
+    const AttnParams& a = p.a;
+    const int lane = ctx.tid % 32, warp = ctx.tid / 32, g = lane / 4, q4 = lane % 4;
+    const int rows = a.lq * a.group, r0 = rb * H::kRows, left = min(H::kRows, rows - r0);
+    const AttnSeq s = attn_seq(a, b);
+    const int i0 = r0 / a.group, i1 = min((r0 + left - 1) / a.group + 1, s.qlen);      // queries of the block
+    const int keys = i0 < s.qlen ? attn_keys(a, s, i1) : 0;
+    const T* const kbase = static_cast<const T*>(p.pages.array[0]) + hk * p.ks[2];
+    const T* const vbase = static_cast<const T*>(p.pages.array[1]) + hk * p.vs[2];
+    const int* const table = p.pages.table + (long)b * p.pages.columns;
+    const int page = p.pages.page, log_page = __ffs(page) - 1;
+
+    Tile t;
+    // the page of every eighth position of a step, one to a lane
+    auto pages_of = [&](int step) {
+      const int j = (step * H::kWarps + warp) * H::kKeys + 8 * lane;
+      return lane < 2 * H::kTiles && step < s1 && j < keys ? table[j >> log_page] : -1;
+    };
+    auto load_keys = [&](int step, int ids) {
+      const int j0 = (step * H::kWarps + warp) * H::kKeys;
+#pragma unroll
+      for (int m = 0; m < 2 * H::kTiles; ++m) {
+        const int id = __shfl_sync(0xffffffffu, ids, m), j = j0 + 8 * m;
+        const int on = step >= s1 || j + g >= keys ? 0 : id < 0 || id >= p.pages.count ? -1 : 1;
+        const T* row = kbase + (on > 0 ? (long)id * p.ks[0] + (long)((j & (page - 1)) + g) * p.ks[1] : 0);
+#pragma unroll
+        for (int c = 0; c < H::kQk; ++c) paged_load<T, 16 / sizeof(T), WIDE>(t.k[m / 2][m % 2][c], row, (4 * c + q4) * (16 / (int)sizeof(T)), a.dim, on);
+      }
+    };
+    auto load_values = [&](int step, int ids) {
+      const int j0 = (step * H::kWarps + warp) * H::kKeys;
+#pragma unroll
+      for (int m = 0; m < 2 * H::kTiles; ++m) {
+        const int id = __shfl_sync(0xffffffffu, ids, m), j = j0 + 8 * m;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = H::kHalf ? 2 * q4 + e : q4 + 4 * e;
+          const int on = step >= s1 || j + r >= keys ? 0 : id < 0 || id >= p.pages.count ? -1 : 1;
+          const T* row = vbase + (on > 0 ? (long)id * p.vs[0] + (long)((j & (page - 1)) + r) * p.vs[1] : 0);
+#pragma unroll
+          for (int c = 0; c < H::kVc; ++c) paged_load<T, H::kVd, WIDE>(t.v[m / 2][2 * (m % 2) + e][c], row, (8 * c + g) * H::kVd, a.dim, on);
+        }
+      }
+    };
+    int ids = pages_of(s0), next = pages_of(s0 + 1);
+    load_keys(s0, ids);
+    load_values(s0, ids);
+
+    // ---- queries as the right operands of the scores, and what each row sees
+    for (int e = ctx.tid; e < H::kQk * NT * 32; e += kThreads) {
+      const int c = e / 32 / NT, nt = e / 32 % NT, l = e % 32, r = r0 + 8 * nt + l / 4, i = r / a.group;
+      unsigned w[4];
+      paged_load<T, 16 / sizeof(T), false>(w, static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + (hk * a.group + r % a.group) * a.qs[2],
+                                           (4 * c + l % 4) * (16 / (int)sizeof(T)), a.dim, r < rows && i < s.qlen && keys > 0);
+      if constexpr (H::kHalf) {
+        query[e] = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        FewSplit x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = few_split(as_float(w[u]));
+        query[2 * e] = make_uint4(x[0].hi, x[1].hi, x[2].hi, x[3].hi);
+        query[2 * e + 1] = make_uint4(x[0].lo, x[1].lo, x[2].lo, x[3].lo);
+      }
+    }
+    int lim[NT][2], pos[NT][2];                          // a row sees the positions before lim
+    float flat[NT][2];
+    const T* bias[NT][2];
+    int all_see = keys;                                  // that every row sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = r0 + 8 * nt + 2 * q4 + e, i = r / a.group;
+        const bool in = r < rows && i < s.qlen;
+        pos[nt][e] = i + s.start;
+        lim[nt][e] = in ? attn_keys(a, s, i + 1) : r < rows ? 0 : keys;
+        all_see = min(all_see, lim[nt][e]);
+        flat[nt][e] = 0.f;
+        bias[nt][e] = nullptr;
+        if (a.bias && r < rows) {
+          bias[nt][e] = static_cast<const T*>(a.bias) + hk * a.group + r % a.group;
+          const int which = a.bucket_of[0];
+          if (which >= 0 && which < a.n_buckets) flat[nt][e] = attn_bias_units(widen(bias[nt][e][(long)which * a.heads]));
+        }
+      }
+    all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 1));
+    all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 2));
+    ctx.sync();                                          // the queries
+
+    const float scale = a.scale * kLog2e;
+    float acc[H::kOut][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int c = 0; c < H::kOut; ++c)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[c][nt][e] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[nt][e] = kNoScore; l[nt][e] = 0.f; }
+
+    for (int step = s0; step < s1; ++step) {
+      const int j0 = (step * H::kWarps + warp) * H::kKeys;
+      ids = next;
+      next = pages_of(step + 2);
+      // ---- scores: 16 positions x 8 rows
+      float x[H::kTiles][NT][4];
+#pragma unroll
+      for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k][nt][e] = 0.f;
+      if constexpr (H::kHalf) {
+#pragma unroll
+        for (int c = 0; c < H::kQk; ++c)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 y = query[(c * NT + nt) * 32 + lane];
+#pragma unroll
+            for (int k = 0; k < H::kTiles; ++k) {
+              paged_mma(x[k][nt], t.k[k][0][c][0], t.k[k][1][c][0], t.k[k][0][c][1], t.k[k][1][c][1], y.x, y.y);
+              paged_mma(x[k][nt], t.k[k][0][c][2], t.k[k][1][c][2], t.k[k][0][c][3], t.k[k][1][c][3], y.z, y.w);
+            }
+          }
+      } else {
+        float z[H::kTiles][NT][4] = {};                  // the small products
+#pragma unroll
+        for (int c = 0; c < H::kQk; ++c)
+#pragma unroll
+          for (int k = 0; k < H::kTiles; ++k) {
+            FewSplit u[2][4];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e / 4][e % 4] = few_split(as_float(t.k[k][e / 4][c][e % 4]));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 hi = query[2 * ((c * NT + nt) * 32 + lane)], lo = query[2 * ((c * NT + nt) * 32 + lane) + 1];
+              paged_mma_tf32(z[k][nt], u[0][0].lo, u[1][0].lo, u[0][1].lo, u[1][1].lo, hi.x, hi.y);
+              paged_mma_tf32(z[k][nt], u[0][0].hi, u[1][0].hi, u[0][1].hi, u[1][1].hi, lo.x, lo.y);
+              paged_mma_tf32(x[k][nt], u[0][0].hi, u[1][0].hi, u[0][1].hi, u[1][1].hi, hi.x, hi.y);
+              paged_mma_tf32(z[k][nt], u[0][2].lo, u[1][2].lo, u[0][3].lo, u[1][3].lo, hi.z, hi.w);
+              paged_mma_tf32(z[k][nt], u[0][2].hi, u[1][2].hi, u[0][3].hi, u[1][3].hi, lo.z, lo.w);
+              paged_mma_tf32(x[k][nt], u[0][2].hi, u[1][2].hi, u[0][3].hi, u[1][3].hi, hi.z, hi.w);
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][nt][e] += z[k][nt][e];
+      }
+      load_keys(step + 1, ids);
+      // ---- weights
+      const bool far = !a.bias || j0 + H::kKeys - 1 - (i0 + s.start) <= -a.reach;    // one bias per head
+      const bool plain = j0 + H::kKeys <= all_see;
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        top[nt][0] = top[nt][1] = kNoScore;
+#pragma unroll
+        for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float add = flat[nt][e % 2];
+            const int j = j0 + 16 * k + g + 8 * (e / 2);
+            if (!far) {
+              add = 0.f;
+              const int which = a.bucket_of[attn_clamp(j - pos[nt][e % 2], -a.reach, a.reach) + a.reach];
+              if (bias[nt][e % 2] && which >= 0 && which < a.n_buckets) add = attn_bias_units(widen(bias[nt][e % 2][(long)which * a.heads]));
+            }
+            float y = fmaf(x[k][nt][e], scale, add);
+            if (!plain && j >= lim[nt][e % 2]) y = kNoScore;
+            x[k][nt][e] = y;
+            top[nt][e % 2] = fmaxf(top[nt][e % 2], y);
+          }
+      }
+      bool more = false;
+      float f[NT][2], base[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& y = top[nt][e];
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+          y = fmaxf(y, m[nt][e]);
+          base[nt][e] = y == kNoScore ? 0.f : y;
+          f[nt][e] = exp2_fast(m[nt][e] - base[nt][e]);
+          more = more || y != m[nt][e];
+        }
+      if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            l[nt][e] *= f[nt][e];
+            m[nt][e] = top[nt][e];
+          }
+#pragma unroll
+          for (int c = 0; c < H::kOut; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][nt][e] *= f[nt][e % 2];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[k][nt][e] = exp2_fast(x[k][nt][e] - base[nt][e % 2]);
+            l[nt][e % 2] += x[k][nt][e];
+          }
+      // ---- outputs
+#pragma unroll
+      for (int k = 0; k < H::kTiles; ++k) {
+        if constexpr (H::kHalf) {
+          unsigned hi[NT][2], lo[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float u = x[k][nt][2 * e], w = x[k][nt][2 * e + 1];
+              const unsigned r = pack_bf16(u, w);
+              hi[nt][e] = paged_movmatrix(r);
+              lo[nt][e] = paged_movmatrix(pack_bf16(u - as_float(r << 16), w - as_float(r & 0xffff0000u)));
+            }
+#pragma unroll
+          for (int c = 0; c < H::kOut; ++c) {
+            const int vc = c / (H::kVd / 2), w = c % (H::kVd / 2);
+            const unsigned a0 = __byte_perm(t.v[k][0][vc][w], t.v[k][1][vc][w], 0x5410), a1 = __byte_perm(t.v[k][0][vc][w], t.v[k][1][vc][w], 0x7632);
+            const unsigned a2 = __byte_perm(t.v[k][2][vc][w], t.v[k][3][vc][w], 0x5410), a3 = __byte_perm(t.v[k][2][vc][w], t.v[k][3][vc][w], 0x7632);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              paged_mma(acc[c][nt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+              paged_mma(acc[c][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
+            }
+          }
+        } else {
+          // a step of 8 positions; row g's weight of position q4 (+ 4) lies in lane 4 q4 (+ 16) + g / 2
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            FewSplit w[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int from = 4 * q4 + 16 * e + g / 2;
+                const float even = __shfl_sync(0xffffffffu, x[k][nt][2 * h], from), odd = __shfl_sync(0xffffffffu, x[k][nt][2 * h + 1], from);
+                w[nt][e] = few_split(g % 2 ? odd : even);
+              }
+#pragma unroll
+            for (int c = 0; c < H::kOut; ++c) {
+              const int vc = c / 2, d = 2 * (c % 2);
+              const FewSplit v0 = few_split(as_float(t.v[k][2 * h][vc][d])), v1 = few_split(as_float(t.v[k][2 * h][vc][d + 1]));
+              const FewSplit v2 = few_split(as_float(t.v[k][2 * h + 1][vc][d])), v3 = few_split(as_float(t.v[k][2 * h + 1][vc][d + 1]));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                paged_mma_tf32(acc[c][nt], v0.lo, v1.lo, v2.lo, v3.lo, w[nt][0].hi, w[nt][1].hi);
+                paged_mma_tf32(acc[c][nt], v0.hi, v1.hi, v2.hi, v3.hi, w[nt][0].lo, w[nt][1].lo);
+                paged_mma_tf32(acc[c][nt], v0.hi, v1.hi, v2.hi, v3.hi, w[nt][0].hi, w[nt][1].hi);
+              }
+            }
+          }
+        }
+      }
+      load_values(step + 1, ids);
+    }
+    // ---- the warps' results: [warp][row][DP values, maximum, sum]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float& y = l[nt][e];
+        y += __shfl_xor_sync(0xffffffffu, y, 4);
+        y += __shfl_xor_sync(0xffffffffu, y, 8);
+        y += __shfl_xor_sync(0xffffffffu, y, 16);
+        float* to = join + (warp * H::kRows + 8 * nt + 2 * q4 + e) * (DP + 2);
+#pragma unroll
+        for (int c = 0; c < H::kOut; ++c) *reinterpret_cast<float2*>(to + H::value(c, lane)) = make_float2(acc[c][nt][e], acc[c][nt][2 + e]);
+        if (g == 0) {
+          to[DP] = m[nt][e];
+          to[DP + 1] = y;
+        }
+      }
+    ctx.sync();
+    for (int e = ctx.tid; e < left * DP; e += kThreads) {
+      const int r = e / DP, c = e % DP;
+      float top = kNoScore;
+#pragma unroll
+      for (int w = 0; w < H::kWarps; ++w) top = fmaxf(top, join[(w * H::kRows + r) * (DP + 2) + DP]);
+      const float base = top == kNoScore ? 0.f : top;
+      float o = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < H::kWarps; ++w) {
+        const float* from = join + (w * H::kRows + r) * (DP + 2);
+        const float f = exp2_fast(from[DP] - base);
+        o = fmaf(from[c], f, o);
+        sum = fmaf(from[DP + 1], f, sum);
+      }
+      if (part) {
+        part[r * (DP + 2) + c] = o;
+        if (c == 0) {
+          part[r * (DP + 2) + DP] = top;
+          part[r * (DP + 2) + DP + 1] = sum;
+        }
+      } else if (c < a.dim) {
+        write(p, b, hk, r0 + r, c, o, sum);
+      }
+    }
+    ctx.sync();                                          // queries and results are written again
+  }
+  static __device__ __forceinline__ void write(const Params& p, int b, int hk, int r, int c, float o, float sum) {
+    const AttnParams& a = p.a;
+    const int i = r / a.group, h = hk * a.group + r % a.group;
+    narrow(static_cast<T*>(a.out) + (((long)b * a.lq + i) * a.heads + h) * a.dim + c, sum == 0.f ? 0.f : o / sum);
+  }
+};
+
+// Joins the blocks' results of an item: a block per row, thread t with column t % DP of every kThreads / DP-th block.
+template <class T, int DP, int NT>
+struct PagedJoin {
+  using Params = PagedParams;
+  using H = PagedShape<T, DP, NT>;
+  static constexpr int kThreads = 128, kBlocks = 8, kSlices = kThreads / DP;
+  static size_t smem(long blocks) { return (blocks + kThreads + 8) * sizeof(float); }
+  static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
+    const AttnParams& a = p.a;
+    const int4 what = p.split[ctx.bid / H::kRows];
+    const int n = what.z, per_batch = a.kv_heads * p.row_blocks, b = what.x / per_batch, within = what.x % per_batch;
+    const int r = ctx.bid % H::kRows, row = within % p.row_blocks * H::kRows + r;
+    if (n == 0 || row >= a.lq * a.group) return;
+    const int t = ctx.tid, lane = t % 32, warp = t / 32;
+    float *red = reinterpret_cast<float*>(smem), *outs = red + 8, *weight = outs + kThreads;
+    // block k's part of it: the first one's lies where what goes on is kept
+    auto part = [&](int k) { return p.part + ((2L * (what.y + k) + (k == 0)) * H::kRows + r) * (DP + 2); };
+    float m = kNoScore;
+    for (int e = t; e < n; e += kThreads) m = fmaxf(m, part(e)[DP]);
+    m = lanes_max<32>(ctx, m);
+    if (lane == 0) red[warp] = m;
+    ctx.sync();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float base = m == kNoScore ? 0.f : m;
+    float l = 0.f;
+    for (int e = t; e < n; e += kThreads) {
+      const float f = exp2_fast(part(e)[DP] - base);
+      weight[e] = f;
+      l = fmaf(part(e)[DP + 1], f, l);
+    }
+    l = lanes_sum<32>(ctx, l);
+    if (lane == 0) red[4 + warp] = l;
+    ctx.sync();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const int c = t % DP;
+    float o = 0.f;
+#pragma unroll 8
+    for (int e = t / DP; e < n; e += kSlices) o = fmaf(part(e)[c], weight[e], o);
+    outs[t] = o;
+    ctx.sync();
+    if (t >= DP) return;
+    for (int e = 1; e < kSlices; ++e) o += outs[e * DP + t];
+    if (t < a.dim) PagedAttention<T, DP, NT, true>::write(p, b, within / p.row_blocks, row, t, o, l);
+  }
+};
+
+}  // namespace s2c
+#endif  // S2C_EMUL

@@ -9,16 +9,12 @@
 #include <cfloat>
 #include <cmath>
 
+#include "attention_kernels.h"
 #include "head_rotation_kernels.h"
 #include "kept_pages.h"
+#include "paged_attention_kernels.h"
 
 namespace s2c {
-
-#define S2C_PAGES_TRY(expr)          \
-  do {                               \
-    int rc__ = (expr);               \
-    if (rc__ != S2C_OK) return rc__; \
-  } while (0)
 
 inline bool on_boundary(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
@@ -27,7 +23,7 @@ constexpr int kHeadMaxDim = 128;
 inline int head_check(const char* who, const s2c_head_desc* d) {
   const std::string w = std::string(who) + ": ";
   if (!d) return fail(S2C_ERR_BAD_ARG, w + "no description");
-  if (d->dtype != kSeqF32 && d->dtype != kSeqBf16) return fail(S2C_ERR_BAD_ARG, w + "dtype is 0 (float32) or 1 (bfloat16)");
+  S2C_SEQ_TRY(seq_check_type(who, d->dtype));
   if (d->batch < 0 || d->length < 0 || d->heads < 0 || d->kv_heads < 0 || d->dim < 1) return fail(S2C_ERR_BAD_ARG, w + "bad sizes");
   if (d->dim > kHeadMaxDim) return fail(S2C_ERR_UNSUPPORTED, w + "at most 128 values per head");
   if (d->pairs < 0 || 2 * d->pairs > d->dim || (d->pairs > 0 && !d->frequencies)) return fail(S2C_ERR_BAD_ARG, w + "more frequencies than pairs of values, or none");
@@ -105,7 +101,7 @@ template <class T>
 int head_backward(HeadParams p, void* dqw, void* dkw, stream_t st) {
   const long blocks = head_backward_blocks<T>(p);
   for (int k = 0; k < 2; ++k) p.kind[k].wide = head_wide(p, p.kind[k], sizeof(T));
-  S2C_PAGES_TRY(head_by_dim<T>(p.dim, [&](auto lanes) {
+  S2C_SEQ_TRY(head_by_dim<T>(p.dim, [&](auto lanes) {
     using K = HeadBackward<T, decltype(lanes)::value, 2>;
     return seq_launch<K>("norm_rotate_backward", blocks, K::smem(), st, p);
   }));
@@ -150,6 +146,84 @@ inline size_t gathered_bytes(const s2c_attention_desc& g) {
   return page_align((size_t)g.batch * g.lk * g.kv_heads * g.dim * (g.dtype == kSeqF32 ? 4 : 2));
 }
 
+#ifndef S2C_EMUL
+inline AttnParams paged_params(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* q, const void* bias, void* out) {
+  AttnParams p = {};
+  p.q = q; p.bias = d->bucket_of ? bias : nullptr; p.out = out;
+  p.bucket_of = d->bucket_of; p.start = d->q_starts; p.q_len = d->q_lengths; p.kv_len = d->kv_lengths;
+  for (int i = 0; i < 3; ++i) p.qs[i] = d->q_stride[i];
+  p.batch = d->batch; p.lq = d->lq; p.lk = pages->columns * pages->page; p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->dim;
+  p.group = d->heads / d->kv_heads;
+  p.causal = d->causal != 0; p.scale = d->scale; p.start_all = d->q_start;
+  p.reach = p.bias ? d->reach : 0; p.n_buckets = p.bias ? d->n_buckets : 0;
+  return p;
+}
+// rows of 16-byte pieces (of four values at least): keys and values as they lie
+template <class T>
+bool paged_wide(const s2c_page_desc* d, const void* keys, const void* values) {
+  bool ok = on_boundary(keys, 16) && on_boundary(values, 16);
+  for (int i = 0; i < 3; ++i) ok = ok && d->key_stride[i] % kVec<T> == 0 && d->value_stride[i] % kVec<T> == 0;
+  return ok;
+}
+struct PagedPlan {
+  long items = 0, blocks = 0;
+  int row_blocks = 0, nt = 1;
+  bool joined = false;
+  size_t part = 0, bytes = 0;
+};
+template <class T, class F>
+int paged_by_shape(int dim, int nt, F f) {
+#define S2C_PAGED(DP) return nt == 1 ? f(std::integral_constant<int, DP>(), std::integral_constant<int, 1>()) : f(std::integral_constant<int, DP>(), std::integral_constant<int, 2>())
+  if (dim <= 32) S2C_PAGED(32);
+  if (dim <= 64) S2C_PAGED(64);
+  S2C_PAGED(128);
+#undef S2C_PAGED
+}
+// How many blocks share the work: as many as run at once, or fewer where the columns hold fewer steps.
+template <class T>
+PagedPlan paged_plan(const AttnParams& a) {
+  PagedPlan plan;
+  const long rows = (long)a.lq * a.group;
+  plan.nt = rows <= 8 ? 1 : 2;
+  plan.row_blocks = (int)((rows + 8 * plan.nt - 1) / (8 * plan.nt));
+  plan.items = (long)a.batch * a.kv_heads * plan.row_blocks;
+  paged_by_shape<T>(a.dim, plan.nt, [&](auto dp, auto nt) {
+    using K = PagedAttention<T, decltype(dp)::value, decltype(nt)::value, true>;
+    const long steps = std::max(1, (a.lk + K::H::kStep - 1) / K::H::kStep);
+    plan.blocks = std::min((long)K::kBlocks * dev_sm_count(), plan.items * steps);
+    plan.joined = steps > 1;
+    plan.part = page_align(2 * (size_t)plan.blocks * K::H::kRows * (decltype(dp)::value + 2) * sizeof(float));
+    return (int)S2C_OK;
+  });
+  plan.bytes = plan.part + (size_t)std::min(plan.items, plan.blocks) * sizeof(int4);
+  return plan;
+}
+template <class T>
+int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* keys, const void* values, void* ws, size_t ws_bytes, stream_t st) {
+  const PagedPlan plan = paged_plan<T>(a);
+  if (plan.items == 0) return S2C_OK;
+  if (plan.items > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, "s2c_paged_attention: too many heads and queries");
+  if (plan.bytes > ws_bytes || !ws) return fail(S2C_ERR_WORKSPACE, "s2c_paged_attention: workspace too small");
+  PagedParams p = {};
+  p.a = a;
+  p.pages = page_table(pages, keys, values);
+  for (int i = 0; i < 3; ++i) { p.ks[i] = pages->key_stride[i]; p.vs[i] = pages->value_stride[i]; }
+  p.row_blocks = plan.row_blocks;
+  p.part = static_cast<float*>(ws);
+  p.split = reinterpret_cast<int4*>(static_cast<char*>(ws) + plan.part);
+  const bool wide = paged_wide<T>(pages, keys, values);
+  return paged_by_shape<T>(a.dim, plan.nt, [&](auto dp, auto nt) {
+    constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;
+    using W = PagedAttention<T, DP, NT, true>;
+    using N = PagedAttention<T, DP, NT, false>;
+    S2C_SEQ_TRY(wide ? seq_launch<W>("paged_attention", plan.blocks, W::smem(), st, p) : seq_launch<N>("paged_attention", plan.blocks, N::smem(), st, p));
+    if (!plan.joined) return (int)S2C_OK;
+    using J = PagedJoin<T, DP, NT>;
+    return seq_launch<J>("paged_join", std::min(plan.items, plan.blocks) * W::H::kRows, J::smem(plan.blocks), st, p);
+  });
+}
+#endif
+
 }  // namespace s2c
 
 using namespace s2c;
@@ -157,7 +231,7 @@ using namespace s2c;
 extern "C" {
 
 int s2c_norm_rotate(const s2c_head_desc* d, const void* q, const void* k, const void* q_weight, const void* k_weight, void* q_out, void* k_out, void* stream) {
-  S2C_PAGES_TRY(head_check("s2c_norm_rotate", d));
+  S2C_SEQ_TRY(head_check("s2c_norm_rotate", d));
   if ((q && !q_out) || (k && !k_out)) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate: a pointer is missing");
   HeadParams p = head_params(d);
   p.lengths = nullptr;
@@ -178,7 +252,7 @@ size_t s2c_norm_rotate_backward_workspace(const s2c_head_desc* d) {
 int s2c_norm_rotate_backward(const s2c_head_desc* d, const void* q, const void* k, const void* q_weight, const void* k_weight, const void* dq_out,
                              const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
                              void* stream) {
-  S2C_PAGES_TRY(head_check("s2c_norm_rotate_backward", d));
+  S2C_SEQ_TRY(head_check("s2c_norm_rotate_backward", d));
   const bool some = d->batch > 0 && d->length > 0;
   if (some && ((d->heads > 0 && (!q || !dq_out)) || (d->kv_heads > 0 && (!k || !dk_out)))) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_backward: a pointer is missing");
   if ((dq_weight || dk_weight) && !d->norm) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_backward: a weight needs a norm");
@@ -200,8 +274,8 @@ int s2c_norm_rotate_backward(const s2c_head_desc* d, const void* q, const void* 
 
 int s2c_norm_rotate_store(const s2c_head_desc* d, const s2c_page_desc* pages, const void* q, const void* k, const void* v, const void* q_weight,
                           const void* k_weight, void* q_out, void* keys, void* values, void* stream) {
-  S2C_PAGES_TRY(head_check("s2c_norm_rotate_store", d));
-  S2C_PAGES_TRY(page_check("s2c_norm_rotate_store", pages));
+  S2C_SEQ_TRY(head_check("s2c_norm_rotate_store", d));
+  S2C_SEQ_TRY(page_check("s2c_norm_rotate_store", pages));
   if (q && !q_out) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_store: a pointer is missing");
   if (d->batch > 0 && d->length > 0 && d->kv_heads > 0 && (!k || !v || (pages->count > 0 && (!keys || !values))))
     return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_store: a pointer is missing");
@@ -224,17 +298,29 @@ int s2c_norm_rotate_store(const s2c_head_desc* d, const s2c_page_desc* pages, co
 }
 
 size_t s2c_paged_attention_workspace(const s2c_attention_desc* d, const s2c_page_desc* pages) {
-  if (!d || page_check("s2c_paged_attention_workspace", pages) != S2C_OK) return 0;
+  if (page_check("s2c_paged_attention_workspace", pages) != S2C_OK || attn_check("s2c_paged_attention_workspace", d) != S2C_OK) return 0;
+#ifndef S2C_EMUL
+  const AttnParams a = paged_params(d, pages, nullptr, nullptr, nullptr);
+  return d->dtype == kSeqF32 ? paged_plan<float>(a).bytes : paged_plan<bf16>(a).bytes;
+#else
   const s2c_attention_desc g = gathered(d, pages);
   return 2 * gathered_bytes(g) + s2c_attention_workspace(&g);
+#endif
 }
 
 int s2c_paged_attention(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* q, const void* keys, const void* values, const void* bias,
                         void* out, void* workspace, size_t workspace_bytes, void* stream) {
-  S2C_PAGES_TRY(page_check("s2c_paged_attention", pages));
-  if (!d) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: no description");
+  S2C_SEQ_TRY(page_check("s2c_paged_attention", pages));
+  S2C_SEQ_TRY(attn_check("s2c_paged_attention", d));
+  if (d->batch > 0 && d->lq > 0 && (!q || !out || (pages->count > 0 && (!keys || !values)))) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: a pointer is missing");
+  if ((bias != nullptr) != (d->bucket_of != nullptr)) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: a bias needs its buckets, and buckets a bias");
+  if (!aligned16(workspace)) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: the workspace starts on a 16-byte boundary");
+#ifndef S2C_EMUL
+  const AttnParams a = paged_params(d, pages, q, bias, out);
+  return d->dtype == kSeqF32 ? paged_launch<float>(a, pages, keys, values, workspace, workspace_bytes, (stream_t)stream)
+                             : paged_launch<bf16>(a, pages, keys, values, workspace, workspace_bytes, (stream_t)stream);
+#else
   const s2c_attention_desc g = gathered(d, pages);
-  if (pages->count > 0 && (!keys || !values)) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: a pointer is missing");
   const size_t need = s2c_paged_attention_workspace(d, pages), part = gathered_bytes(g);
   if (need > workspace_bytes || (need && !workspace)) return fail(S2C_ERR_WORKSPACE, "s2c_paged_attention: workspace too small");
   PageGatherParams p = {};
@@ -244,8 +330,9 @@ int s2c_paged_attention(const s2c_attention_desc* d, const s2c_page_desc* pages,
   for (int i = 0; i < 3; ++i) { p.stride[0][i] = pages->key_stride[i]; p.stride[1][i] = pages->value_stride[i]; }
   p.q_len = d->q_lengths; p.kv_len = d->kv_lengths; p.start = d->q_starts;
   p.batch = d->batch; p.length = g.lk; p.heads = d->kv_heads; p.dim = d->dim; p.lq = d->lq; p.causal = d->causal; p.start_all = d->q_start;
-  if (d->batch > 0 && d->lq > 0) S2C_PAGES_TRY(d->dtype == kSeqF32 ? page_gather<float>(p, (stream_t)stream) : page_gather<bf16>(p, (stream_t)stream));
+  if (d->batch > 0 && d->lq > 0) S2C_SEQ_TRY(d->dtype == kSeqF32 ? page_gather<float>(p, (stream_t)stream) : page_gather<bf16>(p, (stream_t)stream));
   return s2c_attention(&g, q, p.out[0], p.out[1], bias, out, nullptr, at + 2 * part, workspace_bytes - 2 * part, stream);
+#endif
 }
 
 int s2c_copy_pages(void* storage, long page_stride, long page_bytes, int count, const int* source, const int* target, long n, void* stream) {

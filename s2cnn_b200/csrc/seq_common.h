@@ -12,6 +12,17 @@ namespace s2c {
 
 enum SeqType : int { kSeqF32 = 0, kSeqBf16 = 1 };
 
+#define S2C_SEQ_TRY(expr)            \
+  do {                               \
+    int rc__ = (expr);               \
+    if (rc__ != S2C_OK) return rc__; \
+  } while (0)
+
+inline int seq_check_type(const char* who, int dtype) {
+  return dtype == kSeqF32 || dtype == kSeqBf16 ? S2C_OK : fail(S2C_ERR_BAD_ARG, std::string(who) + ": dtype is 0 (float32) or 1 (bfloat16)");
+}
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 struct bf16 {
   unsigned short bits;
 };

@@ -18,17 +18,6 @@
 
 namespace s2c {
 
-#define S2C_SEQ_TRY(expr)            \
-  do {                               \
-    int rc__ = (expr);               \
-    if (rc__ != S2C_OK) return rc__; \
-  } while (0)
-
-inline int seq_check_type(const char* who, int dtype) {
-  return dtype == kSeqF32 || dtype == kSeqBf16 ? S2C_OK : fail(S2C_ERR_BAD_ARG, std::string(who) + ": dtype is 0 (float32) or 1 (bfloat16)");
-}
-inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
 // ---- layer norm --------------------------------------------------------------------------------------------------------
 // A row takes the fewest threads that hold it, and the next one as it lies in memory, in their registers: neighbouring lanes up
 // to 1024 columns (512 of float32), a block of 128 up to 4096 (2048), of 512 beyond.
@@ -104,22 +93,6 @@ inline int dropout(const char* who, int dtype, DropoutParams p, const void* x, c
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
-constexpr int kAttnMaxDim = 128, kAttnMaxReach = 2048, kAttnMaxBuckets = 1024;
-inline int attn_check(const char* who, const s2c_attention_desc* d) {
-  const std::string w = std::string(who) + ": ";
-  if (!d) return fail(S2C_ERR_BAD_ARG, w + "no description");
-  S2C_SEQ_TRY(seq_check_type(who, d->dtype));
-  if (d->batch < 0 || d->lq < 0 || d->lk < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads || d->dim < 1)
-    return fail(S2C_ERR_BAD_ARG, w + "bad sizes (the query heads are a multiple of the key heads)");
-  if (d->dim > kAttnMaxDim) return fail(S2C_ERR_UNSUPPORTED, w + "at most 128 values per head");
-  if (std::max(d->lq, d->lk) > (1 << 28)) return fail(S2C_ERR_UNSUPPORTED, w + "at most 2^28 positions");
-  if ((long)d->batch * d->heads > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, w + "too many heads");
-  if (d->bucket_of && (d->n_buckets < 1 || d->reach < 0)) return fail(S2C_ERR_BAD_ARG, w + "bad buckets");
-  if (d->bucket_of && (d->n_buckets > kAttnMaxBuckets || d->reach > kAttnMaxReach))
-    return fail(S2C_ERR_UNSUPPORTED, w + "at most 1024 buckets and relative positions up to 2048");
-  if (!(std::fabs(d->scale) <= FLT_MAX)) return fail(S2C_ERR_BAD_ARG, w + "the scale is not finite");
-  return S2C_OK;
-}
 // what the library lays out itself; the caller's arrays need no more alignment than their type
 inline int attn_check_own(const char* who, const void* saved, const void* workspace) {
   return aligned16(saved) && aligned16(workspace) ? S2C_OK : fail(S2C_ERR_BAD_ARG, std::string(who) + ": saved and workspace start on 16-byte boundaries");
