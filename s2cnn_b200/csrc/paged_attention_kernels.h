@@ -49,29 +49,42 @@ __device__ __forceinline__ void paged_mma_tf32(float (&d)[4], unsigned a0, unsig
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// N consecutive values of a row from value c on: there where on > 0 and c < dim, NaN where on < 0, zeros otherwise.  WIDE: rows lie on
-// boundaries of N values (a piece that the row ends in is still read value by value).
+// 16 (8) bytes of a row into an operand's registers; where `on` is 0 they stay as they are
+template <int WORDS>
+__device__ __forceinline__ void paged_fetch(unsigned (&w)[WORDS], const void* from) {
+  if constexpr (WORDS == 4)
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(from) : "memory");
+  else
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(from) : "memory");
+}
+template <int WORDS>
+__device__ __forceinline__ void paged_fetch_if(unsigned (&w)[WORDS], const void* from, int on) {
+  if constexpr (WORDS == 4)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(from), "r"(on) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t@p ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}"
+                 : "+r"(w[0]), "+r"(w[1]) : "l"(from), "r"(on) : "memory");
+}
+// N consecutive values of a row from value c on, zeros from `dim` on.  WIDE: rows lie on boundaries of N values, and a piece that the
+// row ends in is read whole (it lies in the 16 bytes that its last value lies in).  Not `on`: zeros.
 template <class T, int N, bool WIDE>
-__device__ __forceinline__ void paged_load(unsigned (&w)[N * sizeof(T) / 4], const T* row, int c, int dim, int on) {
-  constexpr int kWords = N * sizeof(T) / 4;
+__device__ __forceinline__ void paged_load(unsigned (&w)[N * sizeof(T) / 4], const T* row, int c, int dim, bool on) {
+  constexpr int kWords = N * sizeof(T) / 4, kPer = 4 / sizeof(T);
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) w[i] = on < 0 ? 0x7fffffffu : 0u;
-  if (WIDE) {
-    const int whole = on > 0 && c + N <= dim;
-    if constexpr (kWords == 4)
-      asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-                   : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(row + c), "r"(whole) : "memory");
-    else
-      asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t@p ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}"
-                   : "+r"(w[0]), "+r"(w[1]) : "l"(row + c), "r"(whole) : "memory");
-    if (dim % N == 0 || whole || on <= 0 || c >= dim) return;
-  }
-  if (on <= 0) return;
+  for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  if constexpr (WIDE) {
+    paged_fetch_if(w, row + c, on && c < dim);
+    if (c + N > dim)
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    if (c + e >= dim) break;
-    if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const unsigned*>(row)[c + e];
-    else w[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[c + e] << (16 * (e % 2));
+      for (int i = 0; i < kWords; ++i) w[i] = c + (i + 1) * kPer <= dim ? w[i] : c + i * kPer >= dim ? 0u : w[i] & 0xffffu;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (!on || c + e >= dim) break;
+      if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const unsigned*>(row)[c + e];
+      else w[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[c + e] << (16 * (e % 2));
+    }
   }
 }
 
@@ -199,40 +212,59 @@ struct PagedAttention {
     const int page = p.pages.page, log_page = __ffs(page) - 1;
 
     Tile t;
-    // the page of every eighth position of a step, one to a lane
+    // the page of every eighth position of a step, one to a lane; -1: none, or not asked for
     auto pages_of = [&](int step) {
       const int j = (step * H::kWarps + warp) * H::kKeys + 8 * lane;
-      return lane < 2 * H::kTiles && step < s1 && j < keys ? table[j >> log_page] : -1;
+      const int id = lane < 2 * H::kTiles && step < s1 && j < keys ? table[j >> log_page] : -1;
+      return id < p.pages.count ? id : -1;
     };
-    auto load_keys = [&](int step, int ids) {
+    // a step whose positions all lie in the sequence, in pages that are there, with whole rows: loads and nothing else
+    auto all_there = [&](int step, int ids) {
+      const bool there = __all_sync(0xffffffffu, ids >= 0 || lane >= 2 * H::kTiles);
+      return WIDE && a.dim == DP && there && (step * H::kWarps + warp + 1) * H::kKeys <= keys;
+    };
+    constexpr int kPiece = 16 / (int)sizeof(T);
+    const long k_lane = g * p.ks[1] + q4 * kPiece, v_lane = (H::kHalf ? 2 * q4 : q4) * p.vs[1] + g * H::kVd, v_next = (H::kHalf ? 1 : 4) * p.vs[1];
+    auto load_keys = [&](int step, int ids, bool there) {
       const int j0 = (step * H::kWarps + warp) * H::kKeys;
 #pragma unroll
       for (int m = 0; m < 2 * H::kTiles; ++m) {
         const int id = __shfl_sync(0xffffffffu, ids, m), j = j0 + 8 * m;
-        const int on = step >= s1 || j + g >= keys ? 0 : id < 0 || id >= p.pages.count ? -1 : 1;
-        const T* row = kbase + (on > 0 ? (long)id * p.ks[0] + (long)((j & (page - 1)) + g) * p.ks[1] : 0);
+        const T* row = kbase + (id * p.ks[0] + (j & (page - 1)) * p.ks[1] + k_lane);
+        if (there) {
 #pragma unroll
-        for (int c = 0; c < H::kQk; ++c) paged_load<T, 16 / sizeof(T), WIDE>(t.k[m / 2][m % 2][c], row, (4 * c + q4) * (16 / (int)sizeof(T)), a.dim, on);
+          for (int c = 0; c < H::kQk; ++c) paged_fetch(t.k[m / 2][m % 2][c], row + 4 * c * kPiece);
+        } else {
+#pragma unroll
+          for (int c = 0; c < H::kQk; ++c)
+            paged_load<T, kPiece, WIDE>(t.k[m / 2][m % 2][c], row - q4 * kPiece, (4 * c + q4) * kPiece, a.dim, id >= 0 && j + g < keys);
+        }
       }
     };
-    auto load_values = [&](int step, int ids) {
+    auto load_values = [&](int step, int ids, bool there) {
       const int j0 = (step * H::kWarps + warp) * H::kKeys;
 #pragma unroll
       for (int m = 0; m < 2 * H::kTiles; ++m) {
         const int id = __shfl_sync(0xffffffffu, ids, m), j = j0 + 8 * m;
+        const T* row = vbase + (id * p.vs[0] + (j & (page - 1)) * p.vs[1] + v_lane);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = H::kHalf ? 2 * q4 + e : q4 + 4 * e;
-          const int on = step >= s1 || j + r >= keys ? 0 : id < 0 || id >= p.pages.count ? -1 : 1;
-          const T* row = vbase + (on > 0 ? (long)id * p.vs[0] + (long)((j & (page - 1)) + r) * p.vs[1] : 0);
+        for (int e = 0; e < 2; ++e, row += v_next) {
+          if (there) {
 #pragma unroll
-          for (int c = 0; c < H::kVc; ++c) paged_load<T, H::kVd, WIDE>(t.v[m / 2][2 * (m % 2) + e][c], row, (8 * c + g) * H::kVd, a.dim, on);
+            for (int c = 0; c < H::kVc; ++c) paged_fetch(t.v[m / 2][2 * (m % 2) + e][c], row + 8 * c * H::kVd);
+          } else {
+            const int r = H::kHalf ? 2 * q4 + e : q4 + 4 * e;
+#pragma unroll
+            for (int c = 0; c < H::kVc; ++c)
+              paged_load<T, H::kVd, WIDE>(t.v[m / 2][2 * (m % 2) + e][c], row - g * H::kVd, (8 * c + g) * H::kVd, a.dim, id >= 0 && j + r < keys);
+          }
         }
       }
     };
     int ids = pages_of(s0), next = pages_of(s0 + 1);
-    load_keys(s0, ids);
-    load_values(s0, ids);
+    bool there = all_there(s0, ids);
+    load_keys(s0, ids, there);
+    load_values(s0, ids, there);
 
     // ---- queries as the right operands of the scores, and what each row sees
     for (int e = ctx.tid; e < H::kQk * NT * 32; e += kThreads) {
@@ -290,8 +322,11 @@ struct PagedAttention {
 
     for (int step = s0; step < s1; ++step) {
       const int j0 = (step * H::kWarps + warp) * H::kKeys;
+      const int now = ids;
+      const bool now_there = __all_sync(0xffffffffu, now >= 0 || lane >= 2 * H::kTiles || j0 + 8 * lane >= keys);
       ids = next;
       next = pages_of(step + 2);
+      there = all_there(step + 1, ids);
       // ---- scores: 16 positions x 8 rows
       float x[H::kTiles][NT][4];
 #pragma unroll
@@ -339,60 +374,81 @@ struct PagedAttention {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[k][nt][e] += z[k][nt][e];
       }
-      load_keys(step + 1, ids);
+      load_keys(step + 1, ids, there);
       // ---- weights
       const bool far = !a.bias || j0 + H::kKeys - 1 - (i0 + s.start) <= -a.reach;    // one bias per head
-      const bool plain = j0 + H::kKeys <= all_see;
+      const bool plain = j0 + H::kKeys <= all_see && now_there;
       float top[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        top[nt][0] = top[nt][1] = kNoScore;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top[nt][e] = kNoScore;
+      if (plain && far) {
+#pragma unroll
+        for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[k][nt][e] = fmaf(x[k][nt][e], scale, flat[nt][e % 2]);
+              top[nt][e % 2] = fmaxf(top[nt][e % 2], x[k][nt][e]);
+            }
+      } else {
 #pragma unroll
         for (int k = 0; k < H::kTiles; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float add = flat[nt][e % 2];
             const int j = j0 + 16 * k + g + 8 * (e / 2);
-            if (!far) {
-              add = 0.f;
-              const int which = a.bucket_of[attn_clamp(j - pos[nt][e % 2], -a.reach, a.reach) + a.reach];
-              if (bias[nt][e % 2] && which >= 0 && which < a.n_buckets) add = attn_bias_units(widen(bias[nt][e % 2][(long)which * a.heads]));
+            const bool lost = __shfl_sync(0xffffffffu, now, 2 * k + e / 2) < 0;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float add = flat[nt][e % 2];
+              if (!far) {
+                add = 0.f;
+                const int which = a.bucket_of[attn_clamp(j - pos[nt][e % 2], -a.reach, a.reach) + a.reach];
+                if (bias[nt][e % 2] && which >= 0 && which < a.n_buckets) add = attn_bias_units(widen(bias[nt][e % 2][(long)which * a.heads]));
+              }
+              float y = fmaf(x[k][nt][e], scale, add);
+              if (lost) y = as_float(0x7fffffffu);                        // a page that is none
+              if (j >= lim[nt][e % 2]) y = kNoScore;
+              x[k][nt][e] = y;
+              top[nt][e % 2] = fmaxf(top[nt][e % 2], y);
             }
-            float y = fmaf(x[k][nt][e], scale, add);
-            if (!plain && j >= lim[nt][e % 2]) y = kNoScore;
-            x[k][nt][e] = y;
-            top[nt][e % 2] = fmaxf(top[nt][e % 2], y);
           }
       }
+      // The maximum is raised only where a score passes it by 8 (weights up to 2^8), so that hardly any step after a warp's first
+      // exchanges maxima or scales its sums.
       bool more = false;
-      float f[NT][2], base[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& y = top[nt][e];
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
-          y = fmaxf(y, m[nt][e]);
-          base[nt][e] = y == kNoScore ? 0.f : y;
-          f[nt][e] = exp2_fast(m[nt][e] - base[nt][e]);
-          more = more || y != m[nt][e];
-        }
+        for (int e = 0; e < 2; ++e) more = more || top[nt][e] > m[nt][e] + 8.f;
       if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            l[nt][e] *= f[nt][e];
-            m[nt][e] = top[nt][e];
+            float& y = top[nt][e];
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+            y = fmaxf(y, m[nt][e]);
+            f[e] = exp2_fast(m[nt][e] - (y == kNoScore ? 0.f : y));
+            l[nt][e] *= f[e];
+            m[nt][e] = y;
           }
 #pragma unroll
           for (int c = 0; c < H::kOut; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c][nt][e] *= f[nt][e % 2];
+            for (int e = 0; e < 4; ++e) acc[c][nt][e] *= f[e % 2];
         }
       }
+      float base[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) base[nt][e] = m[nt][e] == kNoScore ? 0.f : m[nt][e];
 #pragma unroll
       for (int k = 0; k < H::kTiles; ++k)
 #pragma unroll
@@ -455,7 +511,7 @@ struct PagedAttention {
           }
         }
       }
-      load_values(step + 1, ids);
+      load_values(step + 1, ids, there);
     }
     // ---- the warps' results: [warp][row][DP values, maximum, sum]
 #pragma unroll
