@@ -43,26 +43,6 @@ struct HeadParams {
   float eps, magnitude;
 };
 
-struct alignas(8) Vec8 {
-  unsigned w[2];
-};
-S2C_D void load_four(const float* p, float (&v)[4]) { load_vec(p, v); }
-S2C_D void load_four(const bf16* p, float (&v)[4]) {
-  const Vec8 u = *reinterpret_cast<const Vec8*>(p);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    v[2 * i] = as_float(u.w[i] << 16);
-    v[2 * i + 1] = as_float(u.w[i] & 0xffff0000u);
-  }
-}
-S2C_D void store_four(float* p, const float (&v)[4]) { store_vec(p, v); }
-S2C_D void store_four(bf16* p, const float (&v)[4]) {
-  Vec8 u;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) u.w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-  *reinterpret_cast<Vec8*>(p) = u;
-}
-
 // f in radians per position as a fraction of a turn, in units of 2^-64
 S2C_D unsigned long long turn_units(double f) {
   double t = f * 0.15915494309189533577;

@@ -10,6 +10,8 @@
 //
 // Keys of the next tile are asked for as soon as the scores of this one are done, its values as soon as the outputs are: a warp has
 // up to 8 KB (float32 16) on its way and waits for nobody.  The page of every eighth position comes a tile earlier, by one load per warp.
+// A tile that goes past the last position reads that one again there, with a weight of 0, and where the table names no page, page 0: no
+// load is guarded.  (Guarded ones, whose registers keep what they held, cost 64 x 16384 positions 579 us instead of 313.)
 //
 // Work is dealt in steps of (4 warps x tile) positions of one item (sequence, key head, row block), an equal share to each block as
 // the lengths on the device give it: a block finds where its share begins by adding up the sequences' steps.  Items that lie in
@@ -31,7 +33,9 @@ struct PagedParams {
   PageTable pages;
   long ks[3], vs[3];         // page, position, head
   int row_blocks;
-  float* part;               // [2 blocks][rows][DP + 2]: slot 2 c: an item that began before block c; 2 c + 1: one that goes on behind it
+  Divisor by_group, by_row_blocks, by_buckets;     // of the rows, the items of a sequence, and n_buckets + 1
+  int wide_out;              // out in pieces of four values
+  float* part;               // [2 blocks][rows][DP + 4]: slot 2 c: an item that began before block c; 2 c + 1: one that goes on behind it
   int4* split;               // [min(items, blocks)]: item, first block, blocks of an item that is joined; 0 blocks: none
 };
 
@@ -49,41 +53,28 @@ __device__ __forceinline__ void paged_mma_tf32(float (&d)[4], unsigned a0, unsig
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 (8) bytes of a row into an operand's registers; where `on` is 0 they stay as they are
-template <int WORDS>
-__device__ __forceinline__ void paged_fetch(unsigned (&w)[WORDS], const void* from) {
-  if constexpr (WORDS == 4)
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(from) : "memory");
-  else
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(from) : "memory");
-}
-template <int WORDS>
-__device__ __forceinline__ void paged_fetch_if(unsigned (&w)[WORDS], const void* from, int on) {
-  if constexpr (WORDS == 4)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-                 : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(from), "r"(on) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t@p ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}"
-                 : "+r"(w[0]), "+r"(w[1]) : "l"(from), "r"(on) : "memory");
-}
-// N consecutive values of a row from value c on, zeros from `dim` on.  WIDE: rows lie on boundaries of N values, and a piece that the
-// row ends in is read whole (it lies in the 16 bytes that its last value lies in).  Not `on`: zeros.
-template <class T, int N, bool WIDE>
-__device__ __forceinline__ void paged_load(unsigned (&w)[N * sizeof(T) / 4], const T* row, int c, int dim, bool on) {
-  constexpr int kWords = N * sizeof(T) / 4, kPer = 4 / sizeof(T);
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) w[i] = 0u;
-  if constexpr (WIDE) {
-    paged_fetch_if(w, row + c, on && c < dim);
-    if (c + N > dim)
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = c + (i + 1) * kPer <= dim ? w[i] : c + i * kPer >= dim ? 0u : w[i] & 0xffffu;
+// How rows are read: value by value; in whole pieces of 16 bytes, on whose boundaries they lie, of which the last ones may hold
+// less or nothing of a head; or such that a head fills all pieces.
+enum PagedRows : int { kRowsByValue, kRowsInPieces, kRowsFull };
+// N consecutive values of a row from value c on, as an operand's registers hold them.  Where a head has ended: zeros by value; in
+// pieces what lies behind it in the piece that its last value lies in, and in place of pieces beyond that one, the row's first.
+template <class T, int N, int ROWS>
+__device__ __forceinline__ void paged_load(unsigned (&w)[N * sizeof(T) / 4], const T* row, int c, int dim) {
+  if constexpr (ROWS != kRowsByValue) {
+    const T* from = row + (ROWS == kRowsFull || c < dim ? c : 0);
+    if constexpr (N * sizeof(T) == 16)
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(from) : "memory");
+    else
+      asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(from) : "memory");
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      if (!on || c + e >= dim) break;
-      if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const unsigned*>(row)[c + e];
-      else w[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[c + e] << (16 * (e % 2));
+      if constexpr (sizeof(T) == 4) {
+        w[e] = c + e < dim ? reinterpret_cast<const unsigned*>(row)[c + e] : 0u;
+      } else if (e % 2 == 0) {
+        const unsigned short* at = reinterpret_cast<const unsigned short*>(row) + c + e;
+        w[e / 2] = (c + e < dim ? at[0] : 0u) | (c + e + 1 < dim ? (unsigned)at[1] << 16 : 0u);
+      }
     }
   }
 }
@@ -98,7 +89,7 @@ struct PagedShape {
   static constexpr int kQk = kHalf ? DP / 32 : DP / 16;                       // a row's chunks of four 16-byte pieces
   static constexpr int kVd = kHalf && DP > 32 ? 8 : 4, kVc = DP / (8 * kVd);   // a lane's consecutive values of a row of V, chunks
   static constexpr int kOut = DP / 16;                                        // tiles of 16 rows of O^T
-  static constexpr size_t kQuery = (size_t)kQk * NT * 32 * 16 * (kHalf ? 1 : 2), kJoin = (size_t)kWarps * kRows * (DP + 2) * 4;
+  static constexpr size_t kQuery = (size_t)kQk * NT * 32 * 16 * (kHalf ? 1 : 2), kJoin = (size_t)kWarps * kRows * (DP + 4) * 4 + kRows * 5 * 4;
   // where value `m` (0: of the upper eight rows) of tile t of a lane lies in a head
   static __device__ __forceinline__ int value(int t, int lane) { return t / (kVd / 2) * 8 * kVd + lane / 4 * kVd + 2 * (t % (kVd / 2)); }
 };
@@ -110,13 +101,20 @@ __device__ __forceinline__ int paged_steps(const AttnParams& a, int b, int step)
   return n > 0 ? n : 1;
 }
 
-template <class T, int DP, int NT, bool WIDE>
+template <class T, int DP, int NT, int ROWS>
 struct PagedAttention {
   using Params = PagedParams;
   using H = PagedShape<T, DP, NT>;
   static constexpr int kThreads = H::kThreads;
-  static constexpr int kBlocks = H::kHalf ? (NT == 1 ? 3 : 2) : 2;
-  static size_t smem() { return H::kQuery + H::kJoin + 64; }
+  static constexpr int kBlocks = (H::kHalf ? DP <= 64 || NT == 1 : DP <= 64) ? 3 : 2;      // as registers allow
+  // queries, results, the search for the share; the biases of each row by bucket, 0 behind them, and the bucket of each position
+  static size_t smem(const AttnParams& a) {
+    return H::kQuery + H::kJoin + 64 + (a.bias ? (size_t)H::kRows * (a.n_buckets + 1) * 4 + (size_t)(2 * a.reach + 1) * 2 : 0);
+  }
+  // (64 bits only where they are needed: a division of them is a hundred instructions)
+  static __device__ __forceinline__ long quotient(long x, long y) {
+    return (x | y) >> 32 ? x / y : (long)((unsigned)x / (unsigned)y);
+  }
 
   struct Tile {
     unsigned k[H::kTiles][2][H::kQk][4];
@@ -129,6 +127,8 @@ struct PagedAttention {
     uint4* const query = reinterpret_cast<uint4*>(smem);
     float* const join = reinterpret_cast<float*>(smem + H::kQuery);
     long* const find = reinterpret_cast<long*>(smem + H::kQuery + H::kJoin);      // [0 .. 3] the warps' sums, [4], [5] where the share begins
+    float* const biases = reinterpret_cast<float*>(smem + H::kQuery + H::kJoin + 64);
+    unsigned short* const bucket = reinterpret_cast<unsigned short*>(biases + H::kRows * (a.n_buckets + 1));
     const int per_batch = a.kv_heads * p.row_blocks;                              // items of a sequence
 
     // ---- this block's share: steps [lo, hi) of all
@@ -156,7 +156,13 @@ struct PagedAttention {
       if (!by_item && ctx.tid == 0) p.split[ctx.bid] = make_int4(0, 0, 0, 0);
       return;
     }
-    const long lo = ctx.bid * total / blocks, hi = (ctx.bid + 1) * total / blocks;
+    const long each = quotient(total, blocks), rest = total - each * blocks;       // the first `rest` blocks have one more
+    const long lo = ctx.bid * each + min((long)ctx.bid, rest), hi = lo + each + (ctx.bid < rest);
+    if (a.bias)
+      for (int e = ctx.tid; e <= 2 * a.reach; e += kThreads) {
+        const int which = a.bucket_of[e];
+        bucket[e] = (unsigned short)(which >= 0 && which < a.n_buckets ? which : a.n_buckets);
+      }
     if (before * per_batch <= lo && lo < (before + sum) * per_batch) {
       int b = ctx.tid * mine;
       for (;; ++b) {
@@ -170,20 +176,20 @@ struct PagedAttention {
     ctx.sync();
     int b = (int)find[4];
     int n = paged_steps(a, b, H::kStep);
-    int within = (int)(find[5] / n), s0 = (int)(find[5] % n);
+    int within = (int)quotient(find[5], n), s0 = (int)(find[5] - (long)within * n);
     bool joined = false;
     for (long at = lo; at < hi;) {
       const int s1 = (int)min((long)n, s0 + (hi - at));
-      const int hk = within / p.row_blocks, rb = within % p.row_blocks, item = b * per_batch + within;
+      const int hk = p.by_row_blocks.quotient(within), rb = within - hk * p.row_blocks, item = b * per_batch + within;
       const bool whole = s0 == 0 && s1 == n;
-      float* part = whole ? nullptr : p.part + (2L * ctx.bid + (s0 == 0 ? 1 : 0)) * H::kRows * (DP + 2);
-      piece(ctx, p, query, join, b, hk, rb, s0, s1, part);
+      float* part = whole ? nullptr : p.part + (2L * ctx.bid + (s0 == 0 ? 1 : 0)) * H::kRows * (DP + 4);
+      piece(ctx, p, query, join, biases, bucket, b, hk, rb, s0, s1, part);
       if (ctx.tid == 0) {
         if (by_item) {
           if (whole) p.split[item] = make_int4(0, 0, 0, 0);
         }
         if (!whole && s0 == 0) {
-          const long last = ((at + n) * blocks - 1) / total;
+          const long end = at + n - 1, more = rest * (each + 1), last = end < more ? quotient(end, each + 1) : rest + quotient(end - more, each);
           p.split[by_item ? item : ctx.bid] = make_int4(item, ctx.bid, (int)(last - ctx.bid) + 1, 0);
           joined = true;
         }
@@ -198,80 +204,122 @@ struct PagedAttention {
     if (!by_item && !joined && ctx.tid == 0) p.split[ctx.bid] = make_int4(0, 0, 0, 0);
   }
 
+  // S^T: 16 positions x 8 rows a tile
+  static __device__ __forceinline__ void scores(const uint4* query, int lane, int dim, Tile& t, float (&x)[H::kTiles][NT][4]) {
+    // a piece that the head ends in holds what lies behind it, pieces beyond it the row's first values
+    if (ROWS == kRowsInPieces)
+#pragma unroll
+      for (int c = 0; c < H::kQk; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int left = dim - (4 * c + lane % 4) * (16 / (int)sizeof(T)) - w * (4 / (int)sizeof(T));      // values of the word
+          const unsigned keep = left >= 4 / (int)sizeof(T) ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+#pragma unroll
+          for (int m = 0; m < 2 * H::kTiles; ++m) t.k[m / 2][m % 2][c][w] &= keep;
+        }
+#pragma unroll
+    for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][nt][e] = 0.f;
+    if constexpr (H::kHalf) {
+#pragma unroll
+      for (int c = 0; c < H::kQk; ++c)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 y = query[(c * NT + nt) * 32 + lane];
+#pragma unroll
+          for (int k = 0; k < H::kTiles; ++k) {
+            paged_mma(x[k][nt], t.k[k][0][c][0], t.k[k][1][c][0], t.k[k][0][c][1], t.k[k][1][c][1], y.x, y.y);
+            paged_mma(x[k][nt], t.k[k][0][c][2], t.k[k][1][c][2], t.k[k][0][c][3], t.k[k][1][c][3], y.z, y.w);
+          }
+        }
+    } else {
+      float z[H::kTiles][NT][4] = {};                  // the small products
+#pragma unroll
+      for (int c = 0; c < H::kQk; ++c)
+#pragma unroll
+        for (int k = 0; k < H::kTiles; ++k) {
+          FewSplit u[2][4];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[e / 4][e % 4] = few_split(as_float(t.k[k][e / 4][c][e % 4]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 hi = query[2 * ((c * NT + nt) * 32 + lane)], lo = query[2 * ((c * NT + nt) * 32 + lane) + 1];
+            paged_mma_tf32(z[k][nt], u[0][0].lo, u[1][0].lo, u[0][1].lo, u[1][1].lo, hi.x, hi.y);
+            paged_mma_tf32(z[k][nt], u[0][0].hi, u[1][0].hi, u[0][1].hi, u[1][1].hi, lo.x, lo.y);
+            paged_mma_tf32(x[k][nt], u[0][0].hi, u[1][0].hi, u[0][1].hi, u[1][1].hi, hi.x, hi.y);
+            paged_mma_tf32(z[k][nt], u[0][2].lo, u[1][2].lo, u[0][3].lo, u[1][3].lo, hi.z, hi.w);
+            paged_mma_tf32(z[k][nt], u[0][2].hi, u[1][2].hi, u[0][3].hi, u[1][3].hi, lo.z, lo.w);
+            paged_mma_tf32(x[k][nt], u[0][2].hi, u[1][2].hi, u[0][3].hi, u[1][3].hi, hi.z, hi.w);
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < H::kTiles; ++k)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k][nt][e] += z[k][nt][e];
+    }
+  }
+
   // steps [s0, s1) of one item; to `part`, or to the output where that is null
-  static __device__ __forceinline__ void piece(const Ctx& ctx, const Params& p, uint4* query, float* join, int b, int hk, int rb, int s0, int s1, float* part) {
+  static __device__ __forceinline__ void piece(const Ctx& ctx, const Params& p, uint4* query, float* join, float* biases, const unsigned short* bucket, int b, int hk,
+                                               int rb, int s0, int s1, float* part) {
     const AttnParams& a = p.a;
     const int lane = ctx.tid % 32, warp = ctx.tid / 32, g = lane / 4, q4 = lane % 4;
     const int rows = a.lq * a.group, r0 = rb * H::kRows, left = min(H::kRows, rows - r0);
     const AttnSeq s = attn_seq(a, b);
-    const int i0 = r0 / a.group, i1 = min((r0 + left - 1) / a.group + 1, s.qlen);      // queries of the block
+    const int i0 = p.by_group.quotient(r0), i1 = min((int)p.by_group.quotient(r0 + left - 1) + 1, s.qlen);      // queries of the block
     const int keys = i0 < s.qlen ? attn_keys(a, s, i1) : 0;
     const T* const kbase = static_cast<const T*>(p.pages.array[0]) + hk * p.ks[2];
     const T* const vbase = static_cast<const T*>(p.pages.array[1]) + hk * p.vs[2];
     const int* const table = p.pages.table + (long)b * p.pages.columns;
     const int page = p.pages.page, log_page = __ffs(page) - 1;
 
-    Tile t;
-    // the page of every eighth position of a step, one to a lane; -1: none, or not asked for
+    Tile t = {};
+    // the page of every eighth position of a step, one to a lane; -1: none
     auto pages_of = [&](int step) {
-      const int j = (step * H::kWarps + warp) * H::kKeys + 8 * lane;
-      const int id = lane < 2 * H::kTiles && step < s1 && j < keys ? table[j >> log_page] : -1;
+      const int j = step < s1 ? min((step * H::kWarps + warp) * H::kKeys + 8 * lane, keys - 1) : keys - 1;
+      const int id = lane < 2 * H::kTiles && j >= 0 ? table[j >> log_page] : -1;
       return id < p.pages.count ? id : -1;
     };
-    // a step whose positions all lie in the sequence, in pages that are there, with whole rows: loads and nothing else
-    auto all_there = [&](int step, int ids) {
-      const bool there = __all_sync(0xffffffffu, ids >= 0 || lane >= 2 * H::kTiles);
-      return WIDE && a.dim == DP && there && (step * H::kWarps + warp + 1) * H::kKeys <= keys;
-    };
     constexpr int kPiece = 16 / (int)sizeof(T);
-    const long k_lane = g * p.ks[1] + q4 * kPiece, v_lane = (H::kHalf ? 2 * q4 : q4) * p.vs[1] + g * H::kVd, v_next = (H::kHalf ? 1 : 4) * p.vs[1];
-    auto load_keys = [&](int step, int ids, bool there) {
-      const int j0 = (step * H::kWarps + warp) * H::kKeys;
+    auto load_keys = [&](int step, int ids) {
+      const int j0 = step < s1 ? (step * H::kWarps + warp) * H::kKeys : keys;      // (behind the last step: the last position)
 #pragma unroll
       for (int m = 0; m < 2 * H::kTiles; ++m) {
-        const int id = __shfl_sync(0xffffffffu, ids, m), j = j0 + 8 * m;
-        const T* row = kbase + (id * p.ks[0] + (j & (page - 1)) * p.ks[1] + k_lane);
-        if (there) {
+        const int id = max(__shfl_sync(0xffffffffu, ids, m), 0), j = max(min(j0 + 8 * m + g, keys - 1), 0);
+        const T* row = kbase + (id * p.ks[0] + (j & (page - 1)) * p.ks[1]);
 #pragma unroll
-          for (int c = 0; c < H::kQk; ++c) paged_fetch(t.k[m / 2][m % 2][c], row + 4 * c * kPiece);
-        } else {
+        for (int c = 0; c < H::kQk; ++c) paged_load<T, kPiece, ROWS>(t.k[m / 2][m % 2][c], row, (4 * c + q4) * kPiece, a.dim);
+      }
+    };
+    auto load_values = [&](int step, int ids) {
+      const int j0 = step < s1 ? (step * H::kWarps + warp) * H::kKeys : keys;      // (behind the last step: the last position)
 #pragma unroll
-          for (int c = 0; c < H::kQk; ++c)
-            paged_load<T, kPiece, WIDE>(t.k[m / 2][m % 2][c], row - q4 * kPiece, (4 * c + q4) * kPiece, a.dim, id >= 0 && j + g < keys);
+      for (int m = 0; m < 2 * H::kTiles; ++m) {
+        const int id = max(__shfl_sync(0xffffffffu, ids, m), 0);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = max(min(j0 + 8 * m + (H::kHalf ? 2 * q4 + e : q4 + 4 * e), keys - 1), 0);
+          const T* row = vbase + (id * p.vs[0] + (j & (page - 1)) * p.vs[1]);
+#pragma unroll
+          for (int c = 0; c < H::kVc; ++c) paged_load<T, H::kVd, ROWS>(t.v[m / 2][2 * (m % 2) + e][c], row, (8 * c + g) * H::kVd, a.dim);
         }
       }
     };
-    auto load_values = [&](int step, int ids, bool there) {
-      const int j0 = (step * H::kWarps + warp) * H::kKeys;
-#pragma unroll
-      for (int m = 0; m < 2 * H::kTiles; ++m) {
-        const int id = __shfl_sync(0xffffffffu, ids, m), j = j0 + 8 * m;
-        const T* row = vbase + (id * p.vs[0] + (j & (page - 1)) * p.vs[1] + v_lane);
-#pragma unroll
-        for (int e = 0; e < 2; ++e, row += v_next) {
-          if (there) {
-#pragma unroll
-            for (int c = 0; c < H::kVc; ++c) paged_fetch(t.v[m / 2][2 * (m % 2) + e][c], row + 8 * c * H::kVd);
-          } else {
-            const int r = H::kHalf ? 2 * q4 + e : q4 + 4 * e;
-#pragma unroll
-            for (int c = 0; c < H::kVc; ++c)
-              paged_load<T, H::kVd, WIDE>(t.v[m / 2][2 * (m % 2) + e][c], row - g * H::kVd, (8 * c + g) * H::kVd, a.dim, id >= 0 && j + r < keys);
-          }
-        }
-      }
-    };
-    int ids = pages_of(s0), next = pages_of(s0 + 1);
-    bool there = all_there(s0, ids);
-    load_keys(s0, ids, there);
-    load_values(s0, ids, there);
+    int now = pages_of(s0), ids = pages_of(s0 + 1);
+    load_keys(s0, now);
+    load_values(s0, now);
 
     // ---- queries as the right operands of the scores, and what each row sees
     for (int e = ctx.tid; e < H::kQk * NT * 32; e += kThreads) {
-      const int c = e / 32 / NT, nt = e / 32 % NT, l = e % 32, r = r0 + 8 * nt + l / 4, i = r / a.group;
+      const int c = e / 32 / NT, nt = e / 32 % NT, l = e % 32, r = r0 + 8 * nt + l / 4, i = p.by_group.quotient(r);
       unsigned w[4];
-      paged_load<T, 16 / sizeof(T), false>(w, static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + (hk * a.group + r % a.group) * a.qs[2],
-                                           (4 * c + l % 4) * (16 / (int)sizeof(T)), a.dim, r < rows && i < s.qlen && keys > 0);
+      paged_load<T, kPiece, kRowsByValue>(w, static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + (hk * a.group + r - i * a.group) * a.qs[2],
+                                          (4 * c + l % 4) * kPiece, r < rows && i < s.qlen && keys > 0 ? a.dim : 0);
       if constexpr (H::kHalf) {
         query[e] = make_uint4(w[0], w[1], w[2], w[3]);
       } else {
@@ -282,30 +330,30 @@ struct PagedAttention {
         query[2 * e + 1] = make_uint4(x[0].lo, x[1].lo, x[2].lo, x[3].lo);
       }
     }
-    int lim[NT][2], pos[NT][2];                          // a row sees the positions before lim
-    float flat[NT][2];
-    const T* bias[NT][2];
+    if (a.bias)
+      for (int e = ctx.tid; e < H::kRows * (a.n_buckets + 1); e += kThreads) {
+        const int row = p.by_buckets.quotient(e), r = r0 + row, which = e - row * (a.n_buckets + 1);
+        biases[e] = r < rows && which < a.n_buckets
+                        ? attn_bias_units(widen(static_cast<const T*>(a.bias)[(long)which * a.heads + hk * a.group + p.by_group.rest(r)])) : 0.f;
+      }
+    int lim[NT][2];                                      // a row sees the positions before lim
     int all_see = keys;                                  // that every row sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = r0 + 8 * nt + 2 * q4 + e, i = r / a.group;
-        const bool in = r < rows && i < s.qlen;
-        pos[nt][e] = i + s.start;
-        lim[nt][e] = in ? attn_keys(a, s, i + 1) : r < rows ? 0 : keys;
+        const int r = r0 + 8 * nt + 2 * q4 + e, i = p.by_group.quotient(r);
+        lim[nt][e] = r >= rows ? keys : i < s.qlen ? attn_keys(a, s, i + 1) : 0;
         all_see = min(all_see, lim[nt][e]);
-        flat[nt][e] = 0.f;
-        bias[nt][e] = nullptr;
-        if (a.bias && r < rows) {
-          bias[nt][e] = static_cast<const T*>(a.bias) + hk * a.group + r % a.group;
-          const int which = a.bucket_of[0];
-          if (which >= 0 && which < a.n_buckets) flat[nt][e] = attn_bias_units(widen(bias[nt][e][(long)which * a.heads]));
-        }
       }
     all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 1));
     all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, 2));
-    ctx.sync();                                          // the queries
+    ctx.sync();                                          // queries and biases
+    float flat[NT][2];                                   // the bias of what lies beyond the reach
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) flat[nt][e] = a.bias ? biases[(8 * nt + 2 * q4 + e) * (a.n_buckets + 1) + bucket[0]] : 0.f;
 
     const float scale = a.scale * kLog2e;
     float acc[H::kOut][NT][4], m[NT][2], l[NT][2];
@@ -321,63 +369,14 @@ struct PagedAttention {
       for (int e = 0; e < 2; ++e) { m[nt][e] = kNoScore; l[nt][e] = 0.f; }
 
     for (int step = s0; step < s1; ++step) {
-      const int j0 = (step * H::kWarps + warp) * H::kKeys;
-      const int now = ids;
-      const bool now_there = __all_sync(0xffffffffu, now >= 0 || lane >= 2 * H::kTiles || j0 + 8 * lane >= keys);
-      ids = next;
-      next = pages_of(step + 2);
-      there = all_there(step + 1, ids);
-      // ---- scores: 16 positions x 8 rows
+      const int j0 = (step * H::kWarps + warp) * H::kKeys, next = pages_of(step + 2);
+      const bool there = __all_sync(0xffffffffu, now >= 0 || lane >= 2 * H::kTiles);
       float x[H::kTiles][NT][4];
-#pragma unroll
-      for (int k = 0; k < H::kTiles; ++k)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[k][nt][e] = 0.f;
-      if constexpr (H::kHalf) {
-#pragma unroll
-        for (int c = 0; c < H::kQk; ++c)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint4 y = query[(c * NT + nt) * 32 + lane];
-#pragma unroll
-            for (int k = 0; k < H::kTiles; ++k) {
-              paged_mma(x[k][nt], t.k[k][0][c][0], t.k[k][1][c][0], t.k[k][0][c][1], t.k[k][1][c][1], y.x, y.y);
-              paged_mma(x[k][nt], t.k[k][0][c][2], t.k[k][1][c][2], t.k[k][0][c][3], t.k[k][1][c][3], y.z, y.w);
-            }
-          }
-      } else {
-        float z[H::kTiles][NT][4] = {};                  // the small products
-#pragma unroll
-        for (int c = 0; c < H::kQk; ++c)
-#pragma unroll
-          for (int k = 0; k < H::kTiles; ++k) {
-            FewSplit u[2][4];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e / 4][e % 4] = few_split(as_float(t.k[k][e / 4][c][e % 4]));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint4 hi = query[2 * ((c * NT + nt) * 32 + lane)], lo = query[2 * ((c * NT + nt) * 32 + lane) + 1];
-              paged_mma_tf32(z[k][nt], u[0][0].lo, u[1][0].lo, u[0][1].lo, u[1][1].lo, hi.x, hi.y);
-              paged_mma_tf32(z[k][nt], u[0][0].hi, u[1][0].hi, u[0][1].hi, u[1][1].hi, lo.x, lo.y);
-              paged_mma_tf32(x[k][nt], u[0][0].hi, u[1][0].hi, u[0][1].hi, u[1][1].hi, hi.x, hi.y);
-              paged_mma_tf32(z[k][nt], u[0][2].lo, u[1][2].lo, u[0][3].lo, u[1][3].lo, hi.z, hi.w);
-              paged_mma_tf32(z[k][nt], u[0][2].hi, u[1][2].hi, u[0][3].hi, u[1][3].hi, lo.z, lo.w);
-              paged_mma_tf32(x[k][nt], u[0][2].hi, u[1][2].hi, u[0][3].hi, u[1][3].hi, hi.z, hi.w);
-            }
-          }
-#pragma unroll
-        for (int k = 0; k < H::kTiles; ++k)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[k][nt][e] += z[k][nt][e];
-      }
-      load_keys(step + 1, ids, there);
+      scores(query, lane, a.dim, t, x);
+      load_keys(step + 1, ids);
       // ---- weights
       const bool far = !a.bias || j0 + H::kKeys - 1 - (i0 + s.start) <= -a.reach;    // one bias per head
-      const bool plain = j0 + H::kKeys <= all_see && now_there;
+      const bool plain = j0 + H::kKeys <= all_see && there;
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -402,12 +401,8 @@ struct PagedAttention {
             const bool lost = __shfl_sync(0xffffffffu, now, 2 * k + e / 2) < 0;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float add = flat[nt][e % 2];
-              if (!far) {
-                add = 0.f;
-                const int which = a.bucket_of[attn_clamp(j - pos[nt][e % 2], -a.reach, a.reach) + a.reach];
-                if (bias[nt][e % 2] && which >= 0 && which < a.n_buckets) add = attn_bias_units(widen(bias[nt][e % 2][(long)which * a.heads]));
-              }
+              const int row = 8 * nt + 2 * q4 + e % 2, away = far ? 0 : attn_clamp(j - (int)p.by_group.quotient(r0 + row) - s.start, -a.reach, a.reach) + a.reach;
+              const float add = far ? flat[nt][e % 2] : biases[row * (a.n_buckets + 1) + bucket[away]];
               float y = fmaf(x[k][nt][e], scale, add);
               if (lost) y = as_float(0x7fffffffu);                        // a page that is none
               if (j >= lim[nt][e % 2]) y = kNoScore;
@@ -511,7 +506,9 @@ struct PagedAttention {
           }
         }
       }
-      load_values(step + 1, ids, there);
+      load_values(step + 1, ids);
+      now = ids;
+      ids = next;
     }
     // ---- the warps' results: [warp][row][DP values, maximum, sum]
 #pragma unroll
@@ -522,7 +519,7 @@ struct PagedAttention {
         y += __shfl_xor_sync(0xffffffffu, y, 4);
         y += __shfl_xor_sync(0xffffffffu, y, 8);
         y += __shfl_xor_sync(0xffffffffu, y, 16);
-        float* to = join + (warp * H::kRows + 8 * nt + 2 * q4 + e) * (DP + 2);
+        float* to = join + (warp * H::kRows + 8 * nt + 2 * q4 + e) * (DP + 4);
 #pragma unroll
         for (int c = 0; c < H::kOut; ++c) *reinterpret_cast<float2*>(to + H::value(c, lane)) = make_float2(acc[c][nt][e], acc[c][nt][2 + e]);
         if (g == 0) {
@@ -531,36 +528,58 @@ struct PagedAttention {
         }
       }
     ctx.sync();
-    for (int e = ctx.tid; e < left * DP; e += kThreads) {
-      const int r = e / DP, c = e % DP;
-      float top = kNoScore;
+    float* const factor = join + H::kWarps * H::kRows * (DP + 4);                       // [row][5]: of the warps, 1 / sum
+    if (ctx.tid < H::kRows) {
+      const float* from = join + ctx.tid * (DP + 4);
+      constexpr int kNext = H::kRows * (DP + 4);
+      float top = kNoScore, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < H::kWarps; ++w) top = fmaxf(top, join[(w * H::kRows + r) * (DP + 2) + DP]);
+      for (int w = 0; w < H::kWarps; ++w) top = fmaxf(top, from[w * kNext + DP]);
       const float base = top == kNoScore ? 0.f : top;
-      float o = 0.f, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < H::kWarps; ++w) {
-        const float* from = join + (w * H::kRows + r) * (DP + 2);
-        const float f = exp2_fast(from[DP] - base);
-        o = fmaf(from[c], f, o);
-        sum = fmaf(from[DP + 1], f, sum);
+        const float f = exp2_fast(from[w * kNext + DP] - base);
+        factor[5 * ctx.tid + w] = f;
+        sum = fmaf(from[w * kNext + DP + 1], f, sum);
       }
-      if (part) {
-        part[r * (DP + 2) + c] = o;
-        if (c == 0) {
-          part[r * (DP + 2) + DP] = top;
-          part[r * (DP + 2) + DP + 1] = sum;
-        }
-      } else if (c < a.dim) {
-        write(p, b, hk, r0 + r, c, o, sum);
+      factor[5 * ctx.tid + 4] = sum == 0.f ? 0.f : 1.f / sum;
+      if (part) *reinterpret_cast<float2*>(part + ctx.tid * (DP + 4) + DP) = make_float2(top, sum);
+    }
+    ctx.sync();
+    for (int e = ctx.tid; e < left * (DP / 4); e += kThreads) {
+      const int r = e / (DP / 4), c = e % (DP / 4) * 4;
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < H::kWarps; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(join + (w * H::kRows + r) * (DP + 4) + c);
+        const float f = factor[5 * r + w];
+        o[0] = fmaf(x.x, f, o[0]);
+        o[1] = fmaf(x.y, f, o[1]);
+        o[2] = fmaf(x.z, f, o[2]);
+        o[3] = fmaf(x.w, f, o[3]);
       }
+      if (part) store_four(part + r * (DP + 4) + c, o);
+      else write<4>(p, b, hk, r0 + r, c, o, factor[5 * r + 4]);
     }
     ctx.sync();                                          // queries and results are written again
   }
-  static __device__ __forceinline__ void write(const Params& p, int b, int hk, int r, int c, float o, float sum) {
+  // N values of a row of the output from value c on
+  template <int N>
+  static __device__ __forceinline__ void write(const Params& p, int b, int hk, int r, int c, float (&o)[N], float over_sum) {
     const AttnParams& a = p.a;
-    const int i = r / a.group, h = hk * a.group + r % a.group;
-    narrow(static_cast<T*>(a.out) + (((long)b * a.lq + i) * a.heads + h) * a.dim + c, sum == 0.f ? 0.f : o / sum);
+    const int i = p.by_group.quotient(r), h = hk * a.group + r - i * a.group;
+    T* out = static_cast<T*>(a.out) + (((long)b * a.lq + i) * a.heads + h) * a.dim;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = over_sum == 0.f ? 0.f : o[e] * over_sum;
+    if constexpr (N == 4) {
+      if (p.wide_out) {
+        if (c < a.dim) store_four(out + c, o);
+        return;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < a.dim) narrow(out + c + e, o[e]);
   }
 };
 
@@ -580,7 +599,7 @@ struct PagedJoin {
     const int t = ctx.tid, lane = t % 32, warp = t / 32;
     float *red = reinterpret_cast<float*>(smem), *outs = red + 8, *weight = outs + kThreads;
     // block k's part of it: the first one's lies where what goes on is kept
-    auto part = [&](int k) { return p.part + ((2L * (what.y + k) + (k == 0)) * H::kRows + r) * (DP + 2); };
+    auto part = [&](int k) { return p.part + ((2L * (what.y + k) + (k == 0)) * H::kRows + r) * (DP + 4); };
     float m = kNoScore;
     for (int e = t; e < n; e += kThreads) m = fmaxf(m, part(e)[DP]);
     m = lanes_max<32>(ctx, m);
@@ -606,7 +625,8 @@ struct PagedJoin {
     ctx.sync();
     if (t >= DP) return;
     for (int e = 1; e < kSlices; ++e) o += outs[e * DP + t];
-    if (t < a.dim) PagedAttention<T, DP, NT, true>::write(p, b, within / p.row_blocks, row, t, o, l);
+    float one[1] = {o};
+    PagedAttention<T, DP, NT, kRowsFull>::template write<1>(p, b, within / p.row_blocks, row, t, one, l == 0.f ? 0.f : 1.f / l);
   }
 };
 

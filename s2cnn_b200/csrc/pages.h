@@ -188,11 +188,11 @@ PagedPlan paged_plan(const AttnParams& a) {
   plan.row_blocks = (int)((rows + 8 * plan.nt - 1) / (8 * plan.nt));
   plan.items = (long)a.batch * a.kv_heads * plan.row_blocks;
   paged_by_shape<T>(a.dim, plan.nt, [&](auto dp, auto nt) {
-    using K = PagedAttention<T, decltype(dp)::value, decltype(nt)::value, true>;
+    using K = PagedAttention<T, decltype(dp)::value, decltype(nt)::value, kRowsFull>;
     const long steps = std::max(1, (a.lk + K::H::kStep - 1) / K::H::kStep);
     plan.blocks = std::min((long)K::kBlocks * dev_sm_count(), plan.items * steps);
     plan.joined = steps > 1;
-    plan.part = page_align(2 * (size_t)plan.blocks * K::H::kRows * (decltype(dp)::value + 2) * sizeof(float));
+    plan.part = page_align(2 * (size_t)plan.blocks * K::H::kRows * (decltype(dp)::value + 4) * sizeof(float));
     return (int)S2C_OK;
   });
   plan.bytes = plan.part + (size_t)std::min(plan.items, plan.blocks) * sizeof(int4);
@@ -202,24 +202,35 @@ template <class T>
 int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* keys, const void* values, void* ws, size_t ws_bytes, stream_t st) {
   const PagedPlan plan = paged_plan<T>(a);
   if (plan.items == 0) return S2C_OK;
-  if (plan.items > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, "s2c_paged_attention: too many heads and queries");
+  if (plan.items > 0x7fffffffL || (long)a.lq * a.group > 0x7fffff00L) return fail(S2C_ERR_UNSUPPORTED, "s2c_paged_attention: too many heads and queries");
   if (plan.bytes > ws_bytes || !ws) return fail(S2C_ERR_WORKSPACE, "s2c_paged_attention: workspace too small");
   PagedParams p = {};
   p.a = a;
   p.pages = page_table(pages, keys, values);
   for (int i = 0; i < 3; ++i) { p.ks[i] = pages->key_stride[i]; p.vs[i] = pages->value_stride[i]; }
+  if (pages->count == 0) {                     // what is read in the place of a page that is none, with a score of NaN
+    for (int i = 0; i < 3; ++i) p.ks[i] = p.vs[i] = 0;
+    p.pages.array[0] = p.pages.array[1] = ws;
+  }
   p.row_blocks = plan.row_blocks;
+  p.by_group = Divisor(a.group);
+  p.by_row_blocks = Divisor(plan.row_blocks);
+  p.by_buckets = Divisor(a.n_buckets + 1);
+  p.wide_out = a.dim % 4 == 0 && on_boundary(a.out, 4 * sizeof(T));
   p.part = static_cast<float*>(ws);
   p.split = reinterpret_cast<int4*>(static_cast<char*>(ws) + plan.part);
-  const bool wide = paged_wide<T>(pages, keys, values);
+  const bool wide = paged_wide<T>(pages, p.pages.array[0], p.pages.array[1]);
   return paged_by_shape<T>(a.dim, plan.nt, [&](auto dp, auto nt) {
     constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;
-    using W = PagedAttention<T, DP, NT, true>;
-    using N = PagedAttention<T, DP, NT, false>;
-    S2C_SEQ_TRY(wide ? seq_launch<W>("paged_attention", plan.blocks, W::smem(), st, p) : seq_launch<N>("paged_attention", plan.blocks, N::smem(), st, p));
+    using F = PagedAttention<T, DP, NT, kRowsFull>;
+    using W = PagedAttention<T, DP, NT, kRowsInPieces>;
+    using N = PagedAttention<T, DP, NT, kRowsByValue>;
+    S2C_SEQ_TRY(!wide ? seq_launch<N>("paged_attention", plan.blocks, N::smem(a), st, p)
+                : a.dim < DP ? seq_launch<W>("paged_attention", plan.blocks, W::smem(a), st, p)
+                             : seq_launch<F>("paged_attention", plan.blocks, F::smem(a), st, p));
     if (!plan.joined) return (int)S2C_OK;
     using J = PagedJoin<T, DP, NT>;
-    return seq_launch<J>("paged_join", std::min(plan.items, plan.blocks) * W::H::kRows, J::smem(plan.blocks), st, p);
+    return seq_launch<J>("paged_join", std::min(plan.items, plan.blocks) * F::H::kRows, J::smem(plan.blocks), st, p);
   });
 }
 #endif

@@ -107,6 +107,43 @@ S2C_D void store_vec(bf16* p, const float (&v)[8]) {
   *reinterpret_cast<Vec16*>(p) = u;
 }
 
+// four values on their boundary
+struct alignas(8) Vec8 {
+  unsigned w[2];
+};
+S2C_D void load_four(const float* p, float (&v)[4]) { load_vec(p, v); }
+S2C_D void load_four(const bf16* p, float (&v)[4]) {
+  const Vec8 u = *reinterpret_cast<const Vec8*>(p);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[2 * i] = as_float(u.w[i] << 16);
+    v[2 * i + 1] = as_float(u.w[i] & 0xffff0000u);
+  }
+}
+S2C_D void store_four(float* p, const float (&v)[4]) { store_vec(p, v); }
+S2C_D void store_four(bf16* p, const float (&v)[4]) {
+  Vec8 u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) u.w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<Vec8*>(p) = u;
+}
+
+// n / d for n < 2^31 by a product: m = ceil(2^(31 + l) / d), l = ceil(log2 d) (T. Granlund, P. Montgomery: "Division by invariant
+// integers using multiplication", 1994); a division takes ten times the instructions.
+struct Divisor {
+  unsigned d = 1, m = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(long by) : d((unsigned)by) {
+    unsigned l = 0;
+    while ((1ull << l) < d) ++l;
+    if (l == 0) return;
+    m = (unsigned)((((1ull << (31 + l)) - 1) / d) + 1);
+    shift = l - 1;
+  }
+  S2C_HD unsigned quotient(unsigned n) const { return m ? (unsigned)(((unsigned long long)n * m) >> 32) >> shift : n; }
+  S2C_HD unsigned rest(unsigned n) const { return n - quotient(n) * d; }
+};
+
 // A kernel as a struct: Params, kThreads, kBlocks (per SM, for the register budget) and a static run(ctx, p, smem).
 #ifndef S2C_EMUL
 template <class Impl>
