@@ -2,6 +2,8 @@
 // array for the kernels of whole tiles.
 #pragma once
 
+#include <type_traits>
+
 #include "seq_common.h"
 
 namespace s2c {
@@ -28,29 +30,35 @@ struct PageCopyParams {
   long n, chunks;                 // copies; pieces of kChunk bytes of each
   int count;
 };
-// P: bytes of one access.  A block copies kChunk bytes at a time, all loads before the stores.
+// P: bytes of one access.  A block copies a chunk, all of its loads before its stores.
 template <int P>
 struct PageCopy {
   using Params = PageCopyParams;
-  struct alignas(P) Piece {
-    unsigned char b[P];
-  };
-  static constexpr int kThreads = 256, kBlocks = 4, kAhead = P == 16 ? 4 : 8;
+  using Piece = typename std::conditional<P == 16, Vec16, typename std::conditional<P == 4, unsigned, unsigned char>::type>::type;
+  static constexpr int kThreads = 256, kBlocks = 4, kAhead = 8;
   static constexpr long kChunk = (long)kThreads * kAhead * P;
   static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char*) {
     for (long u = ctx.bid; u < p.n * p.chunks; u += ctx.nblk) {
-      const long i = u / p.chunks, at = u % p.chunks * kChunk + (long)ctx.tid * P;
+      const long i = u / p.chunks, at = (u - i * p.chunks) * kChunk + (long)ctx.tid * P;
       const int from = p.source[i], to = p.target[i];
       if (from < 0 || from >= p.count || to < 0 || to >= p.count) continue;
-      const char* x = p.base + from * p.stride + at;
-      char* y = p.base + to * p.stride + at;
+      const Piece* x = reinterpret_cast<const Piece*>(p.base + from * p.stride + at);
+      Piece* y = reinterpret_cast<Piece*>(p.base + to * p.stride + at);
+      const long left = p.bytes - at;                    // of the chunk, from this thread's first piece on
       Piece v[kAhead];
+      if (left > (long)(kAhead - 1) * kThreads * P) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (at + (long)k * kThreads * P < p.bytes) v[k] = *reinterpret_cast<const Piece*>(x + (long)k * kThreads * P);
+        for (int k = 0; k < kAhead; ++k) v[k] = x[k * kThreads];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (at + (long)k * kThreads * P < p.bytes) *reinterpret_cast<Piece*>(y + (long)k * kThreads * P) = v[k];
+        for (int k = 0; k < kAhead; ++k) y[k * kThreads] = v[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (left > (long)k * kThreads * P) v[k] = x[k * kThreads];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (left > (long)k * kThreads * P) y[k * kThreads] = v[k];
+      }
     }
   }
 };

@@ -355,7 +355,7 @@ int s2c_copy_pages(void* storage, long page_stride, long page_bytes, int count, 
   auto go = [&](auto k) {
     using K = typename decltype(k)::type;
     p.chunks = (page_bytes + K::kChunk - 1) / K::kChunk;
-    return seq_launch<K>("copy_pages", std::min<long>(n * p.chunks, 16L * dev_sm_count()), 0, (stream_t)stream, p);
+    return seq_launch<K>("copy_pages", std::min<long>(n * p.chunks, 0x7fffffffL), 0, (stream_t)stream, p);
   };
   struct A { using type = PageCopy<16>; };
   struct B { using type = PageCopy<4>; };
