@@ -17,6 +17,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(PKG, "csrc", "lib.cu")
 PARTS_SRC = os.path.join(PKG, "csrc", "parts.cu")
 SEQ_SRC = os.path.join(PKG, "csrc", "sequence.cu")
+HEADS_SRC = os.path.join(PKG, "csrc", "heads.cu")
 PAGES_SRC = os.path.join(PKG, "csrc", "pages.cu")
 N_PARTS = 18
 LIB_DIR = os.path.join(PKG, "lib")
@@ -95,6 +96,7 @@ def build(force=False, verbose=False):
         jobs = [(PARTS_SRC, ["-DS2C_PART=%d" % k], os.path.join(tmp, "part%d.o" % k)) for k in range(N_PARTS)]
         jobs.append((SRC, [], os.path.join(tmp, "lib.o")))
         jobs.append((SEQ_SRC, [], os.path.join(tmp, "sequence.o")))
+        jobs.append((HEADS_SRC, [], os.path.join(tmp, "heads.o")))
         jobs.append((PAGES_SRC, [], os.path.join(tmp, "pages.o")))
         with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
             list(pool.map(lambda j: run([nvcc] + flags + j[1] + ["-c", j[0], "-o", j[2]]), jobs))

@@ -373,6 +373,9 @@ struct float4 {
 struct int2 {
   int x, y;
 };
+struct ulonglong2 {
+  unsigned long long x, y;
+};
 struct int4 {
   int x, y, z, w;
 };

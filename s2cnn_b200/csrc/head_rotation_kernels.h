@@ -12,10 +12,13 @@
 // 2^-52, times the position.  The nearest quarter turn is taken off in integers, the rest (an eighth at most) goes through
 // the Taylor series of sine and cosine to x^9 and x^10, whose first terms left out are below 2e-9 and 2e-10 there.
 //
-// A team of 4, 8 or 16 neighbouring lanes holds a head of up to 32, 64 or 128 values, four pairs to a lane, and takes GROUP heads of
-// one position at once: their loads are on the way together, and they share the four sines and cosines.  Blocks are dealt to queries,
-// keys and values, so that a lane has one weight.
+// A team of 4, 8 or 16 neighbouring lanes holds a head of up to 32, 64 or 128 values, four pairs to a lane, and takes several heads of
+// one position, which share the four sines and cosines and, times the weights, the pairs' factors.  Blocks are dealt to queries, keys and
+// values, so that a lane has one weight.
 #pragma once
+
+#include <cstring>
+#include <type_traits>
 
 #include "kept_pages.h"
 #include "seq_common.h"
@@ -25,11 +28,12 @@ namespace s2c {
 struct HeadKind {                // queries, keys or values
   const void* x;                 // [batch][length][heads][dim]
   const void* w;                 // norm weight, null: ones
-  const void* dy;                // backward: gradient of out, contiguous; null: none arrived (zeros)
+  const void* dy;                // backward: gradient of out, contiguous
   void* out;                     // contiguous; the gradient of x in the backward pass; null: pages
   long stride[3], pstride[3];    // of x; of the pages (page, position, head)
   int heads, blocks;             // blocks of this kind
-  int wide;                      // all arrays of this kind in pieces of four values on their boundaries
+  int span;                      // heads of a unit
+  Divisor spans;                 // units of a position
   int turn;                      // norm and rotation (queries, keys)
 };
 struct HeadParams {
@@ -38,9 +42,10 @@ struct HeadParams {
   const int *positions, *lengths;
   float* part;                   // backward: [blocks][dim], sums of the weight gradients
   PageTable pages;
+  Divisor by_length;
   int batch, length, dim, pairs, interleaved, norm;
   int each, first;               // positions: one per position of a sequence, or its first; null: `first` for all
-  float eps, magnitude;
+  float eps, magnitude, over_dim;
 };
 
 // f in radians per position as a fraction of a turn, in units of 2^-64
@@ -69,248 +74,429 @@ S2C_D void turn_cos_sin(unsigned long long turns, float& c, float& s) {
   s = quarter & 2 ? -s0 : s0;
 }
 
-template <class T, int LANES>
+S2C_D int min_of(int a, int b) { return a < b ? a : b; }
+
+// How the values of a head lie to a lane: one by one, or in two pieces of four, the first values of four pairs
+// and their second ones (halves) or eight consecutive values (neighbours).  Pieces off their boundaries (apart) are read and
+// written value by value, so that alignment changes no sum.
+enum HeadRows : int { kHeadByValue, kHeadHalves, kHeadNeighbours, kHeadHalvesApart, kHeadNeighboursApart };
+
+// NP: two pairs of a lane each.  Pieces: NP = 2, pairs 4 t ... 4 t + 3; by value: pairs t, t + LANES, ..., so that what a team reads or writes
+// at a time lies together (3601 positions, 16 heads of 25 float32 values: 6.6 us; in the order of pieces, whose stores are single
+// values 32 bytes apart, 11.0).
+template <class T, int LANES, int ROWS, int NP>
 struct HeadTeam {
-  static constexpr int kThreads = 256, kTeams = kThreads / LANES;
-  // A lane's two pieces of four values, by value e: pairs 4 t ... 4 t + 3.  Halves: the pair's first values and its second ones;
-  // neighbours: eight consecutive values.  What is not turned pairs up in the same way.  -1: no value.
-  static S2C_D int index(const HeadParams& p, int t, int piece, int e) {
-    if (p.interleaved) {
-      const int c = 8 * t + 4 * piece + e;
-      return c < p.dim ? c : -1;
-    }
-    const int i = 4 * t + e, rest = p.dim - 2 * p.pairs, low = (rest + 1) / 2;
-    if (i < p.pairs) return i + piece * p.pairs;
-    const int r = i - p.pairs;
-    return piece == 0 ? (r < low ? 2 * p.pairs + r : -1) : r < rest - low ? 2 * p.pairs + low + r : -1;
+  static constexpr int kThreads = 256, kTeams = kThreads / LANES, kPairs = 2 * NP;
+  static constexpr bool kPieces = ROWS != kHeadByValue, kWide = ROWS == kHeadHalves || ROWS == kHeadNeighbours;
+  static constexpr bool kNext = ROWS == kHeadNeighbours || ROWS == kHeadNeighboursApart;
+  using Four = typename std::conditional<sizeof(T) == 2, Vec8, Vec16>::type;
+  struct Wide {
+    Four piece[2];
+  };
+  struct Narrow {
+    float v[2][kPairs];
+  };
+  using Raw = typename std::conditional<kPieces, Wide, Narrow>::type;      // a lane's values as they were loaded
+
+  int t;                          // lane of the team
+  int at[2][kPieces ? 1 : kPairs];   // where the first and second values of its pairs lie, or its pieces; -1: none
+  unsigned turned;                // bit e: pair e is turned
+
+  static S2C_D int pair(int t, int e) { return kPieces ? 4 * t + e : t + LANES * e; }
+  // where value k of pair i lies: what is not turned pairs up as what is
+  static S2C_D int place(const HeadParams& p, int i, int k) {
+    if (p.interleaved) return 2 * i + k < p.dim ? 2 * i + k : -1;
+    const int rest = p.dim - 2 * p.pairs, low = (rest + 1) / 2, r = i - p.pairs;
+    return r < 0 ? i + k * p.pairs : r < (k ? rest - low : low) ? 2 * p.pairs + k * low + r : -1;
   }
-  static S2C_D void load(const HeadParams& p, int wide, const T* x, int t, float (&v)[2][4]) {
+  S2C_D HeadTeam(const HeadParams& p, int lane) : t(lane), turned(0) {
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e)
+      if (pair(t, e) < p.pairs) turned |= 1u << e;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int c = index(p, t, k, 0);
-      if (wide) {
-        if (c >= 0) load_four(x + c, v[k]);
-        else
+      if constexpr (kPieces) {
+        at[k][0] = kNext ? place(p, pair(t, 2 * k), 0) : place(p, pair(t, 0), k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) at[k][e] = place(p, pair(t, e), k);
+      }
+    }
+  }
+  // (a lane's piece behind the head: its first one, in place of which `open` has zeros)
+  S2C_D void fetch(const T* x, Raw& r) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if constexpr (kPieces) {
+        const T* from = x + (at[k][0] >= 0 ? at[k][0] : 0);
+        if constexpr (kWide) {
+          r.piece[k] = *reinterpret_cast<const Four*>(from);
+        } else {
+          const T v[4] = {from[0], from[1], from[2], from[3]};
+          std::memcpy(&r.piece[k], v, sizeof(v));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) r.v[k][e] = at[k][e] >= 0 ? widen(x[at[k][e]]) : 0.f;
+      }
+    }
+  }
+  // as pairs (a[e], b[e])
+  S2C_D void open(const HeadParams& p, const Raw& r, float2 (&a)[NP], float2 (&b)[NP]) const {
+    if constexpr (kPieces) {
+      float v[2][4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        load_four(reinterpret_cast<const T*>(&r.piece[k]), v[k]);
+        if (p.dim < 8 * LANES && at[k][0] < 0)
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[k][e] = 0.f;
-      } else {
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = index(p, t, k, e);
-          v[k][e] = i >= 0 ? widen(x[i]) : 0.f;
+      for (int e = 0; e < 2; ++e) {
+        a[e] = kNext ? make_float2(v[e][0], v[e][2]) : make_float2(v[0][2 * e], v[0][2 * e + 1]);
+        b[e] = kNext ? make_float2(v[e][1], v[e][3]) : make_float2(v[1][2 * e], v[1][2 * e + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        a[e] = make_float2(r.v[0][2 * e], r.v[0][2 * e + 1]);
+        b[e] = make_float2(r.v[1][2 * e], r.v[1][2 * e + 1]);
+      }
+    }
+  }
+  S2C_D void store(T* y, const float2 (&a)[NP], const float2 (&b)[NP]) const {
+    if constexpr (kPieces) {
+      float v[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        v[0][2 * e] = kNext ? (e ? a[0].y : a[0].x) : a[e].x;
+        v[0][2 * e + 1] = kNext ? (e ? b[0].y : b[0].x) : a[e].y;
+        v[1][2 * e] = kNext ? (e ? a[1].y : a[1].x) : b[e].x;
+        v[1][2 * e + 1] = kNext ? (e ? b[1].y : b[1].x) : b[e].y;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (at[k][0] >= 0) {
+          if constexpr (kWide) {
+            store_four(y + at[k][0], v[k]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) narrow(y + at[k][0] + e, v[k][e]);
+          }
         }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) {
+        if (at[0][e] >= 0) narrow(y + at[0][e], e % 2 ? a[e / 2].y : a[e / 2].x);
+        if (at[1][e] >= 0) narrow(y + at[1][e], e % 2 ? b[e / 2].y : b[e / 2].x);
       }
     }
   }
-  static S2C_D void store(const HeadParams& p, int wide, T* y, int t, const float (&v)[2][4]) {
+  // What is the same for all teams of a block, in shared memory: a unit's sines and cosines are made from it, and a lane's registers
+  // are for heads (with it in registers, and the kind of heads, 110 were taken before the first head).
+  struct Shared {
+    HeadKind kind;
+    float w[2][kPairs][LANES];    // weights of the first and second values of a lane's pairs
+    unsigned long long f[kPairs][LANES];      // frequencies
+  };
+  static S2C_D void share(const Ctx& ctx, const HeadParams& p, const HeadKind& kind, Shared* to) {
+    if (ctx.tid < LANES * kPairs) {
+      const int lane = ctx.tid % LANES, e = ctx.tid / LANES, i = pair(lane, e);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = index(p, t, k, 0);
-      if (wide) {
-        if (c >= 0) store_four(y + c, v[k]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = index(p, t, k, e);
-          if (i >= 0) narrow(y + i, v[k][e]);
-        }
+      for (int k = 0; k < 2; ++k) {
+        const int c = place(p, i, k);
+        to->w[k][e][lane] = kind.w && c >= 0 ? widen(static_cast<const T*>(kind.w)[c]) : 1.f;
       }
+      to->f[e][lane] = kind.turn && i < p.pairs ? turn_units(p.frequencies[i]) : 0ull;
+    }
+    if (ctx.tid == ctx.nthr - 1) to->kind = kind;
+    ctx.sync();
+  }
+  // cosines and sines of the pairs times the magnitude; of what is not turned 1 and 0
+  S2C_D void angles(const HeadParams& p, const Shared* s, long position, float2 (&c)[NP], float2 (&si)[NP]) const {
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      turn_cos_sin(s->f[2 * e][t] * (unsigned long long)position, c[e].x, si[e].x);
+      turn_cos_sin(s->f[2 * e + 1][t] * (unsigned long long)position, c[e].y, si[e].y);
+      if (turned >> 2 * e & 1) c[e].x *= p.magnitude, si[e].x *= p.magnitude;
+      if (turned >> 2 * e & 2) c[e].y *= p.magnitude, si[e].y *= p.magnitude;
     }
   }
-  // the pairs' frequencies; what is not turned has 0
-  static S2C_D void frequencies(const HeadParams& p, int t, unsigned long long (&f)[4]) {
+  S2C_D float2 weights(const Shared* s, int k, int e) const { return make_float2(s->w[k][2 * e][t], s->w[k][2 * e + 1][t]); }
+  static S2C_D float2 square(const float2 (&a)[NP], const float2 (&b)[NP], const float2 (&x)[NP], const float2 (&y)[NP]) {
+    float2 sum = mul2(a[0], x[0]);
+    sum = fma2(b[0], y[0], sum);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = 4 * t + e < p.pairs ? turn_units(p.frequencies[4 * t + e]) : 0ull;
+    for (int e = 1; e < NP; ++e) sum = fma2(a[e], x[e], fma2(b[e], y[e], sum));
+    return sum;
   }
-  // the pairs of two pieces, turned (sign 1) or turned back (-1)
-  static S2C_D void turn(const HeadParams& p, int t, const float (&c)[4], const float (&s)[4], float sign, float (&v)[2][4]) {
-    float a[4], b[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[e] = p.interleaved ? v[e / 2][2 * (e % 2)] : v[0][e];
-      b[e] = p.interleaved ? v[e / 2][2 * (e % 2) + 1] : v[1][e];
-      if (4 * t + e < p.pairs) {                        // (others stay as they are: an infinity times 0 would be none)
-        const float x = a[e], y = b[e], si = sign * s[e];
-        a[e] = x * c[e] - y * si;
-        b[e] = x * si + y * c[e];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[0][e] = p.interleaved ? (e % 2 ? b[e / 2] : a[e / 2]) : a[e];
-      v[1][e] = p.interleaved ? (e % 2 ? b[2 + e / 2] : a[2 + e / 2]) : b[e];
-    }
-  }
-  static S2C_D long position(const HeadParams& p, int b, int i) {
-    if (!p.positions) return (long)p.first + i;
-    return p.each ? p.positions[(long)b * p.length + i] : (long)p.positions[b] + i;
-  }
-  static S2C_D void angles(const HeadParams& p, const unsigned long long (&f)[4], long at, float (&c)[4], float (&s)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      turn_cos_sin(f[e] * (unsigned long long)at, c[e], s[e]);
-      c[e] *= p.magnitude;
-      s[e] *= p.magnitude;
-    }
+  // A unit: `span` neighbouring heads of one position.
+  struct Unit {
+    const T* x;                   // its first head
+    long to, at;                  // where that lies among contiguous heads; position
+    int left, b, i;               // heads of the kind from the first one on; sequence and row of it
+    bool on;
+  };
+  static S2C_D Unit unit(const HeadParams& p, const HeadKind& kind, long u, long units) {
+    Unit n;
+    n.on = u < units;
+    const unsigned v = n.on ? (unsigned)u : 0u, row = kind.spans.quotient(v);
+    const int h = (int)(v - row * kind.spans.d) * kind.span;
+    n.b = (int)p.by_length.quotient(row);
+    n.i = (int)row - n.b * p.length;
+    n.left = kind.heads - h;
+    n.x = static_cast<const T*>(kind.x) + n.b * kind.stride[0] + n.i * kind.stride[1] + h * kind.stride[2];
+    n.to = ((long)row * kind.heads + h) * p.dim;
+    n.at = !p.positions ? (long)p.first + n.i : p.each ? p.positions[row] : (long)p.positions[n.b] + n.i;
+    return n;
   }
 };
 
-// A unit is GROUP neighbouring heads of one position.
-template <class T, int LANES, int GROUP>
-struct HeadForward : HeadTeam<T, LANES> {
-  using Team = HeadTeam<T, LANES>;
+// Per lane: GROUP heads loaded while the GROUP before them are worked on, four sines and cosines for all heads of a unit.
+template <class T, int LANES, int ROWS, int NP, int GROUP>
+struct HeadForward {
+  using Team = HeadTeam<T, LANES, ROWS, NP>;
+  using Unit = typename Team::Unit;
+  using Raw = typename Team::Raw;
   using Params = HeadParams;
-  static constexpr int kBlocks = 3;
-  static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char*) {
+  static constexpr int kThreads = Team::kThreads, kBlocks = 2;
+  static constexpr size_t kSmem = sizeof(typename Team::Shared);
+  static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
     int which = 0, bid = ctx.bid;
     while (which < 2 && bid >= p.kind[which].blocks) bid -= p.kind[which++].blocks;
-    const HeadKind& kind = p.kind[which];
-    const int team = ctx.tid / LANES, t = ctx.tid % LANES;
-    const int groups = (kind.heads + GROUP - 1) / GROUP;
-    const long units = (long)p.batch * p.length * groups, per = (long)kind.blocks * Team::kTeams;
-    unsigned long long f[4];
-    float w[2][4];
-    if (kind.turn) {
-      Team::frequencies(p, t, f);
-      if (kind.w) Team::load(p, 0, static_cast<const T*>(kind.w), t, w);
-    }
-    for (long u0 = (long)bid * Team::kTeams; u0 < units; u0 += per) {     // (every team takes the same number of turns)
-      const bool on = u0 + team < units;
-      const long u = on ? u0 + team : 0, row = u / groups;
-      const int h0 = (int)(u % groups) * GROUP, b = (int)(row / p.length), i = (int)(row % p.length);
-      const bool filled = !p.lengths || i < p.lengths[b];
-      const long at = Team::position(p, b, i);
-      const T* x = static_cast<const T*>(kind.x) + b * kind.stride[0] + i * kind.stride[1];
-      float v[GROUP][2][4];
+    typename Team::Shared* const shared = reinterpret_cast<typename Team::Shared*>(smem);
+    const HeadKind& kind = shared->kind;
+    Team::share(ctx, p, p.kind[which], shared);
+    const Team team(p, ctx.tid % LANES);
+    const long units = (long)p.batch * p.length * kind.spans.d, per = (long)kind.blocks * Team::kTeams, mine = ctx.tid / LANES;
+    const bool rest = 2 * p.pairs < p.dim, turn = kind.turn;
+    const int span = kind.span;
+    const long step = kind.stride[2];
+    Raw raw[GROUP];
+    auto fetch = [&](const T* x, int left) {            // (beyond the last head: the first of the group again)
 #pragma unroll
-      for (int g = 0; g < GROUP; ++g)
-        if (on && filled && h0 + g < kind.heads) Team::load(p, kind.wide, x + (h0 + g) * kind.stride[2], t, v[g]);
-        else
+      for (int g = 0; g < GROUP; ++g) team.fetch(x + (g < left ? g * step : 0), raw[g]);
+    };
+    long u0 = (long)bid * Team::kTeams;
+    Unit now = Team::unit(p, kind, u0 + mine, units);
+    fetch(now.x, now.left);
+    bool next_filled = true;
+    int next_page = 0;
+    auto look_up = [&] {                                // of a store, while the heads before are worked on
+      if (!p.pages.table) return;
+      next_filled = !p.lengths || now.i < p.lengths[now.b];
+      next_page = p.pages.of(now.b, now.at);
+    };
+    look_up();
+    for (; u0 < units; u0 += per) {                     // (every team takes the same number of turns)
+      // where the unit's heads go (null: nowhere), and what is said of a row that has no value
+      const bool filled = next_filled;
+      const int page = next_page;
+      T* y = nullptr;
+      long y_step = p.dim;
+      if (now.on && kind.out) {
+        y = static_cast<T*>(kind.out) + now.to;
+      } else if (now.on && filled && page >= 0) {
+        y_step = kind.pstride[2];
+        y = static_cast<T*>(p.pages.array[which - 1]) + page * kind.pstride[0] + (now.at & (p.pages.page - 1)) * kind.pstride[1] + (kind.heads - now.left) * y_step;
+      }
+      // y_a = x_a k0 + x_b k1, y_b = x_a k2 + x_b k3
+      float2 k0[NP], k1[NP], k2[NP], k3[NP];
+      if (turn) {
+        float2 c[NP], s[NP];
+        team.angles(p, shared, now.at, c, s);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[g][e / 4][e % 4] = 0.f;
-      long slot = 0;
-      const bool stored = p.pages.table && p.pages.at(b, at, slot);
-      if (kind.turn) {
-        float c[4], s[4];
-        Team::angles(p, f, at, c, s);
-#pragma unroll
-        for (int g = 0; g < GROUP; ++g) {
-          if (p.norm) {
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum += v[g][e / 4][e % 4] * v[g][e / 4][e % 4];
-            const float rstd = inv_sqrt(lanes_sum<LANES>(ctx, sum) / (float)p.dim + p.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              v[g][e / 4][e % 4] *= rstd;
-              if (kind.w) v[g][e / 4][e % 4] *= w[e / 4][e % 4];
-            }
-          }
-          Team::turn(p, t, c, s, 1.f, v[g]);
+        for (int e = 0; e < NP; ++e) {
+          const float2 x = team.weights(shared, 0, e), z = team.weights(shared, 1, e);
+          k0[e] = mul2(x, c[e]);
+          k1[e] = mul2(z, make_float2(-s[e].x, -s[e].y));
+          k2[e] = mul2(x, s[e]);
+          k3[e] = mul2(z, c[e]);
         }
       }
-      if (!on) continue;
-      if (kind.out) {
-        T* y = static_cast<T*>(kind.out) + (row * kind.heads + h0) * p.dim;
-        const bool lost = p.pages.table && filled && !stored;              // a query whose key has no place
+      int left = now.left;
+      const T* x = now.x;
+      for (int n = 0; n < span; n += GROUP, left -= GROUP) {
+        Raw old[GROUP];
+#pragma unroll
+        for (int g = 0; g < GROUP; ++g) old[g] = raw[g];
+        if (n + GROUP < span) {
+          if (left > GROUP) fetch(x += GROUP * step, left - GROUP);
+        } else {
+          now = Team::unit(p, kind, u0 + per + mine, units);
+          fetch(now.x, now.left);
+          look_up();
+        }
 #pragma unroll
         for (int g = 0; g < GROUP; ++g) {
-          if (h0 + g >= kind.heads) break;
-          if (!filled || lost)
+          float2 a[NP], b[NP];
+          team.open(p, old[g], a, b);
+          if (turn) {
+            if (p.norm) {
+              const float2 sum = Team::square(a, b, a, b);
+              const float rstd = inv_sqrt(fmaf(lanes_sum<LANES>(ctx, sum.x + sum.y), p.over_dim, p.eps));
+              const float2 r2 = make_float2(rstd, rstd);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[g][e / 4][e % 4] = lost ? as_float(0x7fffffffu) : 0.f;
-          Team::store(p, kind.wide, y + g * p.dim, t, v[g]);
+              for (int e = 0; e < NP; ++e) {
+                a[e] = mul2(a[e], r2);
+                b[e] = mul2(b[e], r2);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < NP; ++e) {
+              const float2 u = a[e], v = b[e];
+              a[e] = fma2(u, k0[e], mul2(v, k1[e]));
+              b[e] = fma2(u, k2[e], mul2(v, k3[e]));
+              if (rest) {                               // what is not turned (an infinity times a sine of 0 would be none)
+                if (!(team.turned >> 2 * e & 1)) a[e].x = u.x * k0[e].x, b[e].x = v.x * k3[e].x;
+                if (!(team.turned >> 2 * e & 2)) a[e].y = u.y * k0[e].y, b[e].y = v.y * k3[e].y;
+              }
+            }
+          }
+          if (!filled || page < 0) {                    // a row that is not filled, and a query whose key has no place
+            const float none = filled ? as_float(0x7fffffffu) : 0.f;
+#pragma unroll
+            for (int e = 0; e < NP; ++e) a[e] = b[e] = make_float2(none, none);
+          }
+          if (y && g < left && n + g < span) team.store(y + g * y_step, a, b);
         }
-      } else if (filled && stored) {
-        T* y = static_cast<T*>(p.pages.array[which - 1]) + slot / p.pages.page * kind.pstride[0] + slot % p.pages.page * kind.pstride[1] + h0 * kind.pstride[2];
-#pragma unroll
-        for (int g = 0; g < GROUP; ++g)
-          if (h0 + g < kind.heads) Team::store(p, kind.wide, y + g * kind.pstride[2], t, v[g]);
+        if (y) y += GROUP * y_step;
       }
     }
   }
 };
 
-template <class T, int LANES, int GROUP>
-struct HeadBackward : HeadTeam<T, LANES> {
-  using Team = HeadTeam<T, LANES>;
+template <class T, int LANES, int ROWS, int NP, int GROUP>
+struct HeadBackward {
+  using Team = HeadTeam<T, LANES, ROWS, NP>;
+  using Unit = typename Team::Unit;
+  using Raw = typename Team::Raw;
   using Params = HeadParams;
-  static constexpr int kBlocks = 2;
-  static size_t smem() { return 8 * LANES * sizeof(float); }
+  static constexpr int kThreads = Team::kThreads, kBlocks = 2;
+  static constexpr size_t kSmem = sizeof(typename Team::Shared) + 8 * LANES * sizeof(float);
   static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
     const int which = ctx.bid >= p.kind[0].blocks ? 1 : 0;
-    const HeadKind& kind = p.kind[which];
-    const int bid = ctx.bid - (which ? p.kind[0].blocks : 0), team = ctx.tid / LANES, t = ctx.tid % LANES;
-    const int groups = (kind.heads + GROUP - 1) / GROUP;
-    const long units = (long)p.batch * p.length * groups, per = (long)kind.blocks * Team::kTeams;
-    unsigned long long f[4];
-    Team::frequencies(p, t, f);
-    float w[2][4], dw[2][4];
-    if (kind.w) Team::load(p, 0, static_cast<const T*>(kind.w), t, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dw[e / 4][e % 4] = 0.f;
-    for (long u0 = (long)bid * Team::kTeams; u0 < units; u0 += per) {
-      const bool on = u0 + team < units;
-      const long u = on ? u0 + team : 0, row = u / groups;
-      const int h0 = (int)(u % groups) * GROUP, b = (int)(row / p.length), i = (int)(row % p.length);
-      const T* x = static_cast<const T*>(kind.x) + b * kind.stride[0] + i * kind.stride[1];
-      const T* dy = static_cast<const T*>(kind.dy) + (row * kind.heads + h0) * p.dim;
-      float v[GROUP][2][4], d[GROUP][2][4];
+    const int bid = ctx.bid - (which ? p.kind[0].blocks : 0);
+    typename Team::Shared* const shared = reinterpret_cast<typename Team::Shared*>(smem);
+    const HeadKind& kind = shared->kind;
+    Team::share(ctx, p, p.kind[which], shared);
+    const Team team(p, ctx.tid % LANES);
+    const long units = (long)p.batch * p.length * kind.spans.d, per = (long)kind.blocks * Team::kTeams, mine = ctx.tid / LANES;
+    const bool rest = 2 * p.pairs < p.dim;
+    const int span = kind.span;
+    const long step = kind.stride[2];
+    Raw raw_x[GROUP], raw_d[GROUP];
+    auto fetch = [&](const T* x, long to, int left) {
+      const T* dy = static_cast<const T*>(kind.dy) + to;
 #pragma unroll
       for (int g = 0; g < GROUP; ++g) {
-        const bool in = on && h0 + g < kind.heads;
-        if (in) Team::load(p, kind.wide, dy + g * p.dim, t, d[g]);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[g][e / 4][e % 4] = 0.f;
-        if (in && p.norm) Team::load(p, kind.wide, x + (h0 + g) * kind.stride[2], t, v[g]);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[g][e / 4][e % 4] = 0.f;
+        team.fetch(dy + (g < left ? g * p.dim : 0), raw_d[g]);
+        if (p.norm) team.fetch(x + (g < left ? g * step : 0), raw_x[g]);
       }
-      float c[4], s[4];
-      Team::angles(p, f, Team::position(p, b, i), c, s);
+    };
+    long u0 = (long)bid * Team::kTeams;
+    Unit now = Team::unit(p, kind, u0 + mine, units);
+    fetch(now.x, now.to, now.left);
+    float2 da[NP], db[NP];
 #pragma unroll
-      for (int g = 0; g < GROUP; ++g) {
-        Team::turn(p, t, c, s, -1.f, d[g]);
-        if (p.norm) {
-          float sum = 0.f, dot = 0.f;
+    for (int e = 0; e < NP; ++e) da[e] = db[e] = make_float2(0.f, 0.f);
+    for (; u0 < units; u0 += per) {
+      float2 c[NP], s[NP], w[2][NP];
+      team.angles(p, shared, now.at, c, s);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum += v[g][e / 4][e % 4] * v[g][e / 4][e % 4];
-          const float rstd = inv_sqrt(lanes_sum<LANES>(ctx, sum) / (float)p.dim + p.eps);
+      for (int e = 0; e < NP; ++e) {
+        w[0][e] = team.weights(shared, 0, e);
+        w[1][e] = team.weights(shared, 1, e);
+      }
+      const bool on = now.on;
+      const T* x = now.x;
+      long to = now.to;
+      int left = now.left;
+      for (int n = 0; n < span; n += GROUP, left -= GROUP, to += GROUP * p.dim) {
+        Raw old_x[GROUP], old_d[GROUP];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float &xh = v[g][e / 4][e % 4], &gr = d[g][e / 4][e % 4];
-            xh *= rstd;
-            dw[e / 4][e % 4] += gr * xh;
-            if (kind.w) gr *= w[e / 4][e % 4];
-            dot += gr * xh;
-          }
-          dot = lanes_sum<LANES>(ctx, dot) / (float)p.dim;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[g][e / 4][e % 4] = rstd * (d[g][e / 4][e % 4] - v[g][e / 4][e % 4] * dot);
+        for (int g = 0; g < GROUP; ++g) {
+          old_x[g] = raw_x[g];
+          old_d[g] = raw_d[g];
         }
-        if (on && h0 + g < kind.heads && kind.out) Team::store(p, kind.wide, static_cast<T*>(kind.out) + (row * kind.heads + h0 + g) * p.dim, t, d[g]);
+        if (n + GROUP < span) {
+          if (left > GROUP) fetch(x += GROUP * step, to + GROUP * p.dim, left - GROUP);
+        } else {
+          now = Team::unit(p, kind, u0 + per + mine, units);
+          fetch(now.x, now.to, now.left);
+        }
+#pragma unroll
+        for (int g = 0; g < GROUP; ++g) {
+          const bool in = on && g < left && n + g < span;
+          float2 ga[NP], gb[NP];
+          team.open(p, old_d[g], ga, gb);
+#pragma unroll
+          for (int e = 0; e < NP; ++e) {
+            const float2 u = ga[e], v = gb[e];
+            ga[e] = fma2(u, c[e], mul2(v, s[e]));
+            gb[e] = fma2(v, c[e], mul2(u, make_float2(-s[e].x, -s[e].y)));
+            if (rest) {
+              if (!(team.turned >> 2 * e & 1)) ga[e].x = u.x, gb[e].x = v.x;
+              if (!(team.turned >> 2 * e & 2)) ga[e].y = u.y, gb[e].y = v.y;
+            }
+          }
+          if (p.norm) {
+            float2 xa[NP], xb[NP];
+            team.open(p, old_x[g], xa, xb);
+            float2 sum = Team::square(xa, xb, xa, xb);
+            const float rstd = inv_sqrt(fmaf(lanes_sum<LANES>(ctx, sum.x + sum.y), p.over_dim, p.eps));
+            const float2 r2 = make_float2(rstd, rstd);
+#pragma unroll
+            for (int e = 0; e < NP; ++e) {
+              xa[e] = mul2(xa[e], r2);
+              xb[e] = mul2(xb[e], r2);
+              if (in) {
+                da[e] = fma2(ga[e], xa[e], da[e]);
+                db[e] = fma2(gb[e], xb[e], db[e]);
+              }
+              ga[e] = mul2(ga[e], w[0][e]);
+              gb[e] = mul2(gb[e], w[1][e]);
+            }
+            sum = Team::square(ga, gb, xa, xb);
+            const float dot = -lanes_sum<LANES>(ctx, sum.x + sum.y) * p.over_dim;
+            const float2 dot2 = make_float2(dot, dot);
+#pragma unroll
+            for (int e = 0; e < NP; ++e) {
+              ga[e] = mul2(r2, fma2(xa[e], dot2, ga[e]));
+              gb[e] = mul2(r2, fma2(xb[e], dot2, gb[e]));
+            }
+          }
+          if (in && kind.out) team.store(static_cast<T*>(kind.out) + to + g * p.dim, ga, gb);
+        }
       }
     }
     if (!p.part || !kind.w) return;                 // (a whole block)
-    // the teams of a warp, then the warps in their order
-    float* red = reinterpret_cast<float*>(smem);
+    // the teams of a warp, then the warps in their order: [value of a pair][pair][lane]
+    float* red = reinterpret_cast<float*>(smem + sizeof(typename Team::Shared));
+    constexpr int kPairs = Team::kPairs;
+    float sums[2][kPairs];
 #pragma unroll
-    for (int m = LANES; m < 32; m *= 2)
+    for (int e = 0; e < kPairs; ++e) {
+      sums[0][e] = e % 2 ? da[e / 2].y : da[e / 2].x;
+      sums[1][e] = e % 2 ? db[e / 2].y : db[e / 2].x;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dw[e / 4][e % 4] += ctx.shfl_xor(dw[e / 4][e % 4], m);
-    for (int k = 0; k < 8; ++k) {
-      if (ctx.tid / 32 == k && ctx.tid % 32 < LANES)
+      for (int m = LANES; m < 32; m *= 2)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) red[e * LANES + t] = (k ? red[e * LANES + t] : 0.f) + dw[e / 4][e % 4];
+        for (int k = 0; k < 2; ++k) sums[k][e] += ctx.shfl_xor(sums[k][e], m);
+    }
+    for (int w = 0; w < 8; ++w) {
+      if (ctx.tid / 32 == w && ctx.tid % 32 < LANES)
+#pragma unroll
+        for (int e = 0; e < 2 * kPairs; ++e) {
+          float* to = red + e * LANES + team.t;
+          *to = (w ? *to : 0.f) + sums[e / kPairs][e % kPairs];
+        }
       ctx.sync();
     }
-    if (team != 0) return;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = Team::index(p, t, e / 4, e % 4);
-      if (c >= 0) p.part[(long)ctx.bid * p.dim + c] = red[e * LANES + t];
+    for (int e = ctx.tid; e < 2 * kPairs * LANES; e += ctx.nthr) {
+      const int c = Team::place(p, Team::pair(e % LANES, e / LANES % kPairs), e / LANES / kPairs);
+      if (c >= 0) p.part[(long)ctx.bid * p.dim + c] = red[e];
     }
   }
 };

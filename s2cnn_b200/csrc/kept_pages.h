@@ -4,6 +4,7 @@
 
 #include <type_traits>
 
+#include "../../include/s2cnn_b200.h"
 #include "seq_common.h"
 
 namespace s2c {
@@ -12,16 +13,31 @@ constexpr int kPageLeast = 8;
 struct PageTable {
   const int* table = nullptr;     // [batch][columns]: the page of positions [c page, (c + 1) page)
   void* array[2] = {};            // keys, values
-  int columns = 0, count = 0, page = 1;     // pages of the pool; positions of a page, a power of two
-  // page * `page` + place in the page of position `at` of sequence b; false: it has none
-  S2C_D bool at(int b, long at, long& slot) const {
-    if (at < 0 || at >= (long)columns * page) return false;
-    const int which = table[(long)b * columns + at / page];
-    slot = (long)which * page + at % page;
-    return which >= 0 && which < count;
+  int columns = 0, count = 0, page = 1, log_page = 0;     // pages of the pool; positions of a page, a power of two
+  // the page of position `at` of sequence b; -1: it has none
+  S2C_D int of(int b, long at) const {
+    if (at < 0 || at >= (long)columns * page) return -1;
+    const int which = table[(long)b * columns + (at >> log_page)];
+    return which < count ? which : -1;
   }
 };
 
+// what every call on pages has to fulfil
+inline int page_check(const char* who, const s2c_page_desc* d) {
+  const std::string w = std::string(who) + ": ";
+  if (!d || !d->table) return fail(S2C_ERR_BAD_ARG, w + "no pages");
+  if (d->columns < 0 || d->count < 0) return fail(S2C_ERR_BAD_ARG, w + "bad sizes");
+  if (d->page < kPageLeast || (d->page & (d->page - 1))) return fail(S2C_ERR_UNSUPPORTED, w + "the positions of a page are a power of two, at least 8");
+  if ((long)d->columns * d->page > (1L << 28) || (long)d->count * d->page > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, w + "at most 2^28 positions in a sequence and 2^31 in a pool");
+  return S2C_OK;
+}
+inline PageTable page_table(const s2c_page_desc* d, const void* keys, const void* values) {
+  PageTable t;
+  t.table = d->table; t.columns = d->columns; t.count = d->count; t.page = d->page;
+  while ((1 << t.log_page) < d->page) ++t.log_page;
+  t.array[0] = const_cast<void*>(keys); t.array[1] = const_cast<void*>(values);
+  return t;
+}
 // ---- pages copied within their pool -----------------------------------------------------------------------------------
 struct PageCopyParams {
   char* base;
@@ -83,13 +99,12 @@ struct PageGather {
       const int b = (int)(r / p.length), j = (int)(r % p.length);
       if (p.kv_len && j >= p.kv_len[b]) continue;
       if (p.causal && j > (long)(p.start ? p.start[b] : p.start_all) + (p.q_len ? p.q_len[b] : p.lq) - 1) continue;
-      long slot = 0;
-      const bool there = p.pages.at(b, j, slot);
+      const int page = p.pages.of(b, j), at = j & (p.pages.page - 1);
       for (int which = 0; which < 2; ++which) {
-        const T* from = static_cast<const T*>(p.pages.array[which]) + (there ? slot / p.pages.page * p.stride[which][0] + slot % p.pages.page * p.stride[which][1] : 0);
+        const T* from = static_cast<const T*>(p.pages.array[which]) + (page >= 0 ? page * p.stride[which][0] + at * p.stride[which][1] : 0);
         T* to = static_cast<T*>(p.out[which]) + r * width;
         for (int e = lane; e < width; e += 32) {
-          if (there) to[e] = from[e / p.dim * p.stride[which][2] + e % p.dim];
+          if (page >= 0) to[e] = from[e / p.dim * p.stride[which][2] + e % p.dim];
           else narrow(to + e, as_float(0x7fffffffu));
         }
       }

@@ -35,6 +35,7 @@
 #include "project_kernels.h"
 #ifdef S2C_EMUL
 #include "sequence.h"
+#include "heads.h"
 #include "pages.h"
 #endif
 

@@ -276,7 +276,7 @@ struct PagedAttention {
     const T* const kbase = static_cast<const T*>(p.pages.array[0]) + hk * p.ks[2];
     const T* const vbase = static_cast<const T*>(p.pages.array[1]) + hk * p.vs[2];
     const int* const table = p.pages.table + (long)b * p.pages.columns;
-    const int page = p.pages.page, log_page = __ffs(page) - 1;
+    const int page = p.pages.page, log_page = p.pages.log_page;
 
     Tile t = {};
     // the page of every eighth position of a step, one to a lane; -1: none

@@ -1,2 +1,2 @@
-// Rotation of heads by position and kept keys in pages, compiled beside lib.cu and sequence.cu (build.py).
+// Attention over pages, and copying them, compiled beside lib.cu (build.py).
 #include "pages.h"

@@ -1,6 +1,5 @@
-// C-ABI entry points of the rotation of heads by position and of kept keys in pages (the end of the section on sequences in
-// include/s2cnn_b200.h): checks and the choice of kernels.  Compiled from pages.cu beside lib.cu; part of lib.cu's translation unit in
-// the host-emulation build.
+// C-ABI entry points of attention over pages and of copying them (the end of the section on sequences in include/s2cnn_b200.h):
+// checks and the choice of kernels.  Compiled from pages.cu beside lib.cu; part of lib.cu's translation unit in the host-emulation build.
 #pragma once
 
 #include "../../include/s2cnn_b200.h"
@@ -10,123 +9,12 @@
 #include <cmath>
 
 #include "attention_kernels.h"
-#include "head_rotation_kernels.h"
 #include "kept_pages.h"
 #include "paged_attention_kernels.h"
 
 namespace s2c {
 
-inline bool on_boundary(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-// ---- heads ---------------------------------------------------------------------------------------------------------------
-constexpr int kHeadMaxDim = 128;
-inline int head_check(const char* who, const s2c_head_desc* d) {
-  const std::string w = std::string(who) + ": ";
-  if (!d) return fail(S2C_ERR_BAD_ARG, w + "no description");
-  S2C_SEQ_TRY(seq_check_type(who, d->dtype));
-  if (d->batch < 0 || d->length < 0 || d->heads < 0 || d->kv_heads < 0 || d->dim < 1) return fail(S2C_ERR_BAD_ARG, w + "bad sizes");
-  if (d->dim > kHeadMaxDim) return fail(S2C_ERR_UNSUPPORTED, w + "at most 128 values per head");
-  if (d->pairs < 0 || 2 * d->pairs > d->dim || (d->pairs > 0 && !d->frequencies)) return fail(S2C_ERR_BAD_ARG, w + "more frequencies than pairs of values, or none");
-  if (!(std::fabs(d->magnitude) <= FLT_MAX) || (d->norm && !(d->eps >= 0.f))) return fail(S2C_ERR_BAD_ARG, w + "magnitude or eps is no number, or eps negative");
-  return S2C_OK;
-}
-inline HeadParams head_params(const s2c_head_desc* d) {
-  HeadParams p = {};
-  p.frequencies = d->frequencies; p.positions = d->positions; p.lengths = d->lengths;
-  p.batch = d->batch; p.length = d->length; p.dim = d->dim; p.pairs = d->pairs; p.interleaved = d->interleaved != 0; p.norm = d->norm != 0;
-  p.each = d->each != 0; p.first = d->start;
-  p.eps = d->eps; p.magnitude = d->magnitude;
-  return p;
-}
-inline void head_kind(HeadKind& k, const void* x, const void* w, void* out, const long (&stride)[3], int heads, int turn) {
-  k.x = x; k.w = w; k.out = out; k.heads = x ? heads : 0; k.turn = turn;
-  for (int i = 0; i < 3; ++i) k.stride[i] = stride[i];
-}
-// Pieces of four values: those of a lane have to lie together (halves: whole pieces of pairs, and of what is not turned), and rows
-// on their boundaries.  (The weights are read value by value, once per block.)
-inline bool head_wide(const HeadParams& p, const HeadKind& k, int size) {
-  bool ok = p.interleaved ? p.dim % 4 == 0 : p.pairs % 4 == 0 && (p.dim - 2 * p.pairs) % 8 == 0;
-  ok = ok && on_boundary(k.x, 4 * size) && on_boundary(k.dy, 4 * size) && on_boundary(k.out, 4 * size);
-  for (int i = 0; i < 3; ++i) ok = ok && k.stride[i] % 4 == 0;
-  return ok;
-}
-// Blocks of each kind: one turn for every team where `most` blocks hold them, and the kinds' share of `most` otherwise.
-inline long head_blocks(HeadParams& p, int kinds, int group, int teams, long most) {
-  long want[3] = {}, all = 0;
-  for (int k = 0; k < kinds; ++k) {
-    want[k] = ((long)p.batch * p.length * ((p.kind[k].heads + group - 1) / group) + teams - 1) / teams;
-    all += want[k];
-  }
-  long sum = 0;
-  for (int k = 0; k < kinds; ++k) {
-    const long n = all <= most ? want[k] : want[k] ? std::max(1L, (long)((double)want[k] / (double)all * (double)most)) : 0;
-    p.kind[k].blocks = (int)n;
-    sum += n;
-  }
-  return sum;
-}
-template <class T, class F>
-int head_by_dim(int dim, F f) {
-  if (dim <= 32) return f(std::integral_constant<int, 4>());
-  if (dim <= 64) return f(std::integral_constant<int, 8>());
-  return f(std::integral_constant<int, 16>());
-}
-template <class T>
-int head_forward(HeadParams p, int kinds, const char* name, stream_t st) {
-  for (int k = 0; k < kinds; ++k) p.kind[k].wide = p.kind[k].wide && head_wide(p, p.kind[k], sizeof(T));
-  return head_by_dim<T>(p.dim, [&](auto lanes) {
-    constexpr int L = decltype(lanes)::value;
-    using Four = HeadForward<T, L, 4>;
-    using One = HeadForward<T, L, 1>;
-    const long most = 2L * Four::kBlocks * dev_sm_count();
-    // four heads to a team where that leaves two blocks for every SM
-    long blocks = head_blocks(p, kinds, 4, Four::kTeams, most);
-    if (blocks >= 2L * dev_sm_count()) return seq_launch<Four>(name, blocks, 0, st, p);
-    blocks = head_blocks(p, kinds, 1, One::kTeams, most);
-    return seq_launch<One>(name, blocks, 0, st, p);
-  });
-}
-// blocks of the backward pass; the same for a workspace query, which knows the sizes alone
-template <class T>
-long head_backward_blocks(HeadParams& p) {
-  long n = 0;
-  head_by_dim<T>(p.dim, [&](auto lanes) {
-    constexpr int L = decltype(lanes)::value;
-    n = head_blocks(p, 2, 2, HeadBackward<T, L, 2>::kTeams, 2L * HeadBackward<T, L, 2>::kBlocks * dev_sm_count());
-    return (int)S2C_OK;
-  });
-  return n;
-}
-template <class T>
-int head_backward(HeadParams p, void* dqw, void* dkw, stream_t st) {
-  const long blocks = head_backward_blocks<T>(p);
-  for (int k = 0; k < 2; ++k) p.kind[k].wide = head_wide(p, p.kind[k], sizeof(T));
-  S2C_SEQ_TRY(head_by_dim<T>(p.dim, [&](auto lanes) {
-    using K = HeadBackward<T, decltype(lanes)::value, 2>;
-    return seq_launch<K>("norm_rotate_backward", blocks, K::smem(), st, p);
-  }));
-  if (!p.part) return S2C_OK;
-  HeadSumParams s = {};
-  s.part = p.part; s.dw[0] = dqw; s.dw[1] = dkw; s.dim = p.dim;
-  s.blocks[0] = p.kind[0].blocks; s.first[1] = p.kind[0].blocks; s.blocks[1] = p.kind[1].blocks;
-  return seq_launch<HeadWeightSum<T>>("norm_rotate_sums", 2L * ((p.dim + 31) / 32), 256 * sizeof(float), st, s);
-}
-
 // ---- pages ---------------------------------------------------------------------------------------------------------------
-inline int page_check(const char* who, const s2c_page_desc* d) {
-  const std::string w = std::string(who) + ": ";
-  if (!d || !d->table) return fail(S2C_ERR_BAD_ARG, w + "no pages");
-  if (d->columns < 0 || d->count < 0) return fail(S2C_ERR_BAD_ARG, w + "bad sizes");
-  if (d->page < kPageLeast || (d->page & (d->page - 1))) return fail(S2C_ERR_UNSUPPORTED, w + "the positions of a page are a power of two, at least 8");
-  if ((long)d->columns * d->page > (1L << 28) || (long)d->count * d->page > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, w + "at most 2^28 positions in a sequence and 2^31 in a pool");
-  return S2C_OK;
-}
-inline PageTable page_table(const s2c_page_desc* d, const void* keys, const void* values) {
-  PageTable t;
-  t.table = d->table; t.columns = d->columns; t.count = d->count; t.page = d->page;
-  t.array[0] = const_cast<void*>(keys); t.array[1] = const_cast<void*>(values);
-  return t;
-}
 template <class T>
 int page_gather(const PageGatherParams& p, stream_t st) {
   const long rows = (long)p.batch * p.length;
@@ -240,73 +128,6 @@ int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* ke
 using namespace s2c;
 
 extern "C" {
-
-int s2c_norm_rotate(const s2c_head_desc* d, const void* q, const void* k, const void* q_weight, const void* k_weight, void* q_out, void* k_out, void* stream) {
-  S2C_SEQ_TRY(head_check("s2c_norm_rotate", d));
-  if ((q && !q_out) || (k && !k_out)) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate: a pointer is missing");
-  HeadParams p = head_params(d);
-  p.lengths = nullptr;
-  head_kind(p.kind[0], q, p.norm ? q_weight : nullptr, q_out, d->q_stride, d->heads, 1);
-  head_kind(p.kind[1], k, p.norm ? k_weight : nullptr, k_out, d->k_stride, d->kv_heads, 1);
-  p.kind[0].wide = p.kind[1].wide = 1;
-  return d->dtype == kSeqF32 ? head_forward<float>(p, 2, "norm_rotate", (stream_t)stream) : head_forward<bf16>(p, 2, "norm_rotate", (stream_t)stream);
-}
-
-size_t s2c_norm_rotate_backward_workspace(const s2c_head_desc* d) {
-  if (head_check("s2c_norm_rotate_backward_workspace", d) != S2C_OK || !d->norm) return 0;
-  HeadParams p = head_params(d);
-  p.kind[0].heads = d->heads;
-  p.kind[1].heads = d->kv_heads;
-  return (size_t)(d->dtype == kSeqF32 ? head_backward_blocks<float>(p) : head_backward_blocks<bf16>(p)) * d->dim * sizeof(float);
-}
-
-int s2c_norm_rotate_backward(const s2c_head_desc* d, const void* q, const void* k, const void* q_weight, const void* k_weight, const void* dq_out,
-                             const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
-                             void* stream) {
-  S2C_SEQ_TRY(head_check("s2c_norm_rotate_backward", d));
-  const bool some = d->batch > 0 && d->length > 0;
-  if (some && ((d->heads > 0 && (!q || !dq_out)) || (d->kv_heads > 0 && (!k || !dk_out)))) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_backward: a pointer is missing");
-  if ((dq_weight || dk_weight) && !d->norm) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_backward: a weight needs a norm");
-  if ((dq_weight && !q_weight) || (dk_weight && !k_weight)) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_backward: the gradient of a weight that is not given");
-  const bool sums = dq_weight || dk_weight;
-  const size_t need = sums ? s2c_norm_rotate_backward_workspace(d) : 0;
-  if (need && (!workspace || workspace_bytes < need)) return fail(S2C_ERR_WORKSPACE, "s2c_norm_rotate_backward: workspace too small");
-  if (!on_boundary(workspace, 4)) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_backward: the workspace starts on a 4-byte boundary");
-  HeadParams p = head_params(d);
-  p.lengths = nullptr;
-  static const float none = 0.f;               // (no rows: the sums are written as zeros, nothing is read)
-  head_kind(p.kind[0], d->heads ? (q ? q : &none) : nullptr, p.norm ? q_weight : nullptr, dq, d->q_stride, d->heads, 1);
-  head_kind(p.kind[1], d->kv_heads ? (k ? k : &none) : nullptr, p.norm ? k_weight : nullptr, dk, d->k_stride, d->kv_heads, 1);
-  p.kind[0].dy = dq_out;
-  p.kind[1].dy = dk_out;
-  p.part = !sums ? nullptr : need ? static_cast<float*>(workspace) : const_cast<float*>(&none);
-  return d->dtype == kSeqF32 ? head_backward<float>(p, dq_weight, dk_weight, (stream_t)stream) : head_backward<bf16>(p, dq_weight, dk_weight, (stream_t)stream);
-}
-
-int s2c_norm_rotate_store(const s2c_head_desc* d, const s2c_page_desc* pages, const void* q, const void* k, const void* v, const void* q_weight,
-                          const void* k_weight, void* q_out, void* keys, void* values, void* stream) {
-  S2C_SEQ_TRY(head_check("s2c_norm_rotate_store", d));
-  S2C_SEQ_TRY(page_check("s2c_norm_rotate_store", pages));
-  if (q && !q_out) return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_store: a pointer is missing");
-  if (d->batch > 0 && d->length > 0 && d->kv_heads > 0 && (!k || !v || (pages->count > 0 && (!keys || !values))))
-    return fail(S2C_ERR_BAD_ARG, "s2c_norm_rotate_store: a pointer is missing");
-  HeadParams p = head_params(d);
-  p.pages = page_table(pages, keys, values);
-  head_kind(p.kind[0], q, p.norm ? q_weight : nullptr, q_out, d->q_stride, d->heads, 1);
-  head_kind(p.kind[1], k, p.norm ? k_weight : nullptr, nullptr, d->k_stride, d->kv_heads, 1);
-  head_kind(p.kind[2], v, nullptr, nullptr, d->v_stride, d->kv_heads, 0);
-  for (int i = 0; i < 3; ++i) {
-    p.kind[1].pstride[i] = pages->key_stride[i];
-    p.kind[2].pstride[i] = pages->value_stride[i];
-  }
-  const int size = d->dtype == kSeqF32 ? 4 : 2;
-  p.kind[0].wide = 1;
-  for (int which = 1; which < 3; ++which) {
-    const HeadKind& kind = p.kind[which];
-    p.kind[which].wide = on_boundary(p.pages.array[which - 1], 4 * size) && kind.pstride[0] % 4 == 0 && kind.pstride[1] % 4 == 0 && kind.pstride[2] % 4 == 0;
-  }
-  return d->dtype == kSeqF32 ? head_forward<float>(p, 3, "norm_rotate_store", (stream_t)stream) : head_forward<bf16>(p, 3, "norm_rotate_store", (stream_t)stream);
-}
 
 size_t s2c_paged_attention_workspace(const s2c_attention_desc* d, const s2c_page_desc* pages) {
   if (page_check("s2c_paged_attention_workspace", pages) != S2C_OK || attn_check("s2c_paged_attention_workspace", d) != S2C_OK) return 0;

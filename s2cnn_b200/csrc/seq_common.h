@@ -21,7 +21,8 @@ enum SeqType : int { kSeqF32 = 0, kSeqBf16 = 1 };
 inline int seq_check_type(const char* who, int dtype) {
   return dtype == kSeqF32 || dtype == kSeqBf16 ? S2C_OK : fail(S2C_ERR_BAD_ARG, std::string(who) + ": dtype is 0 (float32) or 1 (bfloat16)");
 }
-inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline bool on_boundary(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+inline bool aligned16(const void* p) { return on_boundary(p, 16); }
 
 struct bf16 {
   unsigned short bits;
@@ -128,6 +129,17 @@ S2C_D void store_four(bf16* p, const float (&v)[4]) {
   *reinterpret_cast<Vec8*>(p) = u;
 }
 
+// two products in one instruction, as fma2
+#ifndef S2C_EMUL
+S2C_D float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+#else
+inline float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+#endif
 // n / d for n < 2^31 by a product: m = ceil(2^(31 + l) / d), l = ceil(log2 d) (T. Granlund, P. Montgomery: "Division by invariant
 // integers using multiplication", 1994); a division takes ten times the instructions.
 struct Divisor {
