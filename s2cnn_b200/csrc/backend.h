@@ -68,6 +68,8 @@ struct Ctx {
   __device__ __forceinline__ void sync_warp() const { __syncwarp(); }
   // exchange within a warp, by every thread of the block (as sync_warp)
   __device__ __forceinline__ float shfl_xor(float v, int mask) const { return __shfl_xor_sync(0xffffffffu, v, mask); }
+  // whether a warp has work: some thread's `v`, by every thread of the warp (the emulation, whose exchanges are barriers of the block: always)
+  __device__ __forceinline__ bool warp_any(bool v) const { return __any_sync(0xffffffffu, v); }
 };
 
 inline int cuda_check(cudaError_t e, const char* what) {
@@ -422,6 +424,7 @@ struct Ctx {
     sync();
     return r;
   }
+  bool warp_any(bool) const { return true; }
 };
 
 inline void emu_trampoline() {

@@ -123,7 +123,7 @@ struct HeadTeam {
       }
     }
   }
-  // (a lane's piece behind the head: its first one, in place of which `open` has zeros)
+  // (a lane's piece behind the head: the head's first one, which counts in no sum and is stored nowhere)
   S2C_D void fetch(const T* x, Raw& r) const {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -142,15 +142,12 @@ struct HeadTeam {
     }
   }
   // as pairs (a[e], b[e])
-  S2C_D void open(const HeadParams& p, const Raw& r, float2 (&a)[NP], float2 (&b)[NP]) const {
+  S2C_D void open(const Raw& r, float2 (&a)[NP], float2 (&b)[NP]) const {
     if constexpr (kPieces) {
       float v[2][4];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         load_four(reinterpret_cast<const T*>(&r.piece[k]), v[k]);
-        if (p.dim < 8 * LANES && at[k][0] < 0)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[k][e] = 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -200,36 +197,47 @@ struct HeadTeam {
     float w[2][kPairs][LANES];    // weights of the first and second values of a lane's pairs
     unsigned long long f[kPairs][LANES];      // frequencies
   };
+  // FORWARD: the magnitude goes with the weights; otherwise with sines and cosines
+  template <bool FORWARD>
   static S2C_D void share(const Ctx& ctx, const HeadParams& p, const HeadKind& kind, Shared* to) {
     if (ctx.tid < LANES * kPairs) {
       const int lane = ctx.tid % LANES, e = ctx.tid / LANES, i = pair(lane, e);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int c = place(p, i, k);
-        to->w[k][e][lane] = kind.w && c >= 0 ? widen(static_cast<const T*>(kind.w)[c]) : 1.f;
+        to->w[k][e][lane] = (kind.w && c >= 0 ? widen(static_cast<const T*>(kind.w)[c]) : 1.f) * (i < p.pairs && FORWARD ? p.magnitude : 1.f);
       }
       to->f[e][lane] = kind.turn && i < p.pairs ? turn_units(p.frequencies[i]) : 0ull;
     }
     if (ctx.tid == ctx.nthr - 1) to->kind = kind;
     ctx.sync();
   }
-  // cosines and sines of the pairs times the magnitude; of what is not turned 1 and 0
+  // cosines and sines of the pairs; of what is not turned 1 and 0
+  template <bool FORWARD>
   S2C_D void angles(const HeadParams& p, const Shared* s, long position, float2 (&c)[NP], float2 (&si)[NP]) const {
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
       turn_cos_sin(s->f[2 * e][t] * (unsigned long long)position, c[e].x, si[e].x);
       turn_cos_sin(s->f[2 * e + 1][t] * (unsigned long long)position, c[e].y, si[e].y);
-      if (turned >> 2 * e & 1) c[e].x *= p.magnitude, si[e].x *= p.magnitude;
-      if (turned >> 2 * e & 2) c[e].y *= p.magnitude, si[e].y *= p.magnitude;
+      if (!FORWARD && (turned >> 2 * e & 1)) c[e].x *= p.magnitude, si[e].x *= p.magnitude;
+      if (!FORWARD && (turned >> 2 * e & 2)) c[e].y *= p.magnitude, si[e].y *= p.magnitude;
     }
   }
   S2C_D float2 weights(const Shared* s, int k, int e) const { return make_float2(s->w[k][2 * e][t], s->w[k][2 * e + 1][t]); }
-  static S2C_D float2 square(const float2 (&a)[NP], const float2 (&b)[NP], const float2 (&x)[NP], const float2 (&y)[NP]) {
-    float2 sum = mul2(a[0], x[0]);
-    sum = fma2(b[0], y[0], sum);
+  // sum over a head of a x + b y, in every lane
+  S2C_D float product(const Ctx& ctx, const float2 (&a)[NP], const float2 (&b)[NP], const float2 (&x)[NP], const float2 (&y)[NP]) const {
+    float2 sum[NP];
 #pragma unroll
-    for (int e = 1; e < NP; ++e) sum = fma2(a[e], x[e], fma2(b[e], y[e], sum));
-    return sum;
+    for (int e = 0; e < NP; ++e) sum[e] = fma2(b[e], y[e], mul2(a[e], x[e]));
+    if constexpr (kPieces) {      // pieces behind the head
+      const float m = at[0][0] >= 0 ? 1.f : 0.f, n = kNext ? (at[1][0] >= 0 ? 1.f : 0.f) : m;
+      return lanes_sum<LANES>(ctx, fmaf(m, sum[0].x + sum[0].y, n * (sum[1].x + sum[1].y)));
+    } else {
+      float s = sum[0].x + sum[0].y;
+#pragma unroll
+      for (int e = 1; e < NP; ++e) s += sum[e].x + sum[e].y;
+      return lanes_sum<LANES>(ctx, s);
+    }
   }
   // A unit: `span` neighbouring heads of one position.
   struct Unit {
@@ -267,10 +275,11 @@ struct HeadForward {
     while (which < 2 && bid >= p.kind[which].blocks) bid -= p.kind[which++].blocks;
     typename Team::Shared* const shared = reinterpret_cast<typename Team::Shared*>(smem);
     const HeadKind& kind = shared->kind;
-    Team::share(ctx, p, p.kind[which], shared);
+    Team::template share<true>(ctx, p, p.kind[which], shared);
     const Team team(p, ctx.tid % LANES);
     const long units = (long)p.batch * p.length * kind.spans.d, per = (long)kind.blocks * Team::kTeams, mine = ctx.tid / LANES;
-    const bool rest = 2 * p.pairs < p.dim, turn = kind.turn;
+    // values that are not turned: an infinity times a sine of 0 would be none (in a norm's head nothing is left of it)
+    const bool rest = 2 * p.pairs < p.dim && !p.norm, turn = kind.turn;
     const int span = kind.span;
     const long step = kind.stride[2];
     Raw raw[GROUP];
@@ -279,19 +288,23 @@ struct HeadForward {
       for (int g = 0; g < GROUP; ++g) team.fetch(x + (g < left ? g * step : 0), raw[g]);
     };
     long u0 = (long)bid * Team::kTeams;
-    Unit now = Team::unit(p, kind, u0 + mine, units);
-    fetch(now.x, now.left);
-    bool next_filled = true;
+    // the next unit, its heads, and in a store its page, while the heads before are worked on
+    Unit now;
+    bool next_filled = true, next_work = true;          // (rows that are not filled: a warp of them alone has nothing to do)
     int next_page = 0;
-    auto look_up = [&] {                                // of a store, while the heads before are worked on
-      if (!p.pages.table) return;
-      next_filled = !p.lengths || now.i < p.lengths[now.b];
-      next_page = p.pages.of(now.b, now.at);
+    auto open_unit = [&](long u) {
+      now = Team::unit(p, kind, u, units);
+      if (p.pages.table) {
+        next_filled = !p.lengths || now.i < p.lengths[now.b];
+        next_work = ctx.warp_any(next_filled && now.on);
+        if (next_work) next_page = p.pages.of(now.b, now.at);
+      }
+      if (next_work) fetch(now.x, now.left);
     };
-    look_up();
+    open_unit(u0 + mine);
     for (; u0 < units; u0 += per) {                     // (every team takes the same number of turns)
       // where the unit's heads go (null: nowhere), and what is said of a row that has no value
-      const bool filled = next_filled;
+      const bool filled = next_filled, work = next_work;
       const int page = next_page;
       T* y = nullptr;
       long y_step = p.dim;
@@ -303,9 +316,9 @@ struct HeadForward {
       }
       // y_a = x_a k0 + x_b k1, y_b = x_a k2 + x_b k3
       float2 k0[NP], k1[NP], k2[NP], k3[NP];
-      if (turn) {
+      if (turn && work) {
         float2 c[NP], s[NP];
-        team.angles(p, shared, now.at, c, s);
+        team.template angles<true>(p, shared, now.at, c, s);
 #pragma unroll
         for (int e = 0; e < NP; ++e) {
           const float2 x = team.weights(shared, 0, e), z = team.weights(shared, 1, e);
@@ -322,20 +335,17 @@ struct HeadForward {
 #pragma unroll
         for (int g = 0; g < GROUP; ++g) old[g] = raw[g];
         if (n + GROUP < span) {
-          if (left > GROUP) fetch(x += GROUP * step, left - GROUP);
+          if (left > GROUP && work) fetch(x += GROUP * step, left - GROUP);
         } else {
-          now = Team::unit(p, kind, u0 + per + mine, units);
-          fetch(now.x, now.left);
-          look_up();
+          open_unit(u0 + per + mine);
         }
 #pragma unroll
         for (int g = 0; g < GROUP; ++g) {
           float2 a[NP], b[NP];
-          team.open(p, old[g], a, b);
-          if (turn) {
+          team.open(old[g], a, b);
+          if (turn && work) {
             if (p.norm) {
-              const float2 sum = Team::square(a, b, a, b);
-              const float rstd = inv_sqrt(fmaf(lanes_sum<LANES>(ctx, sum.x + sum.y), p.over_dim, p.eps));
+              const float rstd = inv_sqrt(fmaf(team.product(ctx, a, b, a, b), p.over_dim, p.eps));
               const float2 r2 = make_float2(rstd, rstd);
 #pragma unroll
               for (int e = 0; e < NP; ++e) {
@@ -348,7 +358,7 @@ struct HeadForward {
               const float2 u = a[e], v = b[e];
               a[e] = fma2(u, k0[e], mul2(v, k1[e]));
               b[e] = fma2(u, k2[e], mul2(v, k3[e]));
-              if (rest) {                               // what is not turned (an infinity times a sine of 0 would be none)
+              if (rest) {
                 if (!(team.turned >> 2 * e & 1)) a[e].x = u.x * k0[e].x, b[e].x = v.x * k3[e].x;
                 if (!(team.turned >> 2 * e & 2)) a[e].y = u.y * k0[e].y, b[e].y = v.y * k3[e].y;
               }
@@ -380,7 +390,7 @@ struct HeadBackward {
     const int bid = ctx.bid - (which ? p.kind[0].blocks : 0);
     typename Team::Shared* const shared = reinterpret_cast<typename Team::Shared*>(smem);
     const HeadKind& kind = shared->kind;
-    Team::share(ctx, p, p.kind[which], shared);
+    Team::template share<false>(ctx, p, p.kind[which], shared);
     const Team team(p, ctx.tid % LANES);
     const long units = (long)p.batch * p.length * kind.spans.d, per = (long)kind.blocks * Team::kTeams, mine = ctx.tid / LANES;
     const bool rest = 2 * p.pairs < p.dim;
@@ -403,7 +413,7 @@ struct HeadBackward {
     for (int e = 0; e < NP; ++e) da[e] = db[e] = make_float2(0.f, 0.f);
     for (; u0 < units; u0 += per) {
       float2 c[NP], s[NP], w[2][NP];
-      team.angles(p, shared, now.at, c, s);
+      team.template angles<false>(p, shared, now.at, c, s);
 #pragma unroll
       for (int e = 0; e < NP; ++e) {
         w[0][e] = team.weights(shared, 0, e);
@@ -430,7 +440,7 @@ struct HeadBackward {
         for (int g = 0; g < GROUP; ++g) {
           const bool in = on && g < left && n + g < span;
           float2 ga[NP], gb[NP];
-          team.open(p, old_d[g], ga, gb);
+          team.open(old_d[g], ga, gb);
 #pragma unroll
           for (int e = 0; e < NP; ++e) {
             const float2 u = ga[e], v = gb[e];
@@ -443,9 +453,8 @@ struct HeadBackward {
           }
           if (p.norm) {
             float2 xa[NP], xb[NP];
-            team.open(p, old_x[g], xa, xb);
-            float2 sum = Team::square(xa, xb, xa, xb);
-            const float rstd = inv_sqrt(fmaf(lanes_sum<LANES>(ctx, sum.x + sum.y), p.over_dim, p.eps));
+            team.open(old_x[g], xa, xb);
+            const float rstd = inv_sqrt(fmaf(team.product(ctx, xa, xb, xa, xb), p.over_dim, p.eps));
             const float2 r2 = make_float2(rstd, rstd);
 #pragma unroll
             for (int e = 0; e < NP; ++e) {
@@ -458,8 +467,7 @@ struct HeadBackward {
               ga[e] = mul2(ga[e], w[0][e]);
               gb[e] = mul2(gb[e], w[1][e]);
             }
-            sum = Team::square(ga, gb, xa, xb);
-            const float dot = -lanes_sum<LANES>(ctx, sum.x + sum.y) * p.over_dim;
+            const float dot = -team.product(ctx, ga, gb, xa, xb) * p.over_dim;
             const float2 dot2 = make_float2(dot, dot);
 #pragma unroll
             for (int e = 0; e < NP; ++e) {
