@@ -159,9 +159,13 @@ struct PagedAttention {
     const long each = quotient(total, blocks), rest = total - each * blocks;       // the first `rest` blocks have one more
     const long lo = ctx.bid * each + min((long)ctx.bid, rest), hi = lo + each + (ctx.bid < rest);
     if (a.bias)
-      for (int e = ctx.tid; e <= 2 * a.reach; e += kThreads) {
-        const int which = a.bucket_of[e];
-        bucket[e] = (unsigned short)(which >= 0 && which < a.n_buckets ? which : a.n_buckets);
+      for (int e = ctx.tid; e <= 2 * a.reach; e += 4 * kThreads) {               // (four loads on their way)
+        int which[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) which[k] = a.bucket_of[min(e + k * kThreads, 2 * a.reach)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (e + k * kThreads <= 2 * a.reach) bucket[e + k * kThreads] = (unsigned short)(which[k] >= 0 && which[k] < a.n_buckets ? which[k] : a.n_buckets);
       }
     if (before * per_batch <= lo && lo < (before + sum) * per_batch) {
       int b = ctx.tid * mine;
@@ -330,12 +334,23 @@ struct PagedAttention {
         query[2 * e + 1] = make_uint4(x[0].lo, x[1].lo, x[2].lo, x[3].lo);
       }
     }
-    if (a.bias)
-      for (int e = ctx.tid; e < H::kRows * (a.n_buckets + 1); e += kThreads) {
-        const int row = p.by_buckets.quotient(e), r = r0 + row, which = e - row * (a.n_buckets + 1);
-        biases[e] = r < rows && which < a.n_buckets
-                        ? attn_bias_units(widen(static_cast<const T*>(a.bias)[(long)which * a.heads + hk * a.group + p.by_group.rest(r)])) : 0.f;
+    if (a.bias) {
+      const int all = H::kRows * (a.n_buckets + 1);
+      for (int e = ctx.tid; e < all; e += 8 * kThreads) {                         // (eight loads on their way)
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at = min(e + k * kThreads, all - 1), row = p.by_buckets.quotient(at), r = min(r0 + row, rows - 1);
+          const int which = min(at - row * (a.n_buckets + 1), a.n_buckets - 1);
+          v[k] = widen(static_cast<const T*>(a.bias)[(long)which * a.heads + hk * a.group + p.by_group.rest(r)]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at = e + k * kThreads;
+          if (at < all) biases[at] = p.by_buckets.rest(at) < a.n_buckets ? attn_bias_units(v[k]) : 0.f;
+        }
       }
+    }
     int lim[NT][2];                                      // a row sees the positions before lim
     int all_see = keys;                                  // that every row sees
 #pragma unroll
@@ -394,20 +409,19 @@ struct PagedAttention {
             }
       } else {
 #pragma unroll
-        for (int k = 0; k < H::kTiles; ++k)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = j0 + 16 * k + g + 8 * (e / 2);
-            const bool lost = __shfl_sync(0xffffffffu, now, 2 * k + e / 2) < 0;
+          for (int e = 0; e < 2; ++e) {
+            const int row = 8 * nt + 2 * q4 + e, position = (int)p.by_group.quotient(r0 + row) + s.start;
+            const float* const of_row = biases + row * (a.n_buckets + 1);
+            const int away = j0 + g - position + a.reach, sees = lim[nt][e] - j0 - g;      // of position j0 + g
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const int row = 8 * nt + 2 * q4 + e % 2, away = far ? 0 : attn_clamp(j - (int)p.by_group.quotient(r0 + row) - s.start, -a.reach, a.reach) + a.reach;
-              const float add = far ? flat[nt][e % 2] : biases[row * (a.n_buckets + 1) + bucket[away]];
-              float y = fmaf(x[k][nt][e], scale, add);
-              if (lost) y = as_float(0x7fffffffu);                        // a page that is none
-              if (j >= lim[nt][e % 2]) y = kNoScore;
-              x[k][nt][e] = y;
-              top[nt][e % 2] = fmaxf(top[nt][e % 2], y);
+            for (int k = 0; k < 2 * H::kTiles; ++k) {
+              float& y = x[k / 2][nt][2 * (k % 2) + e];
+              y = fmaf(y, scale, far ? flat[nt][e] : of_row[bucket[attn_clamp(away + 8 * k, 0, 2 * a.reach)]]);
+              if (!there && __shfl_sync(0xffffffffu, now, k) < 0) y = as_float(0x7fffffffu);    // a page that is none
+              if (8 * k >= sees) y = kNoScore;
+              top[nt][e] = fmaxf(top[nt][e], y);
             }
           }
       }
@@ -583,50 +597,75 @@ struct PagedAttention {
   }
 };
 
-// Joins the blocks' results of an item: a block per row, thread t with column t % DP of every kThreads / DP-th block.
-template <class T, int DP, int NT>
+// Joins the blocks' results of an item, ROWS rows of it to a block: thread t of a row with four columns of every kSlices-th block's part,
+// the first loads on their way together.  One row to a block where there may be many parts (1 x 16384 positions, of 111 parts: 14.7 us in
+// all, with one column a thread 19.8), four where there are few (32 x 1000 positions of 48 rows, of at most 8: 18.2 us and 21.6).
+template <class T, int DP, int NT, int ROWS>
 struct PagedJoin {
   using Params = PagedParams;
   using H = PagedShape<T, DP, NT>;
-  static constexpr int kThreads = 128, kBlocks = 8, kSlices = kThreads / DP;
-  static size_t smem(long blocks) { return (blocks + kThreads + 8) * sizeof(float); }
+  static constexpr int kThreads = 256, kBlocks = 4, kRowThreads = kThreads / ROWS, kCols = DP / 4, kSlices = kRowThreads / kCols, kWarps = kRowThreads / 32;
+  static size_t smem(long parts) { return (16 + 4 * kThreads + ROWS * (size_t)parts) * sizeof(float); }      // (most parts of an item)
   static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char* smem) {
     const AttnParams& a = p.a;
-    const int4 what = p.split[ctx.bid / H::kRows];
-    const int n = what.z, per_batch = a.kv_heads * p.row_blocks, b = what.x / per_batch, within = what.x % per_batch;
-    const int r = ctx.bid % H::kRows, row = within % p.row_blocks * H::kRows + r;
-    if (n == 0 || row >= a.lq * a.group) return;
-    const int t = ctx.tid, lane = t % 32, warp = t / 32;
-    float *red = reinterpret_cast<float*>(smem), *outs = red + 8, *weight = outs + kThreads;
+    const int4 what = p.split[ctx.bid / (H::kRows / ROWS)];
+    const int n = what.z, per_batch = a.kv_heads * p.row_blocks, b = what.x / per_batch, within = what.x - b * per_batch;
+    const int hk = p.by_row_blocks.quotient(within), which = ctx.tid / kRowThreads;
+    const int r = ctx.bid % (H::kRows / ROWS) * ROWS + which, r0 = (within - hk * p.row_blocks) * H::kRows, row = r0 + r, rows = a.lq * a.group;
+    if (n == 0 || row - which >= rows) return;           // (a whole block)
+    const int t = ctx.tid % kRowThreads, lane = t % 32, warp = t / 32;
+    float *red = reinterpret_cast<float*>(smem) + 2 * kWarps * which, *outs = reinterpret_cast<float*>(smem) + 16 + 4 * kRowThreads * which;
+    float* const weight = reinterpret_cast<float*>(smem) + 16 + 4 * kThreads + n * which;
     // block k's part of it: the first one's lies where what goes on is kept
     auto part = [&](int k) { return p.part + ((2L * (what.y + k) + (k == 0)) * H::kRows + r) * (DP + 4); };
+    // the first columns come while the maxima do
+    const int c = t % kCols * 4, slice = t / kCols;
+    constexpr int kAhead = 4;
+    float4 x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (slice + k * kSlices < n) x[k] = *reinterpret_cast<const float4*>(part(slice + k * kSlices) + c);
     float m = kNoScore;
-    for (int e = t; e < n; e += kThreads) m = fmaxf(m, part(e)[DP]);
+    for (int e = t; e < n; e += kRowThreads) {
+      const float top = part(e)[DP];
+      weight[e] = top;
+      m = fmaxf(m, top);
+    }
     m = lanes_max<32>(ctx, m);
     if (lane == 0) red[warp] = m;
     ctx.sync();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[w]);
     const float base = m == kNoScore ? 0.f : m;
     float l = 0.f;
-    for (int e = t; e < n; e += kThreads) {
-      const float f = exp2_fast(part(e)[DP] - base);
+    for (int e = t; e < n; e += kRowThreads) {
+      const float f = exp2_fast(weight[e] - base);
       weight[e] = f;
       l = fmaf(part(e)[DP + 1], f, l);
     }
     l = lanes_sum<32>(ctx, l);
-    if (lane == 0) red[4 + warp] = l;
+    if (lane == 0) red[kWarps + warp] = l;
     ctx.sync();
-    l = (red[4] + red[5]) + (red[6] + red[7]);
-    const int c = t % DP;
-    float o = 0.f;
-#pragma unroll 8
-    for (int e = t / DP; e < n; e += kSlices) o = fmaf(part(e)[c], weight[e], o);
-    outs[t] = o;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const float4& y, float f) {
+      o[0] = fmaf(y.x, f, o[0]);
+      o[1] = fmaf(y.y, f, o[1]);
+      o[2] = fmaf(y.z, f, o[2]);
+      o[3] = fmaf(y.w, f, o[3]);
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (slice + k * kSlices < n) add(x[k], weight[slice + k * kSlices]);
+#pragma unroll 4
+    for (int e = slice + kAhead * kSlices; e < n; e += kSlices) add(*reinterpret_cast<const float4*>(part(e) + c), weight[e]);
+    store_vec(outs + 4 * t, o);
     ctx.sync();
-    if (t >= DP) return;
-    for (int e = 1; e < kSlices; ++e) o += outs[e * DP + t];
-    float one[1] = {o};
-    PagedAttention<T, DP, NT, kRowsFull>::template write<1>(p, b, within / p.row_blocks, row, t, one, l == 0.f ? 0.f : 1.f / l);
+    if (slice != 0 || row >= rows) return;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) l += red[kWarps + w];
+    for (int e = 1; e < min(n, kSlices); ++e) add(*reinterpret_cast<const float4*>(outs + 4 * (e * kCols + t)), 1.f);
+    PagedAttention<T, DP, NT, kRowsFull>::template write<4>(p, b, hk, row, c, o, l == 0.f ? 0.f : 1.f / l);
   }
 };
 

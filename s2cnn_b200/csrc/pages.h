@@ -56,7 +56,7 @@ bool paged_wide(const s2c_page_desc* d, const void* keys, const void* values) {
 struct PagedPlan {
   long items = 0, blocks = 0;
   int row_blocks = 0, nt = 1;
-  bool joined = false;
+  long parts = 1;              // of an item at most
   size_t part = 0, bytes = 0;
 };
 template <class T, class F>
@@ -79,7 +79,7 @@ PagedPlan paged_plan(const AttnParams& a) {
     using K = PagedAttention<T, decltype(dp)::value, decltype(nt)::value, kRowsFull>;
     const long steps = std::max(1, (a.lk + K::H::kStep - 1) / K::H::kStep);
     plan.blocks = std::min((long)K::kBlocks * dev_sm_count(), plan.items * steps);
-    plan.joined = steps > 1;
+    plan.parts = std::min(steps, plan.blocks);
     plan.part = page_align(2 * (size_t)plan.blocks * K::H::kRows * (decltype(dp)::value + 4) * sizeof(float));
     return (int)S2C_OK;
   });
@@ -116,9 +116,12 @@ int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* ke
     S2C_SEQ_TRY(!wide ? seq_launch<N>("paged_attention", plan.blocks, N::smem(a), st, p)
                 : a.dim < DP ? seq_launch<W>("paged_attention", plan.blocks, W::smem(a), st, p)
                              : seq_launch<F>("paged_attention", plan.blocks, F::smem(a), st, p));
-    if (!plan.joined) return (int)S2C_OK;
-    using J = PagedJoin<T, DP, NT>;
-    return seq_launch<J>("paged_join", std::min(plan.items, plan.blocks) * F::H::kRows, J::smem(plan.blocks), st, p);
+    if (plan.parts == 1) return (int)S2C_OK;
+    using Few = PagedJoin<T, DP, NT, 4>;
+    using Many = PagedJoin<T, DP, NT, 1>;
+    const long rows = std::min(plan.items, plan.blocks) * F::H::kRows;
+    return plan.parts <= 16 ? seq_launch<Few>("paged_join", rows / 4, Few::smem(plan.parts), st, p)
+                            : seq_launch<Many>("paged_join", rows, Many::smem(plan.parts), st, p);
   });
 }
 #endif

@@ -684,17 +684,24 @@ struct Ops {
     check(a.k.sizes() == a.v.sizes(), "attention: keys and values differ in shape");
     check(a.q.size(0) == a.k.size(0) && a.q.size(3) == a.k.size(3), "attention: queries and keys differ in batch or dim");
     check(a.k.size(2) > 0 && a.q.size(2) > 0 && a.q.size(2) % a.k.size(2) == 0, "attention: the query heads are a multiple of the key heads");
+    for (int i = 0; i < 4; ++i) check(a.k.size(i) <= 0x7fffffff, "attention: too large");
+    s2c_attention_desc d = query_desc(a, dtype);
+    d.lk = (int)a.k.size(1); d.kv_heads = (int)a.k.size(2);
+    a.k = unit_stride(a.k);
+    a.v = unit_stride(a.v);
+    for (int i = 0; i < 3; ++i) { d.k_stride[i] = a.k.stride(i); d.v_stride[i] = a.v.stride(i); }
+    return d;
+  }
+  // what the queries, their positions and the bias say
+  s2c_attention_desc query_desc(AttnArgs& a, int dtype) const {
     check(a.bias.defined() == a.buckets.defined(), "attention: bias and buckets come together");
     check(std::abs(a.q_start) <= 0x7fffffff, "attention: q_start is out of range");
-    for (int i = 0; i < 4; ++i) check(a.q.size(i) <= 0x7fffffff && a.k.size(i) <= 0x7fffffff, "attention: too large");
+    for (int i = 0; i < 4; ++i) check(a.q.size(i) <= 0x7fffffff, "attention: too large");
     s2c_attention_desc d = {};
     d.dtype = dtype;
     d.batch = (int)a.q.size(0); d.lq = (int)a.q.size(1); d.heads = (int)a.q.size(2); d.dim = (int)a.q.size(3);
-    d.lk = (int)a.k.size(1); d.kv_heads = (int)a.k.size(2);
     a.q = unit_stride(a.q);
-    a.k = unit_stride(a.k);
-    a.v = unit_stride(a.v);
-    for (int i = 0; i < 3; ++i) { d.q_stride[i] = a.q.stride(i); d.k_stride[i] = a.k.stride(i); d.v_stride[i] = a.v.stride(i); }
+    for (int i = 0; i < 3; ++i) d.q_stride[i] = a.q.stride(i);
     d.causal = a.causal;
     d.scale = (float)a.scale;
     d.q_start = (int)a.q_start;
@@ -807,8 +814,10 @@ struct Ops {
   // consecutive values in the last axis
   static Tensor unit_last(const Tensor& t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
   s2c_head_desc head_desc(HeadArgs& a, const char* who) const {
-    const std::string w = std::string(who) + ": ";
-    auto want = [&](bool ok, const char* what) { check(ok, (w + what).c_str()); };
+    auto want = [&](bool ok, const char* what) {
+      if (!ok) raise(PyExc_AssertionError, std::string(who) + ": " + what);
+    };
+    auto refuse = [&](const char* what) { raise(PyExc_TypeError, std::string(who) + ": " + what); };
     const Tensor& any = a.q.defined() ? a.q : a.k;
     want(any.defined(), "neither queries nor keys");
     s2c_head_desc d = {};
@@ -833,7 +842,7 @@ struct Ops {
     }
     if (a.frequencies.defined()) {
       if (a.frequencies.scalar_type() != at::kDouble || a.frequencies.device() != any.device())
-        raise(PyExc_TypeError, w + "frequencies are a float64 tensor on the device of the heads");
+        refuse("frequencies are a float64 tensor on the device of the heads");
       want(a.frequencies.dim() == 1 && 2 * a.frequencies.size(0) <= d.dim, "a frequency for each pair of values, at most dim / 2");
       a.frequencies = a.frequencies.contiguous();
       d.pairs = (int)a.frequencies.size(0);
@@ -847,7 +856,7 @@ struct Ops {
     d.eps = (float)(d.norm ? a.eps : 0);
     for (Tensor* t : {&a.q_weight, &a.k_weight}) {
       if (!t->defined()) continue;
-      prep_like(*t, any, (w + "weights").c_str());
+      prep_like(*t, any, who);
       want(d.norm, "weights belong to a norm: eps is missing");
       want(t->dim() == 1 && t->size(0) == d.dim, "a weight for each value of a head");
       *t = t->contiguous();
@@ -856,14 +865,14 @@ struct Ops {
     d.start = (int)a.start;
     if (a.positions.defined()) {
       if (a.positions.scalar_type() != at::kInt || a.positions.device() != any.device())
-        raise(PyExc_TypeError, w + "positions are a number or an int32 tensor on the device of the heads");
+        refuse("positions are a number or an int32 tensor on the device of the heads");
       d.each = a.positions.dim() == 2;
       want((d.each || a.positions.dim() == 1) && a.positions.size(0) == d.batch && (!d.each || a.positions.size(1) == d.length),
            "positions [batch] of the first ones, or [batch, length]");
       a.positions = a.positions.contiguous();
       d.positions = a.positions.const_data_ptr<int>();
     }
-    d.lengths = int_ptr(a.lengths, any, d.batch, (w + "lengths").c_str());
+    d.lengths = int_ptr(a.lengths, any, d.batch, who);
     return d;
   }
   std::tuple<Tensor, Tensor> norm_rotate(HeadArgs a) const {
@@ -896,14 +905,16 @@ struct Ops {
 
   // -- kept keys in pages ---------------------------------------------------------------------------------
   s2c_page_desc page_desc(const Tensor& like, const Tensor& keys, const Tensor& values, const Tensor& pages, int64_t batch, const char* who) const {
-    const std::string w = std::string(who) + ": ";
-    auto want = [&](bool ok, const char* what) { check(ok, (w + what).c_str()); };
-    prep_like(keys, like, (w + "keys").c_str());
-    prep_like(values, like, (w + "values").c_str());
+    auto want = [&](bool ok, const char* what) {
+      if (!ok) raise(PyExc_AssertionError, std::string(who) + ": " + what);
+    };
+    auto refuse = [&](const char* what) { raise(PyExc_TypeError, std::string(who) + ": " + what); };
+    prep_like(keys, like, who);
+    prep_like(values, like, who);
     want(keys.dim() == 4 && keys.sizes() == values.sizes(), "keys and values [pages, positions of a page, kv_heads, dim]");
     want(keys.size(3) == like.size(3), "heads of another dim than those in the pages");
     want(keys.size(3) <= 1 || (keys.stride(3) == 1 && values.stride(3) == 1), "keys and values with a contiguous last axis");
-    if (pages.scalar_type() != at::kInt || pages.device() != like.device()) raise(PyExc_TypeError, w + "pages are an int32 tensor on the device of the keys");
+    if (pages.scalar_type() != at::kInt || pages.device() != like.device()) refuse("pages are an int32 tensor on the device of the keys");
     want(pages.dim() == 2 && pages.size(0) == batch && pages.is_contiguous(), "pages [batch, columns], contiguous");
     s2c_page_desc d = {};
     d.table = static_cast<const int*>(vptr(pages));
@@ -942,12 +953,12 @@ struct Ops {
   }
   Tensor paged_attention(AttnArgs a, const Tensor& keys, const Tensor& values, const Tensor& pages) const {
     refuse_grad("paged_attention", {a.q, keys, values, a.bias});
-    prep_seq(a.q);
+    const int dtype = prep_seq(a.q);
     check(a.q.dim() == 4, "paged_attention: queries [batch, length, heads, dim]");
     const s2c_page_desc p = page_desc(a.q, keys, values, pages, a.q.size(0), "paged_attention");
-    a.k = keys.new_empty({a.q.size(0), 0, keys.size(2), keys.size(3)});       // (the checks of attention; the pages are read instead)
-    a.v = a.k;
-    const s2c_attention_desc d = attention_desc(a);
+    check(keys.size(2) > 0 && a.q.size(2) > 0 && a.q.size(2) % keys.size(2) == 0, "paged_attention: the query heads are a multiple of the key heads");
+    s2c_attention_desc d = query_desc(a, dtype);
+    d.kv_heads = (int)keys.size(2);
     Tensor out = at::empty({d.batch, d.lq, d.heads, d.dim}, a.q.options());
     Ctx c(*this, a.q);
     const Scratch ws(paged_attention_workspace_(&d, &p), a.q);
