@@ -85,27 +85,35 @@ struct PageGatherParams {
   void* out[2];                   // [batch][length][heads][dim]
   long stride[2][3];              // page, position, head
   const int *q_len, *kv_len, *start;
+  Divisor by_head, by_length;     // of a position's pieces, of the rows
   int batch, length, heads, dim, lq, causal, start_all;
 };
-// A warp takes the rows of one position; NaN where its page is none.  Rows that no query sees are left as they are.
-template <class T>
+// A warp takes a position, in pieces of N values; NaN where its page is none.  Rows that no query sees are left as they are.
+template <class T, int N>
 struct PageGather {
   using Params = PageGatherParams;
+  using Piece = typename std::conditional<N == 1, T, Vec16>::type;
   static constexpr int kThreads = 256, kBlocks = 4;
   static S2C_D void run(const Ctx& ctx, const Params& p, unsigned char*) {
     const long warps = (long)ctx.nblk * (kThreads / 32), rows = (long)p.batch * p.length;
-    const int lane = ctx.tid % 32, width = p.heads * p.dim;
+    const int lane = ctx.tid % 32, pieces = p.heads * p.dim / N;
+    Piece none;
+    T nan[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) narrow(nan + e, as_float(0x7fffffffu));
+    std::memcpy(&none, nan, sizeof(none));
     for (long r = (long)ctx.bid * (kThreads / 32) + ctx.tid / 32; r < rows; r += warps) {
-      const int b = (int)(r / p.length), j = (int)(r % p.length);
+      const int b = (int)p.by_length.quotient((unsigned)r), j = (int)(r - (long)b * p.length);
       if (p.kv_len && j >= p.kv_len[b]) continue;
       if (p.causal && j > (long)(p.start ? p.start[b] : p.start_all) + (p.q_len ? p.q_len[b] : p.lq) - 1) continue;
       const int page = p.pages.of(b, j), at = j & (p.pages.page - 1);
+#pragma unroll
       for (int which = 0; which < 2; ++which) {
         const T* from = static_cast<const T*>(p.pages.array[which]) + (page >= 0 ? page * p.stride[which][0] + at * p.stride[which][1] : 0);
-        T* to = static_cast<T*>(p.out[which]) + r * width;
-        for (int e = lane; e < width; e += 32) {
-          if (page >= 0) to[e] = from[e / p.dim * p.stride[which][2] + e % p.dim];
-          else narrow(to + e, as_float(0x7fffffffu));
+        Piece* to = static_cast<Piece*>(p.out[which]) + r * pieces;
+        for (int e = lane; e < pieces; e += 32) {
+          const int h = (int)p.by_head.quotient(e);
+          to[e] = page >= 0 ? *reinterpret_cast<const Piece*>(from + h * p.stride[which][2] + (e - h * (p.dim / N)) * N) : none;
         }
       }
     }

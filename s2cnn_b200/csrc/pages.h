@@ -15,11 +15,6 @@
 namespace s2c {
 
 // ---- pages ---------------------------------------------------------------------------------------------------------------
-template <class T>
-int page_gather(const PageGatherParams& p, stream_t st) {
-  const long rows = (long)p.batch * p.length;
-  return seq_launch<PageGather<T>>("page_gather", std::min<long>((rows + 7) / 8, 16L * dev_sm_count()), 0, st, p);
-}
 inline size_t page_align(size_t n) { return (n + 255) / 256 * 256; }
 // the call on gathered keys and values
 inline s2c_attention_desc gathered(const s2c_attention_desc* d, const s2c_page_desc* pages) {
@@ -33,6 +28,26 @@ inline s2c_attention_desc gathered(const s2c_attention_desc* d, const s2c_page_d
 inline size_t gathered_bytes(const s2c_attention_desc& g) {
   return page_align((size_t)g.batch * g.lk * g.kv_heads * g.dim * (g.dtype == kSeqF32 ? 4 : 2));
 }
+template <class T>
+int page_gather(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* keys, const void* values, int length, void* k, void* v, stream_t st) {
+  PageGatherParams p = {};
+  p.pages = page_table(pages, keys, values);
+  p.out[0] = k; p.out[1] = v;
+  bool wide = d->dim % kVec<T> == 0 && aligned16(keys) && aligned16(values);
+  for (int i = 0; i < 3; ++i) {
+    p.stride[0][i] = pages->key_stride[i];
+    p.stride[1][i] = pages->value_stride[i];
+    wide = wide && pages->key_stride[i] % kVec<T> == 0 && pages->value_stride[i] % kVec<T> == 0;
+  }
+  p.q_len = d->q_lengths; p.kv_len = d->kv_lengths; p.start = d->q_starts;
+  p.batch = d->batch; p.length = length; p.heads = d->kv_heads; p.dim = d->dim; p.lq = d->lq; p.causal = d->causal; p.start_all = d->q_start;
+  p.by_length = Divisor(std::max(1, length));
+  p.by_head = Divisor(wide ? d->dim / kVec<T> : d->dim);
+  const long rows = (long)d->batch * length;
+  if (rows > 0x7fffffffL || (long)d->kv_heads * d->dim > 0x7fffffffL) return fail(S2C_ERR_UNSUPPORTED, "s2c_paged_attention: too many positions");
+  const long blocks = std::min<long>((rows + 7) / 8, 16L * dev_sm_count());
+  return wide ? seq_launch<PageGather<T, kVec<T>>>("page_gather", blocks, 0, st, p) : seq_launch<PageGather<T, 1>>("page_gather", blocks, 0, st, p);
+}
 
 #ifndef S2C_EMUL
 inline AttnParams paged_params(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* q, const void* bias, void* out) {
@@ -45,6 +60,13 @@ inline AttnParams paged_params(const s2c_attention_desc* d, const s2c_page_desc*
   p.causal = d->causal != 0; p.scale = d->scale; p.start_all = d->q_start;
   p.reach = p.bias ? d->reach : 0; p.n_buckets = p.bias ? d->n_buckets : 0;
   return p;
+}
+// Many queries: keys and values are brought into one array for the kernels of whole tiles, instead of being read again by every 16 rows.
+// 4 x 4096 positions, 4 key heads of 128, 32, 128, 256 and 512 rows for each: in pages 23, 56, 95 and 174 us (float32 45, 127, 224 and
+// 427), in one array 48 to 49 (253 to 259) and some 11 (17) to bring them there.  Not where that takes more than 1 GB of workspace.
+inline bool paged_gathers(const s2c_attention_desc* d, const s2c_page_desc* pages) {
+  const long rows = (long)d->lq * (d->heads / d->kv_heads);
+  return rows > (d->dtype == kSeqF32 ? 256 : 128) && 2 * gathered_bytes(gathered(d, pages)) <= (1ul << 30);
 }
 // rows of 16-byte pieces (of four values at least): keys and values as they lie
 template <class T>
@@ -87,11 +109,10 @@ PagedPlan paged_plan(const AttnParams& a) {
   return plan;
 }
 template <class T>
-int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* keys, const void* values, void* ws, size_t ws_bytes, stream_t st) {
+int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* keys, const void* values, void* ws, stream_t st) {
   const PagedPlan plan = paged_plan<T>(a);
   if (plan.items == 0) return S2C_OK;
   if (plan.items > 0x7fffffffL || (long)a.lq * a.group > 0x7fffff00L) return fail(S2C_ERR_UNSUPPORTED, "s2c_paged_attention: too many heads and queries");
-  if (plan.bytes > ws_bytes || !ws) return fail(S2C_ERR_WORKSPACE, "s2c_paged_attention: workspace too small");
   PagedParams p = {};
   p.a = a;
   p.pages = page_table(pages, keys, values);
@@ -135,39 +156,38 @@ extern "C" {
 size_t s2c_paged_attention_workspace(const s2c_attention_desc* d, const s2c_page_desc* pages) {
   if (page_check("s2c_paged_attention_workspace", pages) != S2C_OK || attn_check("s2c_paged_attention_workspace", d) != S2C_OK) return 0;
 #ifndef S2C_EMUL
-  const AttnParams a = paged_params(d, pages, nullptr, nullptr, nullptr);
-  return d->dtype == kSeqF32 ? paged_plan<float>(a).bytes : paged_plan<bf16>(a).bytes;
-#else
+  if (!paged_gathers(d, pages)) {
+    const AttnParams a = paged_params(d, pages, nullptr, nullptr, nullptr);
+    return d->dtype == kSeqF32 ? paged_plan<float>(a).bytes : paged_plan<bf16>(a).bytes;
+  }
+#endif
   const s2c_attention_desc g = gathered(d, pages);
   return 2 * gathered_bytes(g) + s2c_attention_workspace(&g);
-#endif
 }
 
 int s2c_paged_attention(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* q, const void* keys, const void* values, const void* bias,
                         void* out, void* workspace, size_t workspace_bytes, void* stream) {
   S2C_SEQ_TRY(page_check("s2c_paged_attention", pages));
   S2C_SEQ_TRY(attn_check("s2c_paged_attention", d));
-  if (d->batch > 0 && d->lq > 0 && (!q || !out || (pages->count > 0 && (!keys || !values)))) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: a pointer is missing");
+  if (d->batch == 0 || d->lq == 0) return S2C_OK;
+  if (!q || !out || (pages->count > 0 && (!keys || !values))) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: a pointer is missing");
   if ((bias != nullptr) != (d->bucket_of != nullptr)) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: a bias needs its buckets, and buckets a bias");
   if (!aligned16(workspace)) return fail(S2C_ERR_BAD_ARG, "s2c_paged_attention: the workspace starts on a 16-byte boundary");
-#ifndef S2C_EMUL
-  const AttnParams a = paged_params(d, pages, q, bias, out);
-  return d->dtype == kSeqF32 ? paged_launch<float>(a, pages, keys, values, workspace, workspace_bytes, (stream_t)stream)
-                             : paged_launch<bf16>(a, pages, keys, values, workspace, workspace_bytes, (stream_t)stream);
-#else
-  const s2c_attention_desc g = gathered(d, pages);
-  const size_t need = s2c_paged_attention_workspace(d, pages), part = gathered_bytes(g);
+  const size_t need = s2c_paged_attention_workspace(d, pages);
   if (need > workspace_bytes || (need && !workspace)) return fail(S2C_ERR_WORKSPACE, "s2c_paged_attention: workspace too small");
-  PageGatherParams p = {};
-  p.pages = page_table(pages, keys, values);
-  char* at = static_cast<char*>(workspace);
-  for (int i = 0; i < 2; ++i) p.out[i] = at + i * part;
-  for (int i = 0; i < 3; ++i) { p.stride[0][i] = pages->key_stride[i]; p.stride[1][i] = pages->value_stride[i]; }
-  p.q_len = d->q_lengths; p.kv_len = d->kv_lengths; p.start = d->q_starts;
-  p.batch = d->batch; p.length = g.lk; p.heads = d->kv_heads; p.dim = d->dim; p.lq = d->lq; p.causal = d->causal; p.start_all = d->q_start;
-  if (d->batch > 0 && d->lq > 0) S2C_SEQ_TRY(d->dtype == kSeqF32 ? page_gather<float>(p, (stream_t)stream) : page_gather<bf16>(p, (stream_t)stream));
-  return s2c_attention(&g, q, p.out[0], p.out[1], bias, out, nullptr, at + 2 * part, workspace_bytes - 2 * part, stream);
+#ifndef S2C_EMUL
+  if (!paged_gathers(d, pages)) {
+    const AttnParams a = paged_params(d, pages, q, bias, out);
+    return d->dtype == kSeqF32 ? paged_launch<float>(a, pages, keys, values, workspace, (stream_t)stream)
+                               : paged_launch<bf16>(a, pages, keys, values, workspace, (stream_t)stream);
+  }
 #endif
+  const s2c_attention_desc g = gathered(d, pages);
+  const size_t part = gathered_bytes(g);
+  char* at = static_cast<char*>(workspace);
+  S2C_SEQ_TRY(d->dtype == kSeqF32 ? page_gather<float>(d, pages, keys, values, g.lk, at, at + part, (stream_t)stream)
+                                  : page_gather<bf16>(d, pages, keys, values, g.lk, at, at + part, (stream_t)stream));
+  return s2c_attention(&g, q, at, at + part, bias, out, nullptr, at + 2 * part, workspace_bytes - 2 * part, stream);
 }
 
 int s2c_copy_pages(void* storage, long page_stride, long page_bytes, int count, const int* source, const int* target, long n, void* stream) {

@@ -112,6 +112,9 @@ LARGE = [
     (300, 1, 70, 2, 1, 40, 16, None, {"kv_lengths": [(37 * i) % 71 for i in range(300)]}),                 # more sequences than threads, empty ones among them
     (2, 3, 3000, 5, 1, 100, 64, (16, 64), {"causal": True, "q_start": [2900, 1000], "kv_lengths": [2903, 1003], "how": "odd"}),
     (2, 40, 900, 4, 2, 64, 64, None, {"causal": True, "q_start": [860, 200], "kv_lengths": [900, 240]}),
+    (2, 70, 700, 8, 2, 64, 32, (16, 64), {"causal": True, "q_start": [600, 100], "kv_lengths": [650, 160], "q_lengths": [70, 33]}),   # one array for whole tiles
+    (1, 100, 500, 6, 2, 25, 16, None, {"kv_lengths": [333], "how": "odd"}),
+    (1, 300, 300, 2, 1, 128, 64, None, {"causal": True}),
 ]
 
 
