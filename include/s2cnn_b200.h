@@ -422,7 +422,9 @@ int s2c_norm_rotate_backward(const s2c_head_desc* desc, const void* q, const voi
 
 /* Kept keys and values in pages of one pool: keys and values [count][page][kv_heads][dim], any strides (in elements, of the first three
  * axes).  table (device int32 [batch][columns]): position j of sequence n lies in page table[n][j / page], at j % page.  page is a
- * power of two, at least 8.  An entry outside 0 .. count - 1 is no page: what would be written there is left out, and reads as NaN. */
+ * power of two, at least 8; columns * page at most 2^28, count * page below 2^31.  An entry outside 0 .. count - 1 is no page: what would
+ * be written there is left out, and reads as NaN.  Arrays need no more alignment than their type.  Where all rows start on 16-byte
+ * boundaries they are read in whole 16-byte pieces, the last one with what lies behind the row in it. */
 typedef struct s2c_page_desc {
   const int* table;
   int columns, count, page;
@@ -434,7 +436,11 @@ typedef struct s2c_page_desc {
 int s2c_norm_rotate_store(const s2c_head_desc* desc, const s2c_page_desc* pages, const void* q, const void* k, const void* v, const void* q_weight,
                           const void* k_weight, void* q_out, void* keys, void* values, void* stream);
 /* s2c_attention on keys and values in pages, without a backward pass; lk, k_stride and v_stride of the description are not used:
- * there are columns * page positions. */
+ * there are columns * page positions.  Weights are kept in float32 (bfloat16: in two parts) for up to 128 rows of queries and heads per key
+ * head, 256 in float32; more rows take the kernels of s2c_attention, on a copy of the keys and values in the workspace, where that
+ * takes no more than 1 GB.  Under `causal` a query's neighbours (16 rows of queries and heads of a key head, or as s2c_attention has it)
+ * may get what it sees that is no number, or lies in an entry that is no page, as 0 times it.  The workspace starts on a 16-byte
+ * boundary; it is needed for every call. */
 size_t s2c_paged_attention_workspace(const s2c_attention_desc* desc, const s2c_page_desc* pages);
 int s2c_paged_attention(const s2c_attention_desc* desc, const s2c_page_desc* pages, const void* q, const void* keys, const void* values,
                         const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -843,6 +843,7 @@ struct Ops {
     if (a.frequencies.defined()) {
       if (a.frequencies.scalar_type() != at::kDouble || a.frequencies.device() != any.device())
         refuse("frequencies are a float64 tensor on the device of the heads");
+      if (at::GradMode::is_enabled() && a.frequencies.requires_grad()) raise(PyExc_RuntimeError, std::string(who) + ": frequencies have no gradient");
       want(a.frequencies.dim() == 1 && 2 * a.frequencies.size(0) <= d.dim, "a frequency for each pair of values, at most dim / 2");
       a.frequencies = a.frequencies.contiguous();
       d.pairs = (int)a.frequencies.size(0);

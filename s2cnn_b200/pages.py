@@ -40,7 +40,9 @@ def _eps(eps):
 
 
 def paged_attention(q, keys, values, pages, bias=None, buckets=None, causal=False, scale=None, q_start=0, q_lengths=None, kv_lengths=None):
-    """``sequence.attention`` (its formula and its other parameters) over keys and values in pages.
+    """``sequence.attention`` (its formula and its other parameters) over keys and values in pages: for new positions, whose keys and
+    values are read once, or more (beyond 128 rows of queries and heads per key head, 256 in float32, they are first copied into
+    one array).
 
     :param q: [batch, queries, heads, dim], dim <= 128; any strides with a contiguous last axis
     :param keys, values: [pages, positions of a page, kv_heads, dim]
@@ -74,7 +76,7 @@ class PagedCache:
 
     Which page is whose is decided on the host, which knows how far each sequence has grown (``lengths``, a list); the
     kernels read ``table`` int32 [sequences, columns] and ``filled`` int32 [sequences] on the device.  These keep their addresses,
-    so that a step may be captured and replayed after ``extend``.
+    so that a step may be captured and replayed after ``extend``.  Everything runs on the current stream; nothing waits for the device.
 
     A step of a model: ``cache.extend(new)`` makes room for new positions, the layers run ``SequenceBlock.step_pages`` with
     ``cache.keys(layer)``, ``cache.values(layer)``, ``cache.table`` and ``cache.filled`` (the positions before this step), and
@@ -148,7 +150,7 @@ class PagedCache:
         if any(self._new):
             self.lengths = [a + b for a, b in zip(self.lengths, self._new)]
             self._new = [0] * len(self.lengths)
-            self.filled.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+            self.filled.copy_(torch.tensor(self.lengths, dtype=torch.int32), non_blocking=True)
 
     def fork(self, source, target):
         """Sequence ``target``, which is empty, continues from all that is filled of ``source``: its pages are shared until one of
@@ -207,7 +209,7 @@ class PagedCache:
 
     def _copy(self, moved):
         if moved:
-            which = torch.tensor(moved, dtype=torch.int32).t().contiguous().to(self.storage.device)
+            which = self._on_device(torch.tensor(moved, dtype=torch.int32).t().contiguous())
             copy_pages(self.storage, which[0], which[1])
 
     def _grown(self, s, length):
@@ -220,4 +222,7 @@ class PagedCache:
             rows = torch.full((len(sequences), self.table.size(1)), -1, dtype=torch.int32)
             for row, s in zip(rows, sequences):
                 row[:len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
-            self.table[torch.tensor(sequences, device=self.table.device)] = rows.to(self.table.device)
+            self.table[self._on_device(torch.tensor(sequences))] = self._on_device(rows)
+
+    def _on_device(self, t):
+        return t.to(self.storage.device, non_blocking=True)       # (from pageable memory: the host does not wait for the device)
