@@ -109,7 +109,7 @@ struct PagedAttention {
   static constexpr int kBlocks = (H::kHalf ? DP <= 64 || NT == 1 : DP <= 64) ? 3 : 2;      // as registers allow
   // queries, results, the search for the share; the biases of each row by bucket, 0 behind them, and the bucket of each position
   static size_t smem(const AttnParams& a) {
-    return H::kQuery + H::kJoin + 64 + (a.bias ? (size_t)H::kRows * (a.n_buckets + 1) * 4 + (size_t)(2 * a.reach + 1) * 2 : 0);
+    return H::kQuery + H::kJoin + 128 + (a.bias ? (size_t)H::kRows * (a.n_buckets + 1) * 4 + (size_t)(2 * a.reach + 1) * 2 : 0);
   }
   // (64 bits only where they are needed: a division of them is a hundred instructions)
   static __device__ __forceinline__ long quotient(long x, long y) {
@@ -126,38 +126,73 @@ struct PagedAttention {
     const int lane = ctx.tid % 32, warp = ctx.tid / 32;
     uint4* const query = reinterpret_cast<uint4*>(smem);
     float* const join = reinterpret_cast<float*>(smem + H::kQuery);
-    long* const find = reinterpret_cast<long*>(smem + H::kQuery + H::kJoin);      // [0 .. 3] the warps' sums, [4], [5] where the share begins
-    float* const biases = reinterpret_cast<float*>(smem + H::kQuery + H::kJoin + 64);
+    long* const find = reinterpret_cast<long*>(smem + H::kQuery + H::kJoin);      // the warps' sums, twice; [4], [5] where the share begins
+    float* const biases = reinterpret_cast<float*>(smem + H::kQuery + H::kJoin + 128);
     unsigned short* const bucket = reinterpret_cast<unsigned short*>(biases + H::kRows * (a.n_buckets + 1));
     const int per_batch = a.kv_heads * p.row_blocks;                              // items of a sequence
 
-    // ---- this block's share: steps [lo, hi) of all
-    const int mine = (a.batch + kThreads - 1) / kThreads;
-    long sum = 0;
-    for (int i = 0; i < mine; ++i)
-      if (ctx.tid * mine + i < a.batch) sum += paged_steps(a, ctx.tid * mine + i, H::kStep);
-    long before = sum;
+    // ---- this block's share
+    const int mine = (a.batch + kThreads - 1) / kThreads;                         // sequences of a thread
+    // the sum of `of` over the sequences before this thread's, over this thread's, and over all
+    const int n_first = ctx.tid * mine < a.batch ? paged_steps(a, ctx.tid * mine, H::kStep) : 0;
+    auto add_up = [&](auto of, long* warps, long& sum, long& all) {
+      sum = n_first ? of(n_first) : 0;
+      for (int i = 1; i < mine; ++i)
+        if (ctx.tid * mine + i < a.batch) sum += of(paged_steps(a, ctx.tid * mine + i, H::kStep));
+      long before = sum;
 #pragma unroll
-    for (int m = 1; m < 32; m *= 2) {
-      const long o = __shfl_up_sync(0xffffffffu, before, m);
-      if (lane >= m) before += o;
-    }
-    if (lane == 31) find[warp] = before;
-    ctx.sync();
-    long all = 0;
-    for (int w = 0; w < H::kWarps; ++w) {
-      if (w == warp) before += all;
-      all += find[w];
-    }
-    before -= sum;
-    const long total = all * per_batch, blocks = min((long)ctx.nblk, total);
+      for (int m = 1; m < 32; m *= 2) {
+        const long o = __shfl_up_sync(0xffffffffu, before, m);
+        if (lane >= m) before += o;
+      }
+      if (lane == 31) warps[warp] = before;
+      ctx.sync();
+      all = 0;
+      for (int w = 0; w < H::kWarps; ++w) {
+        if (w == warp) before += all;
+        all += warps[w];
+      }
+      return before - sum;
+    };
+    long sum, all;
+    long before = add_up([](int n) { return n; }, find, sum, all);
     const bool by_item = (long)a.batch * per_batch <= ctx.nblk;                   // as the host counts the splits
-    if (ctx.bid >= blocks) {
+    // Steps [lo, hi) of all, an equal share, in which an item counts kOpening steps more than it has, in front: beginning one costs about
+    // that (32 x 4000 positions of different lengths, 128 items: 22.4 us, 28.9 without; 1 and 4 steps 24.6 and 23.5).
+    constexpr int kOpening = 2;
+    int opening = kOpening;
+    const long steps = all * per_batch, total = steps + (long)a.batch * per_batch * kOpening, blocks = min((long)ctx.nblk, steps);
+    const long each = quotient(total, blocks), rest = total - each * blocks;       // the first `rest` blocks have one more
+    long lo = ctx.bid * each + min((long)ctx.bid, rest), used = blocks;
+    const long hi = lo + each + (ctx.bid < rest);
+    before += (long)min(ctx.tid * mine, a.batch) * kOpening;
+    sum += (long)max(min(mine, a.batch - ctx.tid * mine), 0) * kOpening;
+    // With few steps a block: pieces of `per` steps of one item each, where the blocks hold them (32 x 1000 positions, 128 items: 16.8 us
+    // instead of 18.2; one step a block: the same without a second sum).
+    const int per = (int)min(quotient(steps + blocks - 1, blocks), 5L);
+    bool pieces = per == 1;
+    if (per <= 4) {
+      long of_thread = sum, of_all = all, first = before;
+      if (per > 1) {
+        first = add_up([&](int n) { return (int)((unsigned)(n + per - 1) / (unsigned)per); }, find + 8, of_thread, of_all);
+        pieces = of_all * per_batch <= ctx.nblk;
+      } else {
+        of_thread -= (long)max(min(mine, a.batch - ctx.tid * mine), 0) * kOpening;
+        first -= (long)min(ctx.tid * mine, a.batch) * kOpening;
+      }
+      if (pieces) {
+        sum = of_thread;
+        before = first;
+        used = of_all * per_batch;
+        lo = ctx.bid;
+        opening = 0;
+      }
+    }
+    if (ctx.bid >= used) {
       if (!by_item && ctx.tid == 0) p.split[ctx.bid] = make_int4(0, 0, 0, 0);
       return;
     }
-    const long each = quotient(total, blocks), rest = total - each * blocks;       // the first `rest` blocks have one more
-    const long lo = ctx.bid * each + min((long)ctx.bid, rest), hi = lo + each + (ctx.bid < rest);
+    auto parts_of = [&](int n) { return pieces ? (int)((unsigned)(n + per - 1) / (unsigned)per) : n + opening; };
     if (a.bias)
       for (int e = ctx.tid; e <= 2 * a.reach; e += 4 * kThreads) {               // (four loads on their way)
         int which[4];
@@ -170,7 +205,7 @@ struct PagedAttention {
     if (before * per_batch <= lo && lo < (before + sum) * per_batch) {
       int b = ctx.tid * mine;
       for (;; ++b) {
-        const int n = paged_steps(a, b, H::kStep);
+        const int n = parts_of(paged_steps(a, b, H::kStep));
         if (lo < (before + n) * per_batch) break;
         before += n;
       }
@@ -180,27 +215,29 @@ struct PagedAttention {
     ctx.sync();
     int b = (int)find[4];
     int n = paged_steps(a, b, H::kStep);
-    int within = (int)quotient(find[5], n), s0 = (int)(find[5] - (long)within * n);
+    const int of_item = parts_of(n);
+    int within = (int)quotient(find[5], of_item), v0 = (int)(find[5] - (long)within * of_item) * (pieces ? per : 1);     // in the item, its opening counted
     bool joined = false;
-    for (long at = lo; at < hi;) {
-      const int s1 = (int)min((long)n, s0 + (hi - at));
-      const int hk = p.by_row_blocks.quotient(within), rb = within - hk * p.row_blocks, item = b * per_batch + within;
-      const bool whole = s0 == 0 && s1 == n;
-      float* part = whole ? nullptr : p.part + (2L * ctx.bid + (s0 == 0 ? 1 : 0)) * H::kRows * (DP + 4);
-      piece(ctx, p, query, join, biases, bucket, b, hk, rb, s0, s1, part);
-      if (ctx.tid == 0) {
-        if (by_item) {
-          if (whole) p.split[item] = make_int4(0, 0, 0, 0);
-        }
-        if (!whole && s0 == 0) {
-          const long end = at + n - 1, more = rest * (each + 1), last = end < more ? quotient(end, each + 1) : rest + quotient(end - more, each);
-          p.split[by_item ? item : ctx.bid] = make_int4(item, ctx.bid, (int)(last - ctx.bid) + 1, 0);
-          joined = true;
+    for (long at = lo, left = pieces ? min(per, n - v0) : hi - lo; left > 0;) {
+      const int v1 = (int)min((long)n + opening, v0 + left), s0 = max(v0 - opening, 0), s1 = max(v1 - opening, 0);
+      if (s0 < s1) {
+        const int hk = p.by_row_blocks.quotient(within), rb = within - hk * p.row_blocks, item = b * per_batch + within;
+        const bool whole = s0 == 0 && s1 == n;
+        float* part = whole ? nullptr : p.part + (2L * ctx.bid + (s0 == 0 ? 1 : 0)) * H::kRows * (DP + 4);
+        piece(ctx, p, query, join, biases, bucket, b, hk, rb, s0, s1, part);
+        if (ctx.tid == 0) {
+          if (by_item && whole) p.split[item] = make_int4(0, 0, 0, 0);
+          if (!whole && s0 == 0) {
+            const long end = at - v0 + opening + n - 1, more = rest * (each + 1), last = end < more ? quotient(end, each + 1) : rest + quotient(end - more, each);
+            p.split[by_item ? item : ctx.bid] = make_int4(item, ctx.bid, pieces ? of_item : (int)(last - ctx.bid) + 1, 0);
+            joined = true;
+          }
         }
       }
-      at += s1 - s0;
-      s0 = 0;
-      if (at < hi && ++within == per_batch) {
+      at += v1 - v0;
+      left -= v1 - v0;
+      v0 = 0;
+      if (left > 0 && ++within == per_batch) {
         within = 0;
         n = paged_steps(a, ++b, H::kStep);
       }

@@ -141,8 +141,8 @@ int paged_launch(const AttnParams& a, const s2c_page_desc* pages, const void* ke
     using Few = PagedJoin<T, DP, NT, 4>;
     using Many = PagedJoin<T, DP, NT, 1>;
     const long rows = std::min(plan.items, plan.blocks) * F::H::kRows;
-    return plan.parts <= 16 ? seq_launch<Few>("paged_join", rows / 4, Few::smem(plan.parts), st, p)
-                            : seq_launch<Many>("paged_join", rows, Many::smem(plan.parts), st, p);
+    return plan.blocks <= 16 * plan.items ? seq_launch<Few>("paged_join", rows / 4, Few::smem(plan.parts), st, p)
+                                          : seq_launch<Many>("paged_join", rows, Many::smem(plan.parts), st, p);
   });
 }
 #endif
