@@ -15,6 +15,12 @@
 // A team of 4, 8 or 16 neighbouring lanes holds a head of up to 32, 64 or 128 values, four pairs to a lane, and takes several heads of
 // one position, which share the four sines and cosines and, times the weights, the pairs' factors.  Blocks are dealt to queries, keys and
 // values, so that a lane has one weight.
+//
+// Bound by instructions and their latencies with 16 warps an SM, half of what memory would take: 4 x 4096 positions, 20 heads of 128
+// bfloat16 values, forward 37 us (4.5 TB/s), without a norm 31 (5.4); backward 53 us (4.8), and 4 for the sums of the blocks.  Two blocks
+// an SM with four heads of a turn loaded ahead (two in float32 and backward): three blocks with two heads 36.6, but 14.0 instead of 12.3
+// where the turns are few (a first pass of 4 x 2049 ragged positions, 20 heads of 64, into pages); backward with one head a turn 111
+// instead of 94 for both passes, with one and three blocks 97.
 #pragma once
 
 #include <cstring>

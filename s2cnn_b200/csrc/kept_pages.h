@@ -46,7 +46,8 @@ struct PageCopyParams {
   long n, chunks;                 // copies; pieces of kChunk bytes of each
   int count;
 };
-// P: bytes of one access.  A block copies a chunk, all of its loads before its stores.
+// P: bytes of one access.  A block copies a chunk, all of its loads before its stores.  Bound by memory: 1024 pages of 256 KB 82 us, 6.5 TB/s
+// read and written, the measured copy rate; with four loads ahead 122.
 template <int P>
 struct PageCopy {
   using Params = PageCopyParams;
