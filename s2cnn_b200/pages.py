@@ -90,7 +90,7 @@ class PagedCache:
         step = 16 // torch.empty(0, dtype=dtype).element_size()
         self.page, self.dim, self.layers = page, dim, layers
         self.storage = torch.zeros(pages, layers, 2, kv_heads, page, -(-dim // step) * step, dtype=dtype, device=device)
-        columns = pages if columns is None else columns
+        columns = min(pages, (1 << 28) // page) if columns is None else columns
         assert columns * page <= 1 << 28, "PagedCache: at most 2^28 positions in a sequence"
         self.table = torch.full((sequences, columns), -1, dtype=torch.int32, device=device)
         self.filled = torch.zeros(sequences, dtype=torch.int32, device=device)

@@ -4,6 +4,7 @@ sphere) and an answer about all of them.
 
 * ``attention`` with a learned bias by buckets of the relative position (``relative_buckets``), its output
   and its gradients computed without storing a score;
+* ``norm_rotate``: heads of queries and keys normed, and turned by their position (``rotary_frequencies``), for attention without a bias;
 * ``layer_norm`` over the last axis;
 * ``dropout`` with a counter-based mask that is never stored, optionally added to a residual;
 
@@ -107,7 +108,7 @@ def norm_rotate(q, k=None, frequencies=None, q_weight=None, k_weight=None, eps=N
     :param q, k: [batch, length, heads, dim] and [batch, length, kv_heads, dim] (None: only the other), dim <= 128; any strides with a
         contiguous last axis
     :param frequencies: float64 [pairs], radians per position, see ``rotary_frequencies``; the first 2 pairs values of a head are turned,
-        the others not (None: no value is)
+        the others not (None: no value is).  They have no gradient
     :param q_weight, k_weight: [dim], of the norm
     :param eps: x / sqrt(mean(x^2) + eps) * weight over the values of a head comes first; None: no norm
     :param positions: of the first row, a number or int32 [batch], or of each row, int32 [batch, length]
