@@ -6,8 +6,8 @@
 //   backward: g the gradient of z (the rotation by -t of that of y, times mu), h = g w:
 //   dx = rstd (h - x^ mean(h x^)),  dw = sum over all heads g x^;  rstd is computed again from x: nothing is stored
 //
-// Angles.  t of a position in the hundred thousands loses its digits in float32.  A lane keeps the frequency of each of its pairs as a
-// fraction of a turn in 64 bits of fixed point, F = round(2^64 f / 2 pi mod 2^64); position F modulo 2^64 is then the angle modulo whole
+// Angles.  t of a position in the hundred thousands loses its digits in float32.  The frequency of each pair is kept as a fraction
+// of a turn in 64 bits of fixed point, F = round(2^64 f / 2 pi mod 2^64); position F modulo 2^64 is then the angle modulo whole
 // turns by one integer product, whatever the position (also a negative one).  What is lost is f / 2 pi's own rounding, a relative
 // 2^-52, times the position.  The nearest quarter turn is taken off in integers, the rest (an eighth at most) goes through
 // the Taylor series of sine and cosine to x^9 and x^10, whose first terms left out are below 2e-9 and 2e-10 there.

@@ -24,8 +24,9 @@ def norm_rotate_store(q, k, v, keys, values, pages, frequencies=None, q_weight=N
     :param q: [batch, new, heads, dim], or None: keys and values alone
     :param k, v: [batch, new, kv_heads, dim]
     :param keys, values: [pages, positions of a page, kv_heads, dim], written in place
-    :param pages: int32 [batch, columns], the pages of each sequence.  No two sequences of a call may write to one place
-    :param positions: of the rows, as in ``norm_rotate``; they are the places among the kept ones, too
+    :param pages: int32 [batch, columns], the pages of each sequence
+    :param positions: of the rows, as in ``norm_rotate``; they are the places among the kept ones, too.  No two rows of a call may have
+        one place (it holds either then, or parts of both)
     :param lengths: int32 [batch], the rows that are filled (None: all); what is beyond them is neither read nor written
     :return: the normed and turned queries; 0 beyond ``lengths``, NaN where the position has no page.  None without q
     """

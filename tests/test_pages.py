@@ -431,6 +431,30 @@ def test_paged_cache_refusals(backend):
 
 
 @pytest.mark.parametrize("backend", backends.BACKENDS)
+def test_steps_of_nothing(backend):
+    """No new positions, no sequences, sequences of which some have none: shapes, zeros where nothing is filled, nothing written."""
+    with backends.active(backend) as (_, dev):
+        torch.manual_seed(23)
+        block = S.SequenceBlock(16, 2, causal=True, p=0.0, rotary=8).to(dev).eval()
+        cache = S.PagedCache(4, 8, 2, 8, 2, device=dev)
+        args = cache.keys(), cache.values(), cache.table, cache.filled
+        assert block.step_pages(torch.randn(2, 0, 16, device=dev), *args).shape == (2, 0, 16)
+        assert block.step_pages(torch.randn(0, 1, 16, device=dev), *args[:2], cache.table[:0], cache.filled[:0]).shape == (0, 1, 16)
+        cache.extend(0)
+        cache.advance()
+        assert cache.lengths == [0, 0] and cache.free_pages == 4 and not cache.storage.any()
+        cache.extend([0, 2])
+        x = torch.randn(2, 2, 16, device=dev)
+        out = block.step_pages(x, *args, lengths=ints([0, 2], dev))
+        cache.advance()
+        alone = block(x[1:]).detach()
+        assert torch.isfinite(out).all() and rel(out[1:], alone) <= 2e-5
+        used = cache._pages[1][0]
+        rest = [p for p in range(4) if p != used]
+        assert cache.storage[used].any() and not cache.storage[rest].any()
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
 @pytest.mark.parametrize("how", ["bias", "rotary", "rotary, head norm"])
 @pytest.mark.parametrize("page", [8, 16])
 def test_block_in_pages_agrees_with_whole_sequences(backend, how, page):
