@@ -93,11 +93,8 @@ def build(force=False, verbose=False):
     # one object per part (the kernels with many instantiations) beside lib.cu, compiled side by side
     # (nvcc's own -split-compile gave 5 % slower kernels)
     with tempfile.TemporaryDirectory(dir=LIB_DIR) as tmp:
-        jobs = [(PARTS_SRC, ["-DS2C_PART=%d" % k], os.path.join(tmp, "part%d.o" % k)) for k in range(N_PARTS)]
-        jobs.append((SRC, [], os.path.join(tmp, "lib.o")))
-        jobs.append((SEQ_SRC, [], os.path.join(tmp, "sequence.o")))
-        jobs.append((HEADS_SRC, [], os.path.join(tmp, "heads.o")))
-        jobs.append((PAGES_SRC, [], os.path.join(tmp, "pages.o")))
+        jobs = [(src, [], os.path.join(tmp, os.path.basename(src)[:-3] + ".o")) for src in (PAGES_SRC, SEQ_SRC, SRC, HEADS_SRC)]   # the longest first
+        jobs += [(PARTS_SRC, ["-DS2C_PART=%d" % k], os.path.join(tmp, "part%d.o" % k)) for k in range(N_PARTS)]
         with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
             list(pool.map(lambda j: run([nvcc] + flags + j[1] + ["-c", j[0], "-o", j[2]]), jobs))
         out = os.path.join(tmp, "lib.so")
