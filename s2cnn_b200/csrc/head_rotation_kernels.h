@@ -235,9 +235,10 @@ struct HeadTeam {
     float2 sum[NP];
 #pragma unroll
     for (int e = 0; e < NP; ++e) sum[e] = fma2(b[e], y[e], mul2(a[e], x[e]));
-    if constexpr (kPieces) {      // pieces behind the head
-      const float m = at[0][0] >= 0 ? 1.f : 0.f, n = kNext ? (at[1][0] >= 0 ? 1.f : 0.f) : m;
-      return lanes_sum<LANES>(ctx, fmaf(m, sum[0].x + sum[0].y, n * (sum[1].x + sum[1].y)));
+    if constexpr (kPieces) {      // without the pieces behind the head (by selection: a factor of 0 would make NaN of what overflows there)
+      const bool in = at[0][0] >= 0;
+      const float first = sum[0].x + sum[0].y, second = sum[1].x + sum[1].y;
+      return lanes_sum<LANES>(ctx, (in ? first : 0.f) + ((kNext ? at[1][0] >= 0 : in) ? second : 0.f));
     } else {
       float s = sum[0].x + sum[0].y;
 #pragma unroll

@@ -110,7 +110,8 @@ def norm_rotate(q, k=None, frequencies=None, q_weight=None, k_weight=None, eps=N
     :param frequencies: float64 [pairs], radians per position, see ``rotary_frequencies``; the first 2 pairs values of a head are turned,
         the others not (None: no value is).  They have no gradient
     :param q_weight, k_weight: [dim], of the norm
-    :param eps: x / sqrt(mean(x^2) + eps) * weight over the values of a head comes first; None: no norm
+    :param eps: x / sqrt(mean(x^2) + eps) * weight over the values of a head comes first (zeros where the sum of squares is beyond float32: values
+        from some 1e19 on); None: no norm
     :param positions: of the first row, a number or int32 [batch], or of each row, int32 [batch, length]
     :param interleaved: pairs are neighbours (2 i, 2 i + 1) instead of halves (i, i + pairs)
     :param magnitude: a factor of what is turned
