@@ -396,8 +396,8 @@ int s2c_dropout_numbers(int dtype, const void* x, const void* residual, void* ou
  *   y_a = magnitude (z_a cos t - z_b sin t),  y_b = magnitude (z_a sin t + z_b cos t),  t = position * frequencies[pair]
  * for the pairs (a, b) = (i, i + pairs), or (2 i, 2 i + 1) where interleaved != 0, i < pairs; the values from 2 pairs on are not
  * turned.  frequencies: device float64 [pairs], radians per position; angles are computed modulo whole turns in 64 bits, so that far
- * positions lose nothing.  The position of row i of batch entry n is start + i, positions[n] + i, or, where each != 0,
- * positions[n * length + i] (device int32).  Arrays need no more alignment than their type. */
+ * positions lose nothing; a frequency that is infinite or NaN makes its pair NaN.  The position of row i of batch entry n is start + i,
+ * positions[n] + i, or, where each != 0, positions[n * length + i] (device int32).  Arrays need no more alignment than their type. */
 typedef struct s2c_head_desc {
   int dtype, batch, length, heads, kv_heads, dim;
   long q_stride[3], k_stride[3], v_stride[3];      /* batch entry, position, head */

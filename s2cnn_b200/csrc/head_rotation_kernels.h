@@ -57,7 +57,7 @@ struct HeadParams {
 // f in radians per position as a fraction of a turn, in units of 2^-64
 S2C_D unsigned long long turn_units(double f) {
   double t = f * 0.15915494309189533577;
-  t -= floor(t);                                             // [0, 1); NaN and infinities: a frequency of 0
+  t -= floor(t);                                             // [0, 1), or 1 by rounding; NaN and infinities: the magnitude tells
   return t >= 0. && t < 1. ? (unsigned long long)(t * 18446744073709551616.) : 0ull;
 }
 // cosine and sine of `turns`, in units of 2^-64
@@ -201,6 +201,7 @@ struct HeadTeam {
   struct Shared {
     HeadKind kind;
     float w[2][kPairs][LANES];    // weights of the first and second values of a lane's pairs
+    float mu[kPairs][LANES];      // magnitudes: 1 where nothing is turned, NaN where the frequency is no number
     unsigned long long f[kPairs][LANES];      // frequencies
   };
   // FORWARD: the magnitude goes with the weights; otherwise with sines and cosines
@@ -208,25 +209,31 @@ struct HeadTeam {
   static S2C_D void share(const Ctx& ctx, const HeadParams& p, const HeadKind& kind, Shared* to) {
     if (ctx.tid < LANES * kPairs) {
       const int lane = ctx.tid % LANES, e = ctx.tid / LANES, i = pair(lane, e);
+      const double f = kind.turn && i < p.pairs ? p.frequencies[i] : 0.;
+      const float mu = f - f != 0. ? as_float(0x7fffffffu) : i < p.pairs ? p.magnitude : 1.f;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int c = place(p, i, k);
-        to->w[k][e][lane] = (kind.w && c >= 0 ? widen(static_cast<const T*>(kind.w)[c]) : 1.f) * (i < p.pairs && FORWARD ? p.magnitude : 1.f);
+        to->w[k][e][lane] = (kind.w && c >= 0 ? widen(static_cast<const T*>(kind.w)[c]) : 1.f) * (FORWARD ? mu : 1.f);
       }
-      to->f[e][lane] = kind.turn && i < p.pairs ? turn_units(p.frequencies[i]) : 0ull;
+      to->mu[e][lane] = mu;
+      to->f[e][lane] = turn_units(f);
     }
     if (ctx.tid == ctx.nthr - 1) to->kind = kind;
     ctx.sync();
   }
   // cosines and sines of the pairs; of what is not turned 1 and 0
   template <bool FORWARD>
-  S2C_D void angles(const HeadParams& p, const Shared* s, long position, float2 (&c)[NP], float2 (&si)[NP]) const {
+  S2C_D void angles(const Shared* s, long position, float2 (&c)[NP], float2 (&si)[NP]) const {
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
       turn_cos_sin(s->f[2 * e][t] * (unsigned long long)position, c[e].x, si[e].x);
       turn_cos_sin(s->f[2 * e + 1][t] * (unsigned long long)position, c[e].y, si[e].y);
-      if (!FORWARD && (turned >> 2 * e & 1)) c[e].x *= p.magnitude, si[e].x *= p.magnitude;
-      if (!FORWARD && (turned >> 2 * e & 2)) c[e].y *= p.magnitude, si[e].y *= p.magnitude;
+      if (!FORWARD) {
+        const float2 mu = make_float2(s->mu[2 * e][t], s->mu[2 * e + 1][t]);
+        c[e] = mul2(c[e], mu);
+        si[e] = mul2(si[e], mu);
+      }
     }
   }
   S2C_D float2 weights(const Shared* s, int k, int e) const { return make_float2(s->w[k][2 * e][t], s->w[k][2 * e + 1][t]); }
@@ -325,7 +332,7 @@ struct HeadForward {
       float2 k0[NP], k1[NP], k2[NP], k3[NP];
       if (turn && work) {
         float2 c[NP], s[NP];
-        team.template angles<true>(p, shared, now.at, c, s);
+        team.template angles<true>(shared, now.at, c, s);
 #pragma unroll
         for (int e = 0; e < NP; ++e) {
           const float2 x = team.weights(shared, 0, e), z = team.weights(shared, 1, e);
@@ -420,7 +427,7 @@ struct HeadBackward {
     for (int e = 0; e < NP; ++e) da[e] = db[e] = make_float2(0.f, 0.f);
     for (; u0 < units; u0 += per) {
       float2 c[NP], s[NP], w[2][NP];
-      team.template angles<false>(p, shared, now.at, c, s);
+      team.template angles<false>(shared, now.at, c, s);
 #pragma unroll
       for (int e = 0; e < NP; ++e) {
         w[0][e] = team.weights(shared, 0, e);

@@ -108,7 +108,7 @@ def norm_rotate(q, k=None, frequencies=None, q_weight=None, k_weight=None, eps=N
     :param q, k: [batch, length, heads, dim] and [batch, length, kv_heads, dim] (None: only the other), dim <= 128; any strides with a
         contiguous last axis
     :param frequencies: float64 [pairs], radians per position, see ``rotary_frequencies``; the first 2 pairs values of a head are turned,
-        the others not (None: no value is).  They have no gradient
+        the others not (None: no value is).  They have no gradient; one that is infinite or NaN makes its pair NaN
     :param q_weight, k_weight: [dim], of the norm
     :param eps: x / sqrt(mean(x^2) + eps) * weight over the values of a head comes first (zeros where the sum of squares is beyond float32: values
         from some 1e19 on); None: no norm

@@ -42,3 +42,37 @@ def test_squares_that_overflow(backend, dtype, shape):
         for a, b in zip(grads[0][:2], grads[1][:2]):
             assert not a[zeros].any() and torch.equal(a[~zeros], b[~zeros])
         assert torch.equal(grads[0][2], grads[1][2])
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(24, 8, False), (64, 64, False), (20, 8, True), (25, 24, True)], ids=str)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_frequencies_that_are_no_numbers(backend, dtype, shape, bad):
+    """Their pair is NaN at every position (an infinity times position 0 is, too), in the gradient as well; other pairs are as they were."""
+    with backends.active(backend) as (_, dev):
+        D, turned, interleaved = shape
+        gen = torch.Generator().manual_seed(61)
+        f, w = S.rotary_frequencies(turned, device=dev), normal(gen, dev, dtype, D, scale=0.3, shift=1.0).requires_grad_(True)
+        wrong, pair = f.clone(), turned // 4
+        wrong[pair] = bad
+        at = torch.zeros(D, dtype=torch.bool, device=dev)
+        at[[2 * pair, 2 * pair + 1] if interleaved else [pair, pair + turned // 2]] = True
+        q, g = normal(gen, dev, dtype, 2, 3, 3, D).requires_grad_(True), normal(gen, dev, dtype, 2, 3, 3, D)
+        for eps in (None, 1e-6):
+            for positions in (0, -4):
+                results = []
+                for x in (f, wrong):
+                    y, _ = S.norm_rotate(q, None, x, None if eps is None else w, eps=eps, positions=positions, interleaved=interleaved)
+                    results.append((y.detach(),) + torch.autograd.grad(y, (q,) if eps is None else (q, w), g))
+                for n, (fine, out) in enumerate(zip(*results)):
+                    if n == 1 and eps is not None:            # through the norm a pair reaches the whole head
+                        assert out.isnan().all()
+                    else:
+                        assert out[..., at].isnan().all() and torch.equal(out[..., ~at], fine[..., ~at])
+        keys, values = (torch.zeros(1, 8, 3, D, dtype=dtype, device=dev) for _ in range(2))
+        with torch.no_grad():
+            out = S.norm_rotate_store(q[:1], q[:1], q[:1], keys, values, torch.zeros(1, 1, dtype=torch.int32, device=dev), wrong, interleaved=interleaved)
+        for t in (out[0], keys[0, :3]):
+            assert t[..., at].isnan().all() and torch.isfinite(t[..., ~at]).all()
+        assert torch.equal(values[0, :3], q[0])
