@@ -198,9 +198,9 @@ struct HeadTeam {
   }
   // What is the same for all teams of a block, in shared memory: a unit's sines and cosines are made from it, and a lane's registers
   // are for heads (with it in registers, and the kind of heads, 110 were taken before the first head).
-  struct Shared {
+  struct alignas(16) Shared {
+    float w[2][kPairs][LANES];    // weights of the first and second values of a lane's pairs (as long as a head, or longer)
     HeadKind kind;
-    float w[2][kPairs][LANES];    // weights of the first and second values of a lane's pairs
     float mu[kPairs][LANES];      // magnitudes: 1 where nothing is turned, NaN where the frequency is no number
     unsigned long long f[kPairs][LANES];      // frequencies
   };
@@ -295,7 +295,7 @@ struct HeadForward {
     // values that are not turned: an infinity times a sine of 0 would be none (in a norm's head nothing is left of it)
     const bool rest = 2 * p.pairs < p.dim && !p.norm, turn = kind.turn;
     const int span = kind.span;
-    const long step = kind.stride[2];
+    long step = kind.stride[2];
     Raw raw[GROUP];
     auto fetch = [&](const T* x, int left) {            // (beyond the last head: the first of the group again)
 #pragma unroll
@@ -312,6 +312,9 @@ struct HeadForward {
         next_filled = !p.lengths || now.i < p.lengths[now.b];
         next_work = ctx.warp_any(next_filled && now.on);
         if (next_work) next_page = p.pages.of(now.b, now.at);
+        // A row that is not filled need not be there: what is read in its place lies in shared memory.
+        step = next_filled && now.on ? kind.stride[2] : 0;
+        if (!(next_filled && now.on)) now.x = reinterpret_cast<const T*>(shared->w);
       }
       if (next_work) fetch(now.x, now.left);
     };

@@ -76,3 +76,69 @@ def test_frequencies_that_are_no_numbers(backend, dtype, shape, bad):
         for t in (out[0], keys[0, :3]):
             assert t[..., at].isnan().all() and torch.isfinite(t[..., ~at]).all()
         assert torch.equal(values[0, :3], q[0])
+
+
+# Rows behind `lengths` that are not there: q, k and v end where memory that may not be read begins.  Run in a process of its own, on the CPU.
+_ENDS = """
+import ctypes, mmap, sys
+import torch
+import backends, emul
+import s2cnn_b200 as S
+from test_pages import ints, pool, shuffled
+from test_pages_calls import head_desc, page_desc
+import s2cnn_b200.ops as ops_mod
+ops_mod._cuda_ops = ops = emul.ops()
+libc = ctypes.CDLL(None, use_errno=True)
+D, dtype, interleaved = int(sys.argv[1]), getattr(torch, sys.argv[2]), sys.argv[3] == "True"
+H, Hk, B, new, half = 12, 5, 3, 4, 1 << 16
+size = torch.empty(0, dtype=dtype).element_size()
+gen = torch.Generator().manual_seed(62)
+f = S.rotary_frequencies(D // 4 * 2)
+pages = shuffled(gen, "cpu", 8, B, 2)
+# the filled rows of the middle sequence end where the closed part begins; those of the first one would lie in it altogether
+lengths = ints([0, 2, 0], "cpu")
+for backwards in (False, True):
+    want, at = {}, {}
+    for name, n in (("q", H), ("k", Hk), ("v", Hk)):
+        room = mmap.mmap(-1, 2 * half)
+        base = ctypes.addressof(ctypes.c_char.from_buffer(room))
+        assert libc.mprotect(ctypes.c_void_p(base + half), half, 0) == 0
+        rows = torch.randn(2, n, D, generator=gen).to(dtype)
+        data = rows.flatten().view(torch.uint8).numpy().tobytes()
+        ctypes.memmove(base + half - len(data), data, len(data))
+        want[name], at[name] = rows, (room, base + half - len(data))
+    q, k, v = (torch.zeros(B, new, n, D, dtype=dtype) for n in (H, Hk, Hk))
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        t[1, :2] = want[name]
+    results = []
+    for there in (True, False):
+        keys, values = pool(torch.Generator().manual_seed(63), "cpu", dtype, 8, 8, Hk, D)
+        d = head_desc(q, k, v, f, norm=1, eps=1e-6, start=3, interleaved=int(interleaved), lengths=lengths.data_ptr())
+        out = torch.full((B, new, H, D), 5.0, dtype=dtype)
+        pointers = [t.data_ptr() for t in (q, k, v)]
+        if not there:
+            # sequence 1 lies at the end of what may be read, its unfilled rows, and sequences 0 and 2 (also before it: backwards), behind
+            for name, n in (("q", H), ("k", Hk), ("v", Hk)):
+                step = 4 * n * D
+                getattr(d, name + "_stride")[0] = -step if backwards else 0
+            pointers = [at[n][1] + (4 * w * D * size if backwards else 0) for n, w in (("q", H), ("k", Hk), ("v", Hk))]
+        pd = page_desc(keys, values, pages)
+        ops.lib.call("s2c_norm_rotate_store", ctypes.byref(d), ctypes.byref(pd), *pointers, None, None, out.data_ptr(), keys.data_ptr(), values.data_ptr(), None)
+        results.append((out, keys, values))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert not results[1][0][0].any() and not results[1][0][1, 2:].any() and results[1][0][1, :2].any()
+print("done")
+"""
+
+
+@pytest.mark.parametrize("case", [(24, "float32", False), (128, "bfloat16", False), (20, "float32", True), (25, "bfloat16", True), (80, "float32", False)], ids=str)
+def test_rows_that_are_not_there(case):
+    import os
+    import subprocess
+    import sys
+    import emul
+    emul.build()
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", _ENDS] + [str(x) for x in case], cwd=here, env=dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(here)))),
+                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert done.returncode == 0 and "done" in done.stdout, done.stdout
