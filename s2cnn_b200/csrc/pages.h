@@ -28,6 +28,22 @@ inline s2c_attention_desc gathered(const s2c_attention_desc* d, const s2c_page_d
 inline size_t gathered_bytes(const s2c_attention_desc& g) {
   return page_align((size_t)g.batch * g.lk * g.kv_heads * g.dim * (g.dtype == kSeqF32 ? 4 : 2));
 }
+// The workspace of `n` sequences: gathered keys and values, and what the call on them wants (packed copies of them, in float32 and for heads
+// that are no whole pieces: 1.5 times as much again, and as much).
+inline size_t gathered_need(const s2c_attention_desc* d, const s2c_page_desc* pages, long n) {
+  s2c_attention_desc g = gathered(d, pages);
+  g.batch = (int)n;
+  return 2 * gathered_bytes(g) + s2c_attention_workspace(&g);
+}
+// How many sequences are brought into one array at a time: all, or equal groups that need at most 1 GB (or single sequences).
+constexpr size_t kGatherMost = 1ul << 30;
+inline long gathered_at_once(const s2c_attention_desc* d, const s2c_page_desc* pages) {
+  long n = std::max(1, d->batch);
+  if (gathered_need(d, pages, 1) > kGatherMost) return 1;
+  for (size_t need; n > 1 && (need = gathered_need(d, pages, n)) > kGatherMost;) n = std::max(1L, std::min(n - 1, (long)((double)n * (double)kGatherMost / (double)need)));
+  const long groups = (std::max(1, d->batch) + n - 1) / n;
+  return (std::max(1, d->batch) + groups - 1) / groups;
+}
 template <class T>
 int page_gather(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* keys, const void* values, int length, void* k, void* v, stream_t st) {
   PageGatherParams p = {};
@@ -63,10 +79,11 @@ inline AttnParams paged_params(const s2c_attention_desc* d, const s2c_page_desc*
 }
 // Many queries: keys and values are brought into one array for the kernels of whole tiles, instead of being read again by every 16 rows.
 // 4 x 4096 positions, 4 key heads of 128, 32, 128, 256 and 512 rows for each: in pages 23, 56, 95 and 174 us (float32 45, 127, 224 and
-// 427), in one array 48 to 49 (253 to 259) and some 11 (17) to bring them there.  Not where that takes more than 1 GB of workspace.
+// 427), in one array 48 to 49 (253 to 259) and some 11 (17) to bring them there.  Not where one sequence alone takes more than 1 GB of
+// workspace: by its columns, since what is kept of them only the device knows.
 inline bool paged_gathers(const s2c_attention_desc* d, const s2c_page_desc* pages) {
   const long rows = (long)d->lq * (d->heads / d->kv_heads);
-  return rows > (d->dtype == kSeqF32 ? 256 : 128) && 2 * gathered_bytes(gathered(d, pages)) <= (1ul << 30);
+  return rows > (d->dtype == kSeqF32 ? 256 : 128) && gathered_need(d, pages, 1) <= kGatherMost;
 }
 // rows of 16-byte pieces (of four values at least): keys and values as they lie
 template <class T>
@@ -161,8 +178,8 @@ size_t s2c_paged_attention_workspace(const s2c_attention_desc* d, const s2c_page
     return d->dtype == kSeqF32 ? paged_plan<float>(a).bytes : paged_plan<bf16>(a).bytes;
   }
 #endif
-  const s2c_attention_desc g = gathered(d, pages);
-  return 2 * gathered_bytes(g) + s2c_attention_workspace(&g);
+  const long n = gathered_at_once(d, pages), rest = d->batch % n;
+  return std::max(gathered_need(d, pages, n), rest ? gathered_need(d, pages, rest) : 0);
 }
 
 int s2c_paged_attention(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* q, const void* keys, const void* values, const void* bias,
@@ -182,12 +199,22 @@ int s2c_paged_attention(const s2c_attention_desc* d, const s2c_page_desc* pages,
                                : paged_launch<bf16>(a, pages, keys, values, workspace, (stream_t)stream);
   }
 #endif
-  const s2c_attention_desc g = gathered(d, pages);
-  const size_t part = gathered_bytes(g);
-  char* at = static_cast<char*>(workspace);
-  S2C_SEQ_TRY(d->dtype == kSeqF32 ? page_gather<float>(d, pages, keys, values, g.lk, at, at + part, (stream_t)stream)
-                                  : page_gather<bf16>(d, pages, keys, values, g.lk, at, at + part, (stream_t)stream));
-  return s2c_attention(&g, q, at, at + part, bias, out, nullptr, at + 2 * part, workspace_bytes - 2 * part, stream);
+  const long at_once = gathered_at_once(d, pages), size = d->dtype == kSeqF32 ? 4 : 2;
+  for (long b = 0; b < d->batch; b += at_once) {
+    s2c_attention_desc g = gathered(d, pages);
+    s2c_page_desc some = *pages;
+    g.batch = (int)std::min(at_once, d->batch - b);
+    some.table += b * pages->columns;
+    for (const int** of : {&g.q_starts, &g.q_lengths, &g.kv_lengths})
+      if (*of) *of += b;
+    const size_t part = gathered_bytes(g);
+    char* at = static_cast<char*>(workspace);
+    S2C_SEQ_TRY(d->dtype == kSeqF32 ? page_gather<float>(&g, &some, keys, values, g.lk, at, at + part, (stream_t)stream)
+                                    : page_gather<bf16>(&g, &some, keys, values, g.lk, at, at + part, (stream_t)stream));
+    S2C_SEQ_TRY(s2c_attention(&g, static_cast<const char*>(q) + b * d->q_stride[0] * size, at, at + part, bias,
+                              static_cast<char*>(out) + b * d->lq * d->heads * d->dim * size, nullptr, at + 2 * part, workspace_bytes - 2 * part, stream));
+  }
+  return S2C_OK;
 }
 
 int s2c_copy_pages(void* storage, long page_stride, long page_bytes, int count, const int* source, const int* target, long n, void* stream) {

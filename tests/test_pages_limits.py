@@ -2,6 +2,7 @@
 
 Tolerances: as in test_norm_rotate.py and test_pages.py; what is compared without one is bits.
 """
+import ctypes
 import math
 
 import pytest
@@ -10,6 +11,9 @@ import torch
 import backends
 import s2cnn_b200 as S
 from test_norm_rotate import normal
+from test_pages import gathered, ints, pool, shuffled
+from test_pages_calls import attention_desc, page_desc
+from test_sequence_ops import TOL, exact_attention, rel
 
 F32, BF16 = torch.float32, torch.bfloat16
 
@@ -142,3 +146,48 @@ def test_rows_that_are_not_there(case):
     done = subprocess.run([sys.executable, "-c", _ENDS] + [str(x) for x in case], cwd=here, env=dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(here)))),
                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     assert done.returncode == 0 and "done" in done.stdout, done.stdout
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_workspace_of_many_queries(backend, dtype):
+    """At most 1 GB where one sequence's columns need no more, and it grows with the sequences until then."""
+    with backends.active(backend) as (ops, dev):
+        q, keys = torch.zeros(1, 1, 1, 1, dtype=dtype, device=dev), torch.zeros(2, 64, 1, 1, dtype=dtype, device=dev)
+        pages = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+        for Hk, D in ((4, 128), (1, 64), (3, 25)):
+            for columns in (1, 40, 1000, 2500):
+                sizes = []
+                for batch in (1, 2, 3, 8, 9, 50, 1000, 100000):
+                    d = attention_desc(q, keys, batch=batch, lq=300, heads=2 * Hk, kv_heads=Hk, dim=D, q_stride=(ctypes.c_long * 3)(600 * Hk * D, 2 * Hk * D, D))
+                    p = page_desc(keys, keys, pages, columns=columns)
+                    sizes.append(ops.lib.s2c_paged_attention_workspace(ctypes.byref(d), ctypes.byref(p)))
+                assert 0 < min(sizes) and max(sizes) <= 1 << 30, (Hk, D, columns, sizes)
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_queries_over_wide_tables(backend, dtype):
+    """Columns that nobody has filled, 2^18 positions for each of five sequences: what a table of seven columns gives to the type's exactness, and
+    to the bit the calls on single sequences (which are what 1 GB of workspace holds)."""
+    with backends.active(backend) as (_, dev):
+        gen = torch.Generator().manual_seed(64)
+        B, lq, H, Hk, D, page, columns = 5, 70, 8, 2 if dtype == F32 else 4, 128, 128, 2048
+        keys, values = pool(gen, dev, dtype, 7 * B + 1, page, Hk, D)
+        narrow = shuffled(gen, dev, 7 * B, B, 7)
+        pages = torch.full((B, columns), -1, dtype=torch.int32, device=dev)
+        pages[:, :7] = narrow
+        q = normal(gen, dev, dtype, B, lq, H, D)
+        table, buckets = normal(gen, dev, dtype, 16, H), S.relative_buckets(16, 30, device=dev)
+        kept = [800, 0, 1, 333, 100]
+        kw = {"causal": True, "q_start": ints([730, 5, 0, 263, 60], dev), "q_lengths": ints([70, 70, 1, 70, 40], dev), "kv_lengths": ints(kept, dev)}
+        out = S.paged_attention(q, keys, values, pages, table, buckets, **kw)
+        k, v = gathered(keys, narrow), gathered(values, narrow)
+        assert rel(out, exact_attention(q, k, v, table, buckets, **kw)[0]) <= TOL[dtype]
+        assert rel(S.paged_attention(q, keys, values, narrow, table, buckets, **kw), out) <= 2 * TOL[dtype]
+        for b in range(B):
+            one = {n: t if n == "causal" else t[b:b + 1] for n, t in kw.items()}
+            assert torch.equal(out[b:b + 1], S.paged_attention(q[b:b + 1], keys, values, pages[b:b + 1], table, buckets, **one))
