@@ -169,13 +169,16 @@ def test_workspace_of_many_queries(backend, dtype):
 
 
 @pytest.mark.parametrize("backend", backends.BACKENDS)
-@pytest.mark.parametrize("dtype", [F32, BF16])
-def test_many_queries_over_wide_tables(backend, dtype):
-    """Columns that nobody has filled, 2^18 positions for each of five sequences: what a table of seven columns gives to the type's exactness, and
-    to the bit the calls on single sequences (which are what 1 GB of workspace holds)."""
+@pytest.mark.parametrize("dtype, Hk", [(F32, 1), (F32, 2), (BF16, 4)])
+def test_many_queries_over_wide_tables(backend, dtype, Hk):
+    """Columns that nobody has filled, 2^18 positions for each of five sequences: what a table of seven columns gives to the type's exactness.  A
+    position takes 2 x 2 bytes of workspace for each value in bfloat16, and 2 x (4 + 6), packed copies counted, in float32: one sequence
+    2^18 x 4 x 128 x 4 = 5.4e8 bytes in bfloat16, and 2^18 x 128 x 20 = 6.7e8 in float32 with one key head, so that groups are single
+    sequences and the calls on these give the same bits.  With two key heads it is 1.3e9, more than 2^30: all rows go over the pages, with shares
+    of the work that depend on the batch."""
     with backends.active(backend) as (_, dev):
         gen = torch.Generator().manual_seed(64)
-        B, lq, H, Hk, D, page, columns = 5, 70, 8, 2 if dtype == F32 else 4, 128, 128, 2048
+        B, lq, H, D, page, columns = 5, 70, 8, 128, 128, 2048
         keys, values = pool(gen, dev, dtype, 7 * B + 1, page, Hk, D)
         narrow = shuffled(gen, dev, 7 * B, B, 7)
         pages = torch.full((B, columns), -1, dtype=torch.int32, device=dev)
@@ -190,4 +193,5 @@ def test_many_queries_over_wide_tables(backend, dtype):
         assert rel(S.paged_attention(q, keys, values, narrow, table, buckets, **kw), out) <= 2 * TOL[dtype]
         for b in range(B):
             one = {n: t if n == "causal" else t[b:b + 1] for n, t in kw.items()}
-            assert torch.equal(out[b:b + 1], S.paged_attention(q[b:b + 1], keys, values, pages[b:b + 1], table, buckets, **one))
+            alone = S.paged_attention(q[b:b + 1], keys, values, pages[b:b + 1], table, buckets, **one)
+            assert torch.equal(out[b:b + 1], alone) if Hk != 2 else rel(out[b:b + 1], alone) <= 2 * TOL[dtype]
