@@ -438,10 +438,12 @@ int s2c_norm_rotate_store(const s2c_head_desc* desc, const s2c_page_desc* pages,
 /* s2c_attention on keys and values in pages, without a backward pass; lk, k_stride and v_stride of the description are not used:
  * there are columns * page positions.  Weights are kept in float32 (bfloat16: in two parts) for up to 128 rows of queries and heads per key
  * head, 256 in float32; more rows take the kernels of s2c_attention (bfloat16: with weights rounded to it), on a copy of the keys and
- * values in the workspace, for as many sequences at a time as 1 GB of workspace holds.  That is counted by the columns, whatever is kept;
- * where one sequence needs more, many rows take the first way, which reads the keys and values again for every 16.  Under `causal` a query's neighbours (16 rows of queries and heads of a key head, or as s2c_attention has it)
- * may get what it sees that is no number, or lies in an entry that is no page, as 0 times it.  The workspace starts on a 16-byte
- * boundary; it is needed for every call. */
+ * values in the workspace, for as many sequences at a time as 1 GB holds (packed copies for the tensor cores come on top: in float32
+ * 1.5 times as much, and of the queries; in bfloat16 as much where heads are no multiple of 8 values).  That is counted by the columns,
+ * whatever is kept; where one sequence takes more, or the sequences that fit have too few tiles of queries for the device, many rows take the
+ * first way, which reads the keys and values again for every 16.  Under `causal` a query's neighbours (16 rows of queries and heads of a
+ * key head, or as s2c_attention has it) may get what it sees that is no number, or lies in an entry that is no page, as 0 times it.  The
+ * workspace starts on a 16-byte boundary; it is needed for every call. */
 size_t s2c_paged_attention_workspace(const s2c_attention_desc* desc, const s2c_page_desc* pages);
 int s2c_paged_attention(const s2c_attention_desc* desc, const s2c_page_desc* pages, const void* q, const void* keys, const void* values,
                         const void* bias, void* out, void* workspace, size_t workspace_bytes, void* stream);

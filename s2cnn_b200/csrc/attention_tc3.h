@@ -36,8 +36,8 @@ struct AttnPack {
   static constexpr int kThreads = 256, kBlocks = 4;
   static __device__ __forceinline__ void run(const Ctx& ctx, const Params& p, unsigned char*) {
     const int t = ctx.bid % p.tensors;                                     // a block has one of the tensors
-    const long pieces = (long)p.batch * p.len[t] * p.heads[t] * p.chunks;
-    for (long e = (long)(ctx.bid / p.tensors) * kThreads + ctx.tid; e < pieces; e += (long)(ctx.nblk / p.tensors) * kThreads) {
+    const long per_entry = (long)p.len[t] * p.heads[t] * p.chunks, pieces = p.batch * per_entry, step = (long)(ctx.nblk / p.tensors) * kThreads;
+    for (long e = (long)(ctx.bid / p.tensors) * kThreads + ctx.tid; e < pieces; e += step) {
       // in the order of memory of the usual [batch][position][head] input
       const int c = (int)(e % p.chunks);
       long r = e / p.chunks;
@@ -45,7 +45,10 @@ struct AttnPack {
       r /= p.heads[t];
       const int i = (int)(r % p.len[t]), b = (int)(r / p.len[t]);
       const AttnSeq s = attn_seq(p.a, b);
-      if (i >= (t == 0 || t == 3 ? s.qlen : attn_keys(p.a, s, s.qlen))) continue;
+      if (i >= (t == 0 || t == 3 ? s.qlen : attn_keys(p.a, s, s.qlen))) {   // nor is what follows of this batch entry: its last turn
+        e += ((b + 1) * per_entry - 1 - e) / step * step;
+        continue;
+      }
       const T* from = static_cast<const T*>(p.src[t]) + b * p.stride[t][0] + i * p.stride[t][1] + h * p.stride[t][2] + 8 * c;
       bf16* to = p.dst[t] + (((long)b * p.heads[t] + h) * p.len[t] + i) * 8 * p.chunks + 8 * c;
       float v[8];

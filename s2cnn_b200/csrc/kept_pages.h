@@ -105,8 +105,10 @@ struct PageGather {
     std::memcpy(&none, nan, sizeof(none));
     for (long r = (long)ctx.bid * (kThreads / 32) + ctx.tid / 32; r < rows; r += warps) {
       const int b = (int)p.by_length.quotient((unsigned)r), j = (int)(r - (long)b * p.length);
-      if (p.kv_len && j >= p.kv_len[b]) continue;
-      if (p.causal && j > (long)(p.start ? p.start[b] : p.start_all) + (p.q_len ? p.q_len[b] : p.lq) - 1) continue;
+      if ((p.kv_len && j >= p.kv_len[b]) || (p.causal && j > (long)(p.start ? p.start[b] : p.start_all) + (p.q_len ? p.q_len[b] : p.lq) - 1)) {
+        r += (unsigned)(p.length - 1 - j) / (unsigned)warps * warps;       // nor is what follows of this sequence: its last turn
+        continue;
+      }
       const int page = p.pages.of(b, j), at = j & (p.pages.page - 1);
 #pragma unroll
       for (int which = 0; which < 2; ++which) {

@@ -28,21 +28,21 @@ inline s2c_attention_desc gathered(const s2c_attention_desc* d, const s2c_page_d
 inline size_t gathered_bytes(const s2c_attention_desc& g) {
   return page_align((size_t)g.batch * g.lk * g.kv_heads * g.dim * (g.dtype == kSeqF32 ? 4 : 2));
 }
-// The workspace of `n` sequences: gathered keys and values, and what the call on them wants (packed copies of them, in float32 and for heads
-// that are no whole pieces: 1.5 times as much again, and as much).
+// How many sequences are brought into one array at a time: all, or equal groups whose keys and values take at most 1 GB; 0: one takes more.
+constexpr size_t kGatherMost = 1ul << 30;
+inline long gathered_at_once(const s2c_attention_desc* d, const s2c_page_desc* pages) {
+  s2c_attention_desc g = gathered(d, pages);
+  g.batch = 1;
+  const size_t one = 2 * gathered_bytes(g);
+  if (one > kGatherMost) return 0;
+  const long batch = std::max(1, d->batch), n = one ? std::min(batch, (long)(kGatherMost / one)) : batch, groups = (batch + n - 1) / n;
+  return (batch + groups - 1) / groups;
+}
+// their workspace: gathered keys and values, and what the call on them wants
 inline size_t gathered_need(const s2c_attention_desc* d, const s2c_page_desc* pages, long n) {
   s2c_attention_desc g = gathered(d, pages);
   g.batch = (int)n;
   return 2 * gathered_bytes(g) + s2c_attention_workspace(&g);
-}
-// How many sequences are brought into one array at a time: all, or equal groups that need at most 1 GB (or single sequences).
-constexpr size_t kGatherMost = 1ul << 30;
-inline long gathered_at_once(const s2c_attention_desc* d, const s2c_page_desc* pages) {
-  long n = std::max(1, d->batch);
-  if (gathered_need(d, pages, 1) > kGatherMost) return 1;
-  for (size_t need; n > 1 && (need = gathered_need(d, pages, n)) > kGatherMost;) n = std::max(1L, std::min(n - 1, (long)((double)n * (double)kGatherMost / (double)need)));
-  const long groups = (std::max(1, d->batch) + n - 1) / n;
-  return (std::max(1, d->batch) + groups - 1) / groups;
 }
 template <class T>
 int page_gather(const s2c_attention_desc* d, const s2c_page_desc* pages, const void* keys, const void* values, int length, void* k, void* v, stream_t st) {
@@ -79,11 +79,15 @@ inline AttnParams paged_params(const s2c_attention_desc* d, const s2c_page_desc*
 }
 // Many queries: keys and values are brought into one array for the kernels of whole tiles, instead of being read again by every 16 rows.
 // 4 x 4096 positions, 4 key heads of 128, 32, 128, 256 and 512 rows for each: in pages 23, 56, 95 and 174 us (float32 45, 127, 224 and
-// 427), in one array 48 to 49 (253 to 259) and some 11 (17) to bring them there.  Not where one sequence alone takes more than 1 GB of
-// workspace: by its columns, since what is kept of them only the device knows.
+// 427), in one array 48 to 49 (253 to 259) and some 11 (17) to bring them there.  Not where that takes more than 1 GB for one sequence (by its
+// columns, since what is kept of them only the device knows; packed copies come on top, in float32 1.5 times as much).  In groups of
+// sequences only where their tiles fill half of the SMs: float32, tables of 65536 positions, 16 heads of 128 on 4, groups of 32, 48, 64 and 96
+// tiles 1194, 2375, 373 and 397 us, in pages 916, 1641, 385 and 916 (16 x 1000 kept and 256 queries, 64 x 300 and 300, 9 x 400 and 400, and the
+// first again with three sequences to a group; bfloat16 99 us and 366, 288 and 751, 55 and 174).
 inline bool paged_gathers(const s2c_attention_desc* d, const s2c_page_desc* pages) {
-  const long rows = (long)d->lq * (d->heads / d->kv_heads);
-  return rows > (d->dtype == kSeqF32 ? 256 : 128) && gathered_need(d, pages, 1) <= kGatherMost;
+  const long rows = (long)d->lq * (d->heads / d->kv_heads), n = gathered_at_once(d, pages);
+  if (rows <= (d->dtype == kSeqF32 ? 256 : 128) || n == 0) return false;
+  return n >= d->batch || n * d->heads * ((d->lq + 127) / 128) >= dev_sm_count() / 2;
 }
 // rows of 16-byte pieces (of four values at least): keys and values as they lie
 template <class T>
@@ -178,7 +182,7 @@ size_t s2c_paged_attention_workspace(const s2c_attention_desc* d, const s2c_page
     return d->dtype == kSeqF32 ? paged_plan<float>(a).bytes : paged_plan<bf16>(a).bytes;
   }
 #endif
-  const long n = gathered_at_once(d, pages), rest = d->batch % n;
+  const long n = std::max(1L, gathered_at_once(d, pages)), rest = d->batch % n;
   return std::max(gathered_need(d, pages, n), rest ? gathered_need(d, pages, rest) : 0);
 }
 
@@ -199,7 +203,7 @@ int s2c_paged_attention(const s2c_attention_desc* d, const s2c_page_desc* pages,
                                : paged_launch<bf16>(a, pages, keys, values, workspace, (stream_t)stream);
   }
 #endif
-  const long at_once = gathered_at_once(d, pages), size = d->dtype == kSeqF32 ? 4 : 2;
+  const long at_once = std::max(1L, gathered_at_once(d, pages)), size = d->dtype == kSeqF32 ? 4 : 2;
   for (long b = 0; b < d->batch; b += at_once) {
     s2c_attention_desc g = gathered(d, pages);
     s2c_page_desc some = *pages;
