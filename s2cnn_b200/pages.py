@@ -134,16 +134,19 @@ class PagedCache:
                 need[s] = columns - len(self._pages[s])
         if len(copies) + sum(need.values()) > len(self._free):
             raise MemoryError("PagedCache: %d more pages are needed, %d are free" % (len(copies) + sum(need.values()), len(self._free)))
-        moved = []
+        moved, entries = [], []
         for s, last in copies:
-            own = self._take()
+            own, column = self._take(), self.lengths[s] // self.page
             self._uses[last] -= 1
-            self._pages[s][self.lengths[s] // self.page] = own
+            self._pages[s][column] = own
             moved.append((last, own))
+            entries.append((s, column, own))
         for s, n in need.items():
-            self._pages[s] += [self._take() for _ in range(n)]
+            for _ in range(n):
+                entries.append((s, len(self._pages[s]), self._take()))
+                self._pages[s].append(entries[-1][2])
         self._copy(moved)
-        self._upload(sorted(set(need) | {s for s, _ in copies}))
+        self._upload(entries)
         self._new = new
 
     def advance(self):
@@ -151,7 +154,7 @@ class PagedCache:
         if any(self._new):
             self.lengths = [a + b for a, b in zip(self.lengths, self._new)]
             self._new = [0] * len(self.lengths)
-            self.filled.copy_(torch.tensor(self.lengths, dtype=torch.int32), non_blocking=True)
+            self.filled.copy_(self._staged(torch.tensor(self.lengths, dtype=torch.int32)), non_blocking=True)
 
     def fork(self, source, target):
         """Sequence ``target``, which is empty, continues from all that is filled of ``source``: its pages are shared until one of
@@ -161,6 +164,7 @@ class PagedCache:
         self._pages[target] = self._pages[source][:-(-self.lengths[source] // self.page)]
         for p in self._pages[target]:
             self._uses[p] += 1
+        self._upload([(target, column, p) for column, p in enumerate(self._pages[target])])
         self._grown(target, self.lengths[source])
 
     def truncate(self, sequence, length):
@@ -170,6 +174,7 @@ class PagedCache:
         keep = -(-length // self.page)
         for p in self._pages[sequence][keep:]:
             self._give(p)
+        self._upload([(sequence, column, -1) for column in range(keep, len(self._pages[sequence]))])
         del self._pages[sequence][keep:]
         self._grown(sequence, length)
 
@@ -188,10 +193,8 @@ class PagedCache:
         for a, b in moved:
             self._uses[b], self._uses[a] = self._uses[a], 0
         self._free = list(range(len(self._uses) - 1, held - 1, -1))
-        changed = [s for s, pages in enumerate(self._pages) if any(p in to for p in pages)]
-        for s in changed:
-            self._pages[s] = [to.get(p, p) for p in self._pages[s]]
-        self._upload(changed)
+        self._upload([(s, column, to[p]) for s, pages in enumerate(self._pages) for column, p in enumerate(pages) if p in to])
+        self._pages = [[to.get(p, p) for p in pages] for pages in self._pages]
         return held
 
     # -- the host's account
@@ -215,15 +218,18 @@ class PagedCache:
 
     def _grown(self, s, length):
         self.lengths[s] = length
-        self._upload([s])
         self.filled[s].fill_(length)
 
-    def _upload(self, sequences):
-        if sequences:
-            rows = torch.full((len(sequences), self.table.size(1)), -1, dtype=torch.int32)
-            for row, s in zip(rows, sequences):
-                row[:len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
-            self.table[self._on_device(torch.tensor(sequences))] = self._on_device(rows)
+    def _upload(self, entries):
+        """the entries (sequence, column, page) of the table that have changed"""
+        if entries:
+            at, pages = self._on_device(torch.tensor([(s * self.table.size(1) + column, page) for s, column, page in entries]).t().contiguous())
+            self.table.view(-1)[at] = pages.int()
+
+    def _staged(self, t):
+        # (from pageable memory the driver may wait for the stream before it copies, and does from 64 KB on; a block of the pinned memory that
+        # torch keeps is not used again before the copy from it has run)
+        return t.pin_memory() if self.storage.is_cuda else t
 
     def _on_device(self, t):
-        return t.to(self.storage.device, non_blocking=True)       # (from pageable memory: the host does not wait for the device)
+        return self._staged(t).to(self.storage.device, non_blocking=True)

@@ -4,6 +4,7 @@ Tolerances: as in test_norm_rotate.py and test_pages.py; what is compared withou
 """
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -198,3 +199,69 @@ def test_many_queries_over_wide_tables(backend, dtype, Hk):
             one = {n: t if n == "causal" else t[b:b + 1] for n, t in kw.items()}
             alone = S.paged_attention(q[b:b + 1], keys, values, pages[b:b + 1], table, buckets, **one)
             assert torch.equal(out[b:b + 1], alone) if Hk != 2 else rel(out[b:b + 1], alone) <= 2 * TOL[dtype]
+
+
+# ---- the account of a pool ----------------------------------------------------------------------------------------------
+
+
+def account(cache, table, filled):
+    """the table and the lengths on the device are the host's"""
+    want = torch.full(table.shape, -1, dtype=torch.int32)
+    for row, pages in zip(want, cache._pages):
+        row[:len(pages)] = torch.tensor(pages, dtype=torch.int32)
+    assert torch.equal(table.cpu(), want) and filled.tolist() == cache.lengths
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+def test_the_table_follows_the_account(backend):
+    with backends.active(backend) as (_, dev):
+        rng = random.Random(70)
+        for columns in (6, 300):
+            cache = S.PagedCache(40, 8, 1, 4, 7, columns=columns, device=dev)
+            for _ in range(120):
+                what, s, t = rng.choice(["extend", "extend", "extend", "fork", "truncate", "free", "compact"]), rng.randrange(7), rng.randrange(7)
+                if what == "extend":
+                    try:
+                        cache.extend([rng.choice([0, 0, 1, 3, 17]) for _ in range(7)])
+                        if rng.random() < 0.3:
+                            cache.extend([rng.choice([0, 1, 5]) for _ in range(7)])
+                    except MemoryError:
+                        pass
+                    cache.advance()
+                elif what == "fork" and s != t:
+                    cache.free(t)
+                    cache.fork(s, t)
+                elif what == "truncate":
+                    cache.truncate(s, rng.randint(0, cache.lengths[s]))
+                elif what == "free":
+                    cache.free(s - 7)                        # (counted from the end)
+                elif what == "compact":
+                    held = cache.compact()
+                    assert all(p < held for pages in cache._pages for p in pages)
+                account(cache, cache.table, cache.filled)
+
+
+@pytest.mark.gpu
+def test_the_account_does_not_wait_for_the_device():
+    """Steps, forks and the rest come back while work that was queued before them still runs, whatever the table's width."""
+    a = torch.randn(8192, 8192, device="cuda", dtype=BF16)
+    for turn in range(2):                                        # (the first one has memory pinned)
+        cache = S.PagedCache(30000, 8, 1, 8, 64, columns=16384, dtype=BF16)
+        cache.extend([8 * n for n in range(64)])
+        cache.advance()
+        torch.cuda.synchronize()
+        for _ in range(300):
+            b = a @ a
+        done = torch.cuda.Event()
+        done.record()
+        for step in range(5):
+            cache.extend(9)
+            cache.advance()
+            cache.free(step)
+            cache.fork(60, step)
+            cache.truncate(50 + step, 20)
+            cache.compact()
+        waited = done.query()
+        account(cache, cache.table, cache.filled)
+        assert not (turn and waited)
+        del b
