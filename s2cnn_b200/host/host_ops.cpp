@@ -692,10 +692,11 @@ struct Ops {
     for (int i = 0; i < 3; ++i) { d.k_stride[i] = a.k.stride(i); d.v_stride[i] = a.v.stride(i); }
     return d;
   }
+  static bool is_position(int64_t n) { return n >= -0x7fffffff && n <= 0x7fffffff; }
   // what the queries, their positions and the bias say
   s2c_attention_desc query_desc(AttnArgs& a, int dtype) const {
     check(a.bias.defined() == a.buckets.defined(), "attention: bias and buckets come together");
-    check(std::abs(a.q_start) <= 0x7fffffff, "attention: q_start is out of range");
+    check(is_position(a.q_start), "attention: q_start is out of range");
     for (int i = 0; i < 4; ++i) check(a.q.size(i) <= 0x7fffffff, "attention: too large");
     s2c_attention_desc d = {};
     d.dtype = dtype;
@@ -862,7 +863,7 @@ struct Ops {
       want(t->dim() == 1 && t->size(0) == d.dim, "a weight for each value of a head");
       *t = t->contiguous();
     }
-    want(std::abs(a.start) <= 0x7fffffff, "positions are out of range");
+    want(is_position(a.start), "positions are out of range");
     d.start = (int)a.start;
     if (a.positions.defined()) {
       if (a.positions.scalar_type() != at::kInt || a.positions.device() != any.device())

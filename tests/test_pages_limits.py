@@ -11,6 +11,7 @@ import torch
 
 import backends
 import s2cnn_b200 as S
+from s2cnn_b200 import _lib
 from test_norm_rotate import normal
 from test_pages import gathered, ints, pool, shuffled
 from test_pages_calls import attention_desc, page_desc
@@ -147,6 +148,20 @@ def test_rows_that_are_not_there(case):
     done = subprocess.run([sys.executable, "-c", _ENDS] + [str(x) for x in case], cwd=here, env=dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(here)))),
                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     assert done.returncode == 0 and "done" in done.stdout, done.stdout
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+def test_first_positions_out_of_range(backend):
+    """Numbers that are no 32-bit positions are refused, the least 64-bit one (whose magnitude is none) among them; 32-bit ones are not."""
+    with backends.active(backend) as (_, dev):
+        q, keys, pages = torch.ones(1, 1, 1, 8, device=dev), torch.ones(1, 8, 1, 8, device=dev), torch.zeros(1, 1, dtype=torch.int32, device=dev)
+        for start in (1 << 31, -(1 << 31), (1 << 63) - 1, -(1 << 63)):
+            for call in (lambda: S.norm_rotate(q, None, positions=start), lambda: S.norm_rotate_store(q, q, q, keys, keys, pages, positions=start),
+                         lambda: S.paged_attention(q, keys, keys, pages, q_start=start), lambda: S.attention(q, q, q, q_start=start)):
+                with pytest.raises((AssertionError, _lib.S2cError), match="range"):
+                    call()
+        for start in ((1 << 31) - 1, 1 - (1 << 31)):
+            assert torch.equal(S.norm_rotate(q, None, positions=start)[0], q) and S.attention(q, q, q, q_start=start).shape == q.shape
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
