@@ -263,5 +263,5 @@ class SequenceBlock(nn.Module):
             q = norm_rotate_store(q, k, v, keys, values, pages, *turning, positions=filled, lengths=lengths)
             bias = (self.bias.weight.to(q.dtype), self.bias.buckets) if self.rotary is None else (None, None)
             a = paged_attention(q, keys, values, pages, *bias, causal=self.causal, q_start=filled, q_lengths=lengths,
-                                kv_lengths=filled + (x.size(1) if lengths is None else lengths))
+                                kv_lengths=filled + (x.size(1) if lengths is None else lengths.clamp(max=x.size(1))))
             return self._rest(x, a)

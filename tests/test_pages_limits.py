@@ -280,3 +280,22 @@ def test_the_account_does_not_wait_for_the_device():
         account(cache, cache.table, cache.filled)
         assert not (turn and waited)
         del b
+
+
+# ---- blocks -------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("backend", backends.BACKENDS)
+@pytest.mark.parametrize("rotary", [None, 8])
+def test_lengths_beyond_the_new_positions(backend, rotary):
+    """Count as all of them, and below 0 as none: what a page holds behind the new positions is not looked at."""
+    with backends.active(backend) as (_, dev):
+        torch.manual_seed(72)
+        block = S.SequenceBlock(32, 4, 2, causal=False, p=0.0, rotary=rotary).to(dev).eval()
+        x, results = torch.randn(3, 4, 32, device=dev), []
+        pages, filled = ints([[0, 1], [2, 3], [4, 5]], dev), ints([5, 3, 1], dev)
+        for lengths in ([4, 2, 0], [9, 2, -3]):
+            keys, values = (torch.randn(6, 8, 2, 8, generator=torch.Generator().manual_seed(73 + n)).to(dev) for n in (0, 1))
+            results.append((block.step_pages(x, keys, values, pages, filled, lengths=ints(lengths, dev)), keys, values))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
