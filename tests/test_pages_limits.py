@@ -13,7 +13,7 @@ import backends
 import s2cnn_b200 as S
 from s2cnn_b200 import _lib
 from test_norm_rotate import normal
-from test_pages import gathered, ints, pool, shuffled
+from test_pages import check_attention, gathered, ints, pool, shuffled
 from test_pages_calls import attention_desc, page_desc
 from test_sequence_ops import TOL, exact_attention, rel
 
@@ -214,6 +214,66 @@ def test_many_queries_over_wide_tables(backend, dtype, Hk):
             one = {n: t if n == "causal" else t[b:b + 1] for n, t in kw.items()}
             alone = S.paged_attention(q[b:b + 1], keys, values, pages[b:b + 1], table, buckets, **one)
             assert torch.equal(out[b:b + 1], alone) if Hk != 2 else rel(out[b:b + 1], alone) <= 2 * TOL[dtype]
+
+
+def lengths_of(batch, most):
+    """from none and one to all, in no order"""
+    return [0, 1, most] + [(37 * i * i + 11 * i) % (most + 1) for i in range(batch - 3)]
+
+
+MANY = [
+    # B, lq, room, H, Hk, D, page, bias, kept; with 148 SMs at most 444 blocks share the items (sequence, key head, 8 or 16 rows)
+    (64, 1, 700, 16, 8, 64, 16, None, lengths_of(64, 700)),                      # 512 items
+    (64, 3, 500, 32, 8, 64, 32, (16, 30), lengths_of(64, 500)),                  # 512, of 12 rows
+    (200, 1, 6000, 8, 4, 32, 64, None, [6000] + [(7 * i) % 50 for i in range(199)]),     # 800, one long sequence among short ones
+    (150, 24, 200, 2, 2, 128, 16, None, lengths_of(150, 200)),                   # 600: 24 rows are two times 16
+    (70, 2, 900, 16, 8, 128, 64, (8, 20), lengths_of(70, 900)),                  # 560
+    (500, 1, 40, 3, 1, 25, 8, None, lengths_of(500, 40)),                        # 500, of one step each; four sequences to a thread that adds up
+    (3, 200, 1500, 8, 8, 40, 16, None, [1500, 700, 0]),                          # 312 of 16 rows in float32; in bfloat16 200 rows take the kernels of whole tiles
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "x".join(map(str, c[:7])))
+def test_more_items_than_blocks(case, causal, dtype):
+    """Each item's share is found, joined and written, with a workspace full of NaN; the same in every call."""
+    B, lq, room, H, Hk, D, page, bias, kept = case
+    kw = {"kv_lengths": kept}
+    if causal:
+        kw |= {"causal": True, "q_start": [n - lq for n in kept]}
+    else:
+        kw |= {"q_lengths": [(i * 5) % (lq + 1) for i in range(B)]}
+    results = []
+    for _ in range(2):
+        stale = torch.full((1 << 26,), math.nan, device="cuda")
+        del stale
+        results.append(check_attention("cuda", dtype, B, lq, room, H, Hk, D, page, bias, seed=65, **kw))
+    assert torch.equal(*results)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_ragged_new_positions(dtype):
+    """A step in which one of sixteen sequences brings 30 positions, one none and the others one: a row of the call on each sequence alone."""
+    gen = torch.Generator().manual_seed(66)
+    B, new, H, Hk, D, page = 16, 30, 16, 4, 64, 32
+    counts = [30, 0] + [1] * 14
+    filled = [100 + 61 * i for i in range(B)]
+    keys, values = pool(gen, "cuda", dtype, B * 36 + 2, page, Hk, D)
+    pages = shuffled(gen, "cuda", B * 36 + 2, B, 36)
+    q, k, v = normal(gen, "cuda", dtype, B, new, H + 2 * Hk, D).split((H, Hk, Hk), 2)
+    f, lengths, at = S.rotary_frequencies(32, device="cuda"), ints(counts, "cuda"), ints(filled, "cuda")
+    turned = S.norm_rotate_store(q, k, v, keys, values, pages, f, positions=at, lengths=lengths)
+    kw = {"causal": True, "q_start": at, "q_lengths": lengths, "kv_lengths": at + lengths}
+    out = S.paged_attention(turned, keys, values, pages, **kw)
+    assert rel(out, exact_attention(turned, gathered(keys, pages), gathered(values, pages), **kw)[0]) <= TOL[dtype]
+    for b, n in enumerate(counts):
+        assert not out[b, n:].any()
+        if n:
+            alone = S.paged_attention(turned[b:b + 1, :n], keys, values, pages[b:b + 1], causal=True, q_start=filled[b], kv_lengths=ints([filled[b] + n], "cuda"))
+            assert rel(out[b:b + 1, :n], alone) <= 2 * TOL[dtype]
 
 
 # ---- the account of a pool ----------------------------------------------------------------------------------------------
