@@ -77,7 +77,8 @@ class PagedCache:
 
     Which page is whose is decided on the host, which knows how far each sequence has grown (``lengths``, a list); the
     kernels read ``table`` int32 [sequences, columns] and ``filled`` int32 [sequences] on the device.  These keep their addresses,
-    so that a step may be captured and replayed after ``extend``.  Everything runs on the current stream; nothing waits for the device.
+    so that a step may be captured and replayed after ``extend`` (the account's own calls are not captured).  Everything runs on the
+    current stream; nothing waits for the device.
 
     A step of a model: ``cache.extend(new)`` makes room for new positions, the layers run ``SequenceBlock.step_pages`` with
     ``cache.keys(layer)``, ``cache.values(layer)``, ``cache.table`` and ``cache.filled`` (the positions before this step), and
@@ -116,6 +117,7 @@ class PagedCache:
         """Begins a step of ``new`` positions for every sequence (a number or one per sequence): pages that they need are taken, and
         a shared page that would be written is copied first.  Raises MemoryError, and changes nothing, if the pool does not hold
         them."""
+        self._uncaptured("extend")
         new = [new] * len(self.lengths) if isinstance(new, int) else list(new)
         assert len(new) == len(self.lengths) and min(new) >= 0, "extend: a number of new positions for each sequence"
         need, copies = {}, []
@@ -151,6 +153,7 @@ class PagedCache:
 
     def advance(self):
         """Ends the step: its positions count as filled."""
+        self._uncaptured("advance")
         if any(self._new):
             self.lengths = [a + b for a, b in zip(self.lengths, self._new)]
             self._new = [0] * len(self.lengths)
@@ -159,8 +162,8 @@ class PagedCache:
     def fork(self, source, target):
         """Sequence ``target``, which is empty, continues from all that is filled of ``source``: its pages are shared until one of
         the two writes to the last of them."""
-        assert source != target and not self._pages[target] and self.lengths[target] == 0, "fork: the target is not empty"
         self._settled("fork")
+        assert source != target and not self._pages[target] and self.lengths[target] == 0, "fork: the target is not empty"
         self._pages[target] = self._pages[source][:-(-self.lengths[source] // self.page)]
         for p in self._pages[target]:
             self._uses[p] += 1
@@ -169,8 +172,8 @@ class PagedCache:
 
     def truncate(self, sequence, length):
         """Forgets the positions of a sequence from ``length`` on."""
-        assert 0 <= length <= self.lengths[sequence], "truncate: the sequence is shorter"
         self._settled("truncate")
+        assert 0 <= length <= self.lengths[sequence], "truncate: the sequence is shorter"
         keep = -(-length // self.page)
         for p in self._pages[sequence][keep:]:
             self._give(p)
@@ -198,7 +201,11 @@ class PagedCache:
         return held
 
     # -- the host's account
+    def _uncaptured(self, what):
+        assert not (self.storage.is_cuda and torch.cuda.is_current_stream_capturing()), what + ": the account changes between captured steps, not in one"
+
     def _settled(self, what):
+        self._uncaptured(what)
         assert not any(self._new), what + ": a step has begun (advance() ends it)"
 
     def _take(self):

@@ -359,3 +359,25 @@ def test_lengths_beyond_the_new_positions(backend, rotary):
             results.append((block.step_pages(x, keys, values, pages, filled, lengths=ints(lengths, dev)), keys, values))
         for a, b in zip(*results):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_the_account_is_not_captured():
+    """A replay would copy from memory that has long been used for something else: refused before anything changes."""
+    cache = S.PagedCache(20, 8, 1, 8, 3)
+    cache.extend(5)
+    cache.advance()
+    x = torch.ones(1, device="cuda")
+    for call in (lambda: cache.extend(9), cache.advance, lambda: cache.fork(0, 2), lambda: cache.truncate(0, 2), lambda: cache.free(1), cache.compact):
+        before = list(cache.lengths), [list(p) for p in cache._pages], list(cache._free)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x.add_(1)
+            with pytest.raises(AssertionError, match="captured"):
+                call()
+        assert before == (cache.lengths, cache._pages, cache._free)
+        account(cache, cache.table, cache.filled)
+        del graph
+    cache.extend(9)
+    cache.advance()
+    account(cache, cache.table, cache.filled)
