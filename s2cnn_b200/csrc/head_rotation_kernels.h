@@ -17,10 +17,11 @@
 // values, so that a lane has one weight.
 //
 // Bound by instructions and their latencies with 16 warps an SM, half of what memory would take: 4 x 4096 positions, 20 heads of 128
-// bfloat16 values, forward 37 us (4.5 TB/s), without a norm 31 (5.4); backward 53 us (4.8), and 4 for the sums of the blocks.  Two blocks
-// an SM with four heads of a turn loaded ahead (two in float32 and backward): three blocks with two heads 36.6, but 14.0 instead of 12.3
-// where the turns are few (a first pass of 4 x 2049 ragged positions, 20 heads of 64, into pages); backward with one head a turn 111
-// instead of 94 for both passes, with one and three blocks 97.
+// bfloat16 values, forward 36 us (4.7 TB/s), without a norm 31 (5.4); backward 53 us (4.8), and 4 for the sums of the blocks; a first pass
+// of 4 x 2049 ragged positions, 20 heads of 64, into pages 12.6.  Two blocks an SM with four heads of a turn loaded ahead (two in float32
+// and backward).  Others, when this was chosen: three blocks with two heads 36.6 us where this had 37, but 14.0 for the first pass, where
+// this had 12.3; backward with one head a turn 111 where this had 94 for both passes, with one and three blocks 97.  Instances of single
+// values with four heads ahead keep up to 274 bytes a thread of them in local memory (bfloat16, heads of 65 to 128 values).
 #pragma once
 
 #include <cstring>

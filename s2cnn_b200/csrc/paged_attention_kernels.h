@@ -11,7 +11,7 @@
 // Keys of the next tile are asked for as soon as the scores of this one are done, its values as soon as the outputs are: a warp has
 // up to 8 KB (float32 16) on its way and waits for nobody.  The page of every eighth position comes a tile earlier, by one load per warp.
 // A tile that goes past the last position reads that one again there, with a weight of 0, and where the table names no page, page 0: no
-// load is guarded.  (Guarded ones, whose registers keep what they held, cost 64 x 16384 positions 579 us instead of 313.)
+// load is guarded.  (Guarded ones, whose registers keep what they held, cost 64 x 16384 positions 579 us.)
 //
 // Work is dealt in steps of (4 warps x tile) positions of one item (sequence, key head, row block), an equal share to each block as
 // the lengths on the device give it: a block finds where its share begins by adding up the sequences' steps.  Items that lie in
@@ -22,7 +22,8 @@
 //
 // Bound by memory where sequences are long: 64 x 16384 positions, 16 heads of 128 on 4, 2.1 GB: 315 us (6.8 TB/s; the measured copy
 // rate is 6.56); 16 ragged ones of up to 16384, 285 MB, 49 us (5.9).  Short ones by the chain of a block's loads, lengths, pages, keys, and
-// the second launch: one step 5 us, 1 x 16384 positions 15 us (2.3 TB/s).
+// the second launch: one step 5 us, 1 x 16384 positions 15 us (2.3 TB/s).  The steps of a sequence are those of its last query for all of
+// its row blocks: rows that see less, or none, take as long.
 #pragma once
 
 #include "attention_few.h"
@@ -110,7 +111,10 @@ struct PagedAttention {
   using Params = PagedParams;
   using H = PagedShape<T, DP, NT>;
   static constexpr int kThreads = H::kThreads;
-  static constexpr int kBlocks = (H::kHalf ? DP <= 64 || NT == 1 : DP <= 64) ? 3 : 2;      // as registers allow
+  // Blocks an SM, and with them 168 or 255 registers a thread.  Those hold a step's keys and values in <bf16, 128, 1> and <float, 64, 1> on
+  // whole rows; other instances keep a part in local memory: 4 to 102 bytes a thread with one row group, with two 78 to 298 at 168
+  // registers, and at 255 4 to 22 (bfloat16) or 334 to 410 (float32).
+  static constexpr int kBlocks = (H::kHalf ? DP <= 64 || NT == 1 : DP <= 64) ? 3 : 2;
   // queries, results, the search for the share; the biases of each row by bucket, 0 behind them, and the bucket of each position
   static size_t smem(const AttnParams& a) {
     return H::kQuery + H::kJoin + 128 + (a.bias ? (size_t)H::kRows * (a.n_buckets + 1) * 4 + (size_t)(2 * a.reach + 1) * 2 : 0);

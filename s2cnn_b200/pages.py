@@ -42,8 +42,11 @@ def _eps(eps):
 
 def paged_attention(q, keys, values, pages, bias=None, buckets=None, causal=False, scale=None, q_start=0, q_lengths=None, kv_lengths=None):
     """``sequence.attention`` (its formula and its other parameters) over keys and values in pages: for new positions, whose keys and
-    values are read once, or more (beyond 128 rows of queries and heads per key head, 256 in float32, they are first copied into
-    one array).
+    values are read once, or, beyond 16 rows of queries and heads per key head, once for every 16.
+
+    Beyond 128 rows (256 in float32) they are first copied into one array, where the whole of their columns takes at most 1 GB for
+    one sequence, whatever is kept, for the kernels of ``attention``, which round bfloat16 weights to 8 bits; otherwise these have 16 (and
+    the float32 ones 22: products of two TF32 parts).
 
     :param q: [batch, queries, heads, dim], dim <= 128; any strides with a contiguous last axis
     :param keys, values: [pages, positions of a page, kv_heads, dim]
@@ -71,6 +74,9 @@ def copy_pages(storage, source, target):
 
 class PagedCache:
     """The kept keys and values of up to ``sequences`` sequences, in all layers of a model, in a pool of ``pages`` pages.
+
+    ``columns`` are the pages that a sequence can have: by default, all of the pool, up to 2^28 positions.  Long first passes want them no
+    larger than needed (see ``paged_attention``); ``table[:, :n].contiguous()`` does for a call on sequences that are known to be short.
 
     ``storage`` [pages, layers, 2, kv_heads, page, dim rounded up to 16 bytes] has the positions of a head in a page one after
     another, so that attention reads them in whole pieces, and all layers of a page together, so that forking copies one piece.
