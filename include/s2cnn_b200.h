@@ -392,7 +392,7 @@ int s2c_dropout_numbers(int dtype, const void* x, const void* residual, void* ou
 
 /* Heads of queries and keys, q [batch][length][heads][dim], k and v [batch][length][kv_heads][dim], any strides (in elements, of the
  * first three axes; the last is contiguous), dim <= 128: normed (norm != 0) head by head and turned by their position,
- *   z = x / sqrt(mean(x^2) + eps) * weight   (weight [dim], NULL: 1;  norm == 0: z = x)
+ *   z = x / sqrt(mean(x^2) + eps) * weight   (weight [dim], NULL: 1;  norm == 0: z = x;  zeros where the sum of squares is beyond float32)
  *   y_a = magnitude (z_a cos t - z_b sin t),  y_b = magnitude (z_a sin t + z_b cos t),  t = position * frequencies[pair]
  * for the pairs (a, b) = (i, i + pairs), or (2 i, 2 i + 1) where interleaved != 0, i < pairs; the values from 2 pairs on are not
  * turned.  frequencies: device float64 [pairs], radians per position; angles are computed modulo whole turns in 64 bits, so that far
